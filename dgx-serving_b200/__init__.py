@@ -41,6 +41,29 @@ class MoeLayout(ctypes.Structure):
                                                "xq_h", "xs_h", "sout", "bytes")]
 
 
+class KVCache(ctypes.Structure):
+    """Mirror of w4a8_kv_cache: codes k, v [num_blocks][heads][block][dim] int8, scales [num_blocks][heads] fp32."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("num_blocks", ctypes.c_int), ("heads", ctypes.c_int), ("block", ctypes.c_int), ("dim", ctypes.c_int)]
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale):
+        """The cache in four tensors, which the object keeps alive."""
+        for t in (k, v, k_scale, v_scale):
+            if not t.is_contiguous():
+                raise ValueError("a KV cache's tensors are contiguous")
+        if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+            raise ValueError("k, v: [num_blocks][heads][block][dim]; k_scale, v_scale: [num_blocks][heads]")
+        if (k.element_size(), v.element_size(), k_scale.element_size(), v_scale.element_size()) != (1, 1, 4, 4):
+            raise ValueError("a KV cache holds int8 codes and fp32 scales")
+        c = cls(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
+        c._tensors = (k, v, k_scale, v_scale)
+        c._ref = ctypes.byref(c)
+        return c
+
+
+DTYPES = {"fp32": 0, "fp16": 1, "bf16": 2}          # W4A8_F32, W4A8_F16, W4A8_BF16: rows of the attention operators
+
 _P, _I, _Z, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_int64
 _SIGNATURES = {
     "w4a8_version": (_I, []),
@@ -63,6 +86,12 @@ _SIGNATURES = {
     "w4a8_moe_layout_for": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(MoeLayout)]),
     "w4a8_moe_block": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "w4a8_moe_block_shard": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P, _Z, ctypes.c_uint32, _I, _I, _P]),
+    "w4a8_kv_plan": (_I, [_P, _P, _I, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
+    "w4a8_kv_append_q8": (_I, [_P, _P, _L, _P, _I, ctypes.POINTER(KVCache), _I, _P]),
+    "w4a8_kv_read_q8": (_I, [ctypes.POINTER(KVCache), _P, _I, _P, _P, _I, _I, _P, _P, _L, _I, _P]),
+    "w4a8_attention_q8_workspace_bytes": (_Z, [ctypes.POINTER(KVCache), _I, _I, _I]),
+    "w4a8_attention_q8": (_I, [_P, _L, ctypes.POINTER(KVCache), _P, _I, _P, _P, _I, _I, _I, _P, _L, _P, ctypes.c_float, _I, _I, ctypes.c_float, _I, _I,
+                               _P, _Z, _P]),
     "w4a8_shard_rows": (_I, [_L, _I, _I, ctypes.POINTER(_L), ctypes.POINTER(_L)]),
     "w4a8_load_qmat_shard": (_I, [ctypes.c_char_p, ctypes.c_char_p, _L, _L, _I, _I, _I, ctypes.POINTER(QMat)]),
     "w4a8_upload_qmat_shard": (_I, [_P, _P, _L, _L, _I, _I, _I, ctypes.POINTER(QMat)]),
@@ -258,6 +287,36 @@ def moe_block_shard(n2, gu_wq, gu_sc, dn_wq, dn_sc, idx, dw, out, S, topk, H, MI
     _check(lib().w4a8_moe_block_shard(_ptr(n2), _ptr(gu_wq), _ptr(gu_sc), _ptr(dn_wq), _ptr(dn_sc), _ptr(idx), _ptr(dw), _ptr(out), S, topk, H, MI,
                                       expert_base, experts_local, scale_dtype, act, _ptr(workspace),
                                       workspace.numel() * workspace.element_size(), arena.handle, sout_offset, epoch, timeout_us, phase, _stream(stream)))
+
+
+def kv_plan(kv_len, new_len, R, block, block_table, table_width, free_blocks, num_free, first_free, seq_len, cu_new, slot, position, T, status, stream=None):
+    """Block tables and slot maps of a step from the requests' lengths, on the GPU (w4a8_kv_plan); position may be None."""
+    _check(lib().w4a8_kv_plan(_ptr(kv_len), _ptr(new_len), R, block, _ptr(block_table), table_width, _ptr(free_blocks), num_free, _ptr(first_free),
+                              _ptr(seq_len), _ptr(cu_new), _ptr(slot), _ptr(position), T, _ptr(status), _stream(stream)))
+
+
+def launch_kv_append_q8(K, V, ld, slot, T, cache, dtype="fp32", stream=None):
+    """Rows K, V [T][heads * dim] (pitch ld elements) into their slots of the 8-bit cache (w4a8_kv_append_q8)."""
+    _check(lib().w4a8_kv_append_q8(_ptr(K), _ptr(V), ld, _ptr(slot), T, cache, DTYPES.get(dtype, dtype), _stream(stream)))
+
+
+def launch_kv_read_q8(cache, block_table, table_width, begin, cu, R, T, K, V, ld, dtype="fp32", stream=None):
+    """The numbers that the cache holds for tokens begin[r] + i of each request, to rows cu[r] + i of K and V (w4a8_kv_read_q8)."""
+    _check(lib().w4a8_kv_read_q8(cache, _ptr(block_table), table_width, _ptr(begin), _ptr(cu), R, T, _ptr(K), _ptr(V), ld, DTYPES.get(dtype, dtype),
+                                 _stream(stream)))
+
+
+def attention_q8_workspace_bytes(heads_q, cache, T=0, max_q=0):
+    return int(lib().w4a8_attention_q8_workspace_bytes(cache, heads_q, T, max_q))
+
+
+def launch_attention_q8(Q, ldq, cache, block_table, table_width, cu_q, seq_len, R, T, heads_q, O, ldo, scale, dtype, workspace, causal=1, window=0,
+                        softcap=0.0, max_q=0, lse=None, stream=None):
+    """Attention of the rows Q[T][heads_q * dim], the last tokens of R requests, over the 8-bit cache (w4a8_attention_q8).  workspace: a device
+    tensor of attention_q8_workspace_bytes(...) bytes, zeroed once."""
+    _check(lib().w4a8_attention_q8(_ptr(Q), ldq, cache, _ptr(block_table), table_width, _ptr(cu_q), _ptr(seq_len), R, T, heads_q, _ptr(O), ldo, _ptr(lse),
+                                   scale, causal, window, softcap, max_q, DTYPES.get(dtype, dtype), _ptr(workspace),
+                                   workspace.numel() * workspace.element_size(), _stream(stream)))
 
 
 def shard_rows(N, rank, world):

@@ -79,7 +79,7 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
 }
 
 // ---- device-side error word (set when a bounded wait runs out) ---------------------------------
-__device__ unsigned int g_dev_error = 0u;  // one translation unit: w4a8_b200.cu includes every kernel file
+static __device__ unsigned int g_dev_error = 0u;  // one word per translation unit; w4a8_device_status reads them all
 __device__ __forceinline__ void dev_set_error(unsigned int code) { atomicCAS(&g_dev_error, 0u, code); }
 
 #ifdef __CUDACC__
@@ -142,7 +142,7 @@ __device__ __forceinline__ int quantize1_div(float x, float d) {
     asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(x / d));
     return max(q, -127);
 }
-__device__ __noinline__ uint32_t quantize4_div(float4 v, float d) {
+static __device__ __noinline__ uint32_t quantize4_div(float4 v, float d) {
     const int q0 = quantize1_div(v.x, d), q1 = quantize1_div(v.y, d), q2 = quantize1_div(v.z, d), q3 = quantize1_div(v.w, d);
     const uint32_t lo = __byte_perm((uint32_t)q0, (uint32_t)q1, 0x0040), hi = __byte_perm((uint32_t)q2, (uint32_t)q3, 0x0040);
     return __byte_perm(lo, hi, 0x5410);

@@ -41,7 +41,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // cost about 180 cycles instead of 34, on every hand-off of the pipeline.  The clock is read once per 64
 // attempts so that it does not delay the wake-up either.  Gives up after `limit_cycles` SM clocks.
 // (Passing a suspend-time hint of 2 us to try_wait changed no kernel's time: measured and left out.)
-__device__ __noinline__ bool mbar_wait_poll(uint32_t bar, uint32_t parity, long long limit_cycles) {
+static __device__ __noinline__ bool mbar_wait_poll(uint32_t bar, uint32_t parity, long long limit_cycles) {
     const long long t0 = clock64();
     for (;;) {
         for (int i = 0; i < 64; i++)

@@ -1,5 +1,5 @@
-// The single translation unit of libw4a8_b200.so: includes every kernel file and defines the C ABI
-// declared in include/w4a8_b200.h.  Build (see dgx-serving_b200/build.py):
+// The matmul path's translation unit of libw4a8_b200.so (the KV cache and attention are kv_cache.cu): includes its kernel
+// files and defines their part of the C ABI declared in include/w4a8_b200.h.  Build (see dgx-serving_b200/build.py):
 //   nvcc -gencode arch=compute_100a,code=sm_100a -O3 -std=c++17 -lineinfo -Xcompiler -fPIC -shared
 #include <cerrno>
 #include <cstdlib>
@@ -21,6 +21,9 @@
 #include "moe_w4a8.cuh"
 
 namespace w4a8 {
+
+cudaError_t kv_take_device_error(unsigned int *v);     // kv_cache.cu
+const char *kv_device_error_text(unsigned int v);
 
 char *err_buf() {
     static thread_local char buf[512] = {0};
@@ -117,8 +120,15 @@ W4A8_API int w4a8_device_status(uint32_t *detail) {
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
     e = cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(v));
     if (e != cudaSuccess) return cuda_fail(e, "read device error word");
+    if (v != 0) cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
+    unsigned int kv_error = 0;
+    e = kv_take_device_error(&kv_error);
+    if (e != cudaSuccess) return cuda_fail(e, "read device error word");
+    if (v == 0 && kv_error != 0) {
+        if (detail) *detail = kv_error;
+        return fail(W4A8_ERR_DEVICE, "%s (code 0x%x)", kv_device_error_text(kv_error), kv_error);
+    }
     if (v != 0) {
-        cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
         if (detail) *detail = v;
         return fail(W4A8_ERR_DEVICE, "a kernel's bounded wait ran out (code 0x%x)", v);
     }

@@ -267,6 +267,66 @@ int w4a8_moe_block_shard(const float *n2, const uint8_t *gu_wq, const void *gu_s
                          int experts_local, int scale_dtype, int act, void *workspace, size_t workspace_bytes,
                          struct w4a8_arena *a, size_t sout_offset, uint32_t epoch, int timeout_us, int phase, void *stream);
 
+/* ---- 8-bit paged KV cache and attention over it -----------------------------------------------------------
+ * What a layer does between its QKV and its output product.  The reference keeps keys and values in fp32 or fp16, contiguous per request
+ * (kernels/kv_store.cuh, kernels/attention*.cuh); here they are int8 codes in blocks of tokens with one fp32 scale per block, kv head and
+ * side, half or a quarter of the bytes that a decode step has to read:
+ *   k, v              [num_blocks][heads][block][dim] int8, contiguous, 16-byte aligned; element = code * scale
+ *   k_scale, v_scale  [num_blocks][heads] fp32
+ * block = 16, 32, 64 or 128 tokens; dim = 64, 128 or 256.  A request's tokens lie in the blocks that its row of the block table names:
+ * token p in block table[r][p / block], place p % block; slot = block * block_size + place.  num_blocks * block < 2^31.
+ * Rows outside the cache (Q, K, V, O) are fp32, fp16 or bf16 (dtype), a token per row of `ld` elements, heads side by side in it, so that
+ * columns of a fused QKV product can be passed as they are; pointers and pitches are multiples of 16 bytes.
+ * Table entries, slots and lengths are read on the device.  One that points outside the cache is not followed: it is left out (a slot) or
+ * taken as block 0 (a table entry, whose request's result is then void), and w4a8_device_status reports it. */
+enum { W4A8_F32 = 0, W4A8_F16 = 1, W4A8_BF16 = 2 };
+typedef struct w4a8_kv_cache {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int num_blocks, heads, block, dim;
+} w4a8_kv_cache;
+
+/* Block tables and slot maps of one step, built on the GPU from the requests' lengths in one launch: kv_len[R] tokens that a request holds
+ * (its first ceil(kv_len / block) table entries are set), new_len[R] that the step brings (negative numbers count as 0).
+ *   need[r] = ceil((kv_len + new_len) / block) - ceil(kv_len / block) fresh blocks, taken in the requests' order from
+ *   free_blocks[*first_free ...num_free) and written into block_table[r][...] (row pitch table_width).
+ *   A request is served if its tokens fit its table row and need[r] = 0 or the free list reaches for it and all requests in front of it
+ *   (those that do not fit their row need nothing).  Others get no block: seq_len[r] = 0, slots -1; kv_len stays theirs for the next step.
+ *   seq_len[r] = kv_len + new_len; cu_new[R + 1] = sums of new_len (the rows' starts, served or not)
+ *   slot[t], position[t] (may be NULL) of row t < T: -1 where there is none (rows of requests not served, rows behind cu_new[R])
+ *   status[4] = index in free_blocks behind the last block taken; requests not served; blocks taken; tokens placed.
+ * Outputs must not overlap inputs.  R <= 16384, sum of new_len < 2^31. */
+int w4a8_kv_plan(const int32_t *kv_len, const int32_t *new_len, int R, int block, int32_t *block_table, int table_width,
+                 const int32_t *free_blocks, int num_free, const int32_t *first_free, int32_t *seq_len, int32_t *cu_new, int32_t *slot,
+                 int32_t *position, int T, int32_t *status, void *stream);
+
+/* Writes the rows K[T][heads * dim], V[T][heads * dim] into their slots (slot < 0: the row is left out).  Rows that go to one block follow
+ * one another with ascending slots, and no two runs of a call go to the same block (what w4a8_kv_plan gives).  For each block, head and
+ * side: scale = max(the scale so far if the first new slot is not the block's first, amax(new rows) / 127); code = rintf(x / scale)
+ * clamped to +-127, the quantizer's arithmetic; codes in front of the first new slot become rintf(code * (scale so far / scale)) where the
+ * scale grew.  Codes behind the last new slot are left as they are.  An infinite element makes its block's scale infinite and the block's
+ * elements NaN (0 * inf); a NaN is stored as 0. */
+int w4a8_kv_append_q8(const void *K, const void *V, int64_t ld, const int32_t *slot, int T, const w4a8_kv_cache *cache, int dtype, void *stream);
+
+/* The numbers that the cache holds for tokens [begin[r], begin[r] + cu[r + 1] - cu[r]) of each request: row t < min(T, cu[R]) of K, V gets
+ * code * scale, rounded once to dtype; rows behind are left as they are. */
+int w4a8_kv_read_q8(const w4a8_kv_cache *cache, const int32_t *block_table, int table_width, const int32_t *begin, const int32_t *cu, int R, int T,
+                    void *K, void *V, int64_t ld, int dtype, void *stream);
+
+/* O[t] = softmax(scale * q k^T) v for the rows Q[T][heads_q * dim]: rows cu_q[r] .. cu_q[r + 1) are the LAST tokens of request r, which holds
+ * seq_len[r] tokens (the step's own are in the cache already).  Query head h reads kv head h / (heads_q / heads).  The query at position p
+ * sees keys j <= p (causal; all j < seq_len without) with j > p - window (window > 0).  softcap > 0: scores become
+ * softcap * tanh(score / softcap).  Rows that see nothing get zeros (and lse -inf); seq_len 0 is such a request.  lse[T][heads_q] (may be
+ * NULL): log of the sum of exp(score).  Scores, sums and weighted values are held in fp32; fp32 rows enter the products in two fp16 terms
+ * each (22 bits), 16-bit rows in one.  max_q: no request has more rows (0: not known); it chooses the kernel, not the result's meaning.
+ * The workspace (256-byte aligned, zeroed once by the caller, left zeroed where that matters) serves one stream at a time; its size holds
+ * for any lengths.  Row order, requests side by side and the GPU's SM count decide how the key axis is cut, so a row's last bits can differ
+ * between batches; the same call gives the same bits. */
+size_t w4a8_attention_q8_workspace_bytes(const w4a8_kv_cache *cache, int heads_q, int T, int max_q);
+int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *cache, const int32_t *block_table, int table_width, const int32_t *cu_q,
+                      const int32_t *seq_len, int R, int T, int heads_q, void *O, int64_t ldo, float *lse, float scale, int causal, int window,
+                      float softcap, int max_q, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a15: N-sharded weight upload --------------------------------------------------------------------
  * Replaces QMat + load_dev()/mat() (runtime/weights_qwen.h:8, runtime/weights_qwen.cu:12-36,
  * runtime/weights_gemma4.cu:12-41): `<name>_q4.bin` holds N*K/2 bytes, `<name>_scale.bin` holds
