@@ -28,6 +28,7 @@ constexpr int TK = 64;                     // tokens of a tile
 constexpr int CW = 4;                      // consumer warps: 16 tokens of the tile each
 constexpr int THREADS = (CW + 1) * 32;
 constexpr int MAX_R = 2048;                // requests of one launch (their sums lie in shared memory)
+constexpr int FEW_ROWS = 64;                // rows (queries x heads of a group) of a request that the streaming kernel takes at most
 constexpr int MIN_TILES = 2;               // a CTA takes at least so many tiles: joining costs about two tiles' time
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;

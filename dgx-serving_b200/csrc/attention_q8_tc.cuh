@@ -1,0 +1,516 @@
+// Attention of many queries a request (prompts) over the 8-bit paged KV cache on the tcgen05 tensor cores.
+//
+// Same formula as attention_q8.cuh.  What bounds it: 4 * dim operations for every (query row, key) pair on the tensor cores, and one
+// exponential for each pair on the special function units, which at dim 128 take as long.
+//  - A CTA takes 256 rows (queries x heads of a group, dim 256: 128) of one kv head as tiles of 128, and walks over the keys in tiles of 128
+//    (dim 256: 64).  S = Q K^T and O += P V are tcgen05.mma kind::f16 with fp32 accumulators in tensor memory: S of both row tiles, in whose
+//    columns the weights P are then written as fp16, and O of both: 512 columns.  While the warps of one row tile turn its S into P, the
+//    tensor core works on the other's.
+//  - The cache's codes come in by bulk copies along the block table, four warps turn them into fp16 (exact) in the operands' layout, rows of
+//    64 elements with the 128-byte swizzle: K is then K-major, V the same bytes read as MN-major, so neither is transposed.
+//  - A thread has one row: maximum, sum and rescaling need no exchange.  The weight that enters the product, exp(s - B) * vs, takes its
+//    block's scale in the exponent: x = exp2(f s + log2 vs - B), one multiply-add and one exp2; the sum divides it out again once per block
+//    and row.  B is such that the largest x was 2^8 when B was chosen; it moves, and O in tensor memory is rescaled, only when an x would
+//    pass 2^15.
+//  - fp32 rows enter as two fp16 terms each, Q and P, as in attention_q8.cuh: twice the products, 22 bits.
+#pragma once
+#include "attention_q8.cuh"
+
+namespace w4a8 {
+namespace attn_tc {
+
+using attn::LOG2E;
+using attn::LN2;
+using attn::ex2;
+using attn::h2_bits;
+constexpr unsigned ERR_WAIT = 0xB00u;
+constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
+constexpr int MAX_R = 2048;
+constexpr int SCALE_SLOTS = 4;
+
+template <typename T, int D> struct Shape {
+    static constexpr bool SPLIT = std::is_same<T, float>::value;
+    static constexpr int KT = D == 256 ? 64 : 128, NT = D == 256 ? 1 : 2, TERMS = SPLIT ? 2 : 1;
+    static constexpr int ST = SPLIT && D >= 128 ? 1 : 2;                    // fp16 stages of K and of V
+    static constexpr int QT = 128 * D * 2, KV = KT * D * 2, RAW = KT * D;    // bytes: one term of a row tile; a stage; its codes
+    static constexpr int OFF_KV = NT * TERMS * QT, OFF_RAW = OFF_KV + 2 * ST * KV, OFF_SCALE = OFF_RAW + 2 * RAW, OFF_BAR = OFF_SCALE + SCALE_SLOTS * 8 * 16;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;
+    static constexpr int S_COLS = KT, O_COL = 2 * KT;                        // TMEM: two S buffers, then O of each row tile
+    static_assert(O_COL + NT * D <= 512 && SMEM <= 227 * 1024, "shape");
+};
+
+enum { RAW_FULL = 0, RAW_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY = 10, S_FULL = 12, P_FULL = 14, PV_DONE = 16, O_FULL = 17, BARS = 19 };
+
+// D[tmem] (+)= A[tmem] B[smem]; A: 128 lanes, two fp16 a column.  B: N x 16 as the descriptor says.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// fp32 accumulators (bits [4,6) = 1), fp16 A and B; bit 16: B is MN-major; N >> 3 in [17,23), M >> 4 in [24,29).
+__host__ __device__ constexpr uint32_t idesc_f16(int N, int b_mn) { return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
+// MN-major operand, 128-byte swizzle: 64 elements of a row (one k) in 128 bytes, 8 rows 1024 bytes, the next 64 elements `mn_stride` on.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t mn_stride) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(mn_stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+                 "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+                 "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// cap * tanh(x) * log2 e with x in units of cap: 1 - 2 / (1 + e^2x), whose error is that of a number near 1
+__device__ __forceinline__ float capped(float x, float cap) {
+    return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E))));
+}
+
+// 8 elements of a row of Q as floats.
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+    const float4 a = attn::load4(p), b = attn::load4(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// Four bytes of codes as two packed pairs of fp16.
+__device__ __forceinline__ void widen(uint32_t w, uint32_t &a, uint32_t &b) {
+    w ^= 0x80808080u;
+    a = attn::codes_f16<0x4140>(w);
+    b = attn::codes_f16<0x4342>(w);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn::Args a, const int8_t *__restrict__ kc, const int8_t *__restrict__ vc) {
+    using S = Shape<T, D>;
+    constexpr int KT = S::KT, NT = S::NT, ST = S::ST, TERMS = S::TERMS;
+    constexpr bool SPLIT = S::SPLIT;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ unsigned wsum[THREADS / 32];
+    __shared__ int item[4];                       // request, kv head, row tile
+    __shared__ uint32_t tmem_slot;
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = ptx::smem_u32(smem), bars = base + S::OFF_BAR, scales = base + S::OFF_SCALE;
+    const auto BAR = [&](int i) { return bars + 8u * i; };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    // ---- which rows: the blockIdx.x-th item of all requests that have more than `few` rows --------------------------------------------
+    if (tid == 0) item[0] = -1;
+    {
+        unsigned carry = 0;
+        __syncthreads();
+        for (int r0 = 0; r0 < a.R; r0 += THREADS) {
+            const int r = r0 + tid;
+            unsigned v = 0;
+            if (r < a.R) {
+                const int q0 = max(0, min(a.cu_q[r], a.T)), n = max(0, min(a.cu_q[r + 1], a.T) - q0), rows = n * a.G;
+                if (rows > a.few) v = (unsigned)((rows + NT * 128 - 1) / (NT * 128)) * (unsigned)a.Hkv;
+            }
+            unsigned s = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const unsigned t = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += t; }
+            if (lane == 31) wsum[warp] = s;
+            __syncthreads();
+            unsigned front = carry;
+            for (int w = 0; w < warp; w++) front += wsum[w];
+            const unsigned lo = front + s - v;
+            if (v != 0 && blockIdx.x >= lo && blockIdx.x < lo + v) {
+                // the request's last rows first: with the causal mask they have the most keys
+                const unsigned in = blockIdx.x - lo, tiles = v / (unsigned)a.Hkv;
+                item[0] = r;
+                item[1] = (int)(in % (unsigned)a.Hkv);
+                item[2] = (int)(tiles - 1 - in / (unsigned)a.Hkv);
+            }
+            for (int w = 0; w < THREADS / 32; w++) carry += wsum[w];
+            __syncthreads();
+            if (item[0] >= 0) break;
+        }
+    }
+    const int r = item[0];
+    if (r < 0) return;
+    const attn::Request x = attn::request(a, r, 1);
+    const int h = item[1], row0 = item[2] * NT * 128, rows = x.n * a.G;
+    const int nt = NT == 2 && row0 + 128 < rows ? 2 : 1;                          // row tiles with rows in them
+    const int last_row = min(row0 + NT * 128, rows) - 1;
+    const int first_q = row0 / a.G, last_q = last_row / a.G;
+    const int lo_all = a.window > 0 ? max(0, x.seq - x.n + first_q - a.window + 1) : 0;
+    const int hi_all = a.causal ? x.seq - x.n + last_q + 1 : x.seq;               // keys [lo_all, hi_all) for some row
+    const int tile0 = lo_all / KT, n = hi_all > lo_all ? (hi_all + KT - 1) / KT - tile0 : 0;
+
+    if (warp == 13) {
+        ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+        ptx::tmem_relinquish();
+    }
+    if (tid == 0) {
+        const int counts[BARS] = {1, 1, 4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, 128, 128, 1, 1, 1};
+        for (int i = 0; i < BARS; i++) ptx::mbar_init(BAR(i), counts[i]);
+        ptx::mbar_fence_init();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+
+    if (warp < 8 && warp / 4 < nt) {
+        // ---- a row tile's warps: thread = row -----------------------------------------------------------------------------------------
+        const int t = warp >> 2, row = row0 + t * 128 + (tid & 127);
+        const int query = min(row, rows - 1) / a.G, head = h * a.G + min(row, rows - 1) % a.G;
+        const int at = x.seq - x.n + query;
+        const int hi = a.causal ? min(at, x.seq - 1) : x.seq - 1, lo = a.window > 0 ? at - a.window + 1 : 0;
+        const int min_hi = __reduce_min_sync(0xffffffffu, hi), max_lo = __reduce_max_sync(0xffffffffu, lo);
+        float fac = 0.f;
+        if (n > 0) {
+            const T *src = static_cast<const T *>(a.q) + (long long)(x.q0 + query) * a.ldq + (long long)head * D;
+            float amax = 0.f;
+            if (row < rows)
+#pragma unroll 4
+                for (int c = 0; c < D / 8; c++) {
+                    float v[8];
+                    load8(src + 8 * c, v);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
+                }
+            float f = attn::row_factor(amax);
+            fac = fabsf(a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f;
+            if (a.scale < 0.f) f = -f;
+            const int lr = tid & 127;
+            const uint32_t dst = base + t * TERMS * S::QT + lr * 128;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; c++) {
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (row < rows) load8(src + 8 * c, v);
+                uint32_t hi2[4], lo2[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = v[2 * e] * f, q = v[2 * e + 1] * f;
+                    const __half2 u = __floats2half2_rn(p, q);
+                    hi2[e] = h2_bits(u);
+                    const float2 b = __half22float2(u);
+                    lo2[e] = h2_bits(__floats2half2_rn(p - b.x, q - b.y));
+                }
+                const uint32_t to = dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (lr & 7)) << 4);
+                sts128(to, hi2[0], hi2[1], hi2[2], hi2[3]);
+                if (SPLIT) sts128(to + S::QT, lo2[0], lo2[1], lo2[2], lo2[3]);
+            }
+            ptx::fence_proxy_async_smem();
+            asm volatile("bar.arrive %0, 160;" ::"r"(1 + t) : "memory");       // the product warp waits for the tile's Q
+        }
+        const float inf = __int_as_float(0x7f800000);
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+        const uint32_t o_at = lanes + S::O_COL + t * D;
+        float B = -inf, l = 0.f;
+        for (int j = 0; j < n; j++) {
+            const int buf = NT == 2 ? t : j & 1;
+            const uint32_t s_at = lanes + buf * S::S_COLS;
+            if (ok && !ptx::mbar_wait_warp(BAR(S_FULL + buf), (NT == 2 ? j : j >> 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 1u); ok = false; }
+            ptx::tc_fence_after_sync();
+            const int key0 = (tile0 + j) * KT;
+            const bool edge = key0 + KT - 1 > min_hi || key0 < max_lo;
+            const uint32_t sc = scales + (j & (SCALE_SLOTS - 1)) * 128;
+            float top = -inf;
+#pragma unroll 1
+            for (int c = 0; c < KT / 32; c++) {
+                uint32_t v[32];
+                ptx::tmem_ld(s_at + 32 * c, v);
+                ptx::tmem_ld_wait();
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const int key = key0 + 32 * c + e;
+                        if (key > hi || key < lo) v[e] = 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float4 k4 = lds_f4(sc + (2 * c + u) * 16);          // ks, log2 vs, 1 / vs, vs == 0
+                    float m = __uint_as_float(v[16 * u]);
+#pragma unroll
+                    for (int e = 1; e < 16; e++) m = fmaxf(m, __uint_as_float(v[16 * u + e]));
+                    const float f = fac * k4.x;
+                    top = fmaxf(top, a.softcap > 0.f ? (m == -inf ? -inf : capped(m * f, a.softcap) + k4.y) : fmaf(m, f, k4.y));
+                }
+            }
+            const auto products_before = [&]() {                     // one S buffer ahead: O is whole when PV of tile j - 1 is done
+                if (ok && !ptx::mbar_wait_warp(BAR(PV_DONE), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 2u); ok = false; }
+                ptx::tc_fence_after_sync();
+            };
+            bool waited = NT == 2 || j == 0;                         // two row tiles: S_t of this tile came after PV_t of the one before
+            const bool again = top > B + 15.f;
+            if (__any_sync(0xffffffffu, again)) {
+                const float Bn = again ? top - 8.f : B;
+                const float shrink = B == -inf ? (Bn == -inf ? 1.f : 0.f) : ex2(B - Bn);
+                B = Bn;
+                l *= shrink;
+                if (j > 0) {
+                    if (!waited) { products_before(); waited = true; }
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[32];
+                        ptx::tmem_ld(o_at + 32 * c, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                        tmem_st32(o_at + 32 * c, o);
+                    }
+                }
+            }
+            const float Bu = B == -inf ? 0.f : B;
+#pragma unroll 1
+            for (int c = 0; c < KT / 32; c++) {
+                uint32_t v[32], ph[16], pl[16];
+                ptx::tmem_ld(s_at + 32 * c, v);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float4 k4 = lds_f4(sc + (2 * c + u) * 16);
+                    const float f = fac * k4.x, add = k4.y - Bu;
+                    float p[16], sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float s = __uint_as_float(v[16 * u + e]);
+                        p[e] = ex2(a.softcap > 0.f ? capped(s * f, a.softcap) + add : fmaf(s, f, add));
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int key = key0 + 32 * c + 16 * u + e;
+                            if (key > hi || key < lo) p[e] = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sum += p[e];
+                    l = fmaf(sum, k4.z, l);
+                    if (k4.w != 0.f)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) p[e] = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const __half2 b = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
+                        ph[8 * u + e] = h2_bits(b);
+                        if (SPLIT) {
+                            const float2 back = __half22float2(b);
+                            pl[8 * u + e] = h2_bits(__floats2half2_rn(p[2 * e] - back.x, p[2 * e + 1] - back.y));
+                        }
+                    }
+                }
+                tmem_st16(s_at + 32 * c, ph);
+                if (SPLIT) tmem_st16(s_at + 32 * c + 16, pl);
+            }
+            if (!waited) products_before();                          // every phase is awaited, so none is mistaken for another
+            tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            ptx::mbar_arrive(BAR(P_FULL + buf));
+        }
+        // ---- the rows out ------------------------------------------------------------------------------------------------------------
+        if (n > 0) {
+            if (ok && !ptx::mbar_wait_warp(BAR(O_FULL + t), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 3u); ok = false; }
+            ptx::tc_fence_after_sync();
+        }
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        T *dst = static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; c++) {
+            uint32_t o[32];
+            if (n > 0) {
+                ptx::tmem_ld(o_at + 32 * c, o);
+                ptx::tmem_ld_wait();
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = 0u;
+            }
+            if (row < rows)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    attn::store4(dst + 32 * c + 4 * e, make_float4(l == 0.f ? 0.f : __uint_as_float(o[4 * e]) * inv, l == 0.f ? 0.f : __uint_as_float(o[4 * e + 1]) * inv,
+                                                                  l == 0.f ? 0.f : __uint_as_float(o[4 * e + 2]) * inv, l == 0.f ? 0.f : __uint_as_float(o[4 * e + 3]) * inv));
+        }
+        if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (B + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
+        ptx::tc_fence_before_sync();
+    } else if (warp >= 8 && warp < 12) {
+        // ---- codes to fp16 -------------------------------------------------------------------------------------------------------------
+        const int ct = tid - 256;
+        for (int j = 0; j < n; j++) {
+            const int st = j % ST;
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                const int full = kv ? V_FULL : K_FULL, empty = kv ? V_EMPTY : K_EMPTY;
+                if (ok && !ptx::mbar_wait_warp(BAR(RAW_FULL + kv), j & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 4u); ok = false; }
+                if (ok && j >= ST && !ptx::mbar_wait_warp(BAR(empty + st), (j / ST - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 5u); ok = false; }
+                const uint32_t src = base + S::OFF_RAW + kv * S::RAW, dst = base + S::OFF_KV + (2 * st + kv) * S::KV;
+                constexpr int CH = D / 16;                        // 16-byte pieces of a token's codes
+                if (ok)
+#pragma unroll 4
+                    for (int e = ct; e < KT * CH; e += 128) {
+                        const int key = e / CH, c = e % CH, par = D == 64 ? 0 : (c >> 2) & 1;
+                        const uint4 w = attn::lds128(src + 16 * e);
+                        uint32_t f[4], g[4];
+                        // half of the lanes write their second eight elements first: no bank twice
+                        widen(par ? w.z : w.x, f[0], f[1]);
+                        widen(par ? w.w : w.y, f[2], f[3]);
+                        widen(par ? w.x : w.z, g[0], g[1]);
+                        widen(par ? w.y : w.w, g[2], g[3]);
+                        const uint32_t to = dst + (c >> 2) * KT * 128 + key * 128;
+                        const int pos = 2 * (c & 3) + par;
+                        sts128(to + ((pos ^ (key & 7)) << 4), f[0], f[1], f[2], f[3]);
+                        sts128(to + (((pos ^ 1) ^ (key & 7)) << 4), g[0], g[1], g[2], g[3]);
+                    }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (ok && lane == 0) {
+                    ptx::mbar_arrive(BAR(RAW_EMPTY + kv));
+                    ptx::mbar_arrive(BAR(full + st));
+                }
+            }
+        }
+    } else if (warp == 12) {
+        // ---- copies: lane = one piece of a tile (a block, or the part of it in the tile) --------------------------------------------------
+        const int piece = min(a.block, KT), pieces = KT / piece, per = piece / 16, bshift = 31 - __clz(a.block);
+        const auto entry = [&](int j) {                             // block id of this lane's piece of tile j; -1: no token that is seen
+            const int first = (tile0 + j) * KT + lane * piece;
+            if (lane >= pieces || j >= n || first >= hi_all || first + piece <= lo_all) return -1;
+            int id = a.table[(size_t)r * a.width + (first >> bshift)];
+            if (id < 0 || id >= a.num_blocks) { dev_set_error(kv::ERR_BLOCK_ID); id = 0; }
+            return id;
+        };
+        int id = entry(0);
+        float ks = 0.f, vs = 1.f;
+        if (id >= 0) { ks = a.ks[(size_t)id * a.Hkv + h]; vs = a.vs[(size_t)id * a.Hkv + h]; }
+        for (int j = 0; j < n && ok; j++) {
+            const int next = entry(j + 1);
+            const unsigned count = __popc(__ballot_sync(0xffffffffu, id >= 0));
+            const int first = (tile0 + j) * KT + lane * piece;
+            const size_t off = id >= 0 ? (((size_t)id * a.Hkv + h) * a.block + (first & (a.block - 1))) * D : 0;
+            if (j > 0 && !ptx::mbar_wait_warp(BAR(RAW_EMPTY), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 6u); ok = false; break; }
+            // the slot's last reader was tile j - 4's rows, done before this K can be awaited (two stages and one tile of codes ahead)
+            if (lane < pieces) {
+                const float none = vs == 0.f ? 1.f : 0.f, v1 = vs == 0.f ? 1.f : vs;
+                for (int u = 0; u < per; u++) {
+                    const uint32_t to = scales + (j & (SCALE_SLOTS - 1)) * 128 + (lane * per + u) * 16;
+                    sts128(to, __float_as_uint(ks), __float_as_uint(lg2(v1)), __float_as_uint(1.f / v1), __float_as_uint(none));
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_expect_tx(BAR(RAW_FULL), count * (unsigned)(piece * D));
+            if (id >= 0) bulk_load(base + S::OFF_RAW + lane * piece * D, kc + off, piece * D, BAR(RAW_FULL));
+            if (j > 0 && !ptx::mbar_wait_warp(BAR(RAW_EMPTY + 1), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 7u); ok = false; break; }
+            if (lane == 0) ptx::mbar_arrive_expect_tx(BAR(RAW_FULL + 1), count * (unsigned)(piece * D));
+            __syncwarp();
+            if (id >= 0) bulk_load(base + S::OFF_RAW + S::RAW + lane * piece * D, vc + off, piece * D, BAR(RAW_FULL + 1));
+            id = next;
+            ks = 0.f; vs = 1.f;
+            if (id >= 0) { ks = a.ks[(size_t)id * a.Hkv + h]; vs = a.vs[(size_t)id * a.Hkv + h]; }
+        }
+        if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
+    } else if (warp == 13 && n > 0) {
+        // ---- products ------------------------------------------------------------------------------------------------------------------
+        for (int t = 0; t < nt; t++) asm volatile("bar.sync %0, 160;" ::"r"(1 + t) : "memory");
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(KT, 0), id_o = idesc_f16(D, 1);
+            const auto wait = [&](int bar, int parity, unsigned code) {
+                if (ok && !ptx::mbar_wait(BAR(bar), parity & 1)) { dev_set_error(ERR_WAIT | code); ok = false; }
+                ptx::tc_fence_after_sync();
+                return ok;
+            };
+            const auto scores = [&](int t, int j, int buf) {
+                const uint32_t kb = base + S::OFF_KV + 2 * (j % ST) * S::KV;
+                uint32_t first = 0;
+#pragma unroll
+                for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint64_t qd = ptx::umma_desc_k_sw128(base + (t * TERMS + term) * S::QT + (k >> 2) * 128 * 128) + (uint64_t)((k & 3) * 2);
+                        const uint64_t kd = ptx::umma_desc_k_sw128(kb + (k >> 2) * KT * 128) + (uint64_t)((k & 3) * 2);
+                        umma_f16_ss(tmem + buf * S::S_COLS, qd, kd, id_s, first);
+                        first = 1;
+                    }
+                ptx::umma_commit(BAR(S_FULL + buf));
+            };
+            const auto values = [&](int t, int j, int buf) {
+                const uint32_t vb = base + S::OFF_KV + (2 * (j % ST) + 1) * S::KV;
+#pragma unroll
+                for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                    for (int k = 0; k < KT / 16; k++)
+                        umma_f16_ts(tmem + S::O_COL + t * D, tmem + buf * S::S_COLS + (k >> 1) * 32 + (k & 1) * 8 + term * 16,
+                                    desc_mn_sw128(vb + k * 16 * 128, KT * 128), id_o, j > 0 || term > 0 || k > 0);
+            };
+            wait(K_FULL, 0, 8u);
+            if (ok) {
+                for (int t = 0; t < nt; t++) scores(t, 0, t);
+                ptx::umma_commit(BAR(K_EMPTY));
+            }
+            for (int j = 0; j < n && ok; j++) {
+                const int st = j % ST, s1 = (j + 1) % ST;
+                if (NT == 1 && j + 1 < n) {
+                    if (!wait(K_FULL + s1, (j + 1) / ST, 9u)) break;
+                    scores(0, j + 1, (j + 1) & 1);
+                    ptx::umma_commit(BAR(K_EMPTY + s1));
+                }
+                for (int t = 0; t < nt; t++) {
+                    const int buf = NT == 2 ? t : j & 1;
+                    if (t == 0 && !wait(V_FULL + st, j / ST, 10u)) break;
+                    if (!wait(P_FULL + buf, NT == 2 ? j : j >> 1, 11u)) break;
+                    values(t, j, buf);
+                    if (t == nt - 1) ptx::umma_commit(BAR(V_EMPTY + st));
+                    if (NT == 1) ptx::umma_commit(BAR(PV_DONE));
+                    if (j == n - 1) ptx::umma_commit(BAR(O_FULL + t));
+                    if (NT == 2 && j + 1 < n) {
+                        if (t == 0 && !wait(K_FULL + s1, (j + 1) / ST, 12u)) break;
+                        scores(t, j + 1, t);
+                        if (t == nt - 1) ptx::umma_commit(BAR(K_EMPTY + s1));
+                    }
+                }
+            }
+            if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    if (warp == 13) ptx::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+inline int launch_t(const attn::Call &c, cudaStream_t st) {
+    using S = Shape<T, D>;
+    auto kern = attention_q8_tc_kernel<T, D>;
+    static PerDevice<bool> configured;
+    if (!configured.get()) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e != cudaSuccess) return cuda_fail(e, "attention_q8_tc smem opt-in");
+        configured.get() = true;
+    }
+    // no more items than full tiles of all rows and a partial one for each request
+    const long long rows = (long long)c.a.T * c.a.G, items = (rows / (S::NT * 128) + (c.a.R < c.a.T ? c.a.R : c.a.T)) * c.a.Hkv;
+    if (items > 0x7fffffffll) return fail(W4A8_ERR_UNSUPPORTED, "attention_q8: %lld row tiles", items);
+    cudaError_t e = launch_pdl(kern, dim3((unsigned)items), dim3(THREADS), S::SMEM, st, c.a, c.k, c.v);
+    return e == cudaSuccess ? launch_status("attention_q8_tc") : cuda_fail(e, "attention_q8_tc launch");
+}
+
+inline int launch(const attn::Call &c, cudaStream_t st) {
+    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) { return launch_t<decltype(t), decltype(d)::value>(c, st); });
+}
+
+}  // namespace attn_tc
+}  // namespace w4a8

@@ -4,6 +4,7 @@
 #include "common.cuh"
 #include "kv_cache.cuh"
 #include "attention_q8.cuh"
+#include "attention_q8_tc.cuh"
 
 namespace w4a8 {
 
@@ -136,7 +137,18 @@ W4A8_API int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *
     a.part_ml = reinterpret_cast<float2 *>(ws + attn::count_bytes());
     a.part = reinterpret_cast<float *>(ws + attn::count_bytes() + slots * attn::MAX_ROWS * 8);
     c.k = cache->k; c.v = cache->v; c.dtype = dtype; c.dim = cache->dim;
-    const int mq = max_q > 0 && max_q < T ? max_q : T;
-    const int64_t rows = (int64_t)mq * a.G;
-    return attn::launch(c, rows < 0x7fffffff ? (int)rows : 0x7fffffff, (cudaStream_t)stream);
+    const int64_t rows = (int64_t)(max_q > 0 && max_q < T ? max_q : T) * a.G;
+    if (rows > attn::FEW_ROWS) {
+        // requests with many rows on the tensor cores' tiles of rows; the others, if there can be any, by the streaming kernel
+        a.few = R == 1 ? 0 : attn::FEW_ROWS;
+        for (int r0 = 0; r0 < R; r0 += attn_tc::MAX_R) {
+            attn::Call part = c;
+            part.a.R = R - r0 < attn_tc::MAX_R ? R - r0 : attn_tc::MAX_R;
+            part.a.cu_q += r0; part.a.seq_len += r0; part.a.table += (size_t)r0 * table_width;
+            if ((rc = attn_tc::launch(part, (cudaStream_t)stream)) != W4A8_OK) return rc;
+        }
+        if (R == 1) return W4A8_OK;
+        return attn::launch(c, attn::FEW_ROWS, (cudaStream_t)stream);
+    }
+    return attn::launch(c, (int)rows, (cudaStream_t)stream);
 }
