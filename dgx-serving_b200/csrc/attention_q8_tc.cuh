@@ -41,14 +41,24 @@ template <typename T, int D> struct Shape {
 
 enum { RAW_FULL = 0, RAW_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY = 10, S_FULL = 12, P_FULL = 14, PV_DONE = 16, O_FULL = 17, BARS = 19 };
 
-// D[tmem] (+)= A[tmem] B[smem]; A: 128 lanes, two fp16 a column.  B: N x 16 as the descriptor says.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// D[tmem] (+)= A[tmem] B[smem]; A: 128 lanes, two fp16 a column.  B: N x 16 as the descriptor says.  The whole warp comes here and the elected
+// lane issues: addresses and descriptors then stay in uniform registers (inside a branch of one lane an instruction took 120 cycles to issue).
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 // fp32 accumulators (bits [4,6) = 1), fp16 A and B; bit 16: B is MN-major; N >> 3 in [17,23), M >> 4 in [24,29).
 __host__ __device__ constexpr uint32_t idesc_f16(int N, int b_mn) { return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
@@ -56,10 +66,9 @@ __host__ __device__ constexpr uint32_t idesc_f16(int N, int b_mn) { return (1u <
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t mn_stride) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(mn_stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
@@ -86,12 +95,6 @@ __device__ __forceinline__ float capped(float x, float cap) {
     return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E))));
 }
 
-// 8 elements of a row of Q as floats.
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
-    const float4 a = attn::load4(p), b = attn::load4(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-
 // Four bytes of codes as two packed pairs of fp16.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &a, uint32_t &b) {
     w ^= 0x80808080u;
@@ -99,15 +102,232 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t &a, uint32_t &b) {
     b = attn::codes_f16<0x4342>(w);
 }
 
+__device__ __forceinline__ uint64_t pack2u(uint32_t a, uint32_t b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint64_t pack2(float a, float b) { return pack2u(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void unpack2(uint64_t x, float &a, float &b) {
+    uint32_t u, v;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(u), "=r"(v) : "l"(x));
+    a = __uint_as_float(u); b = __uint_as_float(v);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// Both passes over a tile's scores are loops over 32 columns whose code stays in the instruction cache nearest to the scheduler: written out
+// over 128 columns a warp waited for instructions a tenth of the time.  The next 16 columns are on their way while 16 are worked on.
+struct RowMask { int key0, hi, lo; };
+template <int N> __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[N]) {   // the loads before this are complete; r is not read earlier
+#pragma unroll
+    for (int e = 0; e < N; e += 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[e]), "+r"(r[e + 1]), "+r"(r[e + 2]), "+r"(r[e + 3]), "+r"(r[e + 4]), "+r"(r[e + 5]), "+r"(r[e + 6]),
+                     "+r"(r[e + 7]), "+r"(r[e + 8]), "+r"(r[e + 9]), "+r"(r[e + 10]), "+r"(r[e + 11]), "+r"(r[e + 12]), "+r"(r[e + 13]), "+r"(r[e + 14]),
+                     "+r"(r[e + 15]) :: "memory");
+}
+// The columns of a tile in steps of N, the next step's on their way while one is worked on: step(registers, first column).
+template <int KT, int N, class Step>
+__device__ __forceinline__ void columns(uint32_t at, Step &&step) {
+    static_assert(KT % (2 * N) == 0, "two steps a trip");
+    uint32_t v[2][N];
+    ptx::tmem_ld(at, v[0]);
+#pragma unroll 1
+    for (int c = 0; c < KT; c += 2 * N) {
+        tmem_arrived(v[0]);
+        ptx::tmem_ld(at + c + N, v[1]);
+        step(v[0], c);
+        tmem_arrived(v[1]);
+        if (c + 2 * N < KT) ptx::tmem_ld(at + c + 2 * N, v[0]);
+        step(v[1], c + N);
+    }
+}
+// log2 of the row's largest weight
+template <int KT, int N, bool EDGE>
+__device__ __forceinline__ float top_of(uint32_t s_at, uint32_t sc, float fac, float cap, const RowMask &k) {
+    const float inf = __int_as_float(0x7f800000);
+    float top = -inf;
+    columns<KT, N>(s_at, [&](uint32_t (&r)[N], int c) {
+        float4 k4[N / 16];                                                   // ks, log2 vs, 1 / vs, vs == 0
+#pragma unroll
+        for (int u = 0; u < N / 16; u++) k4[u] = lds_f4(sc + c + 16 * u);
+        if (EDGE) {
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (k.key0 + c + e > k.hi || k.key0 + c + e < k.lo) r[e] = 0xff800000u;
+        }
+#pragma unroll
+        for (int u = 0; u < N / 16; u++) {
+            float m[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                m[e] = fmaxf(fmaxf(__uint_as_float(r[16 * u + e]), __uint_as_float(r[16 * u + 4 + e])), fmaxf(__uint_as_float(r[16 * u + 8 + e]), __uint_as_float(r[16 * u + 12 + e])));
+            const float mm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), f = fac * k4[u].x;
+            top = fmaxf(top, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap) + k4[u].y) : fmaf(mm, f, k4[u].y));
+        }
+    });
+    return top;
+}
+// The weights in place of the scores: 16 columns of scores become 8 of fp16 pairs (fp32 rows: and 8 of what they round off).  l += their sum.
+template <int KT, int N, bool SPLIT, bool EDGE, bool CAP>
+__device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, float cap, float B, const RowMask &k, float &l) {
+    columns<KT, N>(s_at, [&](const uint32_t (&r)[N], int c) {
+        float4 k4[N / 16];
+        float p[N];
+#pragma unroll
+        for (int u = 0; u < N / 16; u++) k4[u] = lds_f4(sc + c + 16 * u);
+#pragma unroll
+        for (int u = 0; u < N / 16; u++) {
+            const float f = fac * k4[u].x, add = k4[u].y - B;
+            if (CAP) {
+#pragma unroll
+                for (int e = 16 * u; e < 16 * u + 16; e++) p[e] = ex2(capped(__uint_as_float(r[e]) * f, cap) + add);
+            } else {
+                const uint64_t f2 = pack2(f, f), a2 = pack2(add, add);
+#pragma unroll
+                for (int e = 16 * u; e < 16 * u + 16; e += 2) {
+                    unpack2(fma2(pack2u(r[e], r[e + 1]), f2, a2), p[e], p[e + 1]);
+                    p[e] = ex2(p[e]);
+                    p[e + 1] = ex2(p[e + 1]);
+                }
+            }
+        }
+        if (EDGE) {
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (k.key0 + c + e > k.hi || k.key0 + c + e < k.lo) p[e] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < N / 16; u++) {
+            const float *q = p + 16 * u;
+            uint64_t sum[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = add2f(pack2(q[4 * e], q[4 * e + 1]), pack2(q[4 * e + 2], q[4 * e + 3]));
+            float s0, s1;
+            unpack2(add2f(add2f(sum[0], sum[1]), add2f(sum[2], sum[3])), s0, s1);
+            l = fmaf(s0 + s1, k4[u].z, l);
+            uint32_t ph[8], pl[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const __half2 b = __floats2half2_rn(q[2 * e], q[2 * e + 1]);
+                ph[e] = h2_bits(b);
+                if (SPLIT) {
+                    const float2 back = __half22float2(b);
+                    pl[e] = h2_bits(__floats2half2_rn(q[2 * e] - back.x, q[2 * e + 1] - back.y));
+                }
+            }
+            if (k4[u].w != 0.f)
+#pragma unroll
+                for (int e = 0; e < 8; e++) ph[e] = pl[e] = 0u;
+            tmem_st8(s_at + c + 16 * u, ph);
+            if (SPLIT) tmem_st8(s_at + c + 16 * u + 8, pl);
+        }
+    });
+}
+// 32 rows of Q by one warp: whole rows at a time, a row's largest magnitude by shuffles, its scaled fp16 terms into the operand's layout (row 0 of
+// the 32 at `dst`; the second term `term` bytes on).  fac[row]: what brings a score back, without a.scale.  Rows from `there` on are zeros.
+template <typename T, int D, bool SPLIT, class RowAt>
+__device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac, bool minus, int there, int lane, RowAt &&row_at) {
+    constexpr int N = kv::Row<T>::N, LPR = D / N, PER = LPR > 32 ? LPR / 32 : 1, RPW = LPR >= 32 ? 1 : 32 / LPR, BATCH = 32 / RPW < 8 ? 32 / RPW : 8 / PER;
+    const int sub = LPR >= 32 ? 0 : lane / LPR, col = lane & (LPR >= 32 ? 31 : LPR - 1);
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += RPW * BATCH) {
+        uint4 raw[BATCH][PER];
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const int r = r0 + b * RPW + sub;
+#pragma unroll
+            for (int q = 0; q < PER; q++)
+                raw[b][q] = r < there ? *reinterpret_cast<const uint4 *>(row_at(r) + (col + 32 * q) * N) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const int r = r0 + b * RPW + sub;
+            float x[PER][N], amax = 0.f;
+#pragma unroll
+            for (int q = 0; q < PER; q++) {
+                kv::Row<T>::unpack(raw[b][q], x[q]);
+#pragma unroll
+                for (int e = 0; e < N; e++) amax = fmaxf(amax, fabsf(x[q][e]));
+            }
+#pragma unroll
+            for (int o = (LPR >= 32 ? 32 : LPR) / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            float f = attn::row_factor(amax);
+            if (col == 0) fac[r] = 1.f / f;
+            if (minus) f = -f;
+#pragma unroll
+            for (int q = 0; q < PER; q++) {
+                const int at = (col + 32 * q) * N, chunk = at >> 3;            // of 8 elements
+                const uint32_t to = dst + r * 128 + (chunk >> 3) * (128 * 128) + (((chunk & 7) ^ (r & 7)) << 4) + (at & 7) * 2;
+                uint32_t h[N / 2], lo[N / 2];
+#pragma unroll
+                for (int e = 0; e < N / 2; e++) {
+                    const float u = x[q][2 * e] * f, v = x[q][2 * e + 1] * f;
+                    const __half2 t = __floats2half2_rn(u, v);
+                    const float2 back = __half22float2(t);
+                    h[e] = h2_bits(t);
+                    lo[e] = h2_bits(__floats2half2_rn(u - back.x, v - back.y));
+                }
+                if constexpr (N == 8) sts128(to, h[0], h[1], h[2], h[3]);
+                else {
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(h[0]), "r"(h[1]) : "memory");
+                    if (SPLIT) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + term), "r"(lo[0]), "r"(lo[1]) : "memory");
+                }
+            }
+        }
+    }
+}
+
+// The block is launched with 128 registers a thread; the rows' two warpgroups take 200, the others keep 56: 2 * 128 * (200 + 56) = 512 * 128.
+template <int N> __device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Bounded waits without a call: a kernel that moves registers between its warps cannot have one.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    long long since = 0;
+#pragma unroll 1
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (ptx::mbar_try_wait(bar, parity)) return true;
+        const long long now = clock64();
+        if (since == 0) since = now;
+        else if (now - since > (1ll << 28)) return false;
+    }
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
+    const bool ok = wait_one(bar, parity);
+    return __all_sync(0xffffffffu, ok);
+}
+
+// N columns of a row out.
+template <int N, typename T> __device__ __forceinline__ void put(T *dst, const float (&y)[N], float inv) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
+        attn::store4(dst + e, inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv));
+}
+// O = O * by + 128 columns of tensor memory.
+__device__ __forceinline__ void add_columns(float (&O)[128], uint32_t at, float by) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        uint32_t o[32];
+        ptx::tmem_ld(at + 32 * c, o);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e++) O[32 * c + e] = fmaf(O[32 * c + e], by, __uint_as_float(o[e]));
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn::Args a, const int8_t *__restrict__ kc, const int8_t *__restrict__ vc) {
     using S = Shape<T, D>;
     constexpr int KT = S::KT, NT = S::NT, ST = S::ST, TERMS = S::TERMS;
     constexpr bool SPLIT = S::SPLIT;
+    constexpr int STEP = SPLIT ? 16 : 32;          // columns of scores in work; fp32 rows' registers hold O
+    constexpr int OWN = D < 128 ? D : 128;         // columns of O that a thread sums itself (fp32 rows)
     extern __shared__ unsigned char smem_raw[];
     __shared__ unsigned wsum[THREADS / 32];
     __shared__ int item[4];                       // request, kv head, row tile
     __shared__ uint32_t tmem_slot;
+    __shared__ float shrinks[2][128];              // the rows' factors; dim 256, fp32 rows: what O is rescaled by, two tiles' worth
+    float *const facs = NT == 1 ? shrinks[1] : shrinks[0];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = ptx::smem_u32(smem), bars = base + S::OFF_BAR, scales = base + S::OFF_SCALE;
     const auto BAR = [&](int i) { return bars + 8u * i; };
@@ -162,7 +382,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         ptx::tmem_relinquish();
     }
     if (tid == 0) {
-        const int counts[BARS] = {1, 1, 4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, 128, 128, 1, 1, 1};
+        constexpr int P_COUNT = SPLIT && NT == 1 ? 256 : 128;
+        const int counts[BARS] = {1, 1, 4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, P_COUNT, P_COUNT, 1, 1, 1};
         for (int i = 0; i < BARS; i++) ptx::mbar_init(BAR(i), counts[i]);
         ptx::mbar_fence_init();
     }
@@ -174,6 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
 
     if (warp < 8 && warp / 4 < nt) {
         // ---- a row tile's warps: thread = row -----------------------------------------------------------------------------------------
+        raise_registers<200>();
         const int t = warp >> 2, row = row0 + t * 128 + (tid & 127);
         const int query = min(row, rows - 1) / a.G, head = h * a.G + min(row, rows - 1) % a.G;
         const int at = x.seq - x.n + query;
@@ -181,88 +403,63 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         const int min_hi = __reduce_min_sync(0xffffffffu, hi), max_lo = __reduce_max_sync(0xffffffffu, lo);
         float fac = 0.f;
         if (n > 0) {
-            const T *src = static_cast<const T *>(a.q) + (long long)(x.q0 + query) * a.ldq + (long long)head * D;
-            float amax = 0.f;
-            if (row < rows)
-#pragma unroll 4
-                for (int c = 0; c < D / 8; c++) {
-                    float v[8];
-                    load8(src + 8 * c, v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
-                }
-            float f = attn::row_factor(amax);
-            fac = fabsf(a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f;
-            if (a.scale < 0.f) f = -f;
-            const int lr = tid & 127;
-            const uint32_t dst = base + t * TERMS * S::QT + lr * 128;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; c++) {
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (row < rows) load8(src + 8 * c, v);
-                uint32_t hi2[4], lo2[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float p = v[2 * e] * f, q = v[2 * e + 1] * f;
-                    const __half2 u = __floats2half2_rn(p, q);
-                    hi2[e] = h2_bits(u);
-                    const float2 b = __half22float2(u);
-                    lo2[e] = h2_bits(__floats2half2_rn(p - b.x, q - b.y));
-                }
-                const uint32_t to = dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (lr & 7)) << 4);
-                sts128(to, hi2[0], hi2[1], hi2[2], hi2[3]);
-                if (SPLIT) sts128(to + S::QT, lo2[0], lo2[1], lo2[2], lo2[3]);
-            }
+            const int first = row0 + (tid & ~31);                            // of this warp's rows
+            rows_in<T, D, SPLIT>(base + t * TERMS * S::QT + (tid & 96) * 128, S::QT, facs + (tid & ~31), a.scale < 0.f, rows - first, lane, [&](int i) {
+                const int q = (first + i) / a.G;
+                return static_cast<const T *>(a.q) + (long long)(x.q0 + q) * a.ldq + (long long)(h * a.G + first + i - q * a.G) * D;
+            });
+            __syncwarp();
+            fac = fabsf(a.scale) * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) * facs[tid];
             ptx::fence_proxy_async_smem();
             asm volatile("bar.arrive %0, 160;" ::"r"(1 + t) : "memory");       // the product warp waits for the tile's Q
         }
         const float inf = __int_as_float(0x7f800000);
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
         const uint32_t o_at = lanes + S::O_COL + t * D;
-        float B = -inf, l = 0.f;
+        // fp32 rows: the tensor core's sums lose up to a unit in the last place with every sixteen keys (toward zero), so O in tensor memory
+        // is one tile's and the rows' sums over the tiles are held here, in registers
+        float O[SPLIT ? OWN : 1];
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int e = 0; e < OWN; e++) O[e] = 0.f;
+        }
+        float B = -inf, l = 0.f, shrink = 1.f;
+        const auto take = [&](float by) {                            // O of the tile before, complete in tensor memory, into the registers
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int c = 0; c < OWN / 32; c++) {
+                    uint32_t o[32];
+                    ptx::tmem_ld(o_at + 32 * c, o);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; e++) O[32 * c + e] = fmaf(O[32 * c + e], by, __uint_as_float(o[e]));
+                }
+            }
+        };
         for (int j = 0; j < n; j++) {
             const int buf = NT == 2 ? t : j & 1;
             const uint32_t s_at = lanes + buf * S::S_COLS;
-            if (ok && !ptx::mbar_wait_warp(BAR(S_FULL + buf), (NT == 2 ? j : j >> 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 1u); ok = false; }
+            if (ok && !wait_warp(BAR(S_FULL + buf), (NT == 2 ? j : j >> 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 1u); ok = false; }
             ptx::tc_fence_after_sync();
             const int key0 = (tile0 + j) * KT;
             const bool edge = key0 + KT - 1 > min_hi || key0 < max_lo;
             const uint32_t sc = scales + (j & (SCALE_SLOTS - 1)) * 128;
-            float top = -inf;
-#pragma unroll 1
-            for (int c = 0; c < KT / 32; c++) {
-                uint32_t v[32];
-                ptx::tmem_ld(s_at + 32 * c, v);
-                ptx::tmem_ld_wait();
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int key = key0 + 32 * c + e;
-                        if (key > hi || key < lo) v[e] = 0xff800000u;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float4 k4 = lds_f4(sc + (2 * c + u) * 16);          // ks, log2 vs, 1 / vs, vs == 0
-                    float m = __uint_as_float(v[16 * u]);
-#pragma unroll
-                    for (int e = 1; e < 16; e++) m = fmaxf(m, __uint_as_float(v[16 * u + e]));
-                    const float f = fac * k4.x;
-                    top = fmaxf(top, a.softcap > 0.f ? (m == -inf ? -inf : capped(m * f, a.softcap) + k4.y) : fmaf(m, f, k4.y));
-                }
-            }
             const auto products_before = [&]() {                     // one S buffer ahead: O is whole when PV of tile j - 1 is done
-                if (ok && !ptx::mbar_wait_warp(BAR(PV_DONE), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 2u); ok = false; }
+                if (ok && !wait_warp(BAR(PV_DONE), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 2u); ok = false; }
                 ptx::tc_fence_after_sync();
             };
             bool waited = NT == 2 || j == 0;                         // two row tiles: S_t of this tile came after PV_t of the one before
+            if (SPLIT && NT == 2 && j > 0) take(shrink);
+            const RowMask mask = {key0, hi, lo};
+            const float top = edge ? top_of<KT, STEP, true>(s_at, sc, fac, a.softcap, mask) : top_of<KT, STEP, false>(s_at, sc, fac, a.softcap, mask);
             const bool again = top > B + 15.f;
+            shrink = 1.f;
             if (__any_sync(0xffffffffu, again)) {
                 const float Bn = again ? top - 8.f : B;
-                const float shrink = B == -inf ? (Bn == -inf ? 1.f : 0.f) : ex2(B - Bn);
+                shrink = B == -inf ? (Bn == -inf ? 1.f : 0.f) : ex2(B - Bn);
                 B = Bn;
                 l *= shrink;
-                if (j > 0) {
+                if (!SPLIT && j > 0) {
                     if (!waited) { products_before(); waited = true; }
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
@@ -276,105 +473,109 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 }
             }
             const float Bu = B == -inf ? 0.f : B;
-#pragma unroll 1
-            for (int c = 0; c < KT / 32; c++) {
-                uint32_t v[32], ph[16], pl[16];
-                ptx::tmem_ld(s_at + 32 * c, v);
-                ptx::tmem_ld_wait();
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float4 k4 = lds_f4(sc + (2 * c + u) * 16);
-                    const float f = fac * k4.x, add = k4.y - Bu;
-                    float p[16], sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float s = __uint_as_float(v[16 * u + e]);
-                        p[e] = ex2(a.softcap > 0.f ? capped(s * f, a.softcap) + add : fmaf(s, f, add));
-                    }
-                    if (edge) {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const int key = key0 + 32 * c + 16 * u + e;
-                            if (key > hi || key < lo) p[e] = 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sum += p[e];
-                    l = fmaf(sum, k4.z, l);
-                    if (k4.w != 0.f)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) p[e] = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const __half2 b = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
-                        ph[8 * u + e] = h2_bits(b);
-                        if (SPLIT) {
-                            const float2 back = __half22float2(b);
-                            pl[8 * u + e] = h2_bits(__floats2half2_rn(p[2 * e] - back.x, p[2 * e + 1] - back.y));
-                        }
-                    }
-                }
-                tmem_st16(s_at + 32 * c, ph);
-                if (SPLIT) tmem_st16(s_at + 32 * c + 16, pl);
-            }
-            if (!waited) products_before();                          // every phase is awaited, so none is mistaken for another
+            if (a.softcap > 0.f) weights<KT, STEP, SPLIT, true, true>(s_at, sc, fac, a.softcap, Bu, mask, l);
+            else if (edge) weights<KT, STEP, SPLIT, true, false>(s_at, sc, fac, 0.f, Bu, mask, l);
+            else weights<KT, STEP, SPLIT, false, false>(s_at, sc, fac, 0.f, Bu, mask, l);
+            if (SPLIT && NT == 1) {
+                if (j > 0) { products_before(); take(shrinks[(j - 1) & 1][tid]); }
+                shrinks[j & 1][tid] = shrink;                        // for the other half's warps, who read it before PV of tile j + 1
+            } else if (!waited) products_before();                   // every phase is awaited, so none is mistaken for another
             tmem_st_wait();
             ptx::tc_fence_before_sync();
             ptx::mbar_arrive(BAR(P_FULL + buf));
         }
         // ---- the rows out ------------------------------------------------------------------------------------------------------------
         if (n > 0) {
-            if (ok && !ptx::mbar_wait_warp(BAR(O_FULL + t), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 3u); ok = false; }
+            if (ok && !wait_warp(BAR(O_FULL + t), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 3u); ok = false; }
             ptx::tc_fence_after_sync();
+            take(shrink);
         }
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        if (SPLIT && NT == 1) {
+            asm volatile("bar.sync 4, 256;" ::: "memory");           // the other half has read the last factor
+            shrinks[0][tid] = inv;
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+        }
         T *dst = static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D;
+        if constexpr (SPLIT) {
+            if (row < rows) put<OWN>(dst, O, inv);
+        } else {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; c++) {
-            uint32_t o[32];
-            if (n > 0) {
-                ptx::tmem_ld(o_at + 32 * c, o);
-                ptx::tmem_ld_wait();
-            } else {
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[32];
+                float y[32];
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = 0u;
-            }
-            if (row < rows)
+                if (n > 0) {
+                    ptx::tmem_ld(o_at + 32 * c, o);
+                    ptx::tmem_ld_wait();
+                }
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    attn::store4(dst + 32 * c + 4 * e, make_float4(l == 0.f ? 0.f : __uint_as_float(o[4 * e]) * inv, l == 0.f ? 0.f : __uint_as_float(o[4 * e + 1]) * inv,
-                                                                  l == 0.f ? 0.f : __uint_as_float(o[4 * e + 2]) * inv, l == 0.f ? 0.f : __uint_as_float(o[4 * e + 3]) * inv));
+                for (int e = 0; e < 32; e++) y[e] = __uint_as_float(o[e]);
+                if (row < rows) put<32>(dst + 32 * c, y, inv);
+            }
         }
         if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (B + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
         ptx::tc_fence_before_sync();
+    } else if (SPLIT && NT == 1 && warp >= 4 && warp < 8) {
+        // ---- dim 256, fp32 rows: the second half of O's columns ----------------------------------------------------------------------------
+        raise_registers<200>();
+        const int lr = tid & 127, row = row0 + lr, query = min(row, rows - 1) / a.G, head = h * a.G + min(row, rows - 1) % a.G;
+        const uint32_t o_at = tmem + ((uint32_t)(warp & 3) << 21) + S::O_COL + 128;
+        float O[128];
+#pragma unroll
+        for (int e = 0; e < 128; e++) O[e] = 0.f;
+        for (int j = 0; j < n; j++) {
+            if (j > 0) {                                             // the first tile's weights wait for nobody
+                if (ok && !wait_warp(BAR(PV_DONE), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 13u); ok = false; }
+                ptx::tc_fence_after_sync();
+                add_columns(O, o_at, shrinks[(j - 1) & 1][lr]);
+                ptx::tc_fence_before_sync();
+            }
+            ptx::mbar_arrive(BAR(P_FULL + (j & 1)));
+        }
+        if (n > 0) {
+            if (ok && !wait_warp(BAR(O_FULL), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 14u); ok = false; }
+            ptx::tc_fence_after_sync();
+            add_columns(O, o_at, shrinks[(n - 1) & 1][lr]);
+        }
+        asm volatile("bar.sync 4, 256;" ::: "memory");
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        if (row < rows) put<128>(static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, O, shrinks[0][lr]);
+        ptx::tc_fence_before_sync();
     } else if (warp >= 8 && warp < 12) {
         // ---- codes to fp16 -------------------------------------------------------------------------------------------------------------
-        const int ct = tid - 256;
+        lower_registers<56>();
+        const uint32_t k8 = lane >> 2, cq = lane & 3, odd4 = D == 64 ? 0 : (k8 & 1) * 4, my_key = (warp - 8) * 8 + k8;
+        const uint32_t my_src = my_key * D + 16 * cq, my_dst = my_key * 128, pos0 = ((2 * cq) ^ k8) << 4, pos1 = ((2 * cq + 1) ^ k8) << 4;
         for (int j = 0; j < n; j++) {
             const int st = j % ST;
 #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
                 const int full = kv ? V_FULL : K_FULL, empty = kv ? V_EMPTY : K_EMPTY;
-                if (ok && !ptx::mbar_wait_warp(BAR(RAW_FULL + kv), j & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 4u); ok = false; }
-                if (ok && j >= ST && !ptx::mbar_wait_warp(BAR(empty + st), (j / ST - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 5u); ok = false; }
+                if (ok && !wait_warp(BAR(RAW_FULL + kv), j & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 4u); ok = false; }
+                if (ok && j >= ST && !wait_warp(BAR(empty + st), (j / ST - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 5u); ok = false; }
                 const uint32_t src = base + S::OFF_RAW + kv * S::RAW, dst = base + S::OFF_KV + (2 * st + kv) * S::KV;
-                constexpr int CH = D / 16;                        // 16-byte pieces of a token's codes
+                // A warp takes eight tokens and four 16-byte pieces of their codes at a time; odd tokens the other four of eight, so that neither
+                // the reads nor the two writes meet a bank twice.
+                constexpr int CH = D / 16;
                 if (ok)
-#pragma unroll 4
-                    for (int e = ct; e < KT * CH; e += 128) {
-                        const int key = e / CH, c = e % CH, par = D == 64 ? 0 : (c >> 2) & 1;
-                        const uint4 w = attn::lds128(src + 16 * e);
-                        uint32_t f[4], g[4];
-                        // half of the lanes write their second eight elements first: no bank twice
-                        widen(par ? w.z : w.x, f[0], f[1]);
-                        widen(par ? w.w : w.y, f[2], f[3]);
-                        widen(par ? w.x : w.z, g[0], g[1]);
-                        widen(par ? w.y : w.w, g[2], g[3]);
-                        const uint32_t to = dst + (c >> 2) * KT * 128 + key * 128;
-                        const int pos = 2 * (c & 3) + par;
-                        sts128(to + ((pos ^ (key & 7)) << 4), f[0], f[1], f[2], f[3]);
-                        sts128(to + (((pos ^ 1) ^ (key & 7)) << 4), g[0], g[1], g[2], g[3]);
-                    }
+#pragma unroll
+                    for (int k0 = 0; k0 < KT; k0 += 32)
+#pragma unroll
+                        for (int it = 0; it < CH / 4; it++) {
+                            const int flip = D == 64 ? 0 : 4 * (it & 1), off = 8 * (it >> 1);
+                            const uint32_t c4 = odd4 ^ flip;                 // 0 or 4
+                            const uint4 w = attn::lds128(src + my_src + k0 * D + 16 * (c4 + off));
+                            uint32_t f[8];
+                            widen(w.x, f[0], f[1]);
+                            widen(w.y, f[2], f[3]);
+                            widen(w.z, f[4], f[5]);
+                            widen(w.w, f[6], f[7]);
+                            const uint32_t to = dst + my_dst + k0 * 128 + (c4 >> 2) * (KT * 128) + (off >> 2) * (KT * 128);
+                            sts128(to + pos0, f[0], f[1], f[2], f[3]);
+                            sts128(to + pos1, f[4], f[5], f[6], f[7]);
+                        }
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (ok && lane == 0) {
@@ -383,7 +584,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 }
             }
         }
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
+        lower_registers<56>();
+        if (warp == 12) {
         // ---- copies: lane = one piece of a tile (a block, or the part of it in the tile) --------------------------------------------------
         const int piece = min(a.block, KT), pieces = KT / piece, per = piece / 16, bshift = 31 - __clz(a.block);
         const auto entry = [&](int j) {                             // block id of this lane's piece of tile j; -1: no token that is seen
@@ -401,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             const unsigned count = __popc(__ballot_sync(0xffffffffu, id >= 0));
             const int first = (tile0 + j) * KT + lane * piece;
             const size_t off = id >= 0 ? (((size_t)id * a.Hkv + h) * a.block + (first & (a.block - 1))) * D : 0;
-            if (j > 0 && !ptx::mbar_wait_warp(BAR(RAW_EMPTY), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 6u); ok = false; break; }
+            if (j > 0 && !wait_warp(BAR(RAW_EMPTY), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 6u); ok = false; break; }
             // the slot's last reader was tile j - 4's rows, done before this K can be awaited (two stages and one tile of codes ahead)
             if (lane < pieces) {
                 const float none = vs == 0.f ? 1.f : 0.f, v1 = vs == 0.f ? 1.f : vs;
@@ -413,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_expect_tx(BAR(RAW_FULL), count * (unsigned)(piece * D));
             if (id >= 0) bulk_load(base + S::OFF_RAW + lane * piece * D, kc + off, piece * D, BAR(RAW_FULL));
-            if (j > 0 && !ptx::mbar_wait_warp(BAR(RAW_EMPTY + 1), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 7u); ok = false; break; }
+            if (j > 0 && !wait_warp(BAR(RAW_EMPTY + 1), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 7u); ok = false; break; }
             if (lane == 0) ptx::mbar_arrive_expect_tx(BAR(RAW_FULL + 1), count * (unsigned)(piece * D));
             __syncwarp();
             if (id >= 0) bulk_load(base + S::OFF_RAW + S::RAW + lane * piece * D, vc + off, piece * D, BAR(RAW_FULL + 1));
@@ -425,10 +628,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
     } else if (warp == 13 && n > 0) {
         // ---- products ------------------------------------------------------------------------------------------------------------------
         for (int t = 0; t < nt; t++) asm volatile("bar.sync %0, 160;" ::"r"(1 + t) : "memory");
-        if (lane == 0) {
+        const uint32_t lead = elected();
+        {
             constexpr uint32_t id_s = idesc_f16(KT, 0), id_o = idesc_f16(D, 1);
             const auto wait = [&](int bar, int parity, unsigned code) {
-                if (ok && !ptx::mbar_wait(BAR(bar), parity & 1)) { dev_set_error(ERR_WAIT | code); ok = false; }
+                if (ok && !wait_warp(BAR(bar), parity & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | code); ok = false; }
                 ptx::tc_fence_after_sync();
                 return ok;
             };
@@ -441,10 +645,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                     for (int k = 0; k < D / 16; k++) {
                         const uint64_t qd = ptx::umma_desc_k_sw128(base + (t * TERMS + term) * S::QT + (k >> 2) * 128 * 128) + (uint64_t)((k & 3) * 2);
                         const uint64_t kd = ptx::umma_desc_k_sw128(kb + (k >> 2) * KT * 128) + (uint64_t)((k & 3) * 2);
-                        umma_f16_ss(tmem + buf * S::S_COLS, qd, kd, id_s, first);
+                        umma_f16_ss(lead, tmem + buf * S::S_COLS, qd, kd, id_s, first);
                         first = 1;
                     }
-                ptx::umma_commit(BAR(S_FULL + buf));
+                umma_commit(lead, BAR(S_FULL + buf));
             };
             const auto values = [&](int t, int j, int buf) {
                 const uint32_t vb = base + S::OFF_KV + (2 * (j % ST) + 1) * S::KV;
@@ -452,39 +656,40 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 for (int term = 0; term < TERMS; term++)
 #pragma unroll
                     for (int k = 0; k < KT / 16; k++)
-                        umma_f16_ts(tmem + S::O_COL + t * D, tmem + buf * S::S_COLS + (k >> 1) * 32 + (k & 1) * 8 + term * 16,
-                                    desc_mn_sw128(vb + k * 16 * 128, KT * 128), id_o, j > 0 || term > 0 || k > 0);
+                        umma_f16_ts(lead, tmem + S::O_COL + t * D, tmem + buf * S::S_COLS + 16 * k + 8 * term,
+                                    desc_mn_sw128(vb + k * 16 * 128, KT * 128), id_o, (!SPLIT && j > 0) || term > 0 || k > 0);
             };
             wait(K_FULL, 0, 8u);
             if (ok) {
                 for (int t = 0; t < nt; t++) scores(t, 0, t);
-                ptx::umma_commit(BAR(K_EMPTY));
+                umma_commit(lead, BAR(K_EMPTY));
             }
             for (int j = 0; j < n && ok; j++) {
                 const int st = j % ST, s1 = (j + 1) % ST;
                 if (NT == 1 && j + 1 < n) {
                     if (!wait(K_FULL + s1, (j + 1) / ST, 9u)) break;
                     scores(0, j + 1, (j + 1) & 1);
-                    ptx::umma_commit(BAR(K_EMPTY + s1));
+                    umma_commit(lead, BAR(K_EMPTY + s1));
                 }
                 for (int t = 0; t < nt; t++) {
                     const int buf = NT == 2 ? t : j & 1;
                     if (t == 0 && !wait(V_FULL + st, j / ST, 10u)) break;
                     if (!wait(P_FULL + buf, NT == 2 ? j : j >> 1, 11u)) break;
                     values(t, j, buf);
-                    if (t == nt - 1) ptx::umma_commit(BAR(V_EMPTY + st));
-                    if (NT == 1) ptx::umma_commit(BAR(PV_DONE));
-                    if (j == n - 1) ptx::umma_commit(BAR(O_FULL + t));
+                    if (t == nt - 1) umma_commit(lead, BAR(V_EMPTY + st));
+                    if (NT == 1) umma_commit(lead, BAR(PV_DONE));
+                    if (j == n - 1) umma_commit(lead, BAR(O_FULL + t));
                     if (NT == 2 && j + 1 < n) {
                         if (t == 0 && !wait(K_FULL + s1, (j + 1) / ST, 12u)) break;
                         scores(t, j + 1, t);
-                        if (t == nt - 1) ptx::umma_commit(BAR(K_EMPTY + s1));
+                        if (t == nt - 1) umma_commit(lead, BAR(K_EMPTY + s1));
                     }
                 }
             }
             if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
         }
         __syncwarp();
+        }
     }
     __syncthreads();
     ptx::tc_fence_after_sync();
