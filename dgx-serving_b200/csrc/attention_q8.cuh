@@ -11,11 +11,15 @@
 //  - One warp brings the tiles by TMA into a ring (128-byte swizzle), following the block table; a block never has to be a whole tile.
 //  - Four warps take 16 keys of a tile each and keep their own running maximum, sum and weighted values in registers for all rows (queries
 //    x heads of the group); they meet once at the end of a pair.
-//  - mma.sync m16n8k16 with fp16 operands and fp32 sums: codes are exact in fp16 (one permute and one packed subtraction for two of them).
-//    A query row is scaled by a power of two to the middle of fp16's range.  fp32 rows are split in two fp16 terms (22 bits), which lie in
-//    rows g and g + 8 of the instruction; 16-bit rows fit one term.  The same for the weights exp(s - m) * vs: they are scaled by a factor
-//    of the row's own that keeps the largest near 2^8, 16-bit rows round them to fp16 once (2^-12, below the rounding of a 16-bit result),
-//    fp32 rows take two terms.  tcgen05 has nothing to add here: at most 32 rows meet each key, the instruction's 128 would be padding.
+//  - Q K^T: the codes enter mma.sync m16n8k32 (s8, int32 sums, exact) as they lie in memory.  A query row is cut into three signed digits of base
+//    128 relative to its largest magnitude (2^-22 of it); digits one and two lie in rows g and g + 8 of one instruction, the third of rows g and
+//    g + 8 in another.  fp16 operands need five instructions to widen four codes: decode of 64 requests 148 us.
+//  - P V: mma.sync m16n8k16 with fp16 operands and fp32 sums, since the weights need a floating point; codes are exact in fp16 (one permute
+//    and one packed subtraction for two of them).  The weight that enters is x = exp(s - B) * vs, in base 2 with the block's scale in the
+//    exponent: one multiply-add and one exp2, the sum divides vs out again once per block.  B is the row's reference: the largest x was 2^8 when
+//    it was chosen, and it moves, rescaling what is summed, only when an x would pass 2^15.  16-bit rows round x to fp16 once (2^-12, below the
+//    rounding of a 16-bit result), fp32 rows take two terms (22 bits) in rows g and g + 8.
+//    tcgen05 has nothing to add here: at most 32 rows meet each key, the instruction's 128 would be padding.
 #pragma once
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"
@@ -55,6 +59,11 @@ __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cas
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 // Bytes (lo: 0 and 1, hi: 2 and 3) of a word of codes + 128 as two fp16 numbers, minus the 128 again: 0x6400 | u is 1024 + u.
@@ -153,9 +162,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
 
@@ -188,7 +197,18 @@ __device__ __forceinline__ float row_factor(float amax) {
 }
 
 constexpr int SLOT_SCALES = 4;              // blocks of a tile at most (blocks of 16 tokens)
-constexpr size_t CONTROL = 1024;            // barriers and the stages' scales
+constexpr size_t CONTROL = 1280;            // barriers and the stages' scales: ks, log2 vs, 1 / vs, vs == 0
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// cap * tanh(x) * log2 e with x in units of cap: 1 - 2 / (1 + e^2x), whose error is that of a number near 1
+__device__ __forceinline__ float capped(float x, float cap) { return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E)))); }
+
+// Digits of base 128 of four elements, as bytes of a word: v = d1 * 128^(n-1) + ..., |v| <= 127 * 128^(n-1); v becomes what is left.
+__device__ __forceinline__ uint32_t digit4(float4 &v, float unit, float per) {
+    const float a = rintf(v.x * per), b = rintf(v.y * per), c = rintf(v.z * per), d = rintf(v.w * per);
+    v.x = fmaf(a, -unit, v.x); v.y = fmaf(b, -unit, v.y); v.z = fmaf(c, -unit, v.z); v.w = fmaf(d, -unit, v.w);
+    const uint32_t lo = __byte_perm((uint32_t)(int)a, (uint32_t)(int)b, 0x0040), hi = __byte_perm((uint32_t)(int)c, (uint32_t)(int)d, 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
 
 // Position of the f-th float4 of a row of `dim` floats in the buffer where the warps' results meet: no bank twice when the four lane columns
 // write eight (dim 64: four) float4s each, side by side.
@@ -198,28 +218,29 @@ __device__ __forceinline__ int meet_pos(int f, int row) {
     else return (f & ~7) | ((f & 7) ^ (((f >> 3) & 3) + 4 * (row & 1)));
 }
 
-template <typename T, int D, int MT>
+// R rows (queries x heads of a group) to a CTA's tile: 8, 16, 32.  A thread has rows g + 8 i.
+template <typename T, int D, int R>
 struct Shape {
-    static constexpr bool SPLIT = std::is_same<T, float>::value;      // fp32 rows: two terms, rows g and g + 8
-    static constexpr int RT = SPLIT ? 8 : 16, NR = SPLIT ? 1 : 2, ROWS = MT * RT;
-    static constexpr bool QREG = MT * D <= 128;
-    static constexpr size_t MEET_BYTES = (size_t)CW * ROWS * D * 4, Q_BYTES = QREG ? 0 : (size_t)MT * (D / 16) * 32 * 16;
+    static constexpr bool SPLIT = std::is_same<T, float>::value;      // fp32 rows: two terms of the weights
+    static constexpr int NR = R / 8, SETS = NR + (NR + 1) / 2, PM = SPLIT ? NR : (NR + 1) / 2;    // instructions' row tiles of QK and of PV
+    static constexpr bool QREG = SETS * D / 8 <= 64;                  // the digits in registers
+    static constexpr size_t MEET_BYTES = (size_t)CW * R * D * 4, Q_BYTES = QREG ? 0 : (size_t)SETS * (D / 32) * 32 * 16;
     static constexpr size_t STAGE_BYTES = 2 * (size_t)Tile<D>::BYTES;
-    static constexpr size_t FIXED = 1280 + CONTROL + MEET_BYTES + Q_BYTES + (size_t)CW * ROWS * 8 + ROWS * 4;    // and 4 bytes a request
+    static constexpr size_t FIXED = 1280 + CONTROL + MEET_BYTES + Q_BYTES + (size_t)CW * R * 8 + R * 4;    // and 4 bytes a request
     // two CTAs an SM where each still has a ring of four stages and the weighted values fit the registers
-    static constexpr int PER_SM = MT * D <= 128 && FIXED + 1024 + 4 * STAGE_BYTES <= 113 * 1024 ? 2 : 1;
-    static inline size_t fixed_bytes(int R) { return FIXED + ((size_t)R + 4) * 4; }
-    static inline int stages(int R) {
-        const size_t n = ((PER_SM == 2 ? 113 : 226) * 1024 - fixed_bytes(R)) / STAGE_BYTES;
-        return n < 12 ? (int)n : 12;
+    static constexpr int PER_SM = PM * D <= 128 && FIXED + 1024 + 4 * STAGE_BYTES <= 113 * 1024 ? 2 : 1;
+    static inline size_t fixed_bytes(int n) { return FIXED + ((size_t)n + 4) * 4; }
+    static inline int stages(int n) {
+        const size_t k = ((PER_SM == 2 ? 113 : 226) * 1024 - fixed_bytes(n)) / STAGE_BYTES;
+        return k < 12 ? (int)k : 12;
     }
 };
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
-    using S = Shape<T, D, MT>;
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
+    using S = Shape<T, D, R>;
     using L = Tile<D>;
-    constexpr int RT = S::RT, NR = S::NR, ROWS = S::ROWS, KS = D / 16, NT = D / 8;
+    constexpr int NR = S::NR, SETS = S::SETS, PM = S::PM, ROWS = R, KS = D / 32, NT = D / 8;
     constexpr bool SPLIT = S::SPLIT, QREG = S::QREG;
     extern __shared__ unsigned char smem_raw[];
     // ring first (1024-byte aligned for the swizzle), then the rest
@@ -318,7 +339,9 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8
                 const bool here = now.mine && lane / pieces == t;
                 const int pc = lane - t * pieces;
                 if (here) {
-                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(scales_at + (stage * SLOT_SCALES + pc) * 8), "f"(now.ks), "f"(now.vs) : "memory");
+                    const float v1 = now.vs == 0.f ? 1.f : now.vs;
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales_at + (stage * SLOT_SCALES + pc) * 16), "f"(now.ks), "f"(lg2(v1)),
+                                 "f"(1.f / v1), "f"(now.vs == 0.f ? 1.f : 0.f) : "memory");
                 }
                 const unsigned count = __popc(__ballot_sync(0xffffffffu, here));
                 __syncwarp();                                      // the scales are there before the arrival
@@ -350,84 +373,87 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8
     const float inf = __int_as_float(0x7f800000);
     while (walk.next(s)) {
         const int rows = min(ROWS, s.x.n * a.G - s.rg * ROWS);            // of this row group
-        uint4 qf[QREG ? MT * KS : 1];
-        float fac[MT][NR], m[MT][NR], thr[MT][NR], mref[MT][NR], l[MT][NR], wref[MT][NR], ai[MT][NR];
-        int hi[MT][NR], lo[MT][NR];
-        float acc[MT][NT][4];
+        uint4 qf[QREG ? SETS * KS : 1];
+        float fac[NR], B[NR], l[NR];
+        int hi[NR], lo[NR];
+        float acc[PM][NT][4];
         int min_hi = 0x7fffffff, max_lo = 0;
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-            for (int i = 0; i < NR; i++) {
-                const int row = mt * RT + g + 8 * i, rho = s.rg * ROWS + row;
-                const int query = min(rho / a.G, s.x.n - 1), at = s.x.seq - s.x.n + query;
-                hi[mt][i] = a.causal ? at : s.x.seq - 1;
-                lo[mt][i] = a.window > 0 ? at - a.window + 1 : 0;
-                min_hi = min(min_hi, hi[mt][i]);
-                max_lo = max(max_lo, lo[mt][i]);
-                m[mt][i] = thr[mt][i] = -inf;
-                mref[mt][i] = l[mt][i] = wref[mt][i] = 0.f;
-                ai[mt][i] = 1.f;
-            }
+        for (int i = 0; i < NR; i++) {
+            const int row = g + 8 * i, rho = s.rg * ROWS + row;
+            const int query = min(rho / a.G, s.x.n - 1), at = s.x.seq - s.x.n + query;
+            hi[i] = a.causal ? at : s.x.seq - 1;
+            lo[i] = a.window > 0 ? at - a.window + 1 : 0;
+            min_hi = min(min_hi, hi[i]);
+            max_lo = max(max_lo, lo[i]);
+            B[i] = -inf;
+            l[i] = 0.f;
         }
         min_hi = __reduce_min_sync(0xffffffffu, min_hi);
         max_lo = __reduce_max_sync(0xffffffffu, max_lo);
-        // Q: the row's largest magnitude, the row scaled, the fragments.  Element order inside a step is the codes' order in memory.
-        const auto load_rows = [&](int mt, uint4 *dst, int stride) {
-            float4 v[NR][KS];
+        // Q: the row's largest magnitude, the digits.  Element order inside a step is the codes' order in memory: step k of lane column c is
+        // elements 8 (k & 1) ... + 8 of its (k / 2)-th piece.
+        const auto load_rows = [&](int i, uint4 *dst, int stride) {
+            const int row = g + 8 * i, rho = s.rg * ROWS + row, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
+            const bool there = row < rows;
+            const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
+            float4 v[KS][2];
+            float amax = 0.f;
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
-                const int row = mt * RT + g + 8 * i;
-                float amax = 0.f;
-                const bool there = row < rows;
-                const int rho = s.rg * ROWS + row, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
-                const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    const int pq = k >> 2, d = L::qk_plane(pq) * 128 + L::qk_piece(c, pq) * 16 + (k & 3) * 4;
-                    v[i][k] = there ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int e = 0; e < 2; e++) {
+                    const int d = L::qk_plane(k >> 1) * 128 + L::qk_piece(c, k >> 1) * 16 + (k & 1) * 8 + e * 4;
+                    v[k][e] = there ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int k = 0; k < KS; k++)
-                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[i][k].x), fabsf(v[i][k].y))), fmaxf(fabsf(v[i][k].z), fabsf(v[i][k].w)));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const float f = row_factor(amax);
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int k = 0; k < KS; k++) { v[i][k].x *= f; v[i][k].y *= f; v[i][k].z *= f; v[i][k].w *= f; }
-                const float back = a.softcap > 0.f ? a.scale / f : a.scale * LOG2E / f;
-                if constexpr (QREG) fac[mt][i] = back;
-                else if (c == 0) row_fac[row] = back;
-            }
+                for (int e = 0; e < 2; e++)
+                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[k][e].x), fabsf(v[k][e].y))), fmaxf(fabsf(v[k][e].z), fabsf(v[k][e].w)));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // the row in units of its last digit: amax becomes 127 * 128^2; by a power of two first, so that neither factor leaves fp32
+            constexpr float top = 127.f * 16384.f;
+            const float p2 = row_factor(amax), f = amax > 0.f ? top / (amax * p2) : 1.f;
+            float bad = 0.f;                                           // NaN if an element is not a number or infinite: the digits cannot tell
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float4 &x = v[k][e];
+                    bad += (x.x * 0.f + x.y * 0.f) + (x.z * 0.f + x.w * 0.f);
+                    x.x = x.x * p2 * f; x.y = x.y * p2 * f; x.z = x.z * p2 * f; x.w = x.w * p2 * f;
+                }
+            bad += __shfl_xor_sync(0xffffffffu, bad, 1);
+            bad += __shfl_xor_sync(0xffffffffu, bad, 2);
+            const float back = a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad;
+            if constexpr (QREG) fac[i] = back;
+            else if (c == 0) row_fac[row] = back;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const __half2 a0 = __floats2half2_rn(v[0][k].x, v[0][k].y), a2 = __floats2half2_rn(v[0][k].z, v[0][k].w);
-                __half2 a1, a3;
-                if constexpr (SPLIT) {
-                    const float2 f0 = __half22float2(a0), f2 = __half22float2(a2);
-                    a1 = __floats2half2_rn(v[0][k].x - f0.x, v[0][k].y - f0.y);
-                    a3 = __floats2half2_rn(v[0][k].z - f2.x, v[0][k].w - f2.y);
-                } else {
-                    a1 = __floats2half2_rn(v[NR - 1][k].x, v[NR - 1][k].y);
-                    a3 = __floats2half2_rn(v[NR - 1][k].z, v[NR - 1][k].w);
-                }
-                dst[k * stride] = make_uint4(h2_bits(a0), h2_bits(a1), h2_bits(a2), h2_bits(a3));
+                const uint32_t a0 = digit4(v[k][0], 16384.f, 1.f / 16384.f), a2 = digit4(v[k][1], 16384.f, 1.f / 16384.f);
+                const uint32_t a1 = digit4(v[k][0], 128.f, 1.f / 128.f), a3 = digit4(v[k][1], 128.f, 1.f / 128.f);
+                dst[(i * KS + k) * stride] = make_uint4(a0, a1, a2, a3);
+                const uint32_t b0 = digit4(v[k][0], 1.f, 1.f), b1 = digit4(v[k][1], 1.f, 1.f);
+                uint32_t *third = reinterpret_cast<uint32_t *>(dst + ((NR + (i >> 1)) * KS + k) * stride);
+                third[i & 1] = b0;                                     // row g: first of the pairs, row g + 8: second
+                third[2 + (i & 1)] = b1;
+                if (NR == 1) { third[1] = 0u; third[3] = 0u; }
             }
         };
         if constexpr (QREG) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) load_rows(mt, qf + mt * KS, 1);
+            for (int i = 0; i < NR; i++) load_rows(i, qf, 1);
         } else {
-            if (warp < MT) load_rows(warp, qs + warp * KS * 32 + lane, 32);
+            if (warp < NR) load_rows(warp, qs + lane, 32);
             asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int i = 0; i < NR; i++) fac[mt][i] = row_fac[mt * RT + g + 8 * i];
+            for (int i = 0; i < NR; i++) fac[i] = row_fac[g + 8 * i];
         }
 
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int mt = 0; mt < PM; mt++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[mt][j][0] = acc[mt][j][1] = acc[mt][j][2] = acc[mt][j][3] = 0.f;
         for (int t = 0; t < s.tiles; t++) {
@@ -435,116 +461,103 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8
             const int key0 = (s.x.lo / TK + s.tile + t) * TK + warp * 16;
             if (ok && key0 < s.x.seq && key0 + 16 > s.x.lo) {
                 const uint32_t kt = ring_at + (uint32_t)stage * (uint32_t)S::STAGE_BYTES, vt = kt + L::BYTES;
-                const float2 sc = lds_f2(scales_at + (stage * SLOT_SCALES + ((warp * 16) >> pshift)) * 8);
-                float dot[MT][2][4];
+                const float4 sc = lds_f4(scales_at + (stage * SLOT_SCALES + ((warp * 16) >> pshift)) * 16);
+                int dot[SETS][2][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int mt = 0; mt < SETS; mt++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) dot[mt][i][0] = dot[mt][i][1] = dot[mt][i][2] = dot[mt][i][3] = 0.f;
+                    for (int i = 0; i < 2; i++) dot[mt][i][0] = dot[mt][i][1] = dot[mt][i][2] = dot[mt][i][3] = 0;
 #pragma unroll
                 for (int pq = 0; pq < L::STEPS; pq++) {
                     uint4 w[2];
 #pragma unroll
                     for (int i = 0; i < 2; i++) w[i] = lds128(kt + L::piece(warp * 16 + L::token(i, g), L::qk_piece(c, pq), L::qk_plane(pq)));
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t b[2][2];
+                    for (int mt = 0; mt < SETS; mt++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const uint32_t x = (k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w) ^ 0x80808080u;
-                            b[i][0] = codes_f16<0x4140>(x);
-                            b[i][1] = codes_f16<0x4342>(x);
-                        }
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
+                        for (int k = 0; k < 2; k++) {
                             uint4 qa;
-                            if constexpr (QREG) qa = qf[mt * KS + pq * 4 + k];
-                            else qa = qs[(mt * KS + pq * 4 + k) * 32 + lane];
-                            mma_f16(dot[mt][0], qa, b[0][0], b[0][1]);
-                            mma_f16(dot[mt][1], qa, b[1][0], b[1][1]);
+                            if constexpr (QREG) qa = qf[mt * KS + pq * 2 + k];
+                            else qa = qs[(mt * KS + pq * 2 + k) * 32 + lane];
+#pragma unroll
+                            for (int i = 0; i < 2; i++) mma_s8(dot[mt][i], qa, k ? w[i].z : w[i].x, k ? w[i].w : w[i].y);
                         }
-                    }
                 }
                 // scores in base 2, weights
                 const bool edge = key0 + 15 > min_hi || key0 < max_lo || key0 + 15 >= s.x.seq;
-                uint4 pa[MT];
-                float x[MT][NR][4], sv[MT][NR][4], pr[MT][NR][4];
+                float x[NR][4];
                 bool again = false;
+                const auto scores = [&](int i, float (&y)[4]) {
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-                    for (int i = 0; i < NR; i++) {
-                        const float f = fac[mt][i] * sc.x;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float d = SPLIT ? dot[mt][e >> 1][e & 1] + dot[mt][e >> 1][2 + (e & 1)] : dot[mt][e >> 1][2 * i + (e & 1)];
-                            sv[mt][i][e] = d * f;
-                        }
-                        if (a.softcap > 0.f)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) sv[mt][i][e] = a.softcap * LOG2E * tanhf(sv[mt][i][e] / a.softcap);
-                        if (edge)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int key = key0 + L::token(e >> 1, 2 * c + (e & 1));
-                                if (key > hi[mt][i] || key < lo[mt][i] || key >= s.x.seq) sv[mt][i][e] = -inf;
-                            }
-                        const float top = fmaxf(fmaxf(sv[mt][i][0], sv[mt][i][1]), fmaxf(sv[mt][i][2], sv[mt][i][3]));
-                        float big = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            pr[mt][i][e] = ex2(sv[mt][i][e] - mref[mt][i]);
-                            x[mt][i][e] = edge && sv[mt][i][e] == -inf ? 0.f : pr[mt][i][e] * sc.y * ai[mt][i];
-                            big = fmaxf(big, x[mt][i][e]);
-                        }
-                        again = again || top > thr[mt][i] || big > 32768.f;
+                    for (int e = 0; e < 4; e++) {
+                        const float d = fmaf((float)dot[i][e >> 1][e & 1], 16384.f,
+                                             (float)(dot[i][e >> 1][2 + (e & 1)] * 128 + dot[NR + (i >> 1)][e >> 1][2 * (i & 1) + (e & 1)]));
+                        y[e] = d;
                     }
+                    const float f = fac[i] * sc.x;
+                    if (a.softcap > 0.f) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = capped(y[e] * f, a.softcap) + sc.y;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = fmaf(y[e], f, sc.y);
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int key = key0 + L::token(e >> 1, 2 * c + (e & 1));
+                            if (key > hi[i] || key < lo[i] || key >= s.x.seq) y[e] = -inf;
+                        }
+                    }
+                };
+                float top[NR];
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    scores(i, x[i]);
+                    top[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+                    again = again || top[i] > B[i] + 15.f;
                 }
                 if (__any_sync(0xffffffffu, again)) {
-                    // the rows' maxima have grown by more than 7 (in base 2), or their largest weight: new references
+                    // a weight would pass 2^15: the rows' references move to where their largest is 2^8
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
+                    for (int i = 0; i < NR; i++) {
+                        float m = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                        const float now = m > B[i] + 8.f ? m - 8.f : B[i];
+                        const float shrink = B[i] == -inf ? 1.f : ex2(B[i] - now);        // nothing is summed while B is -inf
+                        B[i] = now;
+                        l[i] *= shrink;
 #pragma unroll
-                        for (int i = 0; i < NR; i++) {
-                            float top = fmaxf(fmaxf(sv[mt][i][0], sv[mt][i][1]), fmaxf(sv[mt][i][2], sv[mt][i][3]));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                            const float now = fmaxf(m[mt][i], top);
-                            const float f = m[mt][i] == -inf ? 1.f : ex2(m[mt][i] - now);
-                            m[mt][i] = now;
-                            thr[mt][i] = now + 7.f;
-                            mref[mt][i] = now == -inf ? 0.f : now;
-                            float w = 0.f;
-                            if (sc.y < inf) w = ex2(top - mref[mt][i]) * sc.y;
-                            const float ref = fmaxf(fmaxf(wref[mt][i] * f, w), 0x1p-100f);
-                            const float shrink = f * wref[mt][i] / ref;
-                            wref[mt][i] = ref;
-                            ai[mt][i] = 256.f / ref;
-                            l[mt][i] *= f;
-#pragma unroll
-                            for (int j = 0; j < NT; j++) {
-                                if constexpr (SPLIT) { acc[mt][j][0] *= shrink; acc[mt][j][1] *= shrink; acc[mt][j][2] *= shrink; acc[mt][j][3] *= shrink; }
-                                else { acc[mt][j][2 * i] *= shrink; acc[mt][j][2 * i + 1] *= shrink; }
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                pr[mt][i][e] = ex2(sv[mt][i][e] - mref[mt][i]);
-                                x[mt][i][e] = sv[mt][i][e] == -inf ? 0.f : pr[mt][i][e] * sc.y * ai[mt][i];
-                            }
+                        for (int j = 0; j < NT; j++) {
+                            if constexpr (SPLIT) { acc[i][j][0] *= shrink; acc[i][j][1] *= shrink; acc[i][j][2] *= shrink; acc[i][j][3] *= shrink; }
+                            else { acc[i >> 1][j][2 * (i & 1)] *= shrink; acc[i >> 1][j][2 * (i & 1) + 1] *= shrink; }
                         }
+                    }
                 }
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
+                for (int i = 0; i < NR; i++) {
+                    const float ref = B[i] == -inf ? 0.f : B[i];
 #pragma unroll
-                    for (int i = 0; i < NR; i++) l[mt][i] += (pr[mt][i][0] + pr[mt][i][1]) + (pr[mt][i][2] + pr[mt][i][3]);
-                    const __half2 h0 = __floats2half2_rn(x[mt][0][0], x[mt][0][1]), h1 = __floats2half2_rn(x[mt][0][2], x[mt][0][3]);
+                    for (int e = 0; e < 4; e++) x[i][e] = edge && x[i][e] == -inf ? 0.f : ex2(x[i][e] - ref);
+                    l[i] = fmaf((x[i][0] + x[i][1]) + (x[i][2] + x[i][3]), sc.z, l[i]);
+                }
+                if (sc.w != 0.f) {
+#pragma unroll
+                    for (int i = 0; i < NR; i++) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+                }
+                uint4 pa[PM];
+#pragma unroll
+                for (int mt = 0; mt < PM; mt++) {
+                    const int i = SPLIT ? mt : 2 * mt;
+                    const __half2 h0 = __floats2half2_rn(x[i][0], x[i][1]), h1 = __floats2half2_rn(x[i][2], x[i][3]);
                     if constexpr (SPLIT) {
                         const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                        pa[mt] = make_uint4(h2_bits(h0), h2_bits(__floats2half2_rn(x[mt][0][0] - f0.x, x[mt][0][1] - f0.y)),
-                                            h2_bits(h1), h2_bits(__floats2half2_rn(x[mt][0][2] - f1.x, x[mt][0][3] - f1.y)));
+                        pa[mt] = make_uint4(h2_bits(h0), h2_bits(__floats2half2_rn(x[i][0] - f0.x, x[i][1] - f0.y)),
+                                            h2_bits(h1), h2_bits(__floats2half2_rn(x[i][2] - f1.x, x[i][3] - f1.y)));
                     } else {
-                        pa[mt] = make_uint4(h2_bits(h0), h2_bits(__floats2half2_rn(x[mt][NR - 1][0], x[mt][NR - 1][1])),
-                                            h2_bits(h1), h2_bits(__floats2half2_rn(x[mt][NR - 1][2], x[mt][NR - 1][3])));
+                        constexpr int o = NR > 1 ? 1 : 0;
+                        pa[mt] = make_uint4(h2_bits(h0), o ? h2_bits(__floats2half2_rn(x[i + o][0], x[i + o][1])) : 0u,
+                                            h2_bits(h1), o ? h2_bits(__floats2half2_rn(x[i + o][2], x[i + o][3])) : 0u);
                     }
                 }
                 // values: lane row g holds the 16 (dim 64: 8) elements of a piece, one for each group of eight columns
@@ -572,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8
 #pragma unroll
                         for (int j = 0; j < 4; j++)
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++) mma_f16(acc[mt][pl * 16 + w * 4 + j], pa[mt], b[j][0], b[j][1]);
+                            for (int mt = 0; mt < PM; mt++) mma_f16(acc[mt][pl * 16 + w * 4 + j], pa[mt], b[j][0], b[j][1]);
                     }
                 }
             }
@@ -583,42 +596,38 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, MT>::PER_SM) attention_q8
 
         // ---- the warps meet --------------------------------------------------------------------------------------------------------
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int i = 0; i < NR; i++) {
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 2);
-                if (c == 0) ml[warp * ROWS + mt * RT + g + 8 * i] = make_float2(m[mt][i], l[mt][i]);
-            }
+        for (int i = 0; i < NR; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (c == 0) ml[warp * ROWS + g + 8 * i] = make_float2(B[i], l[i]);
+        }
         asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int i = 0; i < NR; i++) {
+            const int row = g + 8 * i;
+            float top = ml[row].x;
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
-                const int row = mt * RT + g + 8 * i;
-                float top = ml[row].x;
+            for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w * ROWS + row].x);
+            const float f = B[i] == -inf ? 0.f : ex2(B[i] - top);
+            float4 *dst = reinterpret_cast<float4 *>(meet + ((size_t)warp * ROWS + row) * D);
+            if (row < rows) {
 #pragma unroll
-                for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w * ROWS + row].x);
-                const float f = m[mt][i] == -inf ? 0.f : ex2(m[mt][i] - top) * (wref[mt][i] * (1.f / 256.f));
-                float4 *dst = reinterpret_cast<float4 *>(meet + ((size_t)warp * ROWS + row) * D);
-                if (row < rows) {
+                for (int pl = 0; pl < L::PLANES; pl++)
 #pragma unroll
-                    for (int pl = 0; pl < L::PLANES; pl++)
+                    for (int half = 0; half < 2; half++)
 #pragma unroll
-                        for (int half = 0; half < 2; half++)
+                        for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
+                            float o[4];
 #pragma unroll
-                            for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
-                                float o[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const float *q4 = acc[mt][pl * 16 + 4 * k + e];
-                                    o[e] = (SPLIT ? q4[half] + q4[2 + half] : q4[2 * i + half]) * f;
-                                }
-                                const int f4 = D == 64 ? 4 * c + 2 * half + k : 32 * pl + 8 * c + 4 * half + k;
-                                dst[meet_pos<D>(f4, row)] = make_float4(o[0], o[1], o[2], o[3]);
+                            for (int e = 0; e < 4; e++) {
+                                const float *q4 = acc[SPLIT ? i : i >> 1][pl * 16 + 4 * k + e];
+                                o[e] = (SPLIT ? q4[half] + q4[2 + half] : q4[2 * (i & 1) + half]) * f;
                             }
-                }
+                            const int f4 = D == 64 ? 4 * c + 2 * half + k : 32 * pl + 8 * c + 4 * half + k;
+                            dst[meet_pos<D>(f4, row)] = make_float4(o[0], o[1], o[2], o[3]);
+                        }
             }
+        }
         asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
         const bool whole = s.tiles == s.pair_tiles;
         const int slot = 2 * (int)cta + (s.tile == 0 ? 1 : 0);
@@ -698,14 +707,14 @@ inline size_t workspace_bytes(int dim) {
     return count_bytes() + slots * MAX_ROWS * 8 + slots * MAX_ROWS * dim * 4;
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int R>
 inline int launch_t(Call &c, cudaStream_t st) {
-    using S = Shape<T, D, MT>;
+    using S = Shape<T, D, R>;
     Args &a = c.a;
     constexpr int per_sm = S::PER_SM;
     a.stages = S::stages(a.R);
     const size_t smem = S::fixed_bytes(a.R) + a.stages * S::STAGE_BYTES;
-    auto kern = attention_q8_kernel<T, D, MT>;
+    auto kern = attention_q8_kernel<T, D, R>;
     static PerDevice<size_t> configured_dev;
     size_t &configured = configured_dev.get();
     if (smem > configured) {
@@ -724,12 +733,18 @@ inline int launch_t(Call &c, cudaStream_t st) {
     return e == cudaSuccess ? launch_status("attention_q8") : cuda_fail(e, "attention_q8 launch");
 }
 
+template <typename T, int D>
+inline int launch_r(Call &c, int rows, cudaStream_t st) {
+    constexpr int most = (std::is_same<T, float>::value ? 8 : 16) * (D == 256 ? 1 : 2);     // the registers' limit
+    if (rows <= 8) return launch_t<T, D, 8>(c, st);
+    if (rows <= 16 || most == 16) return launch_t<T, D, most < 16 ? most : 16>(c, st);
+    return launch_t<T, D, most>(c, st);
+}
 template <typename T>
 inline int launch_d(Call &c, int rows, cudaStream_t st) {
-    const bool two = rows > (std::is_same<T, float>::value ? 8 : 16);
-    if (c.dim == 64) return two ? launch_t<T, 64, 2>(c, st) : launch_t<T, 64, 1>(c, st);
-    if (c.dim == 128) return two ? launch_t<T, 128, 2>(c, st) : launch_t<T, 128, 1>(c, st);
-    return launch_t<T, 256, 1>(c, st);
+    if (c.dim == 64) return launch_r<T, 64>(c, rows, st);
+    if (c.dim == 128) return launch_r<T, 128>(c, rows, st);
+    return launch_r<T, 256>(c, rows, st);
 }
 
 // `rows`: queries x heads of a group of the request with most of them.

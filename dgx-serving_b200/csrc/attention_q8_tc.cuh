@@ -22,6 +22,9 @@ namespace attn_tc {
 using attn::LOG2E;
 using attn::LN2;
 using attn::ex2;
+using attn::lg2;
+using attn::capped;
+using attn::lds_f4;
 using attn::h2_bits;
 constexpr unsigned ERR_WAIT = 0xB00u;
 constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
@@ -84,17 +87,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// cap * tanh(x) * log2 e with x in units of cap: 1 - 2 / (1 + e^2x), whose error is that of a number near 1
-__device__ __forceinline__ float capped(float x, float cap) {
-    return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E))));
-}
-
 // Four bytes of codes as two packed pairs of fp16.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &a, uint32_t &b) {
     w ^= 0x80808080u;
