@@ -1,25 +1,22 @@
-// Attention of a few queries a request over the 8-bit paged KV cache: a stream of the blocks through shared memory.
+// Attention of few queries a request over the 8-bit paged KV cache: a stream of the blocks through the tensor cores, which take the codes as they are.
 //
 //   s[i,j] = scale * ks[block(j)] * sum_d q[i,d] K[j,d]           (K, V: the int8 codes)
 //   o[i]   = sum_j exp(s[i,j] - m) vs[block(j)] V[j] / sum_j exp(s[i,j] - m),   j over what query i sees
 //
 // What bounds it: the codes have to come from HBM once, 2 * dim bytes a token and kv head.  Everything else is arranged not to be in the way:
-//  - Work is cut evenly: the (request, kv head, row group) pairs' key tiles of 64 tokens, laid one behind the other, are divided into equal
-//    ranges, one per resident CTA, whatever the lengths.  A pair that several CTAs share leaves partial results (sum, maximum, weighted
-//    values) in the workspace; the last of them to finish joins them in the order of the ranges, so the result does not depend on who is
-//    last.  One launch.
-//  - One warp brings the tiles by TMA into a ring (128-byte swizzle), following the block table; a block never has to be a whole tile.
-//  - Four warps take 16 keys of a tile each and keep their own running maximum, sum and weighted values in registers for all rows (queries
-//    x heads of the group); they meet once at the end of a pair.
-//  - Q K^T: the codes enter mma.sync m16n8k32 (s8, int32 sums, exact) as they lie in memory.  A query row is cut into three signed digits of base
-//    128 relative to its largest magnitude (2^-22 of it); digits one and two lie in rows g and g + 8 of one instruction, the third of rows g and
-//    g + 8 in another.  fp16 operands need five instructions to widen four codes: decode of 64 requests 148 us.
-//  - P V: mma.sync m16n8k16 with fp16 operands and fp32 sums, since the weights need a floating point; codes are exact in fp16 (one permute
-//    and one packed subtraction for two of them).  The weight that enters is x = exp(s - B) * vs, in base 2 with the block's scale in the
-//    exponent: one multiply-add and one exp2, the sum divides vs out again once per block.  B is the row's reference: the largest x was 2^8 when
-//    it was chosen, and it moves, rescaling what is summed, only when an x would pass 2^15.  16-bit rows round x to fp16 once (2^-12, below the
-//    rounding of a 16-bit result), fp32 rows take two terms (22 bits) in rows g and g + 8.
-//    tcgen05 has nothing to add here: at most 32 rows meet each key, the instruction's 128 would be padding.
+//  - Work is cut evenly: the (request, kv head, row group) pairs' key tiles of 128 tokens, laid one behind the other, are divided into equal
+//    ranges, one per SM, whatever the lengths.  A pair that several CTAs share leaves partial results (reference, sum, weighted values) in the
+//    workspace; neighbours are joined by the last of them to finish, in the order of the ranges, so the result does not depend on who is last.
+//    One launch.
+//  - Both products are tcgen05.mma kind::i8 with the keys' tile as the 128-row operand, so the codes go from HBM by TMA to shared memory (128-byte
+//    swizzle; along the block table, a block never has to be a whole tile) and no thread touches them: S^T [keys][rows] = K Q^T with K as it
+//    lies, O^T [dim][rows] += V^T P^T with V read as the transposed operand.  Widening the codes to fp16 for mma.sync cost 450 instructions for 16
+//    keys and bound the stream: two requests of 130k tokens 96 us, 64 ragged ones 128.
+//  - A query row is a fixed-point number relative to its largest magnitude, three signed digits of base 256 (2^-23 of it): three columns.  A weight
+//    is a whole number too, x = exp(s - B) * vs up to 2^31, four columns of P.  All sums are whole numbers and exact; O stays in tensor memory over
+//    the tiles.  The row's reference B is such that its largest x was 2^28 when it was chosen; when an x would pass 2^31, O is read out, rescaled
+//    and summed in fp32, and B moves.  So a weight is rounded to 2^-28 of the row's largest, or as fp32 is.
+//  - 128 threads have a key each, about forty instructions for a row.
 #pragma once
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"
@@ -28,14 +25,14 @@
 namespace w4a8 {
 namespace attn {
 
-constexpr int TK = 64;                     // tokens of a tile
-constexpr int CW = 4;                      // consumer warps: 16 tokens of the tile each
-constexpr int THREADS = (CW + 1) * 32;
+constexpr int TK = 128;                    // keys of a tile
+constexpr int THREADS = 256;               // warps 0-3: a key (then a dim) a thread; 4, 5: copies of K, of V; 6: products; 7: queries
 constexpr int MAX_R = 2048;                // requests of one launch (their sums lie in shared memory)
-constexpr int FEW_ROWS = 64;                // rows (queries x heads of a group) of a request that the streaming kernel takes at most
-constexpr int MIN_TILES = 2;               // a CTA takes at least so many tiles: joining costs about two tiles' time
+constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) of a request that this kernel takes at most
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;
+constexpr float TOP = 28.f, LIMIT = 30.9f; // log2 of the largest weight when B is chosen, and beyond which it moves (four signed digits reach 2^30.99)
+constexpr int FLUSH = 900;                 // tiles after which O is read out at the latest: 128 * 128 * 127 * 900 < 2^31
 
 struct Args {
     const void *q;
@@ -48,24 +45,15 @@ struct Args {
     int causal, window;
     float scale, softcap;
     int few;                               // rows (queries * G) of a request that this kernel takes at most; more are another kernel's
-    unsigned *count;                       // workspace: arrivals per CTA, zero between calls
-    float2 *part_ml;                       // [2 * CTAs][rows] maximum, sum
-    float *part;                           // [2 * CTAs][rows][dim]
+    // workspace, by a CTA's two ends: arrivals, zero between calls; [2 * CTAs][rows] reference, sum; [2 * CTAs][rows][dim] values; groups of CTAs alike
+    unsigned *count, *count2;
+    float2 *part_ml, *part2_ml;
+    float *part, *part2;
 };
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_s8(int (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
 // Bytes (lo: 0 and 1, hi: 2 and 3) of a word of codes + 128 as two fp16 numbers, minus the 128 again: 0x6400 | u is 1024 + u.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t u) {
@@ -134,32 +122,9 @@ struct Walk {
     }
 };
 
-// Where the tile's tokens go for the warps' reads to meet no bank twice (checked for each head size): a tile is planes of 128-byte rows, the
-// 16-byte piece c of row r at c ^ (r & 7).  dim 128 and 256: a row is a token, a plane 128 elements.  dim 64: a row is two tokens.
-template <int D> struct Tile {
-    static constexpr int PLANES = D == 256 ? 2 : 1, ROW_TOKENS = D == 64 ? 2 : 1;
-    static constexpr int PLANE_BYTES = TK * D / PLANES, BYTES = TK * D;
-    // token of the instruction's column n (0..7) in the t-th (0, 1) group of eight: QK and PV agree on it
-    static __device__ __forceinline__ int token(int t, int n) { return D == 64 ? 4 * (n >> 1) + (n & 1) + 2 * t : n + 8 * t; }
-    // address of piece c (0..7 of a plane's 128 elements; 0..3 with dim 64) of token k
-    static __device__ __forceinline__ uint32_t piece(int k, int c, int plane) {
-        if constexpr (D == 64) { const int row = k >> 1; return row * 128 + ((((k & 1) * 4 + c) ^ (row & 7)) << 4); }
-        else return plane * PLANE_BYTES + k * 128 + ((c ^ (k & 7)) << 4);
-    }
-    // dim of the first of the 16 elements that lane column c (0..3) reads in the p-th step of QK: piece and plane
-    static constexpr int STEPS = D / 64;
-    static __device__ __forceinline__ int qk_piece(int c, int p) { return D == 64 ? c : 2 * c + (p & 1); }
-    static __device__ __forceinline__ int qk_plane(int p) { return p >> 1; }
-};
-
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
@@ -196,74 +161,152 @@ __device__ __forceinline__ float row_factor(float amax) {
     return __int_as_float((e + 127) << 23);
 }
 
-constexpr int SLOT_SCALES = 4;              // blocks of a tile at most (blocks of 16 tokens)
-constexpr size_t CONTROL = 1280;            // barriers and the stages' scales: ks, log2 vs, 1 / vs, vs == 0
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // cap * tanh(x) * log2 e with x in units of cap: 1 - 2 / (1 + e^2x), whose error is that of a number near 1
 __device__ __forceinline__ float capped(float x, float cap) { return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E)))); }
 
-// Digits of base 128 of four elements, as bytes of a word: v = d1 * 128^(n-1) + ..., |v| <= 127 * 128^(n-1); v becomes what is left.
-__device__ __forceinline__ uint32_t digit4(float4 &v, float unit, float per) {
-    const float a = rintf(v.x * per), b = rintf(v.y * per), c = rintf(v.z * per), d = rintf(v.w * per);
-    v.x = fmaf(a, -unit, v.x); v.y = fmaf(b, -unit, v.y); v.z = fmaf(c, -unit, v.z); v.w = fmaf(d, -unit, v.w);
-    const uint32_t lo = __byte_perm((uint32_t)(int)a, (uint32_t)(int)b, 0x0040), hi = __byte_perm((uint32_t)(int)c, (uint32_t)(int)d, 0x0040);
-    return __byte_perm(lo, hi, 0x5410);
-}
-
-// Position of the f-th float4 of a row of `dim` floats in the buffer where the warps' results meet: no bank twice when the four lane columns
-// write eight (dim 64: four) float4s each, side by side.
-template <int D>
-__device__ __forceinline__ int meet_pos(int f, int row) {
-    if constexpr (D == 64) return (f & ~3) | ((f & 3) ^ (((f >> 3) & 1) + 2 * (row & 1)));
-    else return (f & ~7) | ((f & 7) ^ (((f >> 3) & 3) + 4 * (row & 1)));
-}
-
-// R rows (queries x heads of a group) to a CTA's tile: 8, 16, 32.  A thread has rows g + 8 i.
-template <typename T, int D, int R>
-struct Shape {
-    static constexpr bool SPLIT = std::is_same<T, float>::value;      // fp32 rows: two terms of the weights
-    static constexpr int NR = R / 8, SETS = NR + (NR + 1) / 2, PM = SPLIT ? NR : (NR + 1) / 2;    // instructions' row tiles of QK and of PV
-    static constexpr bool QREG = SETS * D / 8 <= 64;                  // the digits in registers
-    static constexpr size_t MEET_BYTES = (size_t)CW * R * D * 4, Q_BYTES = QREG ? 0 : (size_t)SETS * (D / 32) * 32 * 16;
-    static constexpr size_t STAGE_BYTES = 2 * (size_t)Tile<D>::BYTES;
-    static constexpr size_t FIXED = 1280 + CONTROL + MEET_BYTES + Q_BYTES + (size_t)CW * R * 8 + R * 4;    // and 4 bytes a request
-    // two CTAs an SM where each still has a ring of four stages and the weighted values fit the registers
-    static constexpr int PER_SM = PM * D <= 128 && FIXED + 1024 + 4 * STAGE_BYTES <= 113 * 1024 ? 2 : 1;
-    static inline size_t fixed_bytes(int n) { return FIXED + ((size_t)n + 4) * 4; }
-    static inline int stages(int n) {
-        const size_t k = ((PER_SM == 2 ? 113 : 226) * 1024 - fixed_bytes(n)) / STAGE_BYTES;
-        return k < 12 ? (int)k : 12;
+// Bounded waits without a call: a kernel that moves registers between its warps cannot have one.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    long long since = 0;
+#pragma unroll 1
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (ptx::mbar_try_wait(bar, parity)) return true;
+        const long long now = clock64();
+        if (since == 0) since = now;
+        else if (now - since > (1ll << 28)) return false;
     }
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
+    const bool ok = wait_one(bar, parity);
+    return __all_sync(0xffffffffu, ok);
+}
+// The same for a warp that waits long: it sleeps between the attempts and leaves the issue slots to the others.
+__device__ __forceinline__ bool wait_idle(uint32_t bar, uint32_t parity) {
+    bool ok = ptx::mbar_try_wait(bar, parity);
+#pragma unroll 1
+    for (int i = 0; i < (1 << 21) && !ok; i++) {
+        __nanosleep(100);
+        ok = ptx::mbar_try_wait(bar, parity);
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+template <int N> __device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// What the warps have to know of a segment, left by the one that prepares its queries.  tiles 0: there is no further one.
+struct Work { int tiles, tile0, min_hi, max_lo, n, q0, rg, h, first, pair0, pair_tiles, pad; };   // keys up to min_hi and from max_lo on: every row sees them
+constexpr int WORKS = 4;
+constexpr int FAN = 16, MAX_ROWS = 32;     // CTAs whose partial results are joined at a time; rows of a partial result
+
+// ---- operands ------------------------------------------------------------------------------------------------------------------------------
+// A tile of codes: planes of 128-byte rows, the 16-byte piece c of row r at c ^ (r & 7).  dim 128 and 256: a row is a token, a plane 128 elements.
+// dim 64: K in rows of 64 bytes (piece c of row r at c ^ (r >> 1 & 3)); V in rows of two tokens, so that the instruction's 128 rows are (token's
+// parity, element), the keys of the product pairs of tokens, and the weights' columns come twice, for the even and the odd tokens: half of what
+// the instruction sums is the wrong parity's and is not read.
+template <int D> struct Tile {
+    static constexpr int PLANES = D == 256 ? 2 : 1, BYTES = TK * D, PLANE_BYTES = BYTES / PLANES;
+    static constexpr int K_ROW = D == 64 ? 64 : 128, V_TOKENS = D == 64 ? 2 : 1;             // bytes of a row of K, tokens of a row of V
+};
+// K-major operand of `ROW`-byte rows: 8 rows ROW * 8 bytes; swizzle mode 2 (128 bytes) or 4 (64 bytes).
+template <int ROW> __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(ROW * 8 >> 4) << 32) | (1ull << 46) | ((ROW == 128 ? 2ull : 4ull) << 61);
+}
+// MN-major operand of 128 bytes: a row of 128 elements for each k, 8 of them 1024 bytes.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D = int32, A and B signed bytes, 128 rows, N columns; bit 15: A is MN-major.
+__host__ __device__ constexpr uint32_t idesc_s8(int N, int a_mn) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
+// The whole warp comes here and the elected lane issues: addresses and descriptors then stay in uniform registers.
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void umma_s8(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+}
+__device__ __forceinline__ float out_round(float, float v) { return v; }
+__device__ __forceinline__ __half out_round(__half, float v) { return __float2half_rn(v); }
+__device__ __forceinline__ __nv_bfloat16 out_round(__nv_bfloat16, float v) { return __float2bfloat16_rn(v); }
+// N columns of tensor memory of this lane.
+template <int N> __device__ __forceinline__ void tmem_columns(uint32_t addr, int (&v)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) {
+        uint32_t r[16];
+        ptx::tmem_ld(addr + c, r);
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[c + e] = (int)r[e];
+    }
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < N; c++) asm volatile("" : "+r"(v[c]));        // nothing that reads them moves in front of the wait
+}
+
+// R rows (queries x heads of a group): 3 columns of S and 4 of P for each, in whole sixteens.
+template <int D, int R_> struct Shape {
+    static constexpr int R = R_, N = (3 * R + 15) / 16 * 16, NP = 4 * R, DP = D == 256 ? 2 : 1, OC = D == 64 ? 2 * NP : DP * NP;    // DP: dims of a thread; OC: columns of O
+    static constexpr int STAGE = 2 * Tile<D>::BYTES, QB = N * D, PB = NP * TK;
+    static constexpr int SCALES = 8;                                                   // blocks of a tile at most
+    static constexpr int MAX_STAGES = 8;
+    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 4 * R * 4 + (D == 64 ? 64 * R * 4 : 0);   // and 4 bytes a request
+    static inline int fixed_bytes(int n) { return (FIXED + (n + 4) * 4 + 1023) & ~1023; }
+    static inline int stages(int n) {
+        const int k = (226 * 1024 - fixed_bytes(n)) / STAGE;
+        return k < MAX_STAGES ? k : MAX_STAGES;
+    }
+    static_assert(NP % 16 == 0 && 2 * N + OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 2 * STAGE <= 226 * 1024, "shape");
 };
 
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
-    using S = Shape<T, D, R>;
+__global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
+    using S = Shape<D, R>;
     using L = Tile<D>;
-    constexpr int NR = S::NR, SETS = S::SETS, PM = S::PM, ROWS = R, KS = D / 32, NT = D / 8;
-    constexpr bool SPLIT = S::SPLIT, QREG = S::QREG;
+    constexpr int N = S::N, NP = S::NP, DP = S::DP;
     extern __shared__ unsigned char smem_raw[];
-    // ring first (1024-byte aligned for the swizzle), then the rest
+    // ring, Q and P first (1024-byte aligned for the swizzle), then the rest
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *ring = smem, *p = ring + (size_t)a.stages * S::STAGE_BYTES;
-    unsigned char *control = p; p += CONTROL;
-    float *meet = reinterpret_cast<float *>(p); p += S::MEET_BYTES;
-    uint4 *qs = reinterpret_cast<uint4 *>(p); p += S::Q_BYTES;
-    float2 *ml = reinterpret_cast<float2 *>(p); p += (size_t)CW * ROWS * 8;
-    float *row_fac = reinterpret_cast<float *>(p); p += ROWS * 4;
+    unsigned char *p = smem + (size_t)a.stages * S::STAGE;
+    unsigned char *qs = p; p += 2 * S::QB;
+    unsigned char *ps = p; p += 2 * S::PB;
+    unsigned char *control = p; p += 1024;
+    float4 *scales = reinterpret_cast<float4 *>(p); p += S::MAX_STAGES * S::SCALES * 16;   // ks, log2 vs, 1 / vs of a stage's blocks
+    float4 *rec = reinterpret_cast<float4 *>(p); p += 2 * R * 16;                          // a row's factor, B, last and first key (as int)
+    float *red = reinterpret_cast<float *>(p); p += 4 * R * 4;
+    float *fold = reinterpret_cast<float *>(p); p += D == 64 ? 64 * R * 4 : 0;
     unsigned *cum = reinterpret_cast<unsigned *>(p);
-    const uint32_t bar = ptx::smem_u32(control), scales_at = bar + 256, ring_at = ptx::smem_u32(ring);
-    const auto FULL = [&](int s) { return bar + 8u * s; };
-    const auto EMPTY = [&](int s) { return bar + 128u + 8u * s; };
-    __shared__ unsigned wsum[THREADS / 32], last_flag;
+    const uint32_t bar = ptx::smem_u32(control), ring_at = ptx::smem_u32(smem), q_at = ptx::smem_u32(qs), p_at = ptx::smem_u32(ps);
+    const uint32_t K_FULL = bar, V_FULL = bar + 64u, EMPTY = bar + 128u, S_FULL = bar + 192u, S_EMPTY = bar + 208u, P_FULL = bar + 224u, P_EMPTY = bar + 240u,
+                   Q_FULL = bar + 256u, Q_EMPTY = bar + 272u;
+    __shared__ unsigned wsum[THREADS / 32], last_flag, tmem_slot;
+    __shared__ int fresh[2];                                            // a tile's weights begin new sums in O
+    __shared__ Work works[WORKS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int s = 0; s < a.stages; s++) { ptx::mbar_init(FULL(s), 1); ptx::mbar_init(EMPTY(s), CW); }
+        for (int s = 0; s < S::MAX_STAGES; s++) { ptx::mbar_init(K_FULL + 8 * s, 1); ptx::mbar_init(V_FULL + 8 * s, 1); ptx::mbar_init(EMPTY + 8 * s, 1); }
+        for (int s = 0; s < 2; s++) {
+            ptx::mbar_init(S_FULL + 8 * s, 1);
+            ptx::mbar_init(S_EMPTY + 8 * s, 4);
+            ptx::mbar_init(P_FULL + 8 * s, 4);
+            ptx::mbar_init(P_EMPTY + 8 * s, 1);
+            ptx::mbar_init(Q_FULL + 8 * s, 1);
+            ptx::mbar_init(Q_EMPTY + 8 * s, 5);
+        }
         ptx::mbar_fence_init();
         ptx::tma_prefetch_desc(&map_k);
         ptx::tma_prefetch_desc(&map_v);
     }
+    // columns behind the rows' (and rows that a segment does not have) are sums of zeros
+    for (int i = tid; i < (2 * S::QB + 2 * S::PB) / 16; i += THREADS) reinterpret_cast<uint4 *>(qs)[i] = make_uint4(0, 0, 0, 0);
     pdl_wait();
     pdl_launch_dependents();
     // units in front of each request
@@ -271,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_
     for (int base = 0; base < a.R; base += THREADS) {
         const int r = base + tid;
         unsigned v = 0;
-        if (r < a.R) { const Request x = request(a, r, ROWS); v = (unsigned)x.groups * (unsigned)a.Hkv * (unsigned)x.tiles; }
+        if (r < a.R) { const Request x = request(a, r, R); v = (unsigned)x.groups * (unsigned)a.Hkv * (unsigned)x.tiles; }
         unsigned s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const unsigned t = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += t; }
@@ -284,48 +327,57 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_
         __syncthreads();
     }
     if (tid == 0) cum[a.R] = carry;
-    __syncthreads();
-    const unsigned U = carry;
-    if (U == 0) return;
-    // equal ranges for as many CTAs as get MIN_TILES each
-    const unsigned P = min(gridDim.x, max(1u, U / MIN_TILES)), cta = blockIdx.x;
+    const unsigned U = carry, P = min(gridDim.x, U), cta = blockIdx.x;            // equal ranges
     if (cta >= P) return;
     const auto bound = [&](unsigned i) { return (unsigned)((unsigned long long)i * U / P); };
     const auto cta_of = [&](unsigned u) { return (unsigned)(((unsigned long long)(u + 1) * P - 1) / U); };
     const unsigned u0 = bound(cta), u1 = bound(cta + 1);
-    const int bshift = 31 - __clz(a.block), piece_tokens = min(a.block, TK), pshift = 31 - __clz(piece_tokens), pieces = TK / piece_tokens;
+    if (warp == 6) {
+        ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::fence_proxy_async_smem();
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot, o_cols = tmem + 2 * N;
+    const int bshift = 31 - __clz(a.block), tokens = min(a.block, TK), tshift = 31 - __clz(tokens), pieces = TK / tokens;
+    const float inf = __int_as_float(0x7f800000);
+    bool ok = true;
+    const auto give_up = [&](unsigned code) { if (lane == 0) dev_set_error(ERR_WAIT | code); ok = false; };
 
-    if (warp == CW) {
-        // ---- producer: lane = one piece (the part of a block that lies in a tile); a batch is 32 pieces ------------------------------
-        Walk walk(a, cum, u0, u1, ROWS);
+    if (warp == 4 || warp == 5) {
+        // ---- copies: lane = one piece (a block, or the part of it that lies in a tile); a batch is 32 pieces; this warp brings K or V -----------------
+        const bool is_k = warp == 4;
+        const CUtensorMap *map = is_k ? &map_k : &map_v;
+        const uint32_t full0 = is_k ? K_FULL : V_FULL;
+        Walk walk(a, cum, u0, u1, R);
         Segment s;
-        int stage = 0, used = 0;                                   // used: stages filled so far (the ring's first round needs no wait)
+        int stage = 0, used = 0, t_next = 0;
         uint32_t phase = 0;
-        bool more = walk.next(s), ok = true;
-        int t_next = 0;                                            // next tile of the segment to look up
-        const int per_batch = 32 / pieces;
-        struct Batch { int tiles, row, tok; float ks, vs; bool mine; } b;
-        int phys = 0;
+        bool more = walk.next(s);
+        const int per_batch = 32 / pieces, mine_t = lane / pieces, pc = lane - mine_t * pieces;
+        struct Batch { int tiles, row; float ks, vs; bool mine; } b;
+        int phys = 0, h = 0, tok = 0;
         const auto look_up = [&]() {                               // the table entry of this lane's piece of the next batch
             b.tiles = 0; b.mine = false;
             if (!more) return;
             b.tiles = min(per_batch, s.tiles - t_next);
-            const int t = lane / pieces, pc = lane - t * pieces;
-            const int first = (s.x.lo / TK + s.tile + t_next + t) * TK + pc * piece_tokens;
-            b.mine = t < b.tiles && first < s.x.seq && first + piece_tokens > s.x.lo;
+            const int first = (s.x.lo / TK + s.tile + t_next + mine_t) * TK + pc * tokens;
+            b.mine = mine_t < b.tiles && first < s.x.seq && first + tokens > s.x.lo;
             if (b.mine) phys = a.table[(size_t)s.r * a.width + (first >> bshift)];
-            b.tok = first & (a.block - 1);
-            b.row = s.h;
+            tok = first & (a.block - 1);
+            h = s.h;
             t_next += b.tiles;
             if (t_next == s.tiles) { more = walk.next(s); t_next = 0; }
         };
         const auto resolve = [&]() {                               // its scales and its place in the pool
+            b.ks = 0.f; b.vs = 1.f;
             if (!b.mine) return;
             if (phys < 0 || phys >= a.num_blocks) { dev_set_error(kv::ERR_BLOCK_ID); phys = 0; }
-            const size_t unit = (size_t)phys * a.Hkv + b.row;
-            b.ks = a.ks[unit];
-            b.vs = a.vs[unit];
-            b.row = (int)((unit * a.block + b.tok) / L::ROW_TOKENS);
+            const size_t unit = (size_t)phys * a.Hkv + h;
+            if (is_k) { b.ks = a.ks[unit]; b.vs = a.vs[unit]; }
+            b.row = (int)((unit * a.block + tok) / (is_k ? 1 : L::V_TOKENS));
         };
         look_up();
         resolve();
@@ -333,26 +385,19 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_
             const Batch now = b;
             look_up();
             for (int t = 0; t < now.tiles; t++) {
-                if (used >= a.stages) {
-                    if (!ptx::mbar_wait_warp(EMPTY(stage), phase ^ 1u)) { dev_set_error(ERR_WAIT | 1u); ok = false; break; }
-                }
-                const bool here = now.mine && lane / pieces == t;
-                const int pc = lane - t * pieces;
-                if (here) {
-                    const float v1 = now.vs == 0.f ? 1.f : now.vs;
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales_at + (stage * SLOT_SCALES + pc) * 16), "f"(now.ks), "f"(lg2(v1)),
-                                 "f"(1.f / v1), "f"(now.vs == 0.f ? 1.f : 0.f) : "memory");
+                if (used >= a.stages && !wait_idle(EMPTY + 8 * stage, phase ^ 1u)) { give_up(is_k ? 1u : 2u); break; }
+                const bool in = mine_t == t, here = in && now.mine;
+                if (is_k && in) {                                  // vs 0: its block's weights are as good as 0, and their sum comes out right
+                    const float v1 = fmaxf(now.vs, 0x1p-100f);
+                    scales[stage * S::SCALES + pc] = make_float4(now.ks, lg2(v1), 1.f / v1, 0.f);
                 }
                 const unsigned count = __popc(__ballot_sync(0xffffffffu, here));
                 __syncwarp();                                      // the scales are there before the arrival
-                if (lane == 0) ptx::mbar_arrive_expect_tx(FULL(stage), count * 2u * (unsigned)(piece_tokens * D));
+                if (lane == 0) ptx::mbar_arrive_expect_tx(full0 + 8 * stage, count * (unsigned)(tokens * D));
                 if (here) {
-                    const uint32_t at = ring_at + (uint32_t)stage * (uint32_t)S::STAGE_BYTES + (uint32_t)(pc * piece_tokens / L::ROW_TOKENS) * 128u;
+                    const uint32_t at = ring_at + (uint32_t)stage * S::STAGE + (is_k ? 0 : L::BYTES) + (uint32_t)(pc * tokens * (D == 256 ? 128 : D));
 #pragma unroll
-                    for (int pl = 0; pl < L::PLANES; pl++) {
-                        ptx::tma_load_2d(at + pl * L::PLANE_BYTES, &map_k, pl * 128, now.row, FULL(stage));
-                        ptx::tma_load_2d(at + L::BYTES + pl * L::PLANE_BYTES, &map_v, pl * 128, now.row, FULL(stage));
-                    }
+                    for (int pl = 0; pl < L::PLANES; pl++) ptx::tma_load_2d(at + pl * L::PLANE_BYTES, map, pl * 128, now.row, full0 + 8 * stage);
                 }
                 used++;
                 if (++stage == a.stages) { stage = 0; phase ^= 1u; }
@@ -360,336 +405,366 @@ __global__ void __launch_bounds__(THREADS, Shape<T, D, R>::PER_SM) attention_q8_
             resolve();
         }
         if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);    // copies in flight end before the CTA's shared memory is another's
-        return;
-    }
-
-    // ---- consumers ------------------------------------------------------------------------------------------------------------------
-    const int g = lane >> 2, c = lane & 3;
-    Walk walk(a, cum, u0, u1, ROWS);
-    Segment s;
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    const float inf = __int_as_float(0x7f800000);
-    while (walk.next(s)) {
-        const int rows = min(ROWS, s.x.n * a.G - s.rg * ROWS);            // of this row group
-        uint4 qf[QREG ? SETS * KS : 1];
-        float fac[NR], B[NR], l[NR];
-        int hi[NR], lo[NR];
-        float acc[PM][NT][4];
-        int min_hi = 0x7fffffff, max_lo = 0;
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const int row = g + 8 * i, rho = s.rg * ROWS + row;
-            const int query = min(rho / a.G, s.x.n - 1), at = s.x.seq - s.x.n + query;
-            hi[i] = a.causal ? at : s.x.seq - 1;
-            lo[i] = a.window > 0 ? at - a.window + 1 : 0;
-            min_hi = min(min_hi, hi[i]);
-            max_lo = max(max_lo, lo[i]);
-            B[i] = -inf;
-            l[i] = 0.f;
-        }
-        min_hi = __reduce_min_sync(0xffffffffu, min_hi);
-        max_lo = __reduce_max_sync(0xffffffffu, max_lo);
-        // Q: the row's largest magnitude, the digits.  Element order inside a step is the codes' order in memory: step k of lane column c is
-        // elements 8 (k & 1) ... + 8 of its (k / 2)-th piece.
-        const auto load_rows = [&](int i, uint4 *dst, int stride) {
-            const int row = g + 8 * i, rho = s.rg * ROWS + row, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
-            const bool there = row < rows;
-            const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
-            float4 v[KS][2];
-            float amax = 0.f;
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int d = L::qk_plane(k >> 1) * 128 + L::qk_piece(c, k >> 1) * 16 + (k & 1) * 8 + e * 4;
-                    v[k][e] = there ? load4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else if (warp == 7) {
+        // ---- queries: the next pair's, while the others are at one --------------------------------------------------------------------------
+        constexpr int LPR = D == 64 ? 16 : 32, RPW = 32 / LPR, PER = D == 256 ? 2 : 1;         // lanes to a row, rows at a time, words of four of a lane
+        Walk walk(a, cum, u0, u1, R);
+        Segment s;
+        for (int k = 0;; k++) {
+            const bool more = walk.next(s);
+            if (k >= 2 && !wait_idle(Q_EMPTY + 8 * (k & 1), (k / 2 - 1) & 1)) give_up(3u);
+            if (!ok) break;
+            if (lane == 0) {
+                Work &w = works[k % WORKS];
+                w.tiles = more ? s.tiles : 0;
+                if (more) {
+                    const int q0 = s.x.seq - s.x.n + s.rg * R / a.G, q1 = s.x.seq - s.x.n + min(s.rg * R + R - 1, s.x.n * a.G - 1) / a.G;
+                    w.min_hi = a.causal ? min(q0, s.x.seq - 1) : s.x.seq - 1; w.max_lo = a.window > 0 ? max(0, q1 - a.window + 1) : 0;
+                    w.tile0 = s.x.lo / TK + s.tile; w.n = s.x.n; w.q0 = s.x.q0; w.rg = s.rg; w.h = s.h;
+                    w.first = s.tile == 0; w.pair0 = s.pair0; w.pair_tiles = s.pair_tiles;
                 }
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[k][e].x), fabsf(v[k][e].y))), fmaxf(fabsf(v[k][e].z), fabsf(v[k][e].w)));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // the row in units of its last digit: amax becomes 127 * 128^2; by a power of two first, so that neither factor leaves fp32
-            constexpr float top = 127.f * 16384.f;
-            const float p2 = row_factor(amax), f = amax > 0.f ? top / (amax * p2) : 1.f;
-            float bad = 0.f;                                           // NaN if an element is not a number or infinite: the digits cannot tell
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float4 &x = v[k][e];
-                    bad += (x.x * 0.f + x.y * 0.f) + (x.z * 0.f + x.w * 0.f);
-                    x.x = x.x * p2 * f; x.y = x.y * p2 * f; x.z = x.z * p2 * f; x.w = x.w * p2 * f;
-                }
-            bad += __shfl_xor_sync(0xffffffffu, bad, 1);
-            bad += __shfl_xor_sync(0xffffffffu, bad, 2);
-            const float back = a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad;
-            if constexpr (QREG) fac[i] = back;
-            else if (c == 0) row_fac[row] = back;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const uint32_t a0 = digit4(v[k][0], 16384.f, 1.f / 16384.f), a2 = digit4(v[k][1], 16384.f, 1.f / 16384.f);
-                const uint32_t a1 = digit4(v[k][0], 128.f, 1.f / 128.f), a3 = digit4(v[k][1], 128.f, 1.f / 128.f);
-                dst[(i * KS + k) * stride] = make_uint4(a0, a1, a2, a3);
-                const uint32_t b0 = digit4(v[k][0], 1.f, 1.f), b1 = digit4(v[k][1], 1.f, 1.f);
-                uint32_t *third = reinterpret_cast<uint32_t *>(dst + ((NR + (i >> 1)) * KS + k) * stride);
-                third[i & 1] = b0;                                     // row g: first of the pairs, row g + 8: second
-                third[2 + (i & 1)] = b1;
-                if (NR == 1) { third[1] = 0u; third[3] = 0u; }
             }
-        };
-        if constexpr (QREG) {
+            if (more) {
+                const int rows = min(R, s.x.n * a.G - s.rg * R), sub = lane / LPR, col = lane % LPR;
+                unsigned char *to = qs + (k & 1) * S::QB;
+#pragma unroll 2
+                for (int r0 = 0; r0 < R; r0 += RPW) {
+                    const int r = r0 + sub;
+                    if (r0 >= rows && k >= 2) break;                             // (rows of an earlier segment: what they give is not read)
+                    const int rho = s.rg * R + min(r, rows - 1), query = rho / a.G, head = s.h * a.G + rho - query * a.G;
+                    const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
+                    float4 v[PER];
+                    float amax = 0.f, bad = 0.f;
 #pragma unroll
-            for (int i = 0; i < NR; i++) load_rows(i, qf, 1);
-        } else {
-            if (warp < NR) load_rows(warp, qs + lane, 32);
-            asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
-#pragma unroll
-            for (int i = 0; i < NR; i++) fac[i] = row_fac[g + 8 * i];
-        }
-
-#pragma unroll
-        for (int mt = 0; mt < PM; mt++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[mt][j][0] = acc[mt][j][1] = acc[mt][j][2] = acc[mt][j][3] = 0.f;
-        for (int t = 0; t < s.tiles; t++) {
-            if (ok && !ptx::mbar_wait_warp(FULL(stage), phase)) { if (lane == 0) dev_set_error(ERR_WAIT | 2u); ok = false; }
-            const int key0 = (s.x.lo / TK + s.tile + t) * TK + warp * 16;
-            if (ok && key0 < s.x.seq && key0 + 16 > s.x.lo) {
-                const uint32_t kt = ring_at + (uint32_t)stage * (uint32_t)S::STAGE_BYTES, vt = kt + L::BYTES;
-                const float4 sc = lds_f4(scales_at + (stage * SLOT_SCALES + ((warp * 16) >> pshift)) * 16);
-                int dot[SETS][2][4];
-#pragma unroll
-                for (int mt = 0; mt < SETS; mt++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) dot[mt][i][0] = dot[mt][i][1] = dot[mt][i][2] = dot[mt][i][3] = 0;
-#pragma unroll
-                for (int pq = 0; pq < L::STEPS; pq++) {
-                    uint4 w[2];
-#pragma unroll
-                    for (int i = 0; i < 2; i++) w[i] = lds128(kt + L::piece(warp * 16 + L::token(i, g), L::qk_piece(c, pq), L::qk_plane(pq)));
-#pragma unroll
-                    for (int mt = 0; mt < SETS; mt++)
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            uint4 qa;
-                            if constexpr (QREG) qa = qf[mt * KS + pq * 2 + k];
-                            else qa = qs[(mt * KS + pq * 2 + k) * 32 + lane];
-#pragma unroll
-                            for (int i = 0; i < 2; i++) mma_s8(dot[mt][i], qa, k ? w[i].z : w[i].x, k ? w[i].w : w[i].y);
-                        }
-                }
-                // scores in base 2, weights
-                const bool edge = key0 + 15 > min_hi || key0 < max_lo || key0 + 15 >= s.x.seq;
-                float x[NR][4];
-                bool again = false;
-                const auto scores = [&](int i, float (&y)[4]) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float d = fmaf((float)dot[i][e >> 1][e & 1], 16384.f,
-                                             (float)(dot[i][e >> 1][2 + (e & 1)] * 128 + dot[NR + (i >> 1)][e >> 1][2 * (i & 1) + (e & 1)]));
-                        y[e] = d;
+                    for (int e = 0; e < PER; e++) {
+                        v[e] = r < rows ? load4(src + 4 * (col + 32 * e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[e].x), fabsf(v[e].y))), fmaxf(fabsf(v[e].z), fabsf(v[e].w)));
+                        bad += (v[e].x * 0.f + v[e].y * 0.f) + (v[e].z * 0.f + v[e].w * 0.f);      // NaN if one is not a number or infinite: digits cannot tell
                     }
-                    const float f = fac[i] * sc.x;
-                    if (a.softcap > 0.f) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = capped(y[e] * f, a.softcap) + sc.y;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = fmaf(y[e], f, sc.y);
+                    for (int o = LPR / 2; o > 0; o >>= 1) {
+                        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        bad += __shfl_xor_sync(0xffffffffu, bad, o);
                     }
-                    if (edge) {
+                    // the row in units of its last digit: amax becomes 127 * 256^2; by a power of two first, so that neither factor leaves fp32
+                    const float p2 = row_factor(amax), f = amax > 0.f ? 127.f * 65536.f / (amax * p2) : 1.f;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int key = key0 + L::token(e >> 1, 2 * c + (e & 1));
-                            if (key > hi[i] || key < lo[i] || key >= s.x.seq) y[e] = -inf;
+                    for (int e = 0; e < PER; e++) {
+                        const float y[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+                        uint32_t w[4];
+#pragma unroll
+                        for (int m = 0; m < 4; m++) w[m] = (uint32_t)(__float2int_rn(y[m] * p2 * f) + 0x8080) ^ 0x8080u;     // signed digits in bytes 2, 1, 0
+                        const int d = 4 * col;                                   // of plane e
+#pragma unroll
+                        for (int g = 0; g < 3; g++) {
+                            const int n = 3 * r + g;
+                            const uint32_t sel = g == 0 ? 0x0062u : g == 1 ? 0x0051u : 0x0040u;
+                            const uint32_t word = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
+                            const int at = D == 64 ? n * 64 + (((d >> 4) ^ ((n >> 1) & 3)) << 4) + (d & 15) : e * N * 128 + n * 128 + (((d >> 4) ^ (n & 7)) << 4) + (d & 15);
+                            if (r < R) *reinterpret_cast<uint32_t *>(to + at) = word;
                         }
                     }
-                };
-                float top[NR];
-#pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    scores(i, x[i]);
-                    top[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
-                    again = again || top[i] > B[i] + 15.f;
-                }
-                if (__any_sync(0xffffffffu, again)) {
-                    // a weight would pass 2^15: the rows' references move to where their largest is 2^8
-#pragma unroll
-                    for (int i = 0; i < NR; i++) {
-                        float m = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                        const float now = m > B[i] + 8.f ? m - 8.f : B[i];
-                        const float shrink = B[i] == -inf ? 1.f : ex2(B[i] - now);        // nothing is summed while B is -inf
-                        B[i] = now;
-                        l[i] *= shrink;
-#pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            if constexpr (SPLIT) { acc[i][j][0] *= shrink; acc[i][j][1] *= shrink; acc[i][j][2] *= shrink; acc[i][j][3] *= shrink; }
-                            else { acc[i >> 1][j][2 * (i & 1)] *= shrink; acc[i >> 1][j][2 * (i & 1) + 1] *= shrink; }
-                        }
+                    if (col == 0 && r < R) {
+                        const int pos = s.x.seq - s.x.n + query;
+                        rec[(k & 1) * R + r] = make_float4(a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
+                                                           __int_as_float(a.causal ? min(pos, s.x.seq - 1) : s.x.seq - 1),
+                                                           __int_as_float(a.window > 0 ? max(0, pos - a.window + 1) : 0));
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    const float ref = B[i] == -inf ? 0.f : B[i];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[i][e] = edge && x[i][e] == -inf ? 0.f : ex2(x[i][e] - ref);
-                    l[i] = fmaf((x[i][0] + x[i][1]) + (x[i][2] + x[i][3]), sc.z, l[i]);
-                }
-                if (sc.w != 0.f) {
-#pragma unroll
-                    for (int i = 0; i < NR; i++) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-                }
-                uint4 pa[PM];
-#pragma unroll
-                for (int mt = 0; mt < PM; mt++) {
-                    const int i = SPLIT ? mt : 2 * mt;
-                    const __half2 h0 = __floats2half2_rn(x[i][0], x[i][1]), h1 = __floats2half2_rn(x[i][2], x[i][3]);
-                    if constexpr (SPLIT) {
-                        const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                        pa[mt] = make_uint4(h2_bits(h0), h2_bits(__floats2half2_rn(x[i][0] - f0.x, x[i][1] - f0.y)),
-                                            h2_bits(h1), h2_bits(__floats2half2_rn(x[i][2] - f1.x, x[i][3] - f1.y)));
-                    } else {
-                        constexpr int o = NR > 1 ? 1 : 0;
-                        pa[mt] = make_uint4(h2_bits(h0), o ? h2_bits(__floats2half2_rn(x[i + o][0], x[i + o][1])) : 0u,
-                                            h2_bits(h1), o ? h2_bits(__floats2half2_rn(x[i + o][2], x[i + o][3])) : 0u);
-                    }
-                }
-                // values: lane row g holds the 16 (dim 64: 8) elements of a piece, one for each group of eight columns
-#pragma unroll
-                for (int pl = 0; pl < L::PLANES; pl++) {
-                    uint32_t v[4][4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int tok = warp * 16 + L::token(k >> 1, 2 * c + (k & 1));
-                        if constexpr (D == 64) {
-                            const uint2 w = lds64(vt + L::piece(tok, g >> 1, 0) + (g & 1) * 8);
-                            v[k][0] = w.x; v[k][1] = w.y;
-                        } else {
-                            const uint4 w = lds128(vt + L::piece(tok, g, pl));
-                            v[k][0] = w.x; v[k][1] = w.y; v[k][2] = w.z; v[k][3] = w.w;
-                        }
-                    }
-#pragma unroll
-                    for (int w = 0; w < (D == 64 ? 2 : 4); w++) {
-                        const uint32_t a0 = v[0][w] ^ 0x80808080u, a1 = v[1][w] ^ 0x80808080u, a2 = v[2][w] ^ 0x80808080u, a3 = v[3][w] ^ 0x80808080u;
-                        const uint32_t e0 = __byte_perm(a0, a1, 0x5140), o0 = __byte_perm(a0, a1, 0x7362);
-                        const uint32_t e1 = __byte_perm(a2, a3, 0x5140), o1 = __byte_perm(a2, a3, 0x7362);
-                        const uint32_t b[4][2] = {{codes_f16<0x4140>(e0), codes_f16<0x4140>(e1)}, {codes_f16<0x4342>(e0), codes_f16<0x4342>(e1)},
-                                                  {codes_f16<0x4140>(o0), codes_f16<0x4140>(o1)}, {codes_f16<0x4342>(o0), codes_f16<0x4342>(o1)}};
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int mt = 0; mt < PM; mt++) mma_f16(acc[mt][pl * 16 + w * 4 + j], pa[mt], b[j][0], b[j][1]);
-                    }
-                }
+                ptx::fence_proxy_async_smem();
             }
             __syncwarp();
-            if (ok && lane == 0) ptx::mbar_arrive(EMPTY(stage));
-            if (++stage == a.stages) { stage = 0; phase ^= 1u; }
+            if (lane == 0) ptx::mbar_arrive(Q_FULL + 8 * (k & 1));
+            if (!more) break;
         }
-
-        // ---- the warps meet --------------------------------------------------------------------------------------------------------
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (c == 0) ml[warp * ROWS + g + 8 * i] = make_float2(B[i], l[i]);
-        }
-        asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const int row = g + 8 * i;
-            float top = ml[row].x;
-#pragma unroll
-            for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w * ROWS + row].x);
-            const float f = B[i] == -inf ? 0.f : ex2(B[i] - top);
-            float4 *dst = reinterpret_cast<float4 *>(meet + ((size_t)warp * ROWS + row) * D);
-            if (row < rows) {
-#pragma unroll
-                for (int pl = 0; pl < L::PLANES; pl++)
-#pragma unroll
-                    for (int half = 0; half < 2; half++)
-#pragma unroll
-                        for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
-                            float o[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float *q4 = acc[SPLIT ? i : i >> 1][pl * 16 + 4 * k + e];
-                                o[e] = (SPLIT ? q4[half] + q4[2 + half] : q4[2 * (i & 1) + half]) * f;
-                            }
-                            const int f4 = D == 64 ? 4 * c + 2 * half + k : 32 * pl + 8 * c + 4 * half + k;
-                            dst[meet_pos<D>(f4, row)] = make_float4(o[0], o[1], o[2], o[3]);
-                        }
-            }
-        }
-        asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
-        const bool whole = s.tiles == s.pair_tiles;
-        const int slot = 2 * (int)cta + (s.tile == 0 ? 1 : 0);
-        const auto finish = [&](int row, int f4, float4 v, float top, float sum) {     // v: the weighted values, sum: the weights'
-            const int rho = s.rg * ROWS + row, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // nothing seen: zeros
-            v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-            store4(static_cast<T *>(a.out) + (long long)(s.x.q0 + query) * a.ldo + (long long)head * D + 4 * f4, v);
-            if (a.lse && f4 == 0) a.lse[(size_t)(s.x.q0 + query) * a.Hq + head] = sum > 0.f ? (top + log2f(sum)) * LN2 : (sum == 0.f ? -inf : sum);
+    } else if (warp == 6) {
+        // ---- products: S of a tile, then PV of the tile before it ---------------------------------------------------------------------------------
+        const uint32_t lead = elected();
+        constexpr uint32_t id_s = idesc_s8(N, 0), id_o = idesc_s8(D == 64 ? 2 * NP : NP, 1);
+        int st = 0, pst = 0;
+        uint32_t ph = 0, pph = 0;
+        unsigned j = 0;
+        const auto wait = [&](uint32_t b, uint32_t parity, unsigned code) {
+            if (ok && !wait_warp(b, parity)) give_up(code);
+            ptx::tc_fence_after_sync();
+            return ok;
         };
-        for (int e = tid; e < rows * (D / 4); e += CW * 32) {
-            const int row = e / (D / 4), f4 = e - row * (D / 4);
-            float top = ml[row].x, sum = 0.f;
+        const auto values = [&](unsigned i) {                        // PV of tile i
+            const uint32_t buf = i & 1;
+            if (!wait(P_FULL + 8 * buf, (i >> 1) & 1, 4u) || !wait(V_FULL + 8 * pst, pph, 5u)) return;
+            const uint32_t begin = fresh[buf] != 0, vb = ring_at + pst * S::STAGE + L::BYTES, pb = p_at + buf * S::PB;
 #pragma unroll
-            for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w * ROWS + row].x);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int pl = 0; pl < DP; pl++)
 #pragma unroll
-            for (int w = 0; w < CW; w++) {
-                const float2 x = ml[w * ROWS + row];
-                const float4 o = reinterpret_cast<const float4 *>(meet + ((size_t)w * ROWS + row) * D)[meet_pos<D>(f4, row)];
-                sum += x.x == -inf ? 0.f : x.y * ex2(x.x - top);
-                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-            }
-            if (whole) finish(row, f4, v, top, sum);
-            else {
-                reinterpret_cast<float4 *>(a.part + ((size_t)slot * ROWS + row) * D)[f4] = v;
-                if (f4 == 0) a.part_ml[(size_t)slot * ROWS + row] = make_float2(top, sum);
-            }
-        }
-        if (whole) continue;
-        // ---- the CTAs that share the pair meet: the last to come joins, in the order of the ranges ----------------------------------------
-        const unsigned c0 = cta_of((unsigned)s.pair0), c1 = cta_of((unsigned)(s.pair0 + s.pair_tiles - 1));
-        __threadfence();
-        asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
-        if (tid == 0) {
-            const unsigned seen = atomicAdd(a.count + c0, 1u);
-            last_flag = seen == c1 - c0;
-            if (seen == c1 - c0) a.count[c0] = 0u;                 // as the next call expects it
-        }
-        asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");
-        if (last_flag) {
-            __threadfence();
-            for (int e = tid; e < rows * (D / 4); e += CW * 32) {
-                const int row = e / (D / 4), f4 = e - row * (D / 4);
-                float top = -inf, sum = 0.f;
-                const auto at = [&](unsigned k) { return (size_t)(2 * k + (k == c0 ? 1 : 0)) * ROWS + row; };
-#pragma unroll 4
-                for (unsigned k = c0; k <= c1; k++) top = fmaxf(top, __ldcg(&a.part_ml[at(k)]).x);
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (unsigned k = c0; k <= c1; k++) {
-                    const float2 x = __ldcg(&a.part_ml[at(k)]);
-                    const float4 o = __ldcg(reinterpret_cast<const float4 *>(a.part + at(k) * D) + f4);
-                    const float f = x.x == -inf ? 0.f : ex2(x.x - top);
-                    sum += x.y * f;
-                    v.x += o.x * f; v.y += o.y * f; v.z += o.z * f; v.w += o.w * f;
+                for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
+                    const uint64_t vd = desc_mn(vb + pl * L::PLANE_BYTES + k * 32 * 128);
+                    const uint64_t pd = D == 64 ? desc_k<64>(pb) + (uint64_t)(2 * k) : desc_k<128>(pb) + (uint64_t)(2 * k);
+                    umma_s8(lead, o_cols + pl * NP, vd, pd, id_o, k > 0 || !begin);
                 }
-                finish(row, f4, v, top, sum);
+            umma_commit(lead, EMPTY + 8 * pst);
+            umma_commit(lead, P_EMPTY + 8 * buf);
+            if (++pst == a.stages) { pst = 0; pph ^= 1u; }
+        };
+        for (int nth = 0; ok; nth++) {
+            if (!wait(Q_FULL + 8 * (nth & 1), (nth >> 1) & 1, 6u)) break;
+            const int tiles = works[nth % WORKS].tiles;
+            if (tiles == 0) break;
+            for (int t = 0; t < tiles && ok; t++, j++) {
+                const uint32_t buf = j & 1, kb = ring_at + st * S::STAGE, qb = q_at + (nth & 1) * S::QB;
+                if (!wait(K_FULL + 8 * st, ph, 7u)) break;
+                if (j >= 2 && !wait(S_EMPTY + 8 * buf, ((j >> 1) - 1) & 1, 8u)) break;
+#pragma unroll
+                for (int k = 0; k < D / 32; k++) {
+                    const uint64_t kd = D == 64 ? desc_k<64>(kb) + (uint64_t)(2 * k) : desc_k<128>(kb + (k >> 2) * L::PLANE_BYTES) + (uint64_t)(2 * (k & 3));
+                    const uint64_t qd = D == 64 ? desc_k<64>(qb) + (uint64_t)(2 * k) : desc_k<128>(qb + (k >> 2) * N * 128) + (uint64_t)(2 * (k & 3));
+                    umma_s8(lead, tmem + buf * N, kd, qd, id_s, k > 0);
+                }
+                umma_commit(lead, S_FULL + 8 * buf);
+                if (t == tiles - 1) umma_commit(lead, Q_EMPTY + 8 * (nth & 1));
+                if (++st == a.stages) { st = 0; ph ^= 1u; }
+                if (j > 0) values(j - 1);
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"r"(CW * 32) : "memory");          // last_flag has been read
+        if (ok && j > 0) values(j - 1);
+        if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
+    } else {
+        // ---- thread = key: scores to weights; thread = dim: O --------------------------------------------------------------------------------------
+        const uint32_t lanes = (uint32_t)warp << 21;
+        const int parity = D == 64 ? tid >> 6 : 0;
+        unsigned j = 0;
+        int st = 0;
+        uint32_t ph = 0;
+        float l[R], acc[DP][R], fac[R], B[R];
+        const auto sync = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        // Is it so for any of the 128 threads?  A wait that ran out for one warp is everybody's to know: they leave together.
+        const auto vote = [&](bool mine) {
+            int any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any) : "r"((int)mine) : "memory");
+            return any != 0;
+        };
+        // O of the tiles since it was last read, in units of 2^B
+        const auto read_o = [&]() {
+            const uint32_t i = j - 1;                                              // the last tile whose PV is in it
+            if (ok && !wait_warp(P_EMPTY + 8 * (i & 1), (i >> 1) & 1)) give_up(9u);
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int pl = 0; pl < DP; pl++) {
+                int v[NP];
+                tmem_columns<NP>(o_cols + lanes + pl * NP + parity * NP, v);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    acc[pl][r] += fmaf((float)v[4 * r], 16777216.f, fmaf((float)v[4 * r + 1], 65536.f, fmaf((float)v[4 * r + 2], 256.f, (float)v[4 * r + 3])));
+            }
+            ptx::tc_fence_before_sync();
+        };
+        for (int nth = 0;; nth++) {
+            if (ok && !wait_warp(Q_FULL + 8 * (nth & 1), (nth >> 1) & 1)) give_up(10u);
+            if (vote(!ok)) break;
+            const Work w = works[nth % WORKS];
+            if (w.tiles == 0) break;
+            const int row0 = w.rg * R, rows = min(R, w.n * a.G - row0);
+            float4 *rc = rec + (nth & 1) * R;
+            bool since = false;                                                     // O holds tiles of this segment that have not been read
+            int held = 0;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                l[r] = 0.f;
+                fac[r] = rc[r].x;
+                B[r] = -inf;
+#pragma unroll
+                for (int pl = 0; pl < DP; pl++) acc[pl][r] = 0.f;
+            }
+            for (int t = 0; t < w.tiles; t++, j++) {
+                const uint32_t buf = j & 1;
+                const int key = (w.tile0 + t) * TK + tid;
+                if (ok && !wait_warp(S_FULL + 8 * buf, (j >> 1) & 1)) give_up(11u);
+                if (ok && !wait_warp(K_FULL + 8 * st, ph)) give_up(12u);             // (passed; the stage's scales are what the barrier's phase shows)
+                ptx::tc_fence_after_sync();
+                int v[N];
+                tmem_columns<N>(tmem + lanes + buf * N, v);
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(S_EMPTY + 8 * buf);
+                const float4 sc = scales[st * S::SCALES + (tid >> tshift)];
+                // rows that the segment does not have go along: they are not read
+                float y[R];
+                bool again = held >= FLUSH;
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float s = fmaf((float)v[3 * r], 65536.f, (float)(v[3 * r + 1] * 256 + v[3 * r + 2]));
+                    y[r] = fmaf(s, fac[r] * sc.x, sc.y);
+                }
+                if (a.softcap > 0.f) {
+#pragma unroll
+                    for (int r = 0; r < R; r++) y[r] = capped(y[r] - sc.y, a.softcap) + sc.y;
+                }
+                if (key - tid + TK - 1 > w.min_hi || key - tid < w.max_lo) {
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        if (key > __float_as_int(rc[r].z) || key < __float_as_int(rc[r].w)) y[r] = -inf;
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++) again = again || y[r] > B[r] + LIMIT;
+                if (vote(again || !ok)) {
+                    if (vote(!ok)) { ok = false; break; }
+                    // a weight would pass 2^31: B moves to where the row's largest is 2^28; what is summed, to the new B
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        float m = y[r];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        if (lane == 0) red[warp * R + r] = m;
+                    }
+                    if (since) read_o();
+                    sync();
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float m = fmaxf(fmaxf(red[r], red[R + r]), fmaxf(red[2 * R + r], red[3 * R + r]));
+                        const float now = m > B[r] + TOP ? m - TOP : B[r];
+                        const float shrink = B[r] == -inf || now == B[r] ? 1.f : ex2(B[r] - now);   // nothing is summed while B is -inf
+                        B[r] = now;
+                        l[r] *= shrink;
+#pragma unroll
+                        for (int pl = 0; pl < DP; pl++) acc[pl][r] *= shrink;
+                    }
+                    sync();
+                    since = false;
+                    held = 0;
+                }
+                if (j >= 2 && ok && !wait_warp(P_EMPTY + 8 * buf, ((j >> 1) - 1) & 1)) give_up(13u);
+                if (tid == 0) fresh[buf] = !since;
+                since = true;
+                held++;
+                unsigned char *to = ps + buf * S::PB;
+                const int pc = D == 64 ? tid >> 1 : tid;                               // column of P
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float x = ex2(y[r] - (B[r] == -inf ? 0.f : B[r]));            // a masked score is -inf: 0
+                    l[r] = fmaf(x, sc.z, l[r]);
+                    const uint32_t n = (__float2uint_rn(x) + 0x808080u) ^ 0x808080u;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const int row = 4 * r + g;                                      // dim 64: NP is a multiple of 8, so the odd tokens' rows swizzle alike
+                        const int at = D == 64 ? row * 64 + (((pc >> 4) ^ ((row >> 1) & 3)) << 4) : row * 128 + (((pc >> 4) ^ (row & 7)) << 4);
+                        to[at + (D == 64 ? (tid & 1) * NP * 64 : 0) + (pc & 15)] = (unsigned char)(n >> (24 - 8 * g));
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(P_FULL + 8 * buf);
+                if (++st == a.stages) { st = 0; ph ^= 1u; }
+            }
+            if (vote(!ok)) break;
+            // ---- the pair's rows, or the partial sums of a part of it, out -------------------------------------------------------------------------
+            read_o();
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float sum = l[r];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0) red[warp * R + r] = sum;
+                if (D == 64 && parity == 1) fold[r * 64 + (tid & 63)] = acc[0][r];
+            }
+            sync();
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                l[r] = (red[r] + red[R + r]) + (red[2 * R + r] + red[3 * R + r]);
+                if (D == 64 && parity == 0) acc[0][r] += fold[r * 64 + tid];
+            }
+            sync();                                                                 // red and fold have been read
+            if (lane == 0) ptx::mbar_arrive(Q_EMPTY + 8 * (nth & 1));
+            const bool whole = w.tiles == w.pair_tiles, writes = D != 64 || tid < 64;
+            const auto finish = [&](int r, int pl, float v, float top, float sum) {     // v: a weighted value, sum: the weights'
+                const int rho = row0 + r, query = rho / a.G, head = w.h * a.G + rho - query * a.G;
+                const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // nothing seen: zeros
+                static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + tid] = out_round(T(), sum == 0.f ? 0.f : v * inv);
+                if (a.lse && tid == 0 && pl == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = sum > 0.f ? (top + log2f(sum)) * LN2 : (sum == 0.f ? -inf : sum);
+            };
+            if (whole) {
+                if (writes)
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        if (r < rows)
+#pragma unroll
+                            for (int pl = 0; pl < DP; pl++) finish(r, pl, acc[pl][r], B[r], l[r]);
+                continue;
+            }
+            const size_t slot = (size_t)(2 * cta + (w.first ? 1 : 0)) * MAX_ROWS;
+            if (writes)
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (r < rows) {
+#pragma unroll
+                        for (int pl = 0; pl < DP; pl++) a.part[(slot + r) * D + pl * 128 + tid] = acc[pl][r];
+                        if (tid == 0) a.part_ml[slot + r] = make_float2(B[r], l[r]);
+                    }
+            // ---- the CTAs that share the pair meet: FAN neighbours first, then the groups; the last to come joins, in the order of the ranges ----------------
+            const unsigned c0 = cta_of((unsigned)w.pair0), c1 = cta_of((unsigned)(w.pair0 + w.pair_tiles - 1)), groups = (c1 - c0) / FAN + 1;
+            const auto slot_of = [&](unsigned k) { return 2 * k + (k == c0 ? 1 : 0); };
+            const auto last_of = [&](unsigned *counter, unsigned n) {      // has everybody written?  What was written before is visible then.
+                __threadfence();
+                sync();
+                if (tid == 0) {
+                    const unsigned seen = atomicAdd(counter, 1u);
+                    last_flag = seen == n - 1;
+                    if (seen == n - 1) *counter = 0u;                      // as the next call expects it
+                }
+                sync();
+                const bool last = last_flag;
+                sync();
+                if (last) __threadfence();
+                return last;
+            };
+            const auto join = [&](const float2 *pml, const float *pv, unsigned first, unsigned step, unsigned n, auto &&out) {
+                if (!writes) return;
+#pragma unroll 1
+                for (int e = 0; e < rows * DP; e++) {
+                    const int r = e / DP, pl = e % DP;
+                    float top = -inf, sum = 0.f, v = 0.f;
+#pragma unroll 1
+                    for (unsigned i0 = 0; i0 < n; i0 += 8) {               // eight loads of each kind in flight
+                        float2 x[8];
+                        float o[8];
+#pragma unroll
+                        for (unsigned i = 0; i < 8; i++) {
+                            const size_t at = (size_t)slot_of(first + (i0 + i < n ? i0 + i : 0) * step) * MAX_ROWS + r;
+                            x[i] = __ldcg(pml + at);
+                            o[i] = __ldcg(pv + at * D + pl * 128 + tid);
+                            if (i0 + i >= n) x[i] = make_float2(-inf, 0.f);
+                        }
+                        float m = top;
+#pragma unroll
+                        for (unsigned i = 0; i < 8; i++) m = fmaxf(m, x[i].x);
+                        const float back = top == -inf ? 1.f : ex2(top - m);
+                        top = m;
+                        sum *= back;
+                        v *= back;
+#pragma unroll
+                        for (unsigned i = 0; i < 8; i++) {
+                            if (x[i].x == -inf && x[i].y == 0.f) continue;
+                            const float f = x[i].x == -inf ? 1.f : ex2(x[i].x - top);            // -inf and a sum: not a number
+                            sum += x[i].y * f;
+                            v += o[i] * f;
+                        }
+                    }
+                    out(r, pl, v, top, sum);
+                }
+            };
+            const unsigned g0 = c0 + (cta - c0) / FAN * FAN, in_group = min((unsigned)FAN, c1 - g0 + 1);
+            if (!last_of(a.count + slot_of(g0), in_group)) continue;
+            if (groups == 1) { join(a.part_ml, a.part, g0, 1, in_group, finish); continue; }
+            join(a.part_ml, a.part, g0, 1, in_group, [&](int r, int pl, float v, float top, float sum) {
+                const size_t at = (size_t)slot_of(g0) * MAX_ROWS + r;
+                a.part2[at * D + pl * 128 + tid] = v;
+                if (tid == 0 && pl == 0) a.part2_ml[at] = make_float2(top, sum);
+            });
+            if (last_of(a.count2 + slot_of(c0), groups)) join(a.part2_ml, a.part2, c0, FAN, groups, finish);
+        }
     }
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    if (warp == 6) ptx::tmem_dealloc(tmem, 512);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
@@ -699,67 +774,65 @@ struct Call {
     int dtype, dim;
 };
 
-// Workspace: the arrival counts, then the partial results of 2 ranges' ends per CTA.  32 rows at most.
-constexpr int MAX_CTAS_PER_SM = 3, MAX_ROWS = 32;
-inline size_t count_bytes() { return ((size_t)sm_count() * MAX_CTAS_PER_SM * 4 + 255) & ~(size_t)255; }
-inline size_t workspace_bytes(int dim) {
-    const size_t slots = (size_t)sm_count() * MAX_CTAS_PER_SM * 2;
-    return count_bytes() + slots * MAX_ROWS * 8 + slots * MAX_ROWS * dim * 4;
+// Workspace: the arrival counts, then the partial results of two ends of each CTA's range and of the groups of CTAs.
+inline size_t ends() { return (size_t)sm_count() * 2; }
+inline size_t count_bytes() { return (2 * ends() * 4 + 255) & ~(size_t)255; }
+inline size_t workspace_bytes(int dim) { return count_bytes() + 2 * ends() * MAX_ROWS * (8 + (size_t)dim * 4); }
+inline void lay_out(Args &a, void *workspace, int dim) {
+    unsigned char *p = static_cast<unsigned char *>(workspace);
+    a.count = reinterpret_cast<unsigned *>(p);
+    a.count2 = a.count + ends();
+    a.part_ml = reinterpret_cast<float2 *>(p + count_bytes());
+    a.part2_ml = a.part_ml + ends() * MAX_ROWS;
+    a.part = reinterpret_cast<float *>(a.part2_ml + ends() * MAX_ROWS);
+    a.part2 = a.part + ends() * MAX_ROWS * dim;
 }
 
 template <typename T, int D, int R>
-inline int launch_t(Call &c, cudaStream_t st) {
-    using S = Shape<T, D, R>;
-    Args &a = c.a;
-    constexpr int per_sm = S::PER_SM;
-    a.stages = S::stages(a.R);
-    const size_t smem = S::fixed_bytes(a.R) + a.stages * S::STAGE_BYTES;
+inline int launch_t(const Call &c, cudaStream_t st) {
+    using S = Shape<D, R>;
     auto kern = attention_q8_kernel<T, D, R>;
-    static PerDevice<size_t> configured_dev;
-    size_t &configured = configured_dev.get();
-    if (smem > configured) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return cuda_fail(e, "attention_q8 smem opt-in");
-        configured = smem;
-    }
-    const uint64_t row = D == 256 ? 256 : 128, rows = (uint64_t)a.num_blocks * a.Hkv * a.block * D / row;
-    const uint32_t box = (uint32_t)((a.block < TK ? a.block : TK) / Tile<D>::ROW_TOKENS);
+    const uint64_t tokens = (uint64_t)c.a.num_blocks * c.a.Hkv * c.a.block;
+    const uint32_t box = (uint32_t)(c.a.block < TK ? c.a.block : TK);
     CUtensorMap mk, mv;
-    int rc = tmap_cached(&mk, c.k, row, rows, 128, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
-    if (rc == W4A8_OK) rc = tmap_cached(&mv, c.v, row, rows, 128, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    int rc = tmap_cached(&mk, c.k, D, tokens, D == 64 ? 64 : 128, box, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    if (rc == W4A8_OK)
+        rc = tmap_cached(&mv, c.v, D == 64 ? 128 : D, D == 64 ? tokens / 2 : tokens, 128, D == 64 ? box / 2 : box, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != W4A8_OK) return rc;
-    const int sms = sm_count();
-    cudaError_t e = launch_pdl(kern, dim3(sms * per_sm), dim3(THREADS), smem, st, mk, mv, a);
-    return e == cudaSuccess ? launch_status("attention_q8") : cuda_fail(e, "attention_q8 launch");
-}
-
-template <typename T, int D>
-inline int launch_r(Call &c, int rows, cudaStream_t st) {
-    constexpr int most = (std::is_same<T, float>::value ? 8 : 16) * (D == 256 ? 1 : 2);     // the registers' limit
-    if (rows <= 8) return launch_t<T, D, 8>(c, st);
-    if (rows <= 16 || most == 16) return launch_t<T, D, most < 16 ? most : 16>(c, st);
-    return launch_t<T, D, most>(c, st);
-}
-template <typename T>
-inline int launch_d(Call &c, int rows, cudaStream_t st) {
-    if (c.dim == 64) return launch_r<T, 64>(c, rows, st);
-    if (c.dim == 128) return launch_r<T, 128>(c, rows, st);
-    return launch_r<T, 256>(c, rows, st);
-}
-
-// `rows`: queries x heads of a group of the request with most of them.
-inline int launch(Call &c, int rows, cudaStream_t st) {
-    const Args all = c.a;
-    for (int r0 = 0; r0 < all.R; r0 += MAX_R) {                    // requests beyond MAX_R: further launches
-        c.a = all;
-        c.a.R = all.R - r0 < MAX_R ? all.R - r0 : MAX_R;
-        c.a.cu_q = all.cu_q + r0;
-        c.a.seq_len = all.seq_len + r0;
-        c.a.table = all.table + (size_t)r0 * all.width;
-        int rc = c.dtype == W4A8_F32 ? launch_d<float>(c, rows, st) : c.dtype == W4A8_F16 ? launch_d<__half>(c, rows, st) : launch_d<__nv_bfloat16>(c, rows, st);
-        if (rc != W4A8_OK) return rc;
+    for (int r0 = 0; r0 < c.a.R; r0 += MAX_R) {                    // requests beyond those: further launches
+        Args a = c.a;
+        a.R = c.a.R - r0 < MAX_R ? c.a.R - r0 : MAX_R;
+        a.cu_q += r0;
+        a.seq_len += r0;
+        a.table += (size_t)r0 * a.width;
+        a.stages = S::stages(a.R);
+        const size_t smem = (size_t)S::fixed_bytes(a.R) + (size_t)a.stages * S::STAGE;
+        static PerDevice<size_t> configured_dev;
+        size_t &configured = configured_dev.get();
+        if (smem > configured) {
+            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return cuda_fail(e, "attention_q8 smem opt-in");
+            configured = smem;
+        }
+        cudaError_t e = launch_pdl(kern, dim3(sm_count()), dim3(THREADS), smem, st, mk, mv, a);
+        if (e != cudaSuccess) return cuda_fail(e, "attention_q8 launch");
     }
-    return W4A8_OK;
+    return launch_status("attention_q8");
+}
+
+// The narrowest kernel that takes `rows` (queries x heads of a group of the request with most of them) at once.
+template <typename T, int D>
+inline int launch_d(const Call &c, int rows, cudaStream_t st) {
+    if (rows <= 4) return launch_t<T, D, 4>(c, st);
+    if (rows <= 8) return launch_t<T, D, 8>(c, st);
+    if (rows <= 16) return launch_t<T, D, 16>(c, st);
+    return launch_t<T, D, 24>(c, st);
+}
+
+inline int launch(const Call &c, int rows, cudaStream_t st) {
+    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) { return launch_d<decltype(t), decltype(d)::value>(c, rows, st); });
 }
 
 }  // namespace attn

@@ -25,6 +25,12 @@ using attn::ex2;
 using attn::lg2;
 using attn::capped;
 using attn::lds_f4;
+using attn::elected;
+using attn::umma_commit;
+using attn::wait_one;
+using attn::wait_warp;
+using attn::raise_registers;
+using attn::lower_registers;
 using attn::h2_bits;
 constexpr unsigned ERR_WAIT = 0xB00u;
 constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
@@ -46,11 +52,6 @@ enum { RAW_FULL = 0, RAW_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY
 
 // D[tmem] (+)= A[tmem] B[smem]; A: 128 lanes, two fp16 a column.  B: N x 16 as the descriptor says.  The whole warp comes here and the elected
 // lane issues: addresses and descriptors then stay in uniform registers (inside a branch of one lane an instruction took 120 cycles to issue).
-__device__ __forceinline__ uint32_t elected() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e;
-}
 __device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
                  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
@@ -58,10 +59,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t 
 __device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
                  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t lead, uint32_t bar) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 // fp32 accumulators (bits [4,6) = 1), fp16 A and B; bit 16: B is MN-major; N >> 3 in [17,23), M >> 4 in [24,29).
 __host__ __device__ constexpr uint32_t idesc_f16(int N, int b_mn) { return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
@@ -267,27 +264,6 @@ __device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac,
 }
 
 // The block is launched with 128 registers a thread; the rows' two warpgroups take 200, the others keep 56: 2 * 128 * (200 + 56) = 512 * 128.
-template <int N> __device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// Bounded waits without a call: a kernel that moves registers between its warps cannot have one.
-__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    long long since = 0;
-#pragma unroll 1
-    for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < 64; i++)
-            if (ptx::mbar_try_wait(bar, parity)) return true;
-        const long long now = clock64();
-        if (since == 0) since = now;
-        else if (now - since > (1ll << 28)) return false;
-    }
-}
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
-    const bool ok = wait_one(bar, parity);
-    return __all_sync(0xffffffffu, ok);
-}
 
 // N columns of a row out.
 template <int N, typename T> __device__ __forceinline__ void put(T *dst, const float (&y)[N], float inv) {

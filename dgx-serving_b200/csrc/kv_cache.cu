@@ -131,11 +131,7 @@ W4A8_API int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *
     a.block = cache->block; a.num_blocks = cache->num_blocks;
     a.causal = causal != 0; a.window = window; a.scale = scale; a.softcap = softcap;
     a.few = 0x7fffffff;
-    unsigned char *ws = static_cast<unsigned char *>(workspace);
-    const size_t slots = (size_t)sm_count() * attn::MAX_CTAS_PER_SM * 2;
-    a.count = reinterpret_cast<unsigned *>(ws);
-    a.part_ml = reinterpret_cast<float2 *>(ws + attn::count_bytes());
-    a.part = reinterpret_cast<float *>(ws + attn::count_bytes() + slots * attn::MAX_ROWS * 8);
+    attn::lay_out(a, workspace, cache->dim);
     c.k = cache->k; c.v = cache->v; c.dtype = dtype; c.dim = cache->dim;
     const int64_t rows = (int64_t)(max_q > 0 && max_q < T ? max_q : T) * a.G;
     if (rows > attn::FEW_ROWS) {

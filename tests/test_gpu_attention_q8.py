@@ -234,7 +234,7 @@ def test_blocks_past_two_to_the_31_bytes(w4a8, cuda):
     cache = w4a8.KVCache.of(*dev)
     q, out = c.q.to(cuda).contiguous(), torch.zeros((c.T, 4, 128), device=cuda)
     ws = torch.zeros(w4a8.attention_q8_workspace_bytes(4, cache), dtype=torch.uint8, device=cuda)
-    w4a8.launch_attention_q8(q, 512, cache, to_dev(far, cuda), c.width, to_dev(c.cu, cuda), to_dev(c.seqs, cuda), 1, c.T, 4, out, 512, c.scale, "fp32", ws)
+    w4a8.launch_attention_q8(q, 512, cache, to_dev(far, cuda), c.width, to_dev(c.cu, cuda), to_dev(c.seqs, cuda), 1, c.T, 4, out, 512, c.scale, "fp32", ws, max_q=1)
     w4a8.device_status()
     assert np.array_equal(out[:1].cpu().numpy(), want)
 
