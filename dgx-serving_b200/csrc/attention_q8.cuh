@@ -16,7 +16,8 @@
 //    is a whole number too, x = exp(s - B) * vs up to 2^31, four columns of P.  All sums are whole numbers and exact; O stays in tensor memory over
 //    the tiles.  The row's reference B is such that its largest x was 2^28 when it was chosen; when an x would pass 2^31, O is read out, rescaled
 //    and summed in fp32, and B moves.  So a weight is rounded to 2^-28 of the row's largest, or as fp32 is.
-//  - 128 threads have a key each, about forty instructions for a row.
+//  - 128 threads have a key each, about forty instructions for a row.  Two such groups take the tiles in turn, each with its own S, P, O, reference and
+//    sums, because a tile's chain of steps takes longer than its bytes do; they meet at the end of a pair, one handing over, the other writing.
 #pragma once
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"
@@ -26,12 +27,13 @@ namespace w4a8 {
 namespace attn {
 
 constexpr int TK = 128;                    // keys of a tile
-constexpr int THREADS = 256;               // warps 0-3: a key (then a dim) a thread; 4, 5: copies of K, of V; 6: products; 7: queries
+constexpr int THREADS = 384;               // warps 0-3, 4-7: a key (then a dim) a thread; 8, 9: copies of K, of V; 10: products; 11: queries
 constexpr int MAX_R = 2048;                // requests of one launch (their sums lie in shared memory)
 constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) of a request that this kernel takes at most
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;
 constexpr float TOP = 28.f, LIMIT = 30.9f; // log2 of the largest weight when B is chosen, and beyond which it moves (four signed digits reach 2^30.99)
+constexpr int START = 3;                   // tiles whose time beginning and ending a pair takes
 constexpr int FLUSH = 900;                 // tiles after which O is read out at the latest: 128 * 128 * 127 * 900 < 2^31
 
 struct Args {
@@ -80,10 +82,11 @@ __device__ __forceinline__ Request request(const Args &a, int r, int rows_per_gr
     return x;
 }
 
-// A CTA's range of units cut at the pairs' ends.
+// Units: a pair is START of them and one for each of its tiles, because beginning and ending a pair costs a CTA as much as START tiles; a bound
+// that falls into the START lies in front of the first tile.  A CTA's range cut at the pairs' ends:
 struct Segment {
     int r, h, rg, tile, tiles;               // tiles [tile, tile + tiles) of the pair's
-    int pair0, pair_tiles;                   // the pair's first unit, its tiles
+    int pair0, pair_tiles;                   // the unit of the pair's first tile, its tiles
     Request x;
 };
 struct Walk {
@@ -108,16 +111,18 @@ struct Walk {
             do r++; while (cum[r + 1] <= u);
             x = request(a, r, rpg);
         }
-        const unsigned in = u - cum[r], pair = in / (unsigned)x.tiles, t = in - pair * (unsigned)x.tiles;
+        const unsigned span = (unsigned)(x.tiles + START), in = u - cum[r], pair = in / span, tile0 = cum[r] + pair * span + START;
+        const unsigned t = u > tile0 ? u - tile0 : 0, t1 = end > tile0 ? min(end - tile0, (unsigned)x.tiles) : 0;
+        u = tile0 + x.tiles;
+        if (t1 <= t) return false;
         s.r = r;
         s.h = (int)(pair % (unsigned)a.Hkv);
         s.rg = (int)(pair / (unsigned)a.Hkv);
         s.tile = (int)t;
-        s.tiles = (int)min((unsigned)x.tiles - t, end - u);
-        s.pair0 = (int)(u - t);
+        s.tiles = (int)(t1 - t);
+        s.pair0 = (int)tile0;
         s.pair_tiles = x.tiles;
         s.x = x;
-        u += s.tiles;
         return true;
     }
 };
@@ -131,6 +136,9 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
 // Four consecutive elements of a row of Q as floats.
@@ -218,8 +226,13 @@ template <int ROW> __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// D = int32, A and B signed bytes, 128 rows, N columns; bit 15: A is MN-major.
-__host__ __device__ constexpr uint32_t idesc_s8(int N, int a_mn) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
+// The same of W bytes, all of the operand's N (W 16: not swizzled; else W bytes).
+template <int W> __device__ __forceinline__ uint64_t desc_p(uint32_t addr) {
+    constexpr uint64_t stride = W * 8 >> 4, mode = W == 128 ? 2 : W == 64 ? 4 : W == 32 ? 6 : 0;
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (stride << 16) | (stride << 32) | (1ull << 46) | (mode << 61);
+}
+// D = int32, A and B signed bytes, 128 rows, N columns; bits 15 and 16: A and B are MN-major.
+__host__ __device__ constexpr uint32_t idesc_s8(int N, int mn) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(mn * 3) << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
 // The whole warp comes here and the elected lane issues: addresses and descriptors then stay in uniform registers.
 __device__ __forceinline__ uint32_t elected() {
     uint32_t e;
@@ -237,15 +250,17 @@ __device__ __forceinline__ void umma_commit(uint32_t lead, uint32_t bar) {
 __device__ __forceinline__ float out_round(float, float v) { return v; }
 __device__ __forceinline__ __half out_round(__half, float v) { return __float2half_rn(v); }
 __device__ __forceinline__ __nv_bfloat16 out_round(__nv_bfloat16, float v) { return __float2bfloat16_rn(v); }
-// N columns of tensor memory of this lane.
-template <int N> __device__ __forceinline__ void tmem_columns(uint32_t addr, int (&v)[N]) {
-#pragma unroll
-    for (int c = 0; c < N; c += 16) {
-        uint32_t r[16];
-        ptx::tmem_ld(addr + c, r);
-#pragma unroll
-        for (int e = 0; e < 16; e++) v[c + e] = (int)r[e];
-    }
+// N columns of tensor memory of this lane, on their way until columns_arrived.
+template <int N> __device__ __forceinline__ void columns_load(uint32_t addr, uint32_t (&v)[N]) {
+    if constexpr (N == 12) {
+        ptx::tmem_ld(addr, *reinterpret_cast<uint32_t(*)[8]>(v));
+        ptx::tmem_ld(addr + 8, *reinterpret_cast<uint32_t(*)[4]>(v + 8));
+    } else if constexpr (N == 24) {
+        ptx::tmem_ld(addr, *reinterpret_cast<uint32_t(*)[16]>(v));
+        ptx::tmem_ld(addr + 16, *reinterpret_cast<uint32_t(*)[8]>(v + 16));
+    } else ptx::tmem_ld(addr, v);
+}
+template <int N> __device__ __forceinline__ void columns_arrived(uint32_t (&v)[N]) {
     ptx::tmem_ld_wait();
 #pragma unroll
     for (int c = 0; c < N; c++) asm volatile("" : "+r"(v[c]));        // nothing that reads them moves in front of the wait
@@ -254,16 +269,17 @@ template <int N> __device__ __forceinline__ void tmem_columns(uint32_t addr, int
 // R rows (queries x heads of a group): 3 columns of S and 4 of P for each, in whole sixteens.
 template <int D, int R_> struct Shape {
     static constexpr int R = R_, N = (3 * R + 15) / 16 * 16, NP = 4 * R, DP = D == 256 ? 2 : 1, OC = D == 64 ? 2 * NP : DP * NP;    // DP: dims of a thread; OC: columns of O
+    static constexpr int P_ROW = D == 64 ? 2 * NP : NP;                              // bytes of P of a token (dim 64: of a pair of tokens)
     static constexpr int STAGE = 2 * Tile<D>::BYTES, QB = N * D, PB = NP * TK;
     static constexpr int SCALES = 8;                                                   // blocks of a tile at most
     static constexpr int MAX_STAGES = 8;
-    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 4 * R * 4 + (D == 64 ? 64 * R * 4 : 0);   // and 4 bytes a request
+    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4;   // and 4 bytes a request
     static inline int fixed_bytes(int n) { return (FIXED + (n + 4) * 4 + 1023) & ~1023; }
     static inline int stages(int n) {
         const int k = (226 * 1024 - fixed_bytes(n)) / STAGE;
         return k < MAX_STAGES ? k : MAX_STAGES;
     }
-    static_assert(NP % 16 == 0 && 2 * N + OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 2 * STAGE <= 226 * 1024, "shape");
+    static_assert(NP % 16 == 0 && 2 * N + 2 * OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 2 * STAGE <= 226 * 1024, "shape");
 };
 
 template <typename T, int D, int R>
@@ -280,13 +296,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     unsigned char *control = p; p += 1024;
     float4 *scales = reinterpret_cast<float4 *>(p); p += S::MAX_STAGES * S::SCALES * 16;   // ks, log2 vs, 1 / vs of a stage's blocks
     float4 *rec = reinterpret_cast<float4 *>(p); p += 2 * R * 16;                          // a row's factor, B, last and first key (as int)
-    float *red = reinterpret_cast<float *>(p); p += 4 * R * 4;
-    float *fold = reinterpret_cast<float *>(p); p += D == 64 ? 64 * R * 4 : 0;
+    float *reds = reinterpret_cast<float *>(p); p += 2 * 4 * R * 4;
+    float2 *over_ml = reinterpret_cast<float2 *>(p); p += R * 8;                           // what one group hands over: B, sum; values
+    float *refs = reinterpret_cast<float *>(p); p += 2 * R * 4;                            // B of each group (many rows)
+    float *over = reinterpret_cast<float *>(p); p += R * (D == 64 ? 128 : D) * 4;
     unsigned *cum = reinterpret_cast<unsigned *>(p);
     const uint32_t bar = ptx::smem_u32(control), ring_at = ptx::smem_u32(smem), q_at = ptx::smem_u32(qs), p_at = ptx::smem_u32(ps);
     const uint32_t K_FULL = bar, V_FULL = bar + 64u, EMPTY = bar + 128u, S_FULL = bar + 192u, S_EMPTY = bar + 208u, P_FULL = bar + 224u, P_EMPTY = bar + 240u,
-                   Q_FULL = bar + 256u, Q_EMPTY = bar + 272u;
-    __shared__ unsigned wsum[THREADS / 32], last_flag, tmem_slot;
+                   Q_FULL = bar + 256u, Q_EMPTY = bar + 272u, OVER = bar + 288u;
+    __shared__ unsigned wsum[THREADS / 32], last_flags[2], tmem_slot;
     __shared__ int fresh[2];                                            // a tile's weights begin new sums in O
     __shared__ Work works[WORKS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -299,7 +317,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             ptx::mbar_init(P_FULL + 8 * s, 4);
             ptx::mbar_init(P_EMPTY + 8 * s, 1);
             ptx::mbar_init(Q_FULL + 8 * s, 1);
-            ptx::mbar_init(Q_EMPTY + 8 * s, 5);
+            ptx::mbar_init(Q_EMPTY + 8 * s, 9);
+            ptx::mbar_init(OVER + 8 * s, 4);
         }
         ptx::mbar_fence_init();
         ptx::tma_prefetch_desc(&map_k);
@@ -314,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     for (int base = 0; base < a.R; base += THREADS) {
         const int r = base + tid;
         unsigned v = 0;
-        if (r < a.R) { const Request x = request(a, r, R); v = (unsigned)x.groups * (unsigned)a.Hkv * (unsigned)x.tiles; }
+        if (r < a.R) { const Request x = request(a, r, R); v = (unsigned)x.groups * (unsigned)a.Hkv * (unsigned)(x.tiles + START); }
         unsigned s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const unsigned t = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += t; }
@@ -328,11 +347,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     }
     if (tid == 0) cum[a.R] = carry;
     const unsigned U = carry, P = min(gridDim.x, U), cta = blockIdx.x;            // equal ranges
-    if (cta >= P) return;
     const auto bound = [&](unsigned i) { return (unsigned)((unsigned long long)i * U / P); };
     const auto cta_of = [&](unsigned u) { return (unsigned)(((unsigned long long)(u + 1) * P - 1) / U); };
+    if (cta >= P) return;
     const unsigned u0 = bound(cta), u1 = bound(cta + 1);
-    if (warp == 6) {
+    if (warp == 10) {
         ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
         ptx::tmem_relinquish();
     }
@@ -346,9 +365,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     bool ok = true;
     const auto give_up = [&](unsigned code) { if (lane == 0) dev_set_error(ERR_WAIT | code); ok = false; };
 
-    if (warp == 4 || warp == 5) {
+    if (warp == 8 || warp == 9) {
         // ---- copies: lane = one piece (a block, or the part of it that lies in a tile); a batch is 32 pieces; this warp brings K or V -----------------
-        const bool is_k = warp == 4;
+        const bool is_k = warp == 8;
         const CUtensorMap *map = is_k ? &map_k : &map_v;
         const uint32_t full0 = is_k ? K_FULL : V_FULL;
         Walk walk(a, cum, u0, u1, R);
@@ -405,13 +424,31 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             resolve();
         }
         if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);    // copies in flight end before the CTA's shared memory is another's
-    } else if (warp == 7) {
+    } else if (warp == 11) {
         // ---- queries: the next pair's, while the others are at one --------------------------------------------------------------------------
         constexpr int LPR = D == 64 ? 16 : 32, RPW = 32 / LPR, PER = D == 256 ? 2 : 1;         // lanes to a row, rows at a time, words of four of a lane
+        constexpr int TURNS = R / RPW;                                                         // their loads are all in flight at once
         Walk walk(a, cum, u0, u1, R);
         Segment s;
+        const int sub = lane / LPR, col = lane % LPR;
         for (int k = 0;; k++) {
             const bool more = walk.next(s);
+            const int rows = more ? min(R, s.x.n * a.G - s.rg * R) : 0;
+            float4 v[TURNS][PER];
+            int pos[TURNS] = {};
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) {
+                const int r = i * RPW + sub;
+#pragma unroll
+                for (int e = 0; e < PER; e++) v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < rows) {
+                    const int rho = s.rg * R + r, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
+                    const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
+                    pos[i] = s.x.seq - s.x.n + query;
+#pragma unroll
+                    for (int e = 0; e < PER; e++) v[i][e] = load4(src + 4 * (col + 32 * e));
+                }
+            }
             if (k >= 2 && !wait_idle(Q_EMPTY + 8 * (k & 1), (k / 2 - 1) & 1)) give_up(3u);
             if (!ok) break;
             if (lane == 0) {
@@ -425,32 +462,27 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 }
             }
             if (more) {
-                const int rows = min(R, s.x.n * a.G - s.rg * R), sub = lane / LPR, col = lane % LPR;
                 unsigned char *to = qs + (k & 1) * S::QB;
-#pragma unroll 2
-                for (int r0 = 0; r0 < R; r0 += RPW) {
-                    const int r = r0 + sub;
-                    if (r0 >= rows && k >= 2) break;                             // (rows of an earlier segment: what they give is not read)
-                    const int rho = s.rg * R + min(r, rows - 1), query = rho / a.G, head = s.h * a.G + rho - query * a.G;
-                    const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
-                    float4 v[PER];
-                    float amax = 0.f, bad = 0.f;
 #pragma unroll
-                    for (int e = 0; e < PER; e++) {
-                        v[e] = r < rows ? load4(src + 4 * (col + 32 * e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[e].x), fabsf(v[e].y))), fmaxf(fabsf(v[e].z), fabsf(v[e].w)));
-                        bad += (v[e].x * 0.f + v[e].y * 0.f) + (v[e].z * 0.f + v[e].w * 0.f);      // NaN if one is not a number or infinite: digits cannot tell
-                    }
+                for (int i = 0; i < TURNS; i++) {
+                    if (i * RPW >= rows && k >= 2) break;                        // (rows of an earlier segment: what they give is not read)
+                    const int r = i * RPW + sub;
+                    uint32_t most = 0;                                           // bits of the largest magnitude; from those of infinity on: not a number
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) {
-                        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                        bad += __shfl_xor_sync(0xffffffffu, bad, o);
+                    for (int e = 0; e < PER; e++)
+                        most = max(max(most, max(__float_as_uint(v[i][e].x) & 0x7FFFFFFFu, __float_as_uint(v[i][e].y) & 0x7FFFFFFFu)),
+                                   max(__float_as_uint(v[i][e].z) & 0x7FFFFFFFu, __float_as_uint(v[i][e].w) & 0x7FFFFFFFu));
+                    if constexpr (LPR == 32) most = __reduce_max_sync(0xffffffffu, most);
+                    else {
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                     }
+                    const float amax = __uint_as_float(most), bad = most >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.f;     // digits cannot tell
                     // the row in units of its last digit: amax becomes 127 * 256^2; by a power of two first, so that neither factor leaves fp32
                     const float p2 = row_factor(amax), f = amax > 0.f ? 127.f * 65536.f / (amax * p2) : 1.f;
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
-                        const float y[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+                        const float y[4] = {v[i][e].x, v[i][e].y, v[i][e].z, v[i][e].w};
                         uint32_t w[4];
 #pragma unroll
                         for (int m = 0; m < 4; m++) w[m] = (uint32_t)(__float2int_rn(y[m] * p2 * f) + 0x8080) ^ 0x8080u;     // signed digits in bytes 2, 1, 0
@@ -461,15 +493,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                             const uint32_t sel = g == 0 ? 0x0062u : g == 1 ? 0x0051u : 0x0040u;
                             const uint32_t word = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
                             const int at = D == 64 ? n * 64 + (((d >> 4) ^ ((n >> 1) & 3)) << 4) + (d & 15) : e * N * 128 + n * 128 + (((d >> 4) ^ (n & 7)) << 4) + (d & 15);
-                            if (r < R) *reinterpret_cast<uint32_t *>(to + at) = word;
+                            *reinterpret_cast<uint32_t *>(to + at) = word;
                         }
                     }
-                    if (col == 0 && r < R) {
-                        const int pos = s.x.seq - s.x.n + query;
+                    if (col == 0)
                         rec[(k & 1) * R + r] = make_float4(a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
-                                                           __int_as_float(a.causal ? min(pos, s.x.seq - 1) : s.x.seq - 1),
-                                                           __int_as_float(a.window > 0 ? max(0, pos - a.window + 1) : 0));
-                    }
+                                                           __int_as_float(a.causal ? min(pos[i], s.x.seq - 1) : s.x.seq - 1),
+                                                           __int_as_float(a.window > 0 ? max(0, pos[i] - a.window + 1) : 0));
                 }
                 ptx::fence_proxy_async_smem();
             }
@@ -477,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             if (lane == 0) ptx::mbar_arrive(Q_FULL + 8 * (k & 1));
             if (!more) break;
         }
-    } else if (warp == 6) {
+    } else if (warp == 10) {
         // ---- products: S of a tile, then PV of the tile before it ---------------------------------------------------------------------------------
         const uint32_t lead = elected();
         constexpr uint32_t id_s = idesc_s8(N, 0), id_o = idesc_s8(D == 64 ? 2 * NP : NP, 1);
@@ -498,8 +528,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
                     const uint64_t vd = desc_mn(vb + pl * L::PLANE_BYTES + k * 32 * 128);
-                    const uint64_t pd = D == 64 ? desc_k<64>(pb) + (uint64_t)(2 * k) : desc_k<128>(pb) + (uint64_t)(2 * k);
-                    umma_s8(lead, o_cols + pl * NP, vd, pd, id_o, k > 0 || !begin);
+                    const uint64_t pd = desc_p<S::P_ROW>(pb + k * 32 * S::P_ROW);
+                    umma_s8(lead, o_cols + buf * S::OC + pl * NP, vd, pd, id_o, k > 0 || !begin);
                 }
             umma_commit(lead, EMPTY + 8 * pst);
             umma_commit(lead, P_EMPTY + 8 * buf);
@@ -528,34 +558,45 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         if (ok && j > 0) values(j - 1);
         if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
     } else {
-        // ---- thread = key: scores to weights; thread = dim: O --------------------------------------------------------------------------------------
-        const uint32_t lanes = (uint32_t)warp << 21;
-        const int parity = D == 64 ? tid >> 6 : 0;
-        unsigned j = 0;
+        // ---- thread = key: scores to weights; thread = dim: O.  This group's tiles are every second one --------------------------------------------
+        const uint32_t group = warp >> 2, lanes = (uint32_t)(warp & 3) << 21;
+        const int gt = tid & 127, gw = warp & 3, parity = D == 64 ? gt >> 6 : 0;
+        float *red = reds + group * 4 * R;
+        unsigned j = 0, before = 0;                                                 // tiles so far; this group's last one + 1
         int st = 0;
         uint32_t ph = 0;
-        float l[R], acc[DP][R], fac[R], B[R];
-        const auto sync = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        // what is the same for all threads of a row is in registers for few rows, for many in shared memory
+        constexpr bool HELD = R <= 8;
+        constexpr int STEP = R < 8 ? R : 8;                                          // rows whose scores are in registers at a time
+        float l[R], acc[DP][R], facs[HELD ? R : 1], Bs[HELD ? R : 1];
+        float *ref = refs + group * R;
+        const float4 *rc = rec;
+        const auto fac = [&](int r) { if constexpr (HELD) return facs[r]; else return rc[r].x; };
+        const auto B = [&](int r) { if constexpr (HELD) return Bs[r]; else return ref[r]; };
+        const auto sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         // Is it so for any of the 128 threads?  A wait that ran out for one warp is everybody's to know: they leave together.
         const auto vote = [&](bool mine) {
             int any;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-                         : "=r"(any) : "r"((int)mine) : "memory");
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any) : "r"((int)mine), "r"(1 + group) : "memory");
             return any != 0;
         };
         // O of the tiles since it was last read, in units of 2^B
         const auto read_o = [&]() {
-            const uint32_t i = j - 1;                                              // the last tile whose PV is in it
-            if (ok && !wait_warp(P_EMPTY + 8 * (i & 1), (i >> 1) & 1)) give_up(9u);
+            const uint32_t i = before - 1;                                         // the last tile whose PV is in it
+            if (ok && !wait_warp(P_EMPTY + 8 * group, (i >> 1) & 1)) give_up(9u);
             ptx::tc_fence_after_sync();
 #pragma unroll
-            for (int pl = 0; pl < DP; pl++) {
-                int v[NP];
-                tmem_columns<NP>(o_cols + lanes + pl * NP + parity * NP, v);
+            for (int pl = 0; pl < DP; pl++)
 #pragma unroll
-                for (int r = 0; r < R; r++)
-                    acc[pl][r] += fmaf((float)v[4 * r], 16777216.f, fmaf((float)v[4 * r + 1], 65536.f, fmaf((float)v[4 * r + 2], 256.f, (float)v[4 * r + 3])));
-            }
+                for (int r0 = 0; r0 < R; r0 += 4) {
+                    uint32_t v[16];
+                    columns_load(o_cols + group * S::OC + lanes + pl * NP + parity * NP + 4 * r0, v);
+                    columns_arrived(v);
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        acc[pl][r0 + r] += fmaf((float)(int)v[4 * r + 3], 16777216.f, fmaf((float)(int)v[4 * r + 2], 65536.f, fmaf((float)(int)v[4 * r + 1], 256.f, (float)(int)v[4 * r])));
+                }
             ptx::tc_fence_before_sync();
         };
         for (int nth = 0;; nth++) {
@@ -564,48 +605,57 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             const Work w = works[nth % WORKS];
             if (w.tiles == 0) break;
             const int row0 = w.rg * R, rows = min(R, w.n * a.G - row0);
-            float4 *rc = rec + (nth & 1) * R;
+            rc = rec + (nth & 1) * R;
             bool since = false;                                                     // O holds tiles of this segment that have not been read
             int held = 0;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 l[r] = 0.f;
-                fac[r] = rc[r].x;
-                B[r] = -inf;
+                if constexpr (HELD) { facs[r] = rc[r].x; Bs[r] = -inf; }
 #pragma unroll
                 for (int pl = 0; pl < DP; pl++) acc[pl][r] = 0.f;
             }
+            if constexpr (!HELD) {
+                if (gt < R) ref[gt] = -inf;
+                sync();
+            }
             for (int t = 0; t < w.tiles; t++, j++) {
-                const uint32_t buf = j & 1;
-                const int key = (w.tile0 + t) * TK + tid;
+                const int at_st = st;
+                if (++st == a.stages) { st = 0; ph ^= 1u; }
+                if ((j & 1) != group) continue;
+                const uint32_t buf = group;
+                const int key = (w.tile0 + t) * TK + gt;
                 if (ok && !wait_warp(S_FULL + 8 * buf, (j >> 1) & 1)) give_up(11u);
-                if (ok && !wait_warp(K_FULL + 8 * st, ph)) give_up(12u);             // (passed; the stage's scales are what the barrier's phase shows)
                 ptx::tc_fence_after_sync();
-                int v[N];
-                tmem_columns<N>(tmem + lanes + buf * N, v);
-                ptx::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(S_EMPTY + 8 * buf);
-                const float4 sc = scales[st * S::SCALES + (tid >> tshift)];
+                const float4 sc = scales[at_st * S::SCALES + (gt >> tshift)];
                 // rows that the segment does not have go along: they are not read
                 float y[R];
                 bool again = held >= FLUSH;
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const float s = fmaf((float)v[3 * r], 65536.f, (float)(v[3 * r + 1] * 256 + v[3 * r + 2]));
-                    y[r] = fmaf(s, fac[r] * sc.x, sc.y);
+                for (int r0 = 0; r0 < R; r0 += STEP) {
+                    uint32_t v[3 * STEP];
+                    columns_load(tmem + lanes + buf * N + 3 * r0, v);
+                    columns_arrived(v);
+#pragma unroll
+                    for (int r = 0; r < STEP; r++) {
+                        const float s = fmaf((float)(int)v[3 * r], 65536.f, (float)((int)v[3 * r + 1] * 256 + (int)v[3 * r + 2]));
+                        y[r0 + r] = fmaf(s, fac(r0 + r) * sc.x, sc.y);
+                    }
                 }
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(S_EMPTY + 8 * buf);
                 if (a.softcap > 0.f) {
 #pragma unroll
                     for (int r = 0; r < R; r++) y[r] = capped(y[r] - sc.y, a.softcap) + sc.y;
                 }
-                if (key - tid + TK - 1 > w.min_hi || key - tid < w.max_lo) {
+                if (key - gt + TK - 1 > w.min_hi || key - gt < w.max_lo) {
 #pragma unroll
                     for (int r = 0; r < R; r++)
                         if (key > __float_as_int(rc[r].z) || key < __float_as_int(rc[r].w)) y[r] = -inf;
                 }
 #pragma unroll
-                for (int r = 0; r < R; r++) again = again || y[r] > B[r] + LIMIT;
+                for (int r = 0; r < R; r++) again = again || y[r] > B(r) + LIMIT;
                 if (vote(again || !ok)) {
                     if (vote(!ok)) { ok = false; break; }
                     // a weight would pass 2^31: B moves to where the row's largest is 2^28; what is summed, to the new B
@@ -614,72 +664,111 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                         float m = y[r];
 #pragma unroll
                         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        if (lane == 0) red[warp * R + r] = m;
+                        if (lane == 0) red[gw * R + r] = m;
                     }
                     if (since) read_o();
                     sync();
 #pragma unroll
                     for (int r = 0; r < R; r++) {
                         const float m = fmaxf(fmaxf(red[r], red[R + r]), fmaxf(red[2 * R + r], red[3 * R + r]));
-                        const float now = m > B[r] + TOP ? m - TOP : B[r];
-                        const float shrink = B[r] == -inf || now == B[r] ? 1.f : ex2(B[r] - now);   // nothing is summed while B is -inf
-                        B[r] = now;
+                        const float was = B(r), now = m > was + TOP ? m - TOP : was;
+                        const float shrink = was == -inf || now == was ? 1.f : ex2(was - now);      // nothing is summed while B is -inf
+                        if constexpr (HELD) Bs[r] = now;
                         l[r] *= shrink;
 #pragma unroll
                         for (int pl = 0; pl < DP; pl++) acc[pl][r] *= shrink;
                     }
                     sync();
+                    if constexpr (!HELD) {
+                        if (gt < R) {
+                            const float m = fmaxf(fmaxf(red[gt], red[R + gt]), fmaxf(red[2 * R + gt], red[3 * R + gt]));
+                            if (m > ref[gt] + TOP) ref[gt] = m - TOP;
+                        }
+                        sync();
+                    }
                     since = false;
                     held = 0;
                 }
                 if (j >= 2 && ok && !wait_warp(P_EMPTY + 8 * buf, ((j >> 1) - 1) & 1)) give_up(13u);
-                if (tid == 0) fresh[buf] = !since;
+                if (gt == 0) fresh[buf] = !since;
                 since = true;
+                before = j + 1;
                 held++;
-                unsigned char *to = ps + buf * S::PB;
-                const int pc = D == 64 ? tid >> 1 : tid;                               // column of P
+                // a row of P is a token's (dim 64: a pair's), its digits from the lowest
+                constexpr int SWZ = S::P_ROW == 128 ? 7 : S::P_ROW == 64 ? 3 : S::P_ROW == 32 ? 1 : 0, PER128 = S::P_ROW == 128 ? 0 : S::P_ROW == 64 ? 1 : 2;
+                const int prow = D == 64 ? gt >> 1 : gt, piece = D == 64 ? (gt & 1) * (NP / 16) : 0, turn = (prow >> PER128) & SWZ;
+                const uint32_t to = p_at + buf * S::PB + prow * S::P_ROW;
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const float x = ex2(y[r] - (B[r] == -inf ? 0.f : B[r]));            // a masked score is -inf: 0
-                    l[r] = fmaf(x, sc.z, l[r]);
-                    const uint32_t n = (__float2uint_rn(x) + 0x808080u) ^ 0x808080u;
+                for (int r0 = 0; r0 < R; r0 += 4) {
+                    uint32_t n[4];
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const int row = 4 * r + g;                                      // dim 64: NP is a multiple of 8, so the odd tokens' rows swizzle alike
-                        const int at = D == 64 ? row * 64 + (((pc >> 4) ^ ((row >> 1) & 3)) << 4) : row * 128 + (((pc >> 4) ^ (row & 7)) << 4);
-                        to[at + (D == 64 ? (tid & 1) * NP * 64 : 0) + (pc & 15)] = (unsigned char)(n >> (24 - 8 * g));
+                    for (int r = 0; r < 4; r++) {
+                        const float b = B(r0 + r), x = ex2(y[r0 + r] - (b == -inf ? 0.f : b));      // a masked score is -inf: 0
+                        l[r0 + r] = fmaf(x, sc.z, l[r0 + r]);
+                        n[r] = (__float2uint_rn(x) + 0x808080u) ^ 0x808080u;
                     }
+                    sts128(to + (((piece + r0 / 4) ^ turn) << 4), n[0], n[1], n[2], n[3]);
                 }
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(P_FULL + 8 * buf);
-                if (++st == a.stages) { st = 0; ph ^= 1u; }
             }
             if (vote(!ok)) break;
             // ---- the pair's rows, or the partial sums of a part of it, out -------------------------------------------------------------------------
-            read_o();
+            if (since) read_o();
+            const bool hands_over = (nth & 1) != (int)group;
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 float sum = l[r];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) red[warp * R + r] = sum;
-                if (D == 64 && parity == 1) fold[r * 64 + (tid & 63)] = acc[0][r];
+                if (lane == 0) red[gw * R + r] = sum;
             }
             sync();
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                l[r] = (red[r] + red[R + r]) + (red[2 * R + r] + red[3 * R + r]);
-                if (D == 64 && parity == 0) acc[0][r] += fold[r * 64 + tid];
-            }
-            sync();                                                                 // red and fold have been read
+            for (int r = 0; r < R; r++) l[r] = (red[r] + red[R + r]) + (red[2 * R + r] + red[3 * R + r]);
+            sync();                                                                 // red has been read
             if (lane == 0) ptx::mbar_arrive(Q_EMPTY + 8 * (nth & 1));
-            const bool whole = w.tiles == w.pair_tiles, writes = D != 64 || tid < 64;
+            // dim 64: the odd tokens' threads too have a part of each element.  The group that takes over here was the one that handed over before, so
+            // nobody reads the buffer any more.
+            if (hands_over) {
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+#pragma unroll
+                    for (int pl = 0; pl < DP; pl++) over[r * (D == 64 ? 128 : D) + pl * 128 + gt] = acc[pl][r];
+                    if (gt == 0) over_ml[r] = make_float2(B(r), l[r]);
+                }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(OVER + 8 * (nth & 1));
+                continue;
+            }
+            if (ok && !wait_warp(OVER + 8 * (nth & 1), (nth >> 1) & 1)) give_up(14u);
+            float tops[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float2 x = over_ml[r];
+                const float top = fmaxf(B(r), x.x), f = B(r) == -inf ? 1.f : ex2(B(r) - top), g = x.x == -inf ? 1.f : ex2(x.x - top);  // (-inf: nothing, or not a number)
+                l[r] = l[r] * f + x.y * g;
+                tops[r] = top;
+#pragma unroll
+                for (int pl = 0; pl < DP; pl++) acc[pl][r] = acc[pl][r] * f + over[r * (D == 64 ? 128 : D) + pl * 128 + gt] * g;
+            }
+            if constexpr (D == 64) {                                                 // the two parities' sums
+                sync();
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (parity == 1) over[r * 128 + gt] = acc[0][r];
+                sync();
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (parity == 0) acc[0][r] += over[r * 128 + 64 + gt];
+            }
+            const bool whole = w.tiles == w.pair_tiles, writes = D != 64 || gt < 64;
             const auto finish = [&](int r, int pl, float v, float top, float sum) {     // v: a weighted value, sum: the weights'
                 const int rho = row0 + r, query = rho / a.G, head = w.h * a.G + rho - query * a.G;
                 const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // nothing seen: zeros
-                static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + tid] = out_round(T(), sum == 0.f ? 0.f : v * inv);
-                if (a.lse && tid == 0 && pl == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = sum > 0.f ? (top + log2f(sum)) * LN2 : (sum == 0.f ? -inf : sum);
+                static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), sum == 0.f ? 0.f : v * inv);
+                if (a.lse && gt == 0 && pl == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = sum > 0.f ? (top + log2f(sum)) * LN2 : (sum == 0.f ? -inf : sum);
             };
             if (whole) {
                 if (writes)
@@ -687,7 +776,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     for (int r = 0; r < R; r++)
                         if (r < rows)
 #pragma unroll
-                            for (int pl = 0; pl < DP; pl++) finish(r, pl, acc[pl][r], B[r], l[r]);
+                            for (int pl = 0; pl < DP; pl++) finish(r, pl, acc[pl][r], tops[r], l[r]);
                 continue;
             }
             const size_t slot = (size_t)(2 * cta + (w.first ? 1 : 0)) * MAX_ROWS;
@@ -696,8 +785,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 for (int r = 0; r < R; r++)
                     if (r < rows) {
 #pragma unroll
-                        for (int pl = 0; pl < DP; pl++) a.part[(slot + r) * D + pl * 128 + tid] = acc[pl][r];
-                        if (tid == 0) a.part_ml[slot + r] = make_float2(B[r], l[r]);
+                        for (int pl = 0; pl < DP; pl++) a.part[(slot + r) * D + pl * 128 + gt] = acc[pl][r];
+                        if (gt == 0) a.part_ml[slot + r] = make_float2(tops[r], l[r]);
                     }
             // ---- the CTAs that share the pair meet: FAN neighbours first, then the groups; the last to come joins, in the order of the ranges ----------------
             const unsigned c0 = cta_of((unsigned)w.pair0), c1 = cta_of((unsigned)(w.pair0 + w.pair_tiles - 1)), groups = (c1 - c0) / FAN + 1;
@@ -705,13 +794,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             const auto last_of = [&](unsigned *counter, unsigned n) {      // has everybody written?  What was written before is visible then.
                 __threadfence();
                 sync();
-                if (tid == 0) {
+                if (gt == 0) {
                     const unsigned seen = atomicAdd(counter, 1u);
-                    last_flag = seen == n - 1;
+                    last_flags[group] = seen == n - 1;
                     if (seen == n - 1) *counter = 0u;                      // as the next call expects it
                 }
                 sync();
-                const bool last = last_flag;
+                const bool last = last_flags[group];
                 sync();
                 if (last) __threadfence();
                 return last;
@@ -730,7 +819,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                         for (unsigned i = 0; i < 8; i++) {
                             const size_t at = (size_t)slot_of(first + (i0 + i < n ? i0 + i : 0) * step) * MAX_ROWS + r;
                             x[i] = __ldcg(pml + at);
-                            o[i] = __ldcg(pv + at * D + pl * 128 + tid);
+                            o[i] = __ldcg(pv + at * D + pl * 128 + gt);
                             if (i0 + i >= n) x[i] = make_float2(-inf, 0.f);
                         }
                         float m = top;
@@ -756,15 +845,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             if (groups == 1) { join(a.part_ml, a.part, g0, 1, in_group, finish); continue; }
             join(a.part_ml, a.part, g0, 1, in_group, [&](int r, int pl, float v, float top, float sum) {
                 const size_t at = (size_t)slot_of(g0) * MAX_ROWS + r;
-                a.part2[at * D + pl * 128 + tid] = v;
-                if (tid == 0 && pl == 0) a.part2_ml[at] = make_float2(top, sum);
+                a.part2[at * D + pl * 128 + gt] = v;
+                if (gt == 0 && pl == 0) a.part2_ml[at] = make_float2(top, sum);
             });
             if (last_of(a.count2 + slot_of(c0), groups)) join(a.part2_ml, a.part2, c0, FAN, groups, finish);
         }
     }
     __syncthreads();
     ptx::tc_fence_after_sync();
-    if (warp == 6) ptx::tmem_dealloc(tmem, 512);
+    if (warp == 10) ptx::tmem_dealloc(tmem, 512);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
@@ -827,8 +916,7 @@ template <typename T, int D>
 inline int launch_d(const Call &c, int rows, cudaStream_t st) {
     if (rows <= 4) return launch_t<T, D, 4>(c, st);
     if (rows <= 8) return launch_t<T, D, 8>(c, st);
-    if (rows <= 16) return launch_t<T, D, 16>(c, st);
-    return launch_t<T, D, 24>(c, st);
+    return launch_t<T, D, 16>(c, st);
 }
 
 inline int launch(const Call &c, int rows, cudaStream_t st) {
