@@ -191,6 +191,11 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
     const bool ok = wait_one(bar, parity);
     return __all_sync(0xffffffffu, ok);
 }
+__device__ __forceinline__ bool test_one(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
 // The same for a warp that waits long: it sleeps between the attempts and leaves the issue slots to the others.
 __device__ __forceinline__ bool wait_idle(uint32_t bar, uint32_t parity) {
     bool ok = ptx::mbar_try_wait(bar, parity);
@@ -207,7 +212,7 @@ template <int N> __device__ __forceinline__ void lower_registers() { asm volatil
 // What the warps have to know of a segment, left by the one that prepares its queries.  tiles 0: there is no further one.
 struct Work { int tiles, tile0, min_hi, max_lo, n, q0, rg, h, first, pair0, pair_tiles, pad; };   // keys up to min_hi and from max_lo on: every row sees them
 constexpr int WORKS = 4;
-constexpr int FAN = 16, MAX_ROWS = 32;     // CTAs whose partial results are joined at a time; rows of a partial result
+constexpr int FAN = 16, MAX_ROWS = 16;     // CTAs whose partial results are joined at a time; rows of a partial result
 
 // ---- operands ------------------------------------------------------------------------------------------------------------------------------
 // A tile of codes: planes of 128-byte rows, the 16-byte piece c of row r at c ^ (r & 7).  dim 128 and 256: a row is a token, a plane 128 elements.
@@ -273,7 +278,7 @@ template <int D, int R_> struct Shape {
     static constexpr int STAGE = 2 * Tile<D>::BYTES, QB = N * D, PB = NP * TK;
     static constexpr int SCALES = 8;                                                   // blocks of a tile at most
     static constexpr int MAX_STAGES = 8;
-    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4;   // and 4 bytes a request
+    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4 + 2 * (FAN + 2) * MAX_ROWS * 4;   // and 4 bytes a request
     static inline int fixed_bytes(int n) { return (FIXED + (n + 4) * 4 + 1023) & ~1023; }
     static inline int stages(int n) {
         const int k = (226 * 1024 - fixed_bytes(n)) / STAGE;
@@ -300,6 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     float2 *over_ml = reinterpret_cast<float2 *>(p); p += R * 8;                           // what one group hands over: B, sum; values
     float *refs = reinterpret_cast<float *>(p); p += 2 * R * 4;                            // B of each group (many rows)
     float *over = reinterpret_cast<float *>(p); p += R * (D == 64 ? 128 : D) * 4;
+    float *coefs = reinterpret_cast<float *>(p); p += 2 * (FAN + 2) * MAX_ROWS * 4;         // joining: what a part counts for
     unsigned *cum = reinterpret_cast<unsigned *>(p);
     const uint32_t bar = ptx::smem_u32(control), ring_at = ptx::smem_u32(smem), q_at = ptx::smem_u32(qs), p_at = ptx::smem_u32(ps);
     const uint32_t K_FULL = bar, V_FULL = bar + 64u, EMPTY = bar + 128u, S_FULL = bar + 192u, S_EMPTY = bar + 208u, P_FULL = bar + 224u, P_EMPTY = bar + 240u,
@@ -508,41 +514,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             if (!more) break;
         }
     } else if (warp == 10) {
-        // ---- products: S of a tile, then PV of the tile before it ---------------------------------------------------------------------------------
+        // ---- products: S of the next tile and PV of the oldest, each as soon as what it needs is there.  S runs up to two tiles ahead, also into the
+        // next pair; it must not be waited for before PV, because the next pair's queries may wait for the end of the one before. ------------------
         const uint32_t lead = elected();
         constexpr uint32_t id_s = idesc_s8(N, 0), id_o = idesc_s8(D == 64 ? 2 * NP : NP, 1);
-        int st = 0, pst = 0;
+        int st = 0, pst = 0, nth = 0, left = 0;                      // stages; pair, its tiles that are left
         uint32_t ph = 0, pph = 0;
-        unsigned j = 0;
-        const auto wait = [&](uint32_t b, uint32_t parity, unsigned code) {
-            if (ok && !wait_warp(b, parity)) give_up(code);
-            ptx::tc_fence_after_sync();
-            return ok;
-        };
-        const auto values = [&](unsigned i) {                        // PV of tile i
-            const uint32_t buf = i & 1;
-            if (!wait(P_FULL + 8 * buf, (i >> 1) & 1, 4u) || !wait(V_FULL + 8 * pst, pph, 5u)) return;
-            const uint32_t begin = fresh[buf] != 0, vb = ring_at + pst * S::STAGE + L::BYTES, pb = p_at + buf * S::PB;
-#pragma unroll
-            for (int pl = 0; pl < DP; pl++)
-#pragma unroll
-                for (int k = 0; k < (D == 64 ? 2 : 4); k++) {
-                    const uint64_t vd = desc_mn(vb + pl * L::PLANE_BYTES + k * 32 * 128);
-                    const uint64_t pd = desc_p<S::P_ROW>(pb + k * 32 * S::P_ROW);
-                    umma_s8(lead, o_cols + buf * S::OC + pl * NP, vd, pd, id_o, k > 0 || !begin);
-                }
-            umma_commit(lead, EMPTY + 8 * pst);
-            umma_commit(lead, P_EMPTY + 8 * buf);
-            if (++pst == a.stages) { pst = 0; pph ^= 1u; }
-        };
-        for (int nth = 0; ok; nth++) {
-            if (!wait(Q_FULL + 8 * (nth & 1), (nth >> 1) & 1, 6u)) break;
-            const int tiles = works[nth % WORKS].tiles;
-            if (tiles == 0) break;
-            for (int t = 0; t < tiles && ok; t++, j++) {
+        unsigned j = 0, i = 0;                                       // tiles whose S, whose PV has been issued
+        bool end = false;
+        const auto there = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, test_one(b, parity)) != 0; };
+        long long since = clock64();
+        while (!end || i < j) {
+            bool did = false;
+            if (!end && left == 0 && there(Q_FULL + 8 * (nth & 1), (nth >> 1) & 1)) {
+                left = works[nth % WORKS].tiles;
+                end = left == 0;
+                did = true;
+            }
+            if (left > 0 && there(K_FULL + 8 * st, ph) && (j < 2 || there(S_EMPTY + 8 * (j & 1), ((j >> 1) - 1) & 1))) {
+                ptx::tc_fence_after_sync();
                 const uint32_t buf = j & 1, kb = ring_at + st * S::STAGE, qb = q_at + (nth & 1) * S::QB;
-                if (!wait(K_FULL + 8 * st, ph, 7u)) break;
-                if (j >= 2 && !wait(S_EMPTY + 8 * buf, ((j >> 1) - 1) & 1, 8u)) break;
 #pragma unroll
                 for (int k = 0; k < D / 32; k++) {
                     const uint64_t kd = D == 64 ? desc_k<64>(kb) + (uint64_t)(2 * k) : desc_k<128>(kb + (k >> 2) * L::PLANE_BYTES) + (uint64_t)(2 * (k & 3));
@@ -550,13 +541,30 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     umma_s8(lead, tmem + buf * N, kd, qd, id_s, k > 0);
                 }
                 umma_commit(lead, S_FULL + 8 * buf);
-                if (t == tiles - 1) umma_commit(lead, Q_EMPTY + 8 * (nth & 1));
+                if (--left == 0) { umma_commit(lead, Q_EMPTY + 8 * (nth & 1)); nth++; }
                 if (++st == a.stages) { st = 0; ph ^= 1u; }
-                if (j > 0) values(j - 1);
+                j++;
+                did = true;
             }
+            if (i < j && there(P_FULL + 8 * (i & 1), (i >> 1) & 1) && there(V_FULL + 8 * pst, pph)) {
+                ptx::tc_fence_after_sync();
+                const uint32_t buf = i & 1, begin = fresh[buf] != 0, vb = ring_at + pst * S::STAGE + L::BYTES, pb = p_at + buf * S::PB;
+#pragma unroll
+                for (int pl = 0; pl < DP; pl++)
+#pragma unroll
+                    for (int k = 0; k < (D == 64 ? 2 : 4); k++)
+                        umma_s8(lead, o_cols + buf * S::OC + pl * NP, desc_mn(vb + pl * L::PLANE_BYTES + k * 32 * 128), desc_p<S::P_ROW>(pb + k * 32 * S::P_ROW), id_o, k > 0 || !begin);
+                umma_commit(lead, EMPTY + 8 * pst);
+                umma_commit(lead, P_EMPTY + 8 * buf);
+                if (++pst == a.stages) { pst = 0; pph ^= 1u; }
+                i++;
+                did = true;
+            }
+            const long long now = clock64();
+            if (did) since = now;
+            else if (__any_sync(0xffffffffu, now - since > (1ll << 28))) { give_up(4u); break; }
         }
-        if (ok && j > 0) values(j - 1);
-        if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);
+        if (!ok) for (int n = 0; n < 64; n++) __nanosleep(50000);
     } else {
         // ---- thread = key: scores to weights; thread = dim: O.  This group's tiles are every second one --------------------------------------------
         const uint32_t group = warp >> 2, lanes = (uint32_t)(warp & 3) << 21;
@@ -763,92 +771,114 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 for (int r = 0; r < R; r++)
                     if (parity == 0) acc[0][r] += over[r * 128 + 64 + gt];
             }
-            const bool whole = w.tiles == w.pair_tiles, writes = D != 64 || gt < 64;
-            const auto finish = [&](int r, int pl, float v, float top, float sum) {     // v: a weighted value, sum: the weights'
-                const int rho = row0 + r, query = rho / a.G, head = w.h * a.G + rho - query * a.G;
-                const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // nothing seen: zeros
-                static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), sum == 0.f ? 0.f : v * inv);
-                if (a.lse && gt == 0 && pl == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = sum > 0.f ? (top + log2f(sum)) * LN2 : (sum == 0.f ? -inf : sum);
-            };
-            if (whole) {
-                if (writes)
+            const bool writes = D != 64 || gt < 64;
+            if (w.tiles != w.pair_tiles) {
+                // ---- the CTAs that share the pair meet: FAN neighbours first, then the groups; the last to come joins, in the order of the ranges ------------
+                const auto leave = [&](float2 *pml, float *pv, size_t slot) {
+                    if (writes)
 #pragma unroll
-                    for (int r = 0; r < R; r++)
-                        if (r < rows)
+                        for (int r = 0; r < R; r++)
+                            if (r < rows) {
 #pragma unroll
-                            for (int pl = 0; pl < DP; pl++) finish(r, pl, acc[pl][r], tops[r], l[r]);
-                continue;
-            }
-            const size_t slot = (size_t)(2 * cta + (w.first ? 1 : 0)) * MAX_ROWS;
-            if (writes)
-#pragma unroll
-                for (int r = 0; r < R; r++)
-                    if (r < rows) {
-#pragma unroll
-                        for (int pl = 0; pl < DP; pl++) a.part[(slot + r) * D + pl * 128 + gt] = acc[pl][r];
-                        if (gt == 0) a.part_ml[slot + r] = make_float2(tops[r], l[r]);
+                                for (int pl = 0; pl < DP; pl++) pv[(slot * MAX_ROWS + r) * D + pl * 128 + gt] = acc[pl][r];
+                                if (gt == 0) pml[slot * MAX_ROWS + r] = make_float2(tops[r], l[r]);
+                            }
+                };
+                const unsigned c0 = cta_of((unsigned)w.pair0), c1 = cta_of((unsigned)(w.pair0 + w.pair_tiles - 1)), groups = (c1 - c0) / FAN + 1;
+                const auto slot_of = [&](unsigned k) { return 2 * k + (k == c0 ? 1 : 0); };
+                const auto last_of = [&](unsigned *counter, unsigned n) {      // has everybody written?  What was written before is visible then.
+                    __threadfence();
+                    sync();
+                    if (gt == 0) {
+                        const unsigned seen = atomicAdd(counter, 1u);
+                        last_flags[group] = seen == n - 1;
+                        if (seen == n - 1) *counter = 0u;                      // as the next call expects it
                     }
-            // ---- the CTAs that share the pair meet: FAN neighbours first, then the groups; the last to come joins, in the order of the ranges ----------------
-            const unsigned c0 = cta_of((unsigned)w.pair0), c1 = cta_of((unsigned)(w.pair0 + w.pair_tiles - 1)), groups = (c1 - c0) / FAN + 1;
-            const auto slot_of = [&](unsigned k) { return 2 * k + (k == c0 ? 1 : 0); };
-            const auto last_of = [&](unsigned *counter, unsigned n) {      // has everybody written?  What was written before is visible then.
-                __threadfence();
-                sync();
-                if (gt == 0) {
-                    const unsigned seen = atomicAdd(counter, 1u);
-                    last_flags[group] = seen == n - 1;
-                    if (seen == n - 1) *counter = 0u;                      // as the next call expects it
-                }
-                sync();
-                const bool last = last_flags[group];
-                sync();
-                if (last) __threadfence();
-                return last;
-            };
-            const auto join = [&](const float2 *pml, const float *pv, unsigned first, unsigned step, unsigned n, auto &&out) {
-                if (!writes) return;
-#pragma unroll 1
-                for (int e = 0; e < rows * DP; e++) {
-                    const int r = e / DP, pl = e % DP;
-                    float top = -inf, sum = 0.f, v = 0.f;
-#pragma unroll 1
-                    for (unsigned i0 = 0; i0 < n; i0 += 8) {               // eight loads of each kind in flight
-                        float2 x[8];
-                        float o[8];
+                    sync();
+                    const bool last = last_flags[group];
+                    if (last) __threadfence();
+                    return last;
+                };
+                float *coef = coefs + group * (FAN + 2) * MAX_ROWS;            // [part][row], then the rows' references and sums
+                const auto join = [&](const float2 *pml, const float *pv, unsigned first, unsigned step, unsigned n) {
+                    constexpr int AT_ONCE = 32 / (R * DP) > 0 ? 32 / (R * DP) : 1;
+                    float o[AT_ONCE][DP][R];
+                    const auto fetch = [&](unsigned i0) {
 #pragma unroll
-                        for (unsigned i = 0; i < 8; i++) {
-                            const size_t at = (size_t)slot_of(first + (i0 + i < n ? i0 + i : 0) * step) * MAX_ROWS + r;
-                            x[i] = __ldcg(pml + at);
-                            o[i] = __ldcg(pv + at * D + pl * 128 + gt);
-                            if (i0 + i >= n) x[i] = make_float2(-inf, 0.f);
+                        for (int i = 0; i < AT_ONCE; i++)
+#pragma unroll
+                            for (int r = 0; r < R; r++)
+#pragma unroll
+                                for (int pl = 0; pl < DP; pl++) {
+                                    o[i][pl][r] = 0.f;
+                                    if (i0 + i < n && r < rows && writes) o[i][pl][r] = __ldcg(pv + ((size_t)slot_of(first + (i0 + i) * step) * MAX_ROWS + r) * D + pl * 128 + gt);
+                                }
+                    };
+                    fetch(0);
+                    {                                                          // eight threads to a row, two parts each: what each part counts for
+                        const int r = gt >> 3, i0 = gt & 7;
+                        float2 x[2];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            x[i] = make_float2(-inf, 0.f);
+                            if (r < rows && i0 + 8 * i < (int)n) x[i] = __ldcg(pml + (size_t)slot_of(first + (i0 + 8 * i) * step) * MAX_ROWS + r);
                         }
-                        float m = top;
+                        float top = fmaxf(x[0].x, x[1].x), sum = 0.f;
 #pragma unroll
-                        for (unsigned i = 0; i < 8; i++) m = fmaxf(m, x[i].x);
-                        const float back = top == -inf ? 1.f : ex2(top - m);
-                        top = m;
-                        sum *= back;
-                        v *= back;
+                        for (int k = 4; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
 #pragma unroll
-                        for (unsigned i = 0; i < 8; i++) {
-                            if (x[i].x == -inf && x[i].y == 0.f) continue;
-                            const float f = x[i].x == -inf ? 1.f : ex2(x[i].x - top);            // -inf and a sum: not a number
+                        for (int i = 0; i < 2; i++) {
+                            const float f = x[i].x != -inf ? ex2(x[i].x - top) : x[i].y == 0.f ? 0.f : 1.f;      // -inf and a sum: not a number
                             sum += x[i].y * f;
-                            v += o[i] * f;
+                            coef[(i0 + 8 * i) * MAX_ROWS + r] = f;
                         }
+#pragma unroll
+                        for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                        if (i0 == 0) { coef[FAN * MAX_ROWS + r] = top; coef[(FAN + 1) * MAX_ROWS + r] = sum; }
                     }
-                    out(r, pl, v, top, sum);
+                    sync();
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        tops[r] = coef[FAN * MAX_ROWS + r];
+                        l[r] = coef[(FAN + 1) * MAX_ROWS + r];
+#pragma unroll
+                        for (int pl = 0; pl < DP; pl++) acc[pl][r] = 0.f;
+                    }
+#pragma unroll 1
+                    for (unsigned i0 = 0;;) {
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; i++)
+                            if (i0 + i < n)
+#pragma unroll
+                                for (int r = 0; r < R; r++)
+#pragma unroll
+                                    for (int pl = 0; pl < DP; pl++) acc[pl][r] = fmaf(o[i][pl][r], coef[(i0 + i) * MAX_ROWS + r], acc[pl][r]);
+                        i0 += AT_ONCE;
+                        if (i0 >= n) break;
+                        fetch(i0);
+                    }
+                };
+                leave(a.part_ml, a.part, 2 * cta + (w.first ? 1 : 0));
+                const unsigned g0 = c0 + (cta - c0) / FAN * FAN, in_group = min((unsigned)FAN, c1 - g0 + 1);
+                if (!last_of(a.count + slot_of(g0), in_group)) continue;
+                join(a.part_ml, a.part, g0, 1, in_group);
+                if (groups > 1) {
+                    leave(a.part2_ml, a.part2, slot_of(g0));
+                    if (!last_of(a.count2 + slot_of(c0), groups)) continue;
+                    join(a.part2_ml, a.part2, c0, FAN, groups);
                 }
-            };
-            const unsigned g0 = c0 + (cta - c0) / FAN * FAN, in_group = min((unsigned)FAN, c1 - g0 + 1);
-            if (!last_of(a.count + slot_of(g0), in_group)) continue;
-            if (groups == 1) { join(a.part_ml, a.part, g0, 1, in_group, finish); continue; }
-            join(a.part_ml, a.part, g0, 1, in_group, [&](int r, int pl, float v, float top, float sum) {
-                const size_t at = (size_t)slot_of(g0) * MAX_ROWS + r;
-                a.part2[at * D + pl * 128 + gt] = v;
-                if (gt == 0 && pl == 0) a.part2_ml[at] = make_float2(top, sum);
-            });
-            if (last_of(a.count2 + slot_of(c0), groups)) join(a.part2_ml, a.part2, c0, FAN, groups, finish);
+            }
+            if (!writes) continue;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (r < rows) {
+                    const int rho = row0 + r, query = rho / a.G, head = w.h * a.G + rho - query * a.G;
+                    const float inv = l[r] > 0.f ? 1.f / l[r] : (l[r] == 0.f ? 0.f : l[r]);          // nothing seen: zeros
+#pragma unroll
+                    for (int pl = 0; pl < DP; pl++)
+                        static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), l[r] == 0.f ? 0.f : acc[pl][r] * inv);
+                    if (a.lse && gt == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = l[r] > 0.f ? (tops[r] + log2f(l[r])) * LN2 : (l[r] == 0.f ? -inf : l[r]);
+                }
         }
     }
     __syncthreads();
