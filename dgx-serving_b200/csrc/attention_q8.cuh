@@ -33,7 +33,7 @@ constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;
 constexpr float TOP = 28.f, LIMIT = 30.9f; // log2 of the largest weight when B is chosen, and beyond which it moves (four signed digits reach 2^30.99)
-constexpr int START = 3;                   // tiles whose time beginning and ending a pair takes
+constexpr int START = 4;                   // tiles whose time beginning and ending a pair takes
 constexpr int FLUSH = 900;                 // tiles after which O is read out at the latest: 128 * 128 * 127 * 900 < 2^31
 
 struct Args {
@@ -169,6 +169,7 @@ __device__ __forceinline__ float row_factor(float amax) {
     return __int_as_float((e + 127) << 23);
 }
 
+__device__ __forceinline__ float warp_max(float x) { float y; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // cap * tanh(x) * log2 e with x in units of cap: 1 - 2 / (1 + e^2x), whose error is that of a number near 1
 __device__ __forceinline__ float capped(float x, float cap) { return cap * LOG2E * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.f * LOG2E)))); }
@@ -432,29 +433,32 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         if (!ok) for (int i = 0; i < 64; i++) __nanosleep(50000);    // copies in flight end before the CTA's shared memory is another's
     } else if (warp == 11) {
         // ---- queries: the next pair's, while the others are at one --------------------------------------------------------------------------
+        // The code is kept short: an SM comes here cold, and sixteen rows unrolled took 11 us to fetch.
         constexpr int LPR = D == 64 ? 16 : 32, RPW = 32 / LPR, PER = D == 256 ? 2 : 1;         // lanes to a row, rows at a time, words of four of a lane
-        constexpr int TURNS = R / RPW;                                                         // their loads are all in flight at once
+        constexpr int TURNS = R / RPW < 4 ? R / RPW : 4, BATCH = TURNS * RPW;                  // rows whose loads are in flight together
         Walk walk(a, cum, u0, u1, R);
         Segment s;
         const int sub = lane / LPR, col = lane % LPR;
         for (int k = 0;; k++) {
             const bool more = walk.next(s);
             const int rows = more ? min(R, s.x.n * a.G - s.rg * R) : 0;
+            // lane = row
+            const int rho = s.rg * R + lane, query = more ? rho / a.G : 0, pos = s.x.seq - s.x.n + query;
+            const long long from = (long long)(s.x.q0 + query) * a.ldq + (long long)(s.h * a.G + rho - query * a.G) * D;
             float4 v[TURNS][PER];
-            int pos[TURNS] = {};
+            const auto fetch = [&](int r0) {
 #pragma unroll
-            for (int i = 0; i < TURNS; i++) {
-                const int r = i * RPW + sub;
+                for (int i = 0; i < TURNS; i++) {
+                    const int r = r0 + i * RPW + sub;
+                    const T *src = static_cast<const T *>(a.q) + __shfl_sync(0xffffffffu, from, r);
 #pragma unroll
-                for (int e = 0; e < PER; e++) v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < rows) {
-                    const int rho = s.rg * R + r, query = rho / a.G, head = s.h * a.G + rho - query * a.G;
-                    const T *src = static_cast<const T *>(a.q) + (long long)(s.x.q0 + query) * a.ldq + (long long)head * D;
-                    pos[i] = s.x.seq - s.x.n + query;
-#pragma unroll
-                    for (int e = 0; e < PER; e++) v[i][e] = load4(src + 4 * (col + 32 * e));
+                    for (int e = 0; e < PER; e++) {
+                        v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (r < rows) v[i][e] = load4(src + 4 * (col + 32 * e));
+                    }
                 }
-            }
+            };
+            fetch(0);
             if (k >= 2 && !wait_idle(Q_EMPTY + 8 * (k & 1), (k / 2 - 1) & 1)) give_up(3u);
             if (!ok) break;
             if (lane == 0) {
@@ -469,43 +473,60 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             }
             if (more) {
                 unsigned char *to = qs + (k & 1) * S::QB;
+#pragma unroll 1
+                for (int r0 = 0; r0 < R && (r0 < rows || k < 2); r0 += BATCH) {  // (rows of an earlier segment: what they give is not read)
+                    uint32_t mine = 0;                                           // lane = row: bits of its largest magnitude
 #pragma unroll
-                for (int i = 0; i < TURNS; i++) {
-                    if (i * RPW >= rows && k >= 2) break;                        // (rows of an earlier segment: what they give is not read)
-                    const int r = i * RPW + sub;
-                    uint32_t most = 0;                                           // bits of the largest magnitude; from those of infinity on: not a number
+                    for (int i = 0; i < TURNS; i++) {
+                        uint32_t most = 0;
 #pragma unroll
-                    for (int e = 0; e < PER; e++)
-                        most = max(max(most, max(__float_as_uint(v[i][e].x) & 0x7FFFFFFFu, __float_as_uint(v[i][e].y) & 0x7FFFFFFFu)),
-                                   max(__float_as_uint(v[i][e].z) & 0x7FFFFFFFu, __float_as_uint(v[i][e].w) & 0x7FFFFFFFu));
-                    if constexpr (LPR == 32) most = __reduce_max_sync(0xffffffffu, most);
-                    else {
+                        for (int e = 0; e < PER; e++)
+                            most = max(max(most, max(__float_as_uint(v[i][e].x) & 0x7FFFFFFFu, __float_as_uint(v[i][e].y) & 0x7FFFFFFFu)),
+                                       max(__float_as_uint(v[i][e].z) & 0x7FFFFFFFu, __float_as_uint(v[i][e].w) & 0x7FFFFFFFu));
+                        if constexpr (LPR == 32) {
+                            most = __reduce_max_sync(0xffffffffu, most);
+                            if (lane == r0 + i) mine = most;
+                        } else {
 #pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    }
-                    const float amax = __uint_as_float(most), bad = most >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.f;     // digits cannot tell
-                    // the row in units of its last digit: amax becomes 127 * 256^2; by a power of two first, so that neither factor leaves fp32
-                    const float p2 = row_factor(amax), f = amax > 0.f ? 127.f * 65536.f / (amax * p2) : 1.f;
-#pragma unroll
-                    for (int e = 0; e < PER; e++) {
-                        const float y[4] = {v[i][e].x, v[i][e].y, v[i][e].z, v[i][e].w};
-                        uint32_t w[4];
-#pragma unroll
-                        for (int m = 0; m < 4; m++) w[m] = (uint32_t)(__float2int_rn(y[m] * p2 * f) + 0x8080) ^ 0x8080u;     // signed digits in bytes 2, 1, 0
-                        const int d = 4 * col;                                   // of plane e
-#pragma unroll
-                        for (int g = 0; g < 3; g++) {
-                            const int n = 3 * r + g;
-                            const uint32_t sel = g == 0 ? 0x0062u : g == 1 ? 0x0051u : 0x0040u;
-                            const uint32_t word = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
-                            const int at = D == 64 ? n * 64 + (((d >> 4) ^ ((n >> 1) & 3)) << 4) + (d & 15) : e * N * 128 + n * 128 + (((d >> 4) ^ (n & 7)) << 4) + (d & 15);
-                            *reinterpret_cast<uint32_t *>(to + at) = word;
+                            for (int o = LPR / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, most, 16);
+                            if (lane >> 1 == (r0 >> 1) + i) mine = (lane & 1) == sub ? most : other;
                         }
                     }
-                    if (col == 0)
-                        rec[(k & 1) * R + r] = make_float4(a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
-                                                           __int_as_float(a.causal ? min(pos[i], s.x.seq - 1) : s.x.seq - 1),
-                                                           __int_as_float(a.window > 0 ? max(0, pos[i] - a.window + 1) : 0));
+                    // the row in units of its last digit: amax becomes 127 * 256^2; by a power of two first, so that neither factor leaves fp32
+                    const float amax = __uint_as_float(mine), bad = mine >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.f;     // digits cannot tell infinities
+                    const float p2 = row_factor(amax), f = amax > 0.f ? 127.f * 65536.f / (amax * p2) : 1.f;
+                    if (lane >= r0 && lane < r0 + BATCH)
+                        rec[(k & 1) * R + lane] = make_float4(a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
+                                                              __int_as_float(a.causal ? min(pos, s.x.seq - 1) : s.x.seq - 1),
+                                                              __int_as_float(a.window > 0 ? max(0, pos - a.window + 1) : 0));
+#pragma unroll
+                    for (int i = 0; i < TURNS; i++) {
+                        const int r = r0 + i * RPW + sub;
+                        const float g2 = __shfl_sync(0xffffffffu, p2, r), g1 = __shfl_sync(0xffffffffu, f, r);
+#pragma unroll
+                        for (int e = 0; e < PER; e++) {
+                            const float y[4] = {v[i][e].x, v[i][e].y, v[i][e].z, v[i][e].w};
+                            uint32_t w[4];
+#pragma unroll
+                            for (int m = 0; m < 4; m++) w[m] = (uint32_t)(__float2int_rn(y[m] * g2 * g1) + 0x8080) ^ 0x8080u;     // signed digits in bytes 2, 1, 0
+                            const int d = 4 * col;                               // of plane e
+#pragma unroll
+                            for (int g = 0; g < 3; g++) {
+                                const int n = 3 * r + g;
+                                const uint32_t sel = g == 0 ? 0x0062u : g == 1 ? 0x0051u : 0x0040u;
+                                const uint32_t word = __byte_perm(__byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel), 0x5410);
+                                const int at = D == 64 ? n * 64 + (((d >> 4) ^ ((n >> 1) & 3)) << 4) + (d & 15) : e * N * 128 + n * 128 + (((d >> 4) ^ (n & 7)) << 4) + (d & 15);
+                                *reinterpret_cast<uint32_t *>(to + at) = word;
+                            }
+                        }
+                    }
+                    if (r0 + BATCH < rows) fetch(r0 + BATCH);
+                    else
+#pragma unroll
+                        for (int i = 0; i < TURNS; i++)
+#pragma unroll
+                            for (int e = 0; e < PER; e++) v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
                 ptx::fence_proxy_async_smem();
             }
@@ -646,7 +667,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     columns_arrived(v);
 #pragma unroll
                     for (int r = 0; r < STEP; r++) {
-                        const float s = fmaf((float)(int)v[3 * r], 65536.f, (float)((int)v[3 * r + 1] * 256 + (int)v[3 * r + 2]));
+                        // |sum| <= 128 * 127 * 256 < 2^22: to fp32 by the bits of 1.5 * 2^23, which is quicker than a conversion
+                        const auto whole = [](uint32_t n) { return __uint_as_float(n + 0x4B400000u) - 12582912.f; };
+                        const float s = fmaf(whole(v[3 * r]), 65536.f, fmaf(whole(v[3 * r + 1]), 256.f, whole(v[3 * r + 2])));
                         y[r0 + r] = fmaf(s, fac(r0 + r) * sc.x, sc.y);
                     }
                 }
@@ -669,9 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     // a weight would pass 2^31: B moves to where the row's largest is 2^28; what is summed, to the new B
 #pragma unroll
                     for (int r = 0; r < R; r++) {
-                        float m = y[r];
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const float m = warp_max(y[r]);
                         if (lane == 0) red[gw * R + r] = m;
                     }
                     if (since) read_o();
