@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         constexpr int LPR = D == 64 ? 16 : 32, RPW = 32 / LPR, PER = D == 256 ? 2 : 1;         // lanes to a row, rows at a time, words of four of a lane
         constexpr int TURNS = R / RPW < 4 ? R / RPW : 4, BATCH = TURNS * RPW;                  // rows whose loads are in flight together
         Walk walk(a, cum, u0, u1, R);
-        Segment s;
+        Segment s = {};
         const int sub = lane / LPR, col = lane % LPR;
         for (int k = 0;; k++) {
             const bool more = walk.next(s);
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             const int rho = s.rg * R + lane, query = more ? rho / a.G : 0, pos = s.x.seq - s.x.n + query;
             const long long from = (long long)(s.x.q0 + query) * a.ldq + (long long)(s.h * a.G + rho - query * a.G) * D;
             float4 v[TURNS][PER];
-            const auto fetch = [&](int r0) {
+            const auto fetch = [&](int r0, float4 (&v)[TURNS][PER]) {
 #pragma unroll
                 for (int i = 0; i < TURNS; i++) {
                     const int r = r0 + i * RPW + sub;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     }
                 }
             };
-            fetch(0);
+            fetch(0, v);
             if (k >= 2 && !wait_idle(Q_EMPTY + 8 * (k & 1), (k / 2 - 1) & 1)) give_up(3u);
             if (!ok) break;
             if (lane == 0) {
@@ -475,6 +475,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 unsigned char *to = qs + (k & 1) * S::QB;
 #pragma unroll 1
                 for (int r0 = 0; r0 < R && (r0 < rows || k < 2); r0 += BATCH) {  // (rows of an earlier segment: what they give is not read)
+                    float4 next[TURNS][PER];
+                    if (R > BATCH) fetch(r0 + BATCH, next);
                     uint32_t mine = 0;                                           // lane = row: bits of its largest magnitude
 #pragma unroll
                     for (int i = 0; i < TURNS; i++) {
@@ -521,12 +523,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                             }
                         }
                     }
-                    if (r0 + BATCH < rows) fetch(r0 + BATCH);
-                    else
+                    if (R > BATCH)
 #pragma unroll
                         for (int i = 0; i < TURNS; i++)
 #pragma unroll
-                            for (int e = 0; e < PER; e++) v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            for (int e = 0; e < PER; e++) v[i][e] = next[i][e];
                 }
                 ptx::fence_proxy_async_smem();
             }
