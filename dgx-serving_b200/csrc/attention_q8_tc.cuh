@@ -213,7 +213,7 @@ __device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, f
 // the 32 at `dst`; the second term `term` bytes on).  fac[row]: what brings a score back, without a.scale.  Rows from `there` on are zeros.
 template <typename T, int D, bool SPLIT, class RowAt>
 __device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac, bool minus, int there, int lane, RowAt &&row_at) {
-    constexpr int N = kv::Row<T>::N, LPR = D / N, PER = LPR > 32 ? LPR / 32 : 1, RPW = LPR >= 32 ? 1 : 32 / LPR, BATCH = 32 / RPW < 8 ? 32 / RPW : 8 / PER;
+    constexpr int N = kv::Row<T>::N, LPR = D / N, PER = LPR > 32 ? LPR / 32 : 1, RPW = LPR >= 32 ? 1 : 32 / LPR, BATCH = 32 / RPW < 16 / PER ? 32 / RPW : 16 / PER;
     const int sub = LPR >= 32 ? 0 : lane / LPR, col = lane & (LPR >= 32 ? 31 : LPR - 1);
 #pragma unroll 1
     for (int r0 = 0; r0 < 32; r0 += RPW * BATCH) {
@@ -228,16 +228,20 @@ __device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac,
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
             const int r = r0 + b * RPW + sub;
-            float x[PER][N], amax = 0.f;
+            float x[PER][N];
+            uint32_t most = 0;                                                 // bits of the largest magnitude
 #pragma unroll
             for (int q = 0; q < PER; q++) {
                 kv::Row<T>::unpack(raw[b][q], x[q]);
 #pragma unroll
-                for (int e = 0; e < N; e++) amax = fmaxf(amax, fabsf(x[q][e]));
+                for (int e = 0; e < N; e++) most = max(most, __float_as_uint(x[q][e]) & 0x7FFFFFFFu);
             }
+            if constexpr (LPR >= 32) most = __reduce_max_sync(0xffffffffu, most);
+            else {
 #pragma unroll
-            for (int o = (LPR >= 32 ? 32 : LPR) / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            float f = attn::row_factor(amax);
+                for (int o = LPR / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            }
+            float f = attn::row_factor(__uint_as_float(most));
             if (col == 0) fac[r] = 1.f / f;
             if (minus) f = -f;
 #pragma unroll
@@ -265,11 +269,29 @@ __device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac,
 
 // The block is launched with 128 registers a thread; the rows' two warpgroups take 200, the others keep 56: 2 * 128 * (200 + 56) = 512 * 128.
 
-// N columns of a row out.
-template <int N, typename T> __device__ __forceinline__ void put(T *dst, const float (&y)[N], float inv) {
+// N columns of a thread's row, times inv, into the staging rows of its warp: `bytes` a row, piece c of 16 bytes at c ^ (row & 7).
+template <int N, typename T> __device__ __forceinline__ void stage(uint32_t at, int row, int col, const float (&y)[N], float inv) {
+    constexpr int E = 16 / sizeof(T);
 #pragma unroll
-    for (int e = 0; e < N; e += 4)
-        attn::store4(dst + e, inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv));
+    for (int e = 0; e < N; e += E) {
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = inv == 0.f ? 0.f : y[e + i] * inv;
+        const uint4 w = kv::Row<T>::pack(x);
+        sts128(at + ((((col + e) / E) ^ (row & 7)) << 4), w.x, w.y, w.z, w.w);
+    }
+}
+// The staged 32 rows of a warp (the first at `at`, `stride` bytes apart, pieces from `piece0` on) to memory, whole rows at a time; lane = row of `dst`.
+template <int N, typename T> __device__ __forceinline__ void rows_out(uint32_t at, uint32_t stride, int piece0, T *dst, int there, int lane) {
+    constexpr int PIECES = N * (int)sizeof(T) / 16, ROWS = 32 / PIECES;
+    __syncwarp();
+#pragma unroll 4
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+        const int r = r0 + lane / PIECES, c = lane % PIECES;
+        T *to = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+        const uint4 w = attn::lds128(at + r * stride + (((piece0 + c) ^ (r & 7)) << 4));
+        if (r < there) *reinterpret_cast<uint4 *>(to + c * (16 / (int)sizeof(T))) = w;
+    }
 }
 // O = O * by + 128 columns of tensor memory.
 __device__ __forceinline__ void add_columns(float (&O)[128], uint32_t at, float by) {
@@ -464,9 +486,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             shrinks[0][tid] = inv;
             asm volatile("bar.sync 3, 256;" ::: "memory");
         }
+        // through shared memory, where Q was (every product is done): stored by its own thread a row took 16 bytes of each of 32 rows at a time
         T *dst = static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D;
+        constexpr uint32_t ROW = D * sizeof(T);
+        static_assert(sizeof(T) == 2 * TERMS, "a row of the output takes what its terms took");
+        const uint32_t rows_at = base + t * TERMS * S::QT + (tid & 96) * ROW, row_at = rows_at + lane * ROW;
+        const int there = rows - (row0 + t * 128 + (tid & 96));
         if constexpr (SPLIT) {
-            if (row < rows) put<OWN>(dst, O, inv);
+            stage<OWN, T>(row_at, lane, 0, O, inv);
+            rows_out<OWN, T>(rows_at, ROW, 0, dst, there, lane);
         } else {
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
@@ -480,8 +508,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e++) y[e] = __uint_as_float(o[e]);
-                if (row < rows) put<32>(dst + 32 * c, y, inv);
+                stage<32, T>(row_at, lane, 32 * c, y, inv);
             }
+            rows_out<D, T>(rows_at, ROW, 0, dst, there, lane);
         }
         if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (B + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
         ptx::tc_fence_before_sync();
@@ -509,7 +538,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         }
         asm volatile("bar.sync 4, 256;" ::: "memory");
         asm volatile("bar.sync 3, 256;" ::: "memory");
-        if (row < rows) put<128>(static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, O, shrinks[0][lr]);
+        const uint32_t rows_at = base + (tid & 96) * (D * sizeof(T));
+        stage<128, T>(rows_at + lane * (D * sizeof(T)), lane, 128, O, shrinks[0][lr]);
+        rows_out<128, T>(rows_at, D * sizeof(T), 32, static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, rows - (row0 + (tid & 96)), lane);
         ptx::tc_fence_before_sync();
     } else if (warp >= 8 && warp < 12) {
         // ---- codes to fp16 -------------------------------------------------------------------------------------------------------------
