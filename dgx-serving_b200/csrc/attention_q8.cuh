@@ -11,13 +11,16 @@
 //  - Both products are tcgen05.mma kind::i8 with the keys' tile as the 128-row operand, so the codes go from HBM by TMA to shared memory (128-byte
 //    swizzle; along the block table, a block never has to be a whole tile) and no thread touches them: S^T [keys][rows] = K Q^T with K as it
 //    lies, O^T [dim][rows] += V^T P^T with V read as the transposed operand.  Widening the codes to fp16 for mma.sync cost 450 instructions for 16
-//    keys and bound the stream: two requests of 130k tokens 96 us, 64 ragged ones 128.
+//    keys and bound the stream: two requests of 115k tokens 96 us, 64 ragged ones of up to 8192 tokens 128.  Now 84 us (5.9 TB/s) and 99 (5.5).
 //  - A query row is a fixed-point number relative to its largest magnitude, three signed digits of base 256 (2^-23 of it): three columns.  A weight
 //    is a whole number too, x = exp(s - B) * vs up to 2^31, four columns of P.  All sums are whole numbers and exact; O stays in tensor memory over
 //    the tiles.  The row's reference B is such that its largest x was 2^28 when it was chosen; when an x would pass 2^31, O is read out, rescaled
 //    and summed in fp32, and B moves.  So a weight is rounded to 2^-28 of the row's largest, or as fp32 is.
-//  - 128 threads have a key each, about forty instructions for a row.  Two such groups take the tiles in turn, each with its own S, P, O, reference and
-//    sums, because a tile's chain of steps takes longer than its bytes do; they meet at the end of a pair, one handing over, the other writing.
+//  - 128 threads have a key each, about thirty instructions for a row.  Two such groups take the tiles in turn, each with its own S, P, O, reference and
+//    sums, because a tile's chain of steps (1300 cycles with 4 rows, 3500 with 16) takes longer than its bytes do; they meet at the end of a pair, one
+//    handing over, the other writing.
+//  - What is left: 3 us before the first tile and 3 us for the last join, and for many rows the chain: 16 requests of up to 56 rows and 6000 tokens take
+//    52 us where their bytes take 9.
 #pragma once
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"
@@ -29,11 +32,12 @@ namespace attn {
 constexpr int TK = 128;                    // keys of a tile
 constexpr int THREADS = 384;               // warps 0-3, 4-7: a key (then a dim) a thread; 8, 9: copies of K, of V; 10: products; 11: queries
 constexpr int MAX_R = 2048;                // requests of one launch (their sums lie in shared memory)
-constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) of a request that this kernel takes at most
+constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) of a request that this kernel takes at most: half a row tile of the other
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;
 constexpr float TOP = 28.f, LIMIT = 30.9f; // log2 of the largest weight when B is chosen, and beyond which it moves (four signed digits reach 2^30.99)
-constexpr int START = 4;                   // tiles whose time beginning and ending a pair takes
+constexpr int START = 4;                   // tiles whose time beginning and ending a pair takes (64 ragged requests: 104.5 us with 1, 99.3 with 4, 100.7 with 6)
+constexpr float UNIT = 0x1p-64f;           // sums of exp(s - B) are in units of 2^64, so that weights up to 2^31 times 1 / vs up to 2^100 stay in fp32
 constexpr int FLUSH = 900;                 // tiles after which O is read out at the latest: 128 * 128 * 127 * 900 < 2^31
 
 struct Args {
@@ -55,13 +59,6 @@ struct Args {
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-
-// Bytes (lo: 0 and 1, hi: 2 and 3) of a word of codes + 128 as two fp16 numbers, minus the 128 again: 0x6400 | u is 1024 + u.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t u) {
-    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
-    return h2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480))));   // 1152
-}
 
 // ---- which keys and how much work ----------------------------------------------------------------------------------------------------
 struct Request {
@@ -127,16 +124,6 @@ struct Walk {
     }
 };
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
-}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -152,15 +139,6 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
 }
-__device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
-__device__ __forceinline__ void store4(__half *p, float4 v) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(h2_bits(__floats2half2_rn(v.x, v.y)), h2_bits(__floats2half2_rn(v.z, v.w)));
-}
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-}
-
 // Power of two that brings a row whose largest magnitude is amax near 2^13, and its inverse times `scale`.
 __device__ __forceinline__ float row_factor(float amax) {
     if (!(amax > 0.f) || !(amax < __int_as_float(0x7f800000))) return 1.f;
@@ -207,9 +185,6 @@ __device__ __forceinline__ bool wait_idle(uint32_t bar, uint32_t parity) {
     }
     return __all_sync(0xffffffffu, ok);
 }
-template <int N> __device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 // What the warps have to know of a segment, left by the one that prepares its queries.  tiles 0: there is no further one.
 struct Work { int tiles, tile0, min_hi, max_lo, n, q0, rg, h, first, pair0, pair_tiles, pad; };   // keys up to min_hi and from max_lo on: every row sees them
 constexpr int WORKS = 4;
@@ -415,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 const bool in = mine_t == t, here = in && now.mine;
                 if (is_k && in) {                                  // vs 0: its block's weights are as good as 0, and their sum comes out right
                     const float v1 = fmaxf(now.vs, 0x1p-100f);
-                    scales[stage * S::SCALES + pc] = make_float4(now.ks, lg2(v1), 1.f / v1, 0.f);
+                    scales[stage * S::SCALES + pc] = make_float4(now.ks, lg2(v1), UNIT / v1, 0.f);
                 }
                 const unsigned count = __popc(__ballot_sync(0xffffffffu, here));
                 __syncwarp();                                      // the scales are there before the arrival
@@ -898,8 +873,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     const float inv = l[r] > 0.f ? 1.f / l[r] : (l[r] == 0.f ? 0.f : l[r]);          // nothing seen: zeros
 #pragma unroll
                     for (int pl = 0; pl < DP; pl++)
-                        static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), l[r] == 0.f ? 0.f : acc[pl][r] * inv);
-                    if (a.lse && gt == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = l[r] > 0.f ? (tops[r] + log2f(l[r])) * LN2 : (l[r] == 0.f ? -inf : l[r]);
+                        static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), l[r] == 0.f ? 0.f : acc[pl][r] * UNIT * inv);
+                    if (a.lse && gt == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = l[r] > 0.f ? (tops[r] + (log2f(l[r]) + 64.f)) * LN2 : (l[r] == 0.f ? -inf : l[r]);
                 }
         }
     }

@@ -12,7 +12,11 @@
 //    block's scale in the exponent: x = exp2(f s + log2 vs - B), one multiply-add and one exp2; the sum divides it out again once per block
 //    and row.  B is such that the largest x was 2^8 when B was chosen; it moves, and O in tensor memory is rescaled, only when an x would
 //    pass 2^15.
-//  - fp32 rows enter as two fp16 terms each, Q and P, as in attention_q8.cuh: twice the products, 22 bits.
+//  - fp32 rows enter as two fp16 terms each, Q and P: twice the products, 22 bits.
+// One prompt of 4096 tokens, 32 heads of 128 over 8, causal: 206 us, 668 TFLOP/s of the 1633 that a large product reaches.  A step of two row
+// tiles and 128 keys takes about 4600 cycles where its products take 2100 and its exponentials 2050: the row's warps, two on a scheduler, are in
+// the way, with the maximum (850), the wait for the scores (1450) and the weights (2500).  Steps of 64 keys with two buffers of scores for each row
+// tile hid the wait, and had every step's fixed costs twice: 240 us.
 #pragma once
 #include "attention_q8.cuh"
 
@@ -24,14 +28,12 @@ using attn::LN2;
 using attn::ex2;
 using attn::lg2;
 using attn::capped;
-using attn::lds_f4;
 using attn::elected;
 using attn::umma_commit;
 using attn::wait_one;
 using attn::wait_warp;
-using attn::raise_registers;
-using attn::lower_registers;
 using attn::h2_bits;
+using attn::sts128;
 constexpr unsigned ERR_WAIT = 0xB00u;
 constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
 constexpr int MAX_R = 2048;
@@ -81,14 +83,27 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+// Bytes (lo: 0 and 1, hi: 2 and 3) of a word of codes + 128 as two fp16 numbers, minus the 128 again: 0x6400 | u is 1024 + u.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t u) {
+    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
+    return h2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480))));   // 1152
 }
 // Four bytes of codes as two packed pairs of fp16.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &a, uint32_t &b) {
     w ^= 0x80808080u;
-    a = attn::codes_f16<0x4140>(w);
-    b = attn::codes_f16<0x4342>(w);
+    a = codes_f16<0x4140>(w);
+    b = codes_f16<0x4342>(w);
 }
 
 __device__ __forceinline__ uint64_t pack2u(uint32_t a, uint32_t b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
@@ -268,6 +283,9 @@ __device__ __forceinline__ void rows_in(uint32_t dst, uint32_t term, float *fac,
 }
 
 // The block is launched with 128 registers a thread; the rows' two warpgroups take 200, the others keep 56: 2 * 128 * (200 + 56) = 512 * 128.
+template <int N> __device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 
 // N columns of a thread's row, times inv, into the staging rows of its warp: `bytes` a row, piece c of 16 bytes at c ^ (row & 7).
 template <int N, typename T> __device__ __forceinline__ void stage(uint32_t at, int row, int col, const float (&y)[N], float inv) {
@@ -289,7 +307,7 @@ template <int N, typename T> __device__ __forceinline__ void rows_out(uint32_t a
     for (int r0 = 0; r0 < 32; r0 += ROWS) {
         const int r = r0 + lane / PIECES, c = lane % PIECES;
         T *to = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-        const uint4 w = attn::lds128(at + r * stride + (((piece0 + c) ^ (r & 7)) << 4));
+        const uint4 w = lds128(at + r * stride + (((piece0 + c) ^ (r & 7)) << 4));
         if (r < there) *reinterpret_cast<uint4 *>(to + c * (16 / (int)sizeof(T))) = w;
     }
 }
@@ -565,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                         for (int it = 0; it < CH / 4; it++) {
                             const int flip = D == 64 ? 0 : 4 * (it & 1), off = 8 * (it >> 1);
                             const uint32_t c4 = odd4 ^ flip;                 // 0 or 4
-                            const uint4 w = attn::lds128(src + my_src + k0 * D + 16 * (c4 + off));
+                            const uint4 w = lds128(src + my_src + k0 * D + 16 * (c4 + off));
                             uint32_t f[8];
                             widen(w.x, f[0], f[1]);
                             widen(w.y, f[2], f[3]);

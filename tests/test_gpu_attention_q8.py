@@ -259,3 +259,16 @@ def test_decode_inside_a_graph(w4a8, cuda):
     g.replay()
     w4a8.device_status()
     assert np.array_equal(out[:3].cpu().numpy(), c.run()[0])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("vs", [0.0, 1e-25, 1e15])
+@pytest.mark.parametrize("news", [[1, 1, 5], [70, 1, 90]])
+def test_values_of_extreme_scale(w4a8, cuda, dtype, D, vs, news):
+    """All values zero (as rows of zeros are held: scale 0, codes 0), tiny or huge: the sum of the weights is what it is without them."""
+    c = Case(w4a8, cuda, [100, 17, 300], news, 8, 2, D, 16, dtype, seed=D)
+    c.vs[np.isfinite(c.vs)] = vs
+    if vs == 0.0:
+        c.v[:] = 0
+    c.check()
