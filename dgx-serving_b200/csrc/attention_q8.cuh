@@ -905,7 +905,7 @@ inline void lay_out(Args &a, void *workspace, int dim) {
 }
 
 template <typename T, int D, int R>
-inline int launch_t(const Call &c, cudaStream_t st) {
+inline int launch_t(const Call &c, int rows, cudaStream_t st) {
     using S = Shape<D, R>;
     auto kern = attention_q8_kernel<T, D, R>;
     const uint64_t tokens = (uint64_t)c.a.num_blocks * c.a.Hkv * c.a.block;
@@ -917,9 +917,13 @@ inline int launch_t(const Call &c, cudaStream_t st) {
         rc = tmap_cached(&mv, c.v, D == 64 ? 128 : D, D == 64 ? tokens / 2 : tokens, 128, D == 64 ? box / 2 : box, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != W4A8_OK) return rc;
-    for (int r0 = 0; r0 < c.a.R; r0 += MAX_R) {                    // requests beyond those: further launches
+    // units are counted in 31 bits: so many requests as full tables of them fit, the others in further launches
+    const double units = (double)c.a.Hkv * ((rows + R - 1) / R) * ((double)c.a.width * c.a.block / TK + 1 + START);
+    const int most = units * MAX_R < 2e9 ? MAX_R : (int)(2e9 / units);
+    if (most < 1) return fail(W4A8_ERR_UNSUPPORTED, "attention_q8: %.0f key tiles of a request", units);
+    for (int r0 = 0; r0 < c.a.R; r0 += most) {
         Args a = c.a;
-        a.R = c.a.R - r0 < MAX_R ? c.a.R - r0 : MAX_R;
+        a.R = c.a.R - r0 < most ? c.a.R - r0 : most;
         a.cu_q += r0;
         a.seq_len += r0;
         a.table += (size_t)r0 * a.width;
@@ -941,9 +945,9 @@ inline int launch_t(const Call &c, cudaStream_t st) {
 // The narrowest kernel that takes `rows` (queries x heads of a group of the request with most of them) at once.
 template <typename T, int D>
 inline int launch_d(const Call &c, int rows, cudaStream_t st) {
-    if (rows <= 4) return launch_t<T, D, 4>(c, st);
-    if (rows <= 8) return launch_t<T, D, 8>(c, st);
-    return launch_t<T, D, 16>(c, st);
+    if (rows <= 4) return launch_t<T, D, 4>(c, rows, st);
+    if (rows <= 8) return launch_t<T, D, 8>(c, rows, st);
+    return launch_t<T, D, 16>(c, rows, st);
 }
 
 inline int launch(const Call &c, int rows, cudaStream_t st) {
