@@ -47,7 +47,7 @@ struct Args {
     const float *ks, *vs;
     const int32_t *table, *cu_q, *seq_len;
     long long ldq, ldo;
-    int R, T, width, Hq, Hkv, G, block, num_blocks, stages;
+    int R, T, width, Hq, Hkv, G, block, num_blocks, k_stages, v_stages;
     int causal, window;
     float scale, softcap;
     int few;                               // rows (queries * G) of a request that this kernel takes at most; more are another kernel's
@@ -251,16 +251,19 @@ template <int N> __device__ __forceinline__ void columns_arrived(uint32_t (&v)[N
 template <int D, int R_> struct Shape {
     static constexpr int R = R_, N = (3 * R + 15) / 16 * 16, NP = 4 * R, DP = D == 256 ? 2 : 1, OC = D == 64 ? 2 * NP : DP * NP;    // DP: dims of a thread; OC: columns of O
     static constexpr int P_ROW = D == 64 ? 2 * NP : NP;                              // bytes of P of a token (dim 64: of a pair of tokens)
-    static constexpr int STAGE = 2 * Tile<D>::BYTES, QB = N * D, PB = NP * TK;
+    static constexpr int STAGE = Tile<D>::BYTES, QB = N * D, PB = NP * TK;             // a stage: a tile of K or of V
     static constexpr int SCALES = 8;                                                   // blocks of a tile at most
-    static constexpr int MAX_STAGES = 8;
-    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + MAX_STAGES * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4 + 2 * (FAN + 2) * MAX_ROWS * 4;   // and 4 bytes a request
+    // K may leave as soon as its product is issued, V only when its weights are.  At dim 256 there are five stages in all, and K's leave early (requests with a
+    // window of 1024 tokens 44.7 -> 40.1 us); at the others K's loads would then run ahead of V's (two of 115k tokens 83.7 -> 87), so both leave together.
+    static constexpr bool EARLY = D == 256;
+    static constexpr int MAX_STAGES = 8, SLOTS = 16;                                   // of each side; tiles' scales, more than are between copy and scores
+    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + SLOTS * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4 + 2 * (FAN + 2) * MAX_ROWS * 4;   // and 4 bytes a request
     static inline int fixed_bytes(int n) { return (FIXED + (n + 4) * 4 + 1023) & ~1023; }
-    static inline int stages(int n) {
+    static inline int stages(int n) {                                                  // of both sides together
         const int k = (226 * 1024 - fixed_bytes(n)) / STAGE;
-        return k < MAX_STAGES ? k : MAX_STAGES;
+        return k < 2 * MAX_STAGES ? k : 2 * MAX_STAGES;
     }
-    static_assert(NP % 16 == 0 && 2 * N + 2 * OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 2 * STAGE <= 226 * 1024, "shape");
+    static_assert(NP % 16 == 0 && 2 * N + 2 * OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 4 * STAGE <= 226 * 1024, "shape");
 };
 
 template <typename T, int D, int R>
@@ -271,11 +274,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     extern __shared__ unsigned char smem_raw[];
     // ring, Q and P first (1024-byte aligned for the swizzle), then the rest
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *p = smem + (size_t)a.stages * S::STAGE;
+    unsigned char *p = smem + (size_t)(a.k_stages + a.v_stages) * S::STAGE;
     unsigned char *qs = p; p += 2 * S::QB;
     unsigned char *ps = p; p += 2 * S::PB;
     unsigned char *control = p; p += 1024;
-    float4 *scales = reinterpret_cast<float4 *>(p); p += S::MAX_STAGES * S::SCALES * 16;   // ks, log2 vs, 1 / vs of a stage's blocks
+    float4 *scales = reinterpret_cast<float4 *>(p); p += S::SLOTS * S::SCALES * 16;   // ks, log2 vs, 1 / vs of a tile's blocks
     float4 *rec = reinterpret_cast<float4 *>(p); p += 2 * R * 16;                          // a row's factor, B, last and first key (as int)
     float *reds = reinterpret_cast<float *>(p); p += 2 * 4 * R * 4;
     float2 *over_ml = reinterpret_cast<float2 *>(p); p += R * 8;                           // what one group hands over: B, sum; values
@@ -284,15 +287,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     float *coefs = reinterpret_cast<float *>(p); p += 2 * (FAN + 2) * MAX_ROWS * 4;         // joining: what a part counts for
     unsigned *cum = reinterpret_cast<unsigned *>(p);
     const uint32_t bar = ptx::smem_u32(control), ring_at = ptx::smem_u32(smem), q_at = ptx::smem_u32(qs), p_at = ptx::smem_u32(ps);
-    const uint32_t K_FULL = bar, V_FULL = bar + 64u, EMPTY = bar + 128u, S_FULL = bar + 192u, S_EMPTY = bar + 208u, P_FULL = bar + 224u, P_EMPTY = bar + 240u,
-                   Q_FULL = bar + 256u, Q_EMPTY = bar + 272u, OVER = bar + 288u;
+    const uint32_t K_FULL = bar, V_FULL = bar + 64u, K_EMPTY = bar + 128u, V_EMPTY = bar + 192u, S_FULL = bar + 256u, S_EMPTY = bar + 272u, P_FULL = bar + 288u,
+                   P_EMPTY = bar + 304u, Q_FULL = bar + 320u, Q_EMPTY = bar + 336u, OVER = bar + 352u, v_ring = ring_at + (uint32_t)a.k_stages * S::STAGE;
     __shared__ unsigned wsum[THREADS / 32], last_flags[2], tmem_slot;
     __shared__ int fresh[2];                                            // a tile's weights begin new sums in O
     __shared__ Work works[WORKS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int s = 0; s < S::MAX_STAGES; s++) { ptx::mbar_init(K_FULL + 8 * s, 1); ptx::mbar_init(V_FULL + 8 * s, 1); ptx::mbar_init(EMPTY + 8 * s, 1); }
+        for (int s = 0; s < S::MAX_STAGES; s++) { ptx::mbar_init(K_FULL + 8 * s, 1); ptx::mbar_init(V_FULL + 8 * s, 1); ptx::mbar_init(K_EMPTY + 8 * s, 1); ptx::mbar_init(V_EMPTY + 8 * s, 1); }
         for (int s = 0; s < 2; s++) {
             ptx::mbar_init(S_FULL + 8 * s, 1);
             ptx::mbar_init(S_EMPTY + 8 * s, 4);
@@ -351,7 +354,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         // ---- copies: lane = one piece (a block, or the part of it that lies in a tile); a batch is 32 pieces; this warp brings K or V -----------------
         const bool is_k = warp == 8;
         const CUtensorMap *map = is_k ? &map_k : &map_v;
-        const uint32_t full0 = is_k ? K_FULL : V_FULL;
+        const uint32_t full0 = is_k ? K_FULL : V_FULL, empty0 = is_k ? K_EMPTY : V_EMPTY, ring = is_k ? ring_at : v_ring;
+        const int stages = is_k ? a.k_stages : a.v_stages;
         Walk walk(a, cum, u0, u1, R);
         Segment s;
         int stage = 0, used = 0, t_next = 0;
@@ -386,22 +390,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             const Batch now = b;
             look_up();
             for (int t = 0; t < now.tiles; t++) {
-                if (used >= a.stages && !wait_idle(EMPTY + 8 * stage, phase ^ 1u)) { give_up(is_k ? 1u : 2u); break; }
+                if (used >= stages && !wait_idle(empty0 + 8 * stage, phase ^ 1u)) { give_up(is_k ? 1u : 2u); break; }
                 const bool in = mine_t == t, here = in && now.mine;
                 if (is_k && in) {                                  // vs 0: its block's weights are as good as 0, and their sum comes out right
                     const float v1 = fmaxf(now.vs, 0x1p-100f);
-                    scales[stage * S::SCALES + pc] = make_float4(now.ks, lg2(v1), UNIT / v1, 0.f);
+                    // the slot's last reader, the scores of tile used - SLOTS: this stage was free only after S of tile used - stages, and that came after them
+                    scales[(used & (S::SLOTS - 1)) * S::SCALES + pc] = make_float4(now.ks, lg2(v1), UNIT / v1, 0.f);
                 }
                 const unsigned count = __popc(__ballot_sync(0xffffffffu, here));
                 __syncwarp();                                      // the scales are there before the arrival
                 if (lane == 0) ptx::mbar_arrive_expect_tx(full0 + 8 * stage, count * (unsigned)(tokens * D));
                 if (here) {
-                    const uint32_t at = ring_at + (uint32_t)stage * S::STAGE + (is_k ? 0 : L::BYTES) + (uint32_t)(pc * tokens * (D == 256 ? 128 : D));
+                    const uint32_t at = ring + (uint32_t)stage * S::STAGE + (uint32_t)(pc * tokens * (D == 256 ? 128 : D));
 #pragma unroll
                     for (int pl = 0; pl < L::PLANES; pl++) ptx::tma_load_2d(at + pl * L::PLANE_BYTES, map, pl * 128, now.row, full0 + 8 * stage);
                 }
                 used++;
-                if (++stage == a.stages) { stage = 0; phase ^= 1u; }
+                if (++stage == stages) { stage = 0; phase ^= 1u; }
             }
             resolve();
         }
@@ -538,22 +543,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     umma_s8(lead, tmem + buf * N, kd, qd, id_s, k > 0);
                 }
                 umma_commit(lead, S_FULL + 8 * buf);
+                if (S::EARLY) umma_commit(lead, K_EMPTY + 8 * st);
                 if (--left == 0) { umma_commit(lead, Q_EMPTY + 8 * (nth & 1)); nth++; }
-                if (++st == a.stages) { st = 0; ph ^= 1u; }
+                if (++st == a.k_stages) { st = 0; ph ^= 1u; }
                 j++;
                 did = true;
             }
             if (i < j && there(P_FULL + 8 * (i & 1), (i >> 1) & 1) && there(V_FULL + 8 * pst, pph)) {
                 ptx::tc_fence_after_sync();
-                const uint32_t buf = i & 1, begin = fresh[buf] != 0, vb = ring_at + pst * S::STAGE + L::BYTES, pb = p_at + buf * S::PB;
+                const uint32_t buf = i & 1, begin = fresh[buf] != 0, vb = v_ring + pst * S::STAGE, pb = p_at + buf * S::PB;
 #pragma unroll
                 for (int pl = 0; pl < DP; pl++)
 #pragma unroll
                     for (int k = 0; k < (D == 64 ? 2 : 4); k++)
                         umma_s8(lead, o_cols + buf * S::OC + pl * NP, desc_mn(vb + pl * L::PLANE_BYTES + k * 32 * 128), desc_p<S::P_ROW>(pb + k * 32 * S::P_ROW), id_o, k > 0 || !begin);
-                umma_commit(lead, EMPTY + 8 * pst);
+                if (!S::EARLY) umma_commit(lead, K_EMPTY + 8 * pst);            // (as many stages as V)
+                umma_commit(lead, V_EMPTY + 8 * pst);
                 umma_commit(lead, P_EMPTY + 8 * buf);
-                if (++pst == a.stages) { pst = 0; pph ^= 1u; }
+                if (++pst == a.v_stages) { pst = 0; pph ^= 1u; }
                 i++;
                 did = true;
             }
@@ -568,8 +575,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         const int gt = tid & 127, gw = warp & 3, parity = D == 64 ? gt >> 6 : 0;
         float *red = reds + group * 4 * R;
         unsigned j = 0, before = 0;                                                 // tiles so far; this group's last one + 1
-        int st = 0;
-        uint32_t ph = 0;
         // what is the same for all threads of a row is in registers for few rows, for many in shared memory
         constexpr bool HELD = R <= 8;
         constexpr int STEP = R < 8 ? R : 8;                                          // rows whose scores are in registers at a time
@@ -625,14 +630,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 sync();
             }
             for (int t = 0; t < w.tiles; t++, j++) {
-                const int at_st = st;
-                if (++st == a.stages) { st = 0; ph ^= 1u; }
                 if ((j & 1) != group) continue;
                 const uint32_t buf = group;
                 const int key = (w.tile0 + t) * TK + gt;
                 if (ok && !wait_warp(S_FULL + 8 * buf, (j >> 1) & 1)) give_up(11u);
                 ptx::tc_fence_after_sync();
-                const float4 sc = scales[at_st * S::SCALES + (gt >> tshift)];
+                const float4 sc = scales[(j & (S::SLOTS - 1)) * S::SCALES + (gt >> tshift)];
                 // rows that the segment does not have go along: they are not read
                 float y[R];
                 bool again = held >= FLUSH;
@@ -927,8 +930,10 @@ inline int launch_t(const Call &c, int rows, cudaStream_t st) {
         a.cu_q += r0;
         a.seq_len += r0;
         a.table += (size_t)r0 * a.width;
-        a.stages = S::stages(a.R);
-        const size_t smem = (size_t)S::fixed_bytes(a.R) + (size_t)a.stages * S::STAGE;
+        const int stages = S::stages(a.R);                          // at most 2 * MAX_STAGES: neither side has more than MAX_STAGES
+        a.k_stages = stages / 2;
+        a.v_stages = S::EARLY ? stages - a.k_stages : a.k_stages;
+        const size_t smem = (size_t)S::fixed_bytes(a.R) + (size_t)(a.k_stages + a.v_stages) * S::STAGE;
         static PerDevice<size_t> configured_dev;
         size_t &configured = configured_dev.get();
         if (smem > configured) {
