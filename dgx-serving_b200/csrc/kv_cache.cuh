@@ -387,22 +387,35 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(ReadArgs a) {
     const int8_t *codes = blockIdx.y ? a.vc : a.kc;
     const float *scales = blockIdx.y ? a.vs : a.ks;
     T *out = static_cast<T *>(blockIdx.y ? a.v : a.k);
-    const int per = a.heads * VPR, total = a.tokens * per;
+    // piece c of token i, without a division for each; codes to fp32 through the bits of 2^23 + code + 128 (8192 tokens of 8 heads of 128, keys and
+    // values, to bf16: 9.7 us, 10.1 with a conversion each and divisions; the bytes alone take 7.7)
+    const int per = a.heads * VPR, total = a.tokens * per, step_i = READ_THREADS / per, step_c = READ_THREADS - step_i * per;
+    int i = tid / per, c = tid - i * per;
 #pragma unroll 4
     for (int e = tid; e < total; e += READ_THREADS) {
-        const int i = e / per, c = e - i * per, h = c / VPR, x = (c - h * VPR) * N;
-        if (unit[i] < 0) continue;
-        const size_t u = (size_t)unit[i] * a.heads + h;
-        const int8_t *p = codes + (u * a.block + place[i]) * D + x;
-        const float s = scales[u];
-        float y[N];
+        const int at = unit[i];
+        if (at >= 0) {
+            const int h = c / VPR, x = (c - h * VPR) * N;
+            const size_t u = (size_t)at * a.heads + h;
+            const int8_t *p = codes + (u * a.block + place[i]) * D + x;
+            const float s = scales[u];
+            uint32_t w[N / 4];
+            if constexpr (N == 4) w[0] = *reinterpret_cast<const uint32_t *>(p);
+            else {
+                const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                w[0] = v.x;
+                w[1] = v.y;
+            }
+            float y[N];
 #pragma unroll
-        for (int q = 0; q < N / 4; q++) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(p + 4 * q);
+            for (int q = 0; q < N / 4; q++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[4 * q + j] = (float)(int8_t)(w >> (8 * j)) * s;
+                for (int j = 0; j < 4; j++) y[4 * q + j] = (__uint_as_float(__byte_perm(w[q] ^ 0x80808080u, 0x4B000000u, 0x7540 + j)) - 8388736.f) * s;
+            *reinterpret_cast<uint4 *>(out + (size_t)(t0 + i) * a.ldo + h * D + x) = Row<T>::pack(y);
         }
-        *reinterpret_cast<uint4 *>(out + (size_t)(t0 + i) * a.ldo + h * D + x) = Row<T>::pack(y);
+        i += step_i;
+        c += step_c;
+        if (c >= per) { c -= per; i++; }
     }
 }
 
