@@ -4,7 +4,9 @@ Tolerance, from the number formats alone.  A score is a sum of dim products, eac
 rows), added in fp32 in at most dim / 16 + 2 roundings of 2^-23 of what is summed so far, then scaled twice: its error is at most
 A * 2^-23 * (dim / 16 + 8) with A = scale * sum |q| |k|.  A weight's relative error is that plus 2^-21 (exp2, its argument's rounding at
 magnitudes up to 64: 2^-18), and 2^-11 for the fp16 rounding of 16-bit rows.  The numerator and the denominator each carry it once, the
-fp32 sums over the keys add 2^-18: |o - o'| <= 2 * weight error * max |v|.  16-bit results add their own rounding, 2^-11 or 2^-8 of |o|.
+fp32 sums over the keys add 2^-18: |o - o'| <= 2 * weight error * max |v|.  (Requests of few rows: an element is held to 2^-24 of its row's largest
+magnitude and everything behind it is exact, which stays within A * 2^-23 * (dim / 16 + 8) while that largest is at most 2 * (dim / 16 + 8) = 24 times
+the rows' mean magnitude weighted by the keys; normally distributed rows have 4.)  16-bit results add their own rounding, 2^-11 or 2^-8 of |o|.
 """
 import numpy as np
 import pytest
