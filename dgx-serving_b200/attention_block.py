@@ -32,9 +32,12 @@ class PagedTables:
         self.cu = torch.zeros(requests + 1, **i32)
         self.status = torch.zeros(4, **i32)                  # [0]: the first free block of the next step
         self.first = torch.zeros(1, **i32)
+        self.slot = torch.empty(0, **i32)                    # of the step's rows
 
     def step(self, new_len, T):
-        """Room for new_len[r] tokens of each request (a tensor on the GPU), T rows in all; slots of the rows, -1 where there was none."""
+        """Room for new_len[r] tokens of each request (int32, on the GPU), T rows in all; slots of the rows, -1 where there was none."""
+        if new_len.dtype != torch.int32 or new_len.shape != (self.R,) or not new_len.is_contiguous() or new_len.device != self.table.device:
+            raise ValueError("new_len: %d int32 numbers, contiguous, on %s" % (self.R, self.table.device))
         self.slot = torch.empty(T, dtype=torch.int32, device=new_len.device)
         w4a8.kv_plan(self.kv_len, new_len, self.R, self.block, self.table, self.width, self.free, self.num_blocks, self.first, self.seq_len, self.cu,
                      self.slot, None, T, self.status)
@@ -52,12 +55,16 @@ class AttentionBlock:
 
     def __init__(self, wqkv, wo, hidden, heads_q, heads, dim, tables, max_rows, scale=None, window=0, softcap=0.0):
         self.wqkv, self.wo, self.hidden, self.heads_q, self.heads, self.dim, self.tables = wqkv, wo, hidden, heads_q, heads, dim, tables
+        self.max_rows = max_rows
         self.scale, self.window, self.softcap = dim ** -0.5 if scale is None else scale, window, softcap
         dev = tables.table.device
         codes = (tables.num_blocks, heads, tables.block, dim)
         self.cache = w4a8.KVCache.of(torch.zeros(codes, dtype=torch.int8, device=dev), torch.zeros(codes, dtype=torch.int8, device=dev),
                                      torch.zeros(codes[:2], device=dev), torch.zeros(codes[:2], device=dev))
         self.cols = (heads_q + 2 * heads) * dim
+        for (wq, sc), n, k, name in ((wqkv, self.cols, hidden, "wqkv"), (wo, hidden, heads_q * dim, "wo")):
+            if wq.numel() * wq.element_size() != n * k // 2 or sc.dtype != torch.float32 or sc.numel() != n * k // 32 or not (wq.is_contiguous() and sc.is_contiguous()):
+                raise ValueError("%s: %d rows of %d packed int4 and %d fp32 scales, contiguous" % (name, n, k, k // 32))
         self.qkv = torch.empty(max_rows, self.cols, device=dev)
         self.mix = torch.empty(max_rows, heads_q * dim, device=dev)
         widest = max(hidden, heads_q * dim)
@@ -66,9 +73,21 @@ class AttentionBlock:
         self.xsum = torch.empty(max_rows * widest // 32, dtype=torch.int32, device=dev)
         self.workspace = torch.zeros(w4a8.attention_q8_workspace_bytes(heads_q, self.cache), dtype=torch.uint8, device=dev)
 
+    def _check(self, X):
+        """The launches below take pointers: what does not fit the buffers or the step's plan is refused here."""
+        if X.dim() != 2 or X.shape[1] != self.hidden or X.dtype != torch.float32 or not X.is_contiguous():
+            raise ValueError("X: contiguous fp32 rows of %d" % self.hidden)
+        if X.shape[0] > self.max_rows:
+            raise ValueError("%d rows: this block has room for %d" % (X.shape[0], self.max_rows))
+        if X.shape[0] != self.tables.slot.numel():
+            raise ValueError("%d rows: the step was planned for %d" % (X.shape[0], self.tables.slot.numel()))
+        if not X.is_cuda or X.device != self.qkv.device:
+            raise ValueError("X is on %s, the block on %s" % (X.device, self.qkv.device))
+
     def __call__(self, X, max_q=0):
         """X[T][hidden] fp32, the step's rows in the order of the requests -> the block's output [T][hidden].  max_q: no request has more rows."""
         t, T = self.tables, X.shape[0]
+        self._check(X)
         Y = torch.empty_like(X)
         q, k, v = self.qkv, self.qkv[:, self.heads_q * self.dim:], self.qkv[:, (self.heads_q + self.heads) * self.dim:]
         w4a8.linear(X, self.xq, self.xs, self.xsum, *self.wqkv, self.qkv, T, self.cols, self.hidden)
