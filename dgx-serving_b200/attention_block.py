@@ -85,11 +85,13 @@ class AttentionBlock:
             raise ValueError("X is on %s, the block on %s" % (X.device, self.qkv.device))
 
     def __call__(self, X, max_q=0):
-        """X[T][hidden] fp32, the step's rows in the order of the requests -> the block's output [T][hidden].  max_q: no request has more rows."""
+        """X[T][hidden] fp32, the step's rows in the order of the requests -> the block's output [T][hidden], zeros in rows that no request
+        owns (a padded step).  max_q: no request has more rows."""
         t, T = self.tables, X.shape[0]
         self._check(X)
         Y = torch.empty_like(X)
         q, k, v = self.qkv, self.qkv[:, self.heads_q * self.dim:], self.qkv[:, (self.heads_q + self.heads) * self.dim:]
+        self.mix[:T].zero_()                                 # rows behind the last request's (a padded step) are left as they are by the attention
         w4a8.linear(X, self.xq, self.xs, self.xsum, *self.wqkv, self.qkv, T, self.cols, self.hidden)
         w4a8.launch_kv_append_q8(k, v, self.cols, t.slot, T, self.cache)
         w4a8.launch_attention_q8(q, self.cols, self.cache, t.table, t.width, t.cu, t.seq_len, t.R, T, self.heads_q, self.mix, self.heads_q * self.dim,
