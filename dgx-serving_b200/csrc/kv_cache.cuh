@@ -422,12 +422,12 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_q8_kernel(ReadArgs a) {
 // ---- launches -----------------------------------------------------------------------------------------------------------------------
 inline int launch_plan(const PlanArgs &a, cudaStream_t st) {
     const size_t smem = (size_t)(a.R + 1) * 2 * sizeof(int);
-    static PerDevice<size_t> configured_dev;
-    size_t &configured = configured_dev.get();
-    if (smem > 48 * 1024 && smem > configured) {
-        cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // what a launch gets without asking, 48 KB, has to hold the kernel's own arrays too: asked for once, for the most requests
+    static PerDevice<bool> configured;
+    if (!configured.get()) {
+        cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (PLAN_MAX_R + 1) * 2 * (int)sizeof(int));
         if (e != cudaSuccess) return cuda_fail(e, "kv_plan smem opt-in");
-        configured = smem;
+        configured.get() = true;
     }
     const int want = (a.T + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS), most = sm_count();
     const int grid = want < 1 ? 1 : (want < most ? want : most);
