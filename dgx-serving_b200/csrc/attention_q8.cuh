@@ -13,9 +13,13 @@
 //    lies, O^T [dim][rows] += V^T P^T with V read as the transposed operand.  Widening the codes to fp16 for mma.sync cost 450 instructions for 16
 //    keys and bound the stream: two requests of 115k tokens 96 us, 64 ragged ones of up to 8192 tokens 128.  Now 84 us (5.9 TB/s) and 99 (5.5).
 //  - A query row is a fixed-point number relative to its largest magnitude, three signed digits of base 256 (2^-23 of it): three columns.  A weight
-//    is a whole number too, x = exp(s - B) * vs up to 2^31, four columns of P.  All sums are whole numbers and exact; O stays in tensor memory over
-//    the tiles.  The row's reference B is such that its largest x was 2^28 when it was chosen; when an x would pass 2^31, O is read out, rescaled
-//    and summed in fp32, and B moves.  So a weight is rounded to 2^-28 of the row's largest, or as fp32 is.
+//    times its block's scale is a whole number too, x = exp(s) 2^-A * vs 2^-E * 2^25 up to 2^31, four columns of P.  All sums are whole numbers and
+//    exact; O stays in tensor memory over the tiles.  The row's reference A is such that its largest weight was in [1, 2) when it was chosen, E is the
+//    largest exponent of the scales of blocks that the row has seen of.  When a weight would pass 2^4.9 or E grows, O is read out, rescaled and summed in
+//    fp32.  So a weight times its scale is rounded to 2^-26 of the row's largest of either, or as fp32 is; A and E are whole numbers and rescaling is
+//    exact.  The sum of the weights, l = sum exp(s) 2^-A, knows nothing of the scales.  (One reference for the products, 2^28 for the largest, with l
+//    taken from them by 1 / vs, took 51.4, 40 and 98.9 us where few queries, a window and ragged tokens now take 55.4, 41.1 and 100.3; but l left fp32
+//    at scales above 2^62, and lost the weights of tokens whose scale is 2^-150 of another's.)
 //  - 128 threads have a key each, about thirty instructions for a row.  Two such groups take the tiles in turn, each with its own S, P, O, reference and
 //    sums, because a tile's chain of steps (1300 cycles with 4 rows, 3500 with 16) takes longer than its bytes do; they meet at the end of a pair, one
 //    handing over, the other writing.
@@ -35,9 +39,11 @@ constexpr int MAX_R = 2048;                // requests of one launch (their sums
 constexpr int FEW_ROWS = 64;               // rows (queries x heads of a group) of a request that this kernel takes at most: half a row tile of the other
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr unsigned ERR_WAIT = 0xA00u;
-constexpr float TOP = 28.f, LIMIT = 30.9f; // log2 of the largest weight when B is chosen, and beyond which it moves (four signed digits reach 2^30.99)
+// log2 of a weight's whole number when A is chosen, and of a weight before A moves: with a scale's mantissa in [1, 2) they make 30.9, and four signed
+// digits reach 2^30.99.  (27 and 2.9 move A more often: 1.7 us more of 54.)
+constexpr float TOP = 25.f, LIMIT = 4.9f;
+constexpr float NONE = -1e30f;             // A before a key was seen
 constexpr int START = 4;                   // tiles whose time beginning and ending a pair takes (64 ragged requests: 104.5 us with 1, 99.3 with 4, 100.7 with 6)
-constexpr float UNIT = 0x1p-64f;           // sums of exp(s - B) are in units of 2^64, so that weights up to 2^31 times 1 / vs up to 2^100 stay in fp32
 constexpr int FLUSH = 900;                 // tiles after which O is read out at the latest: 128 * 128 * 127 * 900 < 2^31
 
 struct Args {
@@ -51,14 +57,23 @@ struct Args {
     int causal, window;
     float scale, softcap;
     int few;                               // rows (queries * G) of a request that this kernel takes at most; more are another kernel's
-    // workspace, by a CTA's two ends: arrivals, zero between calls; [2 * CTAs][rows] reference, sum; [2 * CTAs][rows][dim] values; groups of CTAs alike
+    // workspace, by a CTA's two ends: arrivals, zero between calls; [2 * CTAs][rows] A, E, sum; [2 * CTAs][rows][dim] values; groups of CTAs alike
     unsigned *count, *count2;
-    float2 *part_ml, *part2_ml;
+    float4 *part_ml, *part2_ml;
     float *part, *part2;
 };
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }          // -126 <= e <= 127
+// The exponent of a scale (0 and what is not a number: that of the smallest there are).
+constexpr int LEAST = -150;
+__device__ __forceinline__ int exponent_of(float vs) {
+    const int e = (int)(__float_as_uint(vs) >> 23) - 127;
+    return !(vs > 0.f && vs < __int_as_float(0x7f800000)) ? LEAST : e > -127 ? e : (int)(__float_as_uint(vs * 0x1p64f) >> 23) - 127 - 64;
+}
+// 2^d for a whole number d, -250 <= d <= 250, as a product of two powers of two.
+__device__ __forceinline__ float2 pow2_parts(int d) { return make_float2(pow2(d >> 1), pow2(d - (d >> 1))); }
 
 // ---- which keys and how much work ----------------------------------------------------------------------------------------------------
 struct Request {
@@ -257,7 +272,7 @@ template <int D, int R_> struct Shape {
     // window of 1024 tokens 44.7 -> 40.1 us); at the others K's loads would then run ahead of V's (two of 115k tokens 83.7 -> 87), so both leave together.
     static constexpr bool EARLY = D == 256;
     static constexpr int MAX_STAGES = 8, SLOTS = 16;                                   // of each side; tiles' scales, more than are between copy and scores
-    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + SLOTS * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 8 + 2 * R * 4 + R * (D == 64 ? 128 : D) * 4 + 2 * (FAN + 2) * MAX_ROWS * 4;   // and 4 bytes a request
+    static constexpr int FIXED = 1024 + 2 * QB + 2 * PB + 1024 + SLOTS * SCALES * 16 + 2 * R * 16 + 2 * 4 * R * 4 + R * 16 + 2 * R * 24 + R * (D == 64 ? 128 : D) * 4 + 2 * (FAN + 3) * MAX_ROWS * 4;   // and 4 bytes a request
     static inline int fixed_bytes(int n) { return (FIXED + (n + 4) * 4 + 1023) & ~1023; }
     static inline int stages(int n) {                                                  // of both sides together
         const int k = (226 * 1024 - fixed_bytes(n)) / STAGE;
@@ -278,19 +293,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
     unsigned char *qs = p; p += 2 * S::QB;
     unsigned char *ps = p; p += 2 * S::PB;
     unsigned char *control = p; p += 1024;
-    float4 *scales = reinterpret_cast<float4 *>(p); p += S::SLOTS * S::SCALES * 16;   // ks, log2 vs, 1 / vs of a tile's blocks
-    float4 *rec = reinterpret_cast<float4 *>(p); p += 2 * R * 16;                          // a row's factor, B, last and first key (as int)
+    float4 *scales = reinterpret_cast<float4 *>(p); p += S::SLOTS * S::SCALES * 16;   // a tile's blocks: ks; vs; their largest exponent (below); 0, or not a number where vs is none
+    float4 *rec = reinterpret_cast<float4 *>(p); p += 2 * R * 16;                          // a row's factor, -, last and first key (as int)
+    float4 *over_ml = reinterpret_cast<float4 *>(p); p += R * 16;                          // what one group hands over: A, E, sum; values
     float *reds = reinterpret_cast<float *>(p); p += 2 * 4 * R * 4;
-    float2 *over_ml = reinterpret_cast<float2 *>(p); p += R * 8;                           // what one group hands over: B, sum; values
-    float *refs = reinterpret_cast<float *>(p); p += 2 * R * 4;                            // B of each group (many rows)
+    float *refs = reinterpret_cast<float *>(p); p += 2 * R * 4;                            // of each group's rows: A; E; 2^(25 - E) as a product;
+    int *exps = reinterpret_cast<int *>(p); p += 2 * R * 4;
+    float2 *units = reinterpret_cast<float2 *>(p); p += 2 * R * 8;
+    float2 *changes = reinterpret_cast<float2 *>(p); p += 2 * R * 8;                       // what l and what is summed of O change by
     float *over = reinterpret_cast<float *>(p); p += R * (D == 64 ? 128 : D) * 4;
-    float *coefs = reinterpret_cast<float *>(p); p += 2 * (FAN + 2) * MAX_ROWS * 4;         // joining: what a part counts for
+    float *coefs = reinterpret_cast<float *>(p); p += 2 * (FAN + 3) * MAX_ROWS * 4;         // joining: what a part counts for
     unsigned *cum = reinterpret_cast<unsigned *>(p);
     const uint32_t bar = ptx::smem_u32(control), ring_at = ptx::smem_u32(smem), q_at = ptx::smem_u32(qs), p_at = ptx::smem_u32(ps);
     const uint32_t K_FULL = bar, V_FULL = bar + 64u, K_EMPTY = bar + 128u, V_EMPTY = bar + 192u, S_FULL = bar + 256u, S_EMPTY = bar + 272u, P_FULL = bar + 288u,
                    P_EMPTY = bar + 304u, Q_FULL = bar + 320u, Q_EMPTY = bar + 336u, OVER = bar + 352u, v_ring = ring_at + (uint32_t)a.k_stages * S::STAGE;
     __shared__ unsigned wsum[THREADS / 32], last_flags[2], tmem_slot;
-    __shared__ int fresh[2];                                            // a tile's weights begin new sums in O
+    __shared__ int fresh[2], least_e[2];                                // a tile's weights begin new sums in O; the least E of a group's rows
     __shared__ Work works[WORKS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -362,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         uint32_t phase = 0;
         bool more = walk.next(s);
         const int per_batch = 32 / pieces, mine_t = lane / pieces, pc = lane - mine_t * pieces;
-        struct Batch { int tiles, row; float ks, vs; bool mine; } b;
+        struct Batch { int tiles, row; float ks, vs; bool mine, inner; } b;       // inner: every row sees all keys of the tile
         int phys = 0, h = 0, tok = 0;
         const auto look_up = [&]() {                               // the table entry of this lane's piece of the next batch
             b.tiles = 0; b.mine = false;
@@ -370,6 +388,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             b.tiles = min(per_batch, s.tiles - t_next);
             const int first = (s.x.lo / TK + s.tile + t_next + mine_t) * TK + pc * tokens;
             b.mine = mine_t < b.tiles && first < s.x.seq && first + tokens > s.x.lo;
+            const int key0 = first - pc * tokens, pos0 = s.x.seq - s.x.n;
+            b.inner = mine_t < b.tiles && (s.x.n == 1 || (key0 + TK <= (a.causal ? pos0 + 1 : s.x.seq) && (a.window == 0 || key0 > s.x.seq - 1 - a.window)));
             if (b.mine) phys = a.table[(size_t)s.r * a.width + (first >> bshift)];
             tok = first & (a.block - 1);
             h = s.h;
@@ -389,13 +409,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         while (b.tiles > 0 && ok) {
             const Batch now = b;
             look_up();
+            float most = 0.f;
+            if (is_k) {                                            // of tiles that all rows see whole: their largest exponent in the batch; of others, that of all
+                const int e = now.mine ? exponent_of(now.vs) : LEAST, ahead = __reduce_max_sync(0xffffffffu, now.inner ? e : LEAST), any = __reduce_max_sync(0xffffffffu, e);
+                most = now.inner ? (float)ahead : (float)any + 0.5f;   // (a half: it bounds the rows' own)
+            }
             for (int t = 0; t < now.tiles; t++) {
                 if (used >= stages && !wait_idle(empty0 + 8 * stage, phase ^ 1u)) { give_up(is_k ? 1u : 2u); break; }
                 const bool in = mine_t == t, here = in && now.mine;
-                if (is_k && in) {                                  // vs 0: its block's weights are as good as 0, and their sum comes out right
-                    const float v1 = fmaxf(now.vs, 0x1p-100f);
+                if (is_k && in) {
                     // the slot's last reader, the scores of tile used - SLOTS: this stage was free only after S of tile used - stages, and that came after them
-                    scales[(used & (S::SLOTS - 1)) * S::SCALES + pc] = make_float4(now.ks, lg2(v1), UNIT / v1, 0.f);
+                    scales[(used & (S::SLOTS - 1)) * S::SCALES + pc] = make_float4(now.ks, now.vs, most, now.vs >= 0.f ? now.vs * 0.f : __int_as_float(0x7FC00000));
                 }
                 const unsigned count = __popc(__ballot_sync(0xffffffffu, here));
                 __syncwarp();                                      // the scales are there before the arrival
@@ -578,11 +602,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
         // what is the same for all threads of a row is in registers for few rows, for many in shared memory
         constexpr bool HELD = R <= 8;
         constexpr int STEP = R < 8 ? R : 8;                                          // rows whose scores are in registers at a time
-        float l[R], acc[DP][R], facs[HELD ? R : 1], Bs[HELD ? R : 1];
+        float l[R], acc[DP][R], facs[HELD ? R : 1], As[HELD ? R : 1];
         float *ref = refs + group * R;
+        int *exp_of = exps + group * R;
+        float2 *unit = units + group * R, *change = changes + group * R;
         const float4 *rc = rec;
         const auto fac = [&](int r) { if constexpr (HELD) return facs[r]; else return rc[r].x; };
-        const auto B = [&](int r) { if constexpr (HELD) return Bs[r]; else return ref[r]; };
+        const auto A = [&](int r) { if constexpr (HELD) return As[r]; else return ref[r]; };
         const auto sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         // Is it so for any of the 128 threads?  A wait that ran out for one warp is everybody's to know: they leave together.
         const auto vote = [&](bool mine) {
@@ -591,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                          : "=r"(any) : "r"((int)mine), "r"(1 + group) : "memory");
             return any != 0;
         };
-        // O of the tiles since it was last read, in units of 2^B
+        // O of the tiles since it was last read, in units of 2^(A + E - 25)
         const auto read_o = [&]() {
             const uint32_t i = before - 1;                                         // the last tile whose PV is in it
             if (ok && !wait_warp(P_EMPTY + 8 * group, (i >> 1) & 1)) give_up(9u);
@@ -618,16 +644,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             rc = rec + (nth & 1) * R;
             bool since = false;                                                     // O holds tiles of this segment that have not been read
             int held = 0;
+            bool begun = false;                                                     // A and E are this segment's
+            float least = 0.f;                                                      // the least E of a row
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 l[r] = 0.f;
-                if constexpr (HELD) { facs[r] = rc[r].x; Bs[r] = -inf; }
+                if constexpr (HELD) { facs[r] = rc[r].x; As[r] = NONE; }
 #pragma unroll
                 for (int pl = 0; pl < DP; pl++) acc[pl][r] = 0.f;
-            }
-            if constexpr (!HELD) {
-                if (gt < R) ref[gt] = -inf;
-                sync();
             }
             for (int t = 0; t < w.tiles; t++, j++) {
                 if ((j & 1) != group) continue;
@@ -637,8 +661,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 ptx::tc_fence_after_sync();
                 const float4 sc = scales[(j & (S::SLOTS - 1)) * S::SCALES + (gt >> tshift)];
                 // rows that the segment does not have go along: they are not read
-                float y[R];
-                bool again = held >= FLUSH;
+                float y[R];                                                        // log2 of exp(s)
+                const bool grows = !begun || sc.z > least;
+                bool again = grows || held >= FLUSH;
 #pragma unroll
                 for (int r0 = 0; r0 < R; r0 += STEP) {
                     uint32_t v[3 * STEP];
@@ -649,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                         // |sum| <= 128 * 127 * 256 < 2^22: to fp32 by the bits of 1.5 * 2^23, which is quicker than a conversion
                         const auto whole = [](uint32_t n) { return __uint_as_float(n + 0x4B400000u) - 12582912.f; };
                         const float s = fmaf(whole(v[3 * r]), 65536.f, fmaf(whole(v[3 * r + 1]), 256.f, whole(v[3 * r + 2])));
-                        y[r0 + r] = fmaf(s, fac(r0 + r) * sc.x, sc.y);
+                        y[r0 + r] = fmaf(s, fac(r0 + r) * sc.x, sc.w);
                     }
                 }
                 ptx::tc_fence_before_sync();
@@ -657,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 if (lane == 0) ptx::mbar_arrive(S_EMPTY + 8 * buf);
                 if (a.softcap > 0.f) {
 #pragma unroll
-                    for (int r = 0; r < R; r++) y[r] = capped(y[r] - sc.y, a.softcap) + sc.y;
+                    for (int r = 0; r < R; r++) y[r] = capped(y[r], a.softcap);
                 }
                 if (key - gt + TK - 1 > w.min_hi || key - gt < w.max_lo) {
 #pragma unroll
@@ -665,10 +690,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                         if (key > __float_as_int(rc[r].z) || key < __float_as_int(rc[r].w)) y[r] = -inf;
                 }
 #pragma unroll
-                for (int r = 0; r < R; r++) again = again || y[r] > B(r) + LIMIT;
+                for (int r = 0; r < R; r++) again = again || y[r] > A(r) + LIMIT;
                 if (vote(again || !ok)) {
                     if (vote(!ok)) { ok = false; break; }
-                    // a weight would pass 2^31: B moves to where the row's largest is 2^28; what is summed, to the new B
+                    // a weight would be too large, or a scale is: A moves to the row's largest weight, E to the largest scale of the blocks that it sees of.  A
+                    // thread has a row: this is code that few tiles come to, so it is kept short.
 #pragma unroll
                     for (int r = 0; r < R; r++) {
                         const float m = warp_max(y[r]);
@@ -676,24 +702,35 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     }
                     if (since) read_o();
                     sync();
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        const float m = fmaxf(fmaxf(red[r], red[R + r]), fmaxf(red[2 * R + r], red[3 * R + r]));
-                        const float was = B(r), now = m > was + TOP ? m - TOP : was;
-                        const float shrink = was == -inf || now == was ? 1.f : ex2(was - now);      // nothing is summed while B is -inf
-                        if constexpr (HELD) Bs[r] = now;
-                        l[r] *= shrink;
-#pragma unroll
-                        for (int pl = 0; pl < DP; pl++) acc[pl][r] *= shrink;
+                    if (gw == 0) {
+                        int E = LEAST;
+                        if (gt < R) {
+                            const float was = begun ? ref[gt] : NONE, now = fmaxf(was, floorf(fmaxf(fmaxf(red[gt], red[R + gt]), fmaxf(red[2 * R + gt], red[3 * R + gt]))));
+                            const int hi = __float_as_int(rc[gt].z), lo = __float_as_int(rc[gt].w), E0 = begun ? exp_of[gt] : LEAST;
+                            const bool each = sc.z != floorf(sc.z);                 // rows that may not see all blocks
+                            E = each || !grows ? E0 : max(E0, (int)sc.z);
+#pragma unroll 1
+                            for (int i = 0, k = key - gt; i < pieces && each && grows; i++, k += tokens)
+                                if (k <= hi && k + tokens > lo) E = max(E, exponent_of(scales[(j & (S::SLOTS - 1)) * S::SCALES + i].y));
+                            ref[gt] = now;
+                            exp_of[gt] = E;
+                            unit[gt] = pow2_parts((int)TOP - E);
+                            change[gt] = make_float2(ex2(was - now), ex2(was - now) * ex2((float)(E0 - E)));
+                        }
+                        const int least_of = __reduce_min_sync(0xffffffffu, gt < rows ? E : 0x7fffffff);
+                        if (gt == 0) least_e[group] = least_of;
                     }
                     sync();
-                    if constexpr (!HELD) {
-                        if (gt < R) {
-                            const float m = fmaxf(fmaxf(red[gt], red[R + gt]), fmaxf(red[2 * R + gt], red[3 * R + gt]));
-                            if (m > ref[gt] + TOP) ref[gt] = m - TOP;
-                        }
-                        sync();
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float2 by = change[r];
+                        if constexpr (HELD) As[r] = ref[r];
+                        l[r] *= by.x;
+#pragma unroll
+                        for (int pl = 0; pl < DP; pl++) acc[pl][r] *= by.y;
                     }
+                    least = (float)least_e[group];
+                    begun = true;
                     since = false;
                     held = 0;
                 }
@@ -711,9 +748,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     uint32_t n[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float b = B(r0 + r), x = ex2(y[r0 + r] - (b == -inf ? 0.f : b));      // a masked score is -inf: 0
-                        l[r0 + r] = fmaf(x, sc.z, l[r0 + r]);
-                        n[r] = (__float2uint_rn(x) + 0x808080u) ^ 0x808080u;
+                        const float weight = ex2(y[r0 + r] - A(r0 + r));                           // a masked score is -inf: 0
+                        const float2 by = unit[r0 + r];                                            // (no product in this order leaves fp32 before the last does)
+                        l[r0 + r] += weight;
+                        n[r] = (__float2uint_rn(weight * by.x * sc.y * by.y) + 0x808080u) ^ 0x808080u;
                     }
                     sts128(to + (((piece + r0 / 4) ^ turn) << 4), n[0], n[1], n[2], n[3]);
                 }
@@ -744,19 +782,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 for (int r = 0; r < R; r++) {
 #pragma unroll
                     for (int pl = 0; pl < DP; pl++) over[r * (D == 64 ? 128 : D) + pl * 128 + gt] = acc[pl][r];
-                    if (gt == 0) over_ml[r] = make_float2(B(r), l[r]);
+                    if (gt == 0) over_ml[r] = make_float4(begun ? A(r) : NONE, (float)(begun ? exp_of[r] : LEAST), l[r], 0.f);
                 }
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(OVER + 8 * (nth & 1));
                 continue;
             }
             if (ok && !wait_warp(OVER + 8 * (nth & 1), (nth >> 1) & 1)) give_up(14u);
-            float tops[R];
+            float2 tops[R];                                                          // A, E
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const float2 x = over_ml[r];
-                const float top = fmaxf(B(r), x.x), f = B(r) == -inf ? 1.f : ex2(B(r) - top), g = x.x == -inf ? 1.f : ex2(x.x - top);  // (-inf: nothing, or not a number)
-                l[r] = l[r] * f + x.y * g;
+                const float4 x = over_ml[r];
+                const float2 mine = begun ? make_float2(A(r), (float)exp_of[r]) : make_float2(NONE, (float)LEAST), top = make_float2(fmaxf(mine.x, x.x), fmaxf(mine.y, x.y));
+                float f = ex2(mine.x - top.x), g = ex2(x.x - top.x);
+                l[r] = l[r] * f + x.z * g;
+                f *= ex2(mine.y - top.y);
+                g *= ex2(x.y - top.y);
                 tops[r] = top;
 #pragma unroll
                 for (int pl = 0; pl < DP; pl++) acc[pl][r] = acc[pl][r] * f + over[r * (D == 64 ? 128 : D) + pl * 128 + gt] * g;
@@ -774,14 +815,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
             const bool writes = D != 64 || gt < 64;
             if (w.tiles != w.pair_tiles) {
                 // ---- the CTAs that share the pair meet: FAN neighbours first, then the groups; the last to come joins, in the order of the ranges ------------
-                const auto leave = [&](float2 *pml, float *pv, size_t slot) {
+                const auto leave = [&](float4 *pml, float *pv, size_t slot) {
                     if (writes)
 #pragma unroll
                         for (int r = 0; r < R; r++)
                             if (r < rows) {
 #pragma unroll
                                 for (int pl = 0; pl < DP; pl++) pv[(slot * MAX_ROWS + r) * D + pl * 128 + gt] = acc[pl][r];
-                                if (gt == 0) pml[slot * MAX_ROWS + r] = make_float2(tops[r], l[r]);
+                                if (gt == 0) pml[slot * MAX_ROWS + r] = make_float4(tops[r].x, tops[r].y, l[r], 0.f);
                             }
                 };
                 const unsigned c0 = cta_of((unsigned)w.pair0), c1 = cta_of((unsigned)(w.pair0 + w.pair_tiles - 1)), groups = (c1 - c0) / FAN + 1;
@@ -799,8 +840,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     if (last) __threadfence();
                     return last;
                 };
-                float *coef = coefs + group * (FAN + 2) * MAX_ROWS;            // [part][row], then the rows' references and sums
-                const auto join = [&](const float2 *pml, const float *pv, unsigned first, unsigned step, unsigned n) {
+                float *coef = coefs + group * (FAN + 3) * MAX_ROWS;            // [part][row], then the rows' A, E and sums
+                const auto join = [&](const float4 *pml, const float *pv, unsigned first, unsigned step, unsigned n) {
                     constexpr int AT_ONCE = 32 / (R * DP) > 0 ? 32 / (R * DP) : 1;
                     float o[AT_ONCE][DP][R];
                     const auto fetch = [&](unsigned i0) {
@@ -817,30 +858,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     fetch(0);
                     {                                                          // eight threads to a row, two parts each: what each part counts for
                         const int r = gt >> 3, i0 = gt & 7;
-                        float2 x[2];
+                        float4 x[2];
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            x[i] = make_float2(-inf, 0.f);
+                            x[i] = make_float4(NONE, (float)LEAST, 0.f, 0.f);
                             if (r < rows && i0 + 8 * i < (int)n) x[i] = __ldcg(pml + (size_t)slot_of(first + (i0 + 8 * i) * step) * MAX_ROWS + r);
                         }
-                        float top = fmaxf(x[0].x, x[1].x), sum = 0.f;
+                        float top_a = fmaxf(x[0].x, x[1].x), top_e = fmaxf(x[0].y, x[1].y), sum = 0.f;
 #pragma unroll
-                        for (int k = 4; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        for (int k = 4; k > 0; k >>= 1) {
+                            top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, k));
+                            top_e = fmaxf(top_e, __shfl_xor_sync(0xffffffffu, top_e, k));
+                        }
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const float f = x[i].x != -inf ? ex2(x[i].x - top) : x[i].y == 0.f ? 0.f : 1.f;      // -inf and a sum: not a number
-                            sum += x[i].y * f;
-                            coef[(i0 + 8 * i) * MAX_ROWS + r] = f;
+                            const float f = ex2(x[i].x - top_a);
+                            sum += x[i].z * f;
+                            coef[(i0 + 8 * i) * MAX_ROWS + r] = f * ex2(x[i].y - top_e);
                         }
 #pragma unroll
                         for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                        if (i0 == 0) { coef[FAN * MAX_ROWS + r] = top; coef[(FAN + 1) * MAX_ROWS + r] = sum; }
+                        if (i0 == 0) { coef[FAN * MAX_ROWS + r] = top_a; coef[(FAN + 1) * MAX_ROWS + r] = top_e; coef[(FAN + 2) * MAX_ROWS + r] = sum; }
                     }
                     sync();
 #pragma unroll
                     for (int r = 0; r < R; r++) {
-                        tops[r] = coef[FAN * MAX_ROWS + r];
-                        l[r] = coef[(FAN + 1) * MAX_ROWS + r];
+                        tops[r] = make_float2(coef[FAN * MAX_ROWS + r], coef[(FAN + 1) * MAX_ROWS + r]);
+                        l[r] = coef[(FAN + 2) * MAX_ROWS + r];
 #pragma unroll
                         for (int pl = 0; pl < DP; pl++) acc[pl][r] = 0.f;
                     }
@@ -874,10 +918,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 if (r < rows) {
                     const int rho = row0 + r, query = rho / a.G, head = w.h * a.G + rho - query * a.G;
                     const float inv = l[r] > 0.f ? 1.f / l[r] : (l[r] == 0.f ? 0.f : l[r]);          // nothing seen: zeros
+                    const float2 back = pow2_parts((int)(tops[r].y - TOP));
 #pragma unroll
                     for (int pl = 0; pl < DP; pl++)
-                        static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), l[r] == 0.f ? 0.f : acc[pl][r] * UNIT * inv);
-                    if (a.lse && gt == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = l[r] > 0.f ? (tops[r] + (log2f(l[r]) + 64.f)) * LN2 : (l[r] == 0.f ? -inf : l[r]);
+                        static_cast<T *>(a.out)[(long long)(w.q0 + query) * a.ldo + (long long)head * D + pl * 128 + gt] = out_round(T(), l[r] == 0.f ? 0.f : acc[pl][r] * inv * back.x * back.y);
+                    if (a.lse && gt == 0) a.lse[(size_t)(w.q0 + query) * a.Hq + head] = l[r] > 0.f ? (tops[r].x + log2f(l[r])) * LN2 : (l[r] == 0.f ? -inf : l[r]);
                 }
         }
     }
@@ -896,12 +941,12 @@ struct Call {
 // Workspace: the arrival counts, then the partial results of two ends of each CTA's range and of the groups of CTAs.
 inline size_t ends() { return (size_t)sm_count() * 2; }
 inline size_t count_bytes() { return (2 * ends() * 4 + 255) & ~(size_t)255; }
-inline size_t workspace_bytes(int dim) { return count_bytes() + 2 * ends() * MAX_ROWS * (8 + (size_t)dim * 4); }
+inline size_t workspace_bytes(int dim) { return count_bytes() + 2 * ends() * MAX_ROWS * (16 + (size_t)dim * 4); }
 inline void lay_out(Args &a, void *workspace, int dim) {
     unsigned char *p = static_cast<unsigned char *>(workspace);
     a.count = reinterpret_cast<unsigned *>(p);
     a.count2 = a.count + ends();
-    a.part_ml = reinterpret_cast<float2 *>(p + count_bytes());
+    a.part_ml = reinterpret_cast<float4 *>(p + count_bytes());
     a.part2_ml = a.part_ml + ends() * MAX_ROWS;
     a.part = reinterpret_cast<float *>(a.part2_ml + ends() * MAX_ROWS);
     a.part2 = a.part + ends() * MAX_ROWS * dim;

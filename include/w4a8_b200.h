@@ -317,9 +317,11 @@ int w4a8_kv_read_q8(const w4a8_kv_cache *cache, const int32_t *block_table, int 
  * seq_len[r] tokens (the step's own are in the cache already).  Query head h reads kv head h / (heads_q / heads).  The query at position p
  * sees keys j <= p (causal; all j < seq_len without) with j > p - window (window > 0).  softcap > 0: scores become
  * softcap * tanh(score / softcap).  Rows that see nothing get zeros (and lse -inf); seq_len 0 is such a request.  lse[T][heads_q] (may be
- * NULL): log of the sum of exp(score).  Scales are not negative.  Scores, sums and weighted values are held in fp32 or exactly.  Rows of
- * requests with few (rows * heads_q / heads <= 64) are whole numbers in units of 2^-23 of their largest magnitude, their weights of 2^-28 of
- * the row's largest; rows of prompts and their weights enter the products in one fp16 term each, fp32 rows' in two (22 bits).
+ * NULL): log of the sum of exp(score).  Scales are not negative; where one is infinite or not a number, rows that see its block are not numbers
+ * and the others as without it.  Scores, sums and weighted values are held in fp32 or exactly.  Rows of requests with few (rows * heads_q /
+ * heads <= 64) are whole numbers in units of 2^-23 of their largest magnitude, their weights times values' scales of 2^-25 of the row's largest
+ * weight times the largest scale that it sees; rows of prompts and their weights enter the products in one fp16 term each, fp32 rows' in two (22
+ * bits).
  * max_q: no request has more rows (0: not known); it chooses the kernel, not the result's meaning.
  * The workspace (256-byte aligned, zeroed once by the caller, left zeroed where that matters) serves one stream at a time; its size holds
  * for any lengths.  Row order, requests side by side and the GPU's SM count decide how the key axis is cut, so a row's last bits can differ
