@@ -10,10 +10,13 @@
 //    64 elements with the 128-byte swizzle: K is then K-major, V the same bytes read as MN-major, so neither is transposed.
 //  - A thread has one row: maximum, sum and rescaling need no exchange.  The weight that enters the product, exp(s - B) * vs, takes its
 //    block's scale in the exponent: x = exp2(f s + log2 vs - B), one multiply-add and one exp2; the sum divides it out again once per block
-//    and row.  B is such that the largest x was 2^8 when B was chosen; it moves, and O in tensor memory is rescaled, only when an x would
-//    pass 2^15.
+//    and row.  B is such that the largest x was in [2^7, 2^9) when B was chosen; it moves, and O in tensor memory is rescaled, only when an x would
+//    pass 2^15.  (The whole numbers in log2 vs decide that; what is left of them is below 2.)
+//  - That holds while scales are between 2^-40 and 2^40.  From the first tile on with one that is not (zero, say), the sum has a reference of its
+//    own, A, and a block's x are taken back from B to A by powers of two, or, where they are less than 2^-60 of what B stands for, are the sum's alone.
+//    Both ways give the same bits where both can, so a row's result does not depend on scales that it does not see.
 //  - fp32 rows enter as two fp16 terms each, Q and P: twice the products, 22 bits.
-// One prompt of 4096 tokens, 32 heads of 128 over 8, causal: 206 us, 668 TFLOP/s of the 1633 that a large product reaches.  A step of two row
+// One prompt of 4096 tokens, 32 heads of 128 over 8, causal: 208 us, 661 TFLOP/s of the 1633 that a large product reaches.  A step of two row
 // tiles and 128 keys takes about 4600 cycles where its products take 2100 and its exponentials 2050: the row's warps, two on a scheduler, are in
 // the way, with the maximum (850), the wait for the scores (1450) and the weights (2500).  Steps of 64 keys with two buffers of scores for each row
 // tile hid the wait, and had every step's fixed costs twice: 240 us.
@@ -34,10 +37,22 @@ using attn::wait_one;
 using attn::wait_warp;
 using attn::h2_bits;
 using attn::sts128;
+using attn::NONE;
 constexpr unsigned ERR_WAIT = 0xB00u;
 constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
 constexpr int MAX_R = 2048;
 constexpr int SCALE_SLOTS = 4;
+constexpr int ORDINARY = 40;                   // exponents of ordinary scales, either way
+constexpr float DEAD = -60.f;                  // log2 of a block's largest weight, in what B stands for, below which it is nothing to the products
+
+// A block's scales as the rows take them: ks; the whole number in log2 vs; the rest of it, in [0, 1); 1 / vs.  Once a scale is not ordinary, the last is
+// -2^-rest, without the whole number; not a number if vs is none.  0 is 2^-inf.
+__device__ __forceinline__ float4 scale_entry(float ks, float vs, bool far) {
+    const float e = vs == 0.f ? -__int_as_float(0x7f800000) : (float)attn::exponent_of(vs);
+    const uint32_t b = __float_as_uint(vs < 0x1p-100f ? vs * 0x1p64f : vs);
+    const float rest = vs == 0.f ? 0.f : lg2(__uint_as_float((b & 0x7FFFFFu) | 0x3F800000u)), back = ex2(-rest);
+    return make_float4(ks, e, rest, !far ? back * attn::pow2(-(int)e) : vs < __int_as_float(0x7f800000) && vs >= 0.f ? -back : __int_as_float(0x7FC00000));
+}
 
 template <typename T, int D> struct Shape {
     static constexpr bool SPLIT = std::is_same<T, float>::value;
@@ -142,13 +157,13 @@ __device__ __forceinline__ void columns(uint32_t at, Step &&step) {
         step(v[1], c + N);
     }
 }
-// log2 of the row's largest weight
-template <int KT, int N, bool EDGE>
-__device__ __forceinline__ float top_of(uint32_t s_at, uint32_t sc, float fac, float cap, const RowMask &k) {
+// log2 of the row's largest exp(s) * 2^e, e the whole number in log2 vs; FAR: and of its largest exp(s).
+template <int KT, int N, bool EDGE, bool FAR>
+__device__ __forceinline__ float2 top_of(uint32_t s_at, uint32_t sc, float fac, float cap, const RowMask &k) {
     const float inf = __int_as_float(0x7f800000);
-    float top = -inf;
+    float top = -inf, top_z = -inf;
     columns<KT, N>(s_at, [&](uint32_t (&r)[N], int c) {
-        float4 k4[N / 16];                                                   // ks, log2 vs, 1 / vs, vs == 0
+        float4 k4[N / 16];                                                   // scale_entry
 #pragma unroll
         for (int u = 0; u < N / 16; u++) k4[u] = lds_f4(sc + c + 16 * u);
         if (EDGE) {
@@ -163,25 +178,40 @@ __device__ __forceinline__ float top_of(uint32_t s_at, uint32_t sc, float fac, f
             for (int e = 0; e < 4; e++)
                 m[e] = fmaxf(fmaxf(__uint_as_float(r[16 * u + e]), __uint_as_float(r[16 * u + 4 + e])), fmaxf(__uint_as_float(r[16 * u + 8 + e]), __uint_as_float(r[16 * u + 12 + e])));
             const float mm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), f = fac * k4[u].x;
+            if (FAR) {
+                top_z = fmaxf(top_z, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap)) : mm * f);
+            }
             top = fmaxf(top, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap) + k4[u].y) : fmaf(mm, f, k4[u].y));
         }
     });
-    return top;
+    return make_float2(top, top_z);
 }
 // The weights in place of the scores: 16 columns of scores become 8 of fp16 pairs (fp32 rows: and 8 of what they round off).  l += their sum.
-template <int KT, int N, bool SPLIT, bool EDGE, bool CAP>
-__device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, float cap, float B, const RowMask &k, float &l) {
+template <int KT, int N, bool SPLIT, bool EDGE, bool CAP, bool FAR>
+__device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, float cap, float A, float B, const RowMask &k, float &l) {
     columns<KT, N>(s_at, [&](const uint32_t (&r)[N], int c) {
         float4 k4[N / 16];
         float p[N];
 #pragma unroll
         for (int u = 0; u < N / 16; u++) k4[u] = lds_f4(sc + c + 16 * u);
+        float back[N / 16];                                                  // what brings the block's x to the sum's units
+        bool dead[N / 16];
 #pragma unroll
         for (int u = 0; u < N / 16; u++) {
-            const float f = fac * k4[u].x, add = k4[u].y - B;
+            const float f = fac * k4[u].x;
+            float add = (k4[u].y - B) + k4[u].z;
+            back[u] = k4[u].w;
+            dead[u] = false;
+            if (FAR) {
+                const float d = B - A;
+                dead[u] = k4[u].y - d < DEAD;
+                if (dead[u]) add = -A;
+                add += 0.f * k4[u].w;                                        // (not a number where the scale is none)
+                back[u] = dead[u] ? 1.f : -k4[u].w * ex2(d - k4[u].y);
+            }
             if (CAP) {
 #pragma unroll
-                for (int e = 16 * u; e < 16 * u + 16; e++) p[e] = ex2(capped(__uint_as_float(r[e]) * f, cap) + add);
+                for (int e = 16 * u; e < 16 * u + 16; e++) p[e] = ex2(!FAR || cap > 0.f ? capped(__uint_as_float(r[e]) * f, cap) + add : fmaf(__uint_as_float(r[e]), f, add));
             } else {
                 const uint64_t f2 = pack2(f, f), a2 = pack2(add, add);
 #pragma unroll
@@ -205,7 +235,7 @@ __device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, f
             for (int e = 0; e < 4; e++) sum[e] = add2f(pack2(q[4 * e], q[4 * e + 1]), pack2(q[4 * e + 2], q[4 * e + 3]));
             float s0, s1;
             unpack2(add2f(add2f(sum[0], sum[1]), add2f(sum[2], sum[3])), s0, s1);
-            l = fmaf(s0 + s1, k4[u].z, l);
+            if (!FAR || s0 + s1 != 0.f) l = fmaf(s0 + s1, back[u], l);       // (a block that is all masked may have a scale that is not a number)
             uint32_t ph[8], pl[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -216,7 +246,7 @@ __device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, f
                     pl[e] = h2_bits(__floats2half2_rn(q[2 * e] - back.x, q[2 * e + 1] - back.y));
                 }
             }
-            if (k4[u].w != 0.f)
+            if (FAR && dead[u])
 #pragma unroll
                 for (int e = 0; e < 8; e++) ph[e] = pl[e] = 0u;
             tmem_st8(s_at + c + 16 * u, ph);
@@ -287,14 +317,14 @@ template <int N> __device__ __forceinline__ void raise_registers() { asm volatil
 template <int N> __device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 
-// N columns of a thread's row, times inv, into the staging rows of its warp: `bytes` a row, piece c of 16 bytes at c ^ (row & 7).
-template <int N, typename T> __device__ __forceinline__ void stage(uint32_t at, int row, int col, const float (&y)[N], float inv) {
+// N columns of a thread's row, times inv (a product of two), into the staging rows of its warp: `bytes` a row, piece c of 16 bytes at c ^ (row & 7).
+template <int N, typename T> __device__ __forceinline__ void stage(uint32_t at, int row, int col, const float (&y)[N], float2 inv) {
     constexpr int E = 16 / sizeof(T);
 #pragma unroll
     for (int e = 0; e < N; e += E) {
         float x[E];
 #pragma unroll
-        for (int i = 0; i < E; i++) x[i] = inv == 0.f ? 0.f : y[e + i] * inv;
+        for (int i = 0; i < E; i++) x[i] = inv.x == 0.f ? 0.f : y[e + i] * inv.x * inv.y;
         const uint4 w = kv::Row<T>::pack(x);
         sts128(at + ((((col + e) / E) ^ (row & 7)) << 4), w.x, w.y, w.z, w.w);
     }
@@ -334,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
     __shared__ unsigned wsum[THREADS / 32];
     __shared__ int item[4];                       // request, kv head, row tile
     __shared__ uint32_t tmem_slot;
-    __shared__ float shrinks[2][128];              // the rows' factors; dim 256, fp32 rows: what O is rescaled by, two tiles' worth
+    __shared__ float shrinks[2][128];              // the rows' factors; dim 256, fp32 rows: what O is rescaled by, two tiles' worth, then what divides it
     float *const facs = NT == 1 ? shrinks[1] : shrinks[0];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = ptx::smem_u32(smem), bars = base + S::OFF_BAR, scales = base + S::OFF_SCALE;
@@ -431,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
 #pragma unroll
             for (int e = 0; e < OWN; e++) O[e] = 0.f;
         }
-        float B = -inf, l = 0.f, shrink = 1.f;
+        float A = NONE, B = NONE, l = 0.f, shrink = 1.f;             // A follows B until a tile is far
         const auto take = [&](float by) {                            // O of the tile before, complete in tensor memory, into the registers
             if constexpr (SPLIT) {
 #pragma unroll
@@ -444,14 +474,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 }
             }
         };
-        for (int j = 0; j < n; j++) {
+        // One tile's scores to weights.  false, and nothing done, where it is the first with a scale that is not ordinary and `kind` does not know them.
+        const auto tile = [&](auto kind, int j) {
+            constexpr bool FAR = decltype(kind)::value;
             const int buf = NT == 2 ? t : j & 1;
             const uint32_t s_at = lanes + buf * S::S_COLS;
             if (ok && !wait_warp(BAR(S_FULL + buf), (NT == 2 ? j : j >> 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 1u); ok = false; }
             ptx::tc_fence_after_sync();
+            const uint32_t sc = scales + (j & (SCALE_SLOTS - 1)) * 128;
+            if (!FAR && !(lds_f4(sc).w > 0.f)) return false;
             const int key0 = (tile0 + j) * KT;
             const bool edge = key0 + KT - 1 > min_hi || key0 < max_lo;
-            const uint32_t sc = scales + (j & (SCALE_SLOTS - 1)) * 128;
             const auto products_before = [&]() {                     // one S buffer ahead: O is whole when PV of tile j - 1 is done
                 if (ok && !wait_warp(BAR(PV_DONE), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 2u); ok = false; }
                 ptx::tc_fence_after_sync();
@@ -459,14 +492,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             bool waited = NT == 2 || j == 0;                         // two row tiles: S_t of this tile came after PV_t of the one before
             if (SPLIT && NT == 2 && j > 0) take(shrink);
             const RowMask mask = {key0, hi, lo};
-            const float top = edge ? top_of<KT, STEP, true>(s_at, sc, fac, a.softcap, mask) : top_of<KT, STEP, false>(s_at, sc, fac, a.softcap, mask);
-            const bool again = top > B + 15.f;
+            float2 top;
+            if constexpr (FAR) top = top_of<KT, 16, true, true>(s_at, sc, fac, a.softcap, mask);
+            else top = edge ? top_of<KT, STEP, true, false>(s_at, sc, fac, a.softcap, mask) : top_of<KT, STEP, false, false>(s_at, sc, fac, a.softcap, mask);
+            const bool again = top.x > B + 14.f || (FAR && top.y > A + 60.f);
             shrink = 1.f;
             if (__any_sync(0xffffffffu, again)) {
-                const float Bn = again ? top - 8.f : B;
-                shrink = B == -inf ? (Bn == -inf ? 1.f : 0.f) : ex2(B - Bn);
+                const float Bn = top.x > B + 14.f ? floorf(top.x) - 7.f : B, An = !FAR ? Bn : top.y > A + 60.f ? floorf(top.y) : A;
+                shrink = ex2(B - Bn);                                // nothing is summed before the first
+                l *= ex2(A - An);
+                A = An;
                 B = Bn;
-                l *= shrink;
                 if (!SPLIT && j > 0) {
                     if (!waited) { products_before(); waited = true; }
 #pragma unroll 1
@@ -480,10 +516,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                     }
                 }
             }
-            const float Bu = B == -inf ? 0.f : B;
-            if (a.softcap > 0.f) weights<KT, STEP, SPLIT, true, true>(s_at, sc, fac, a.softcap, Bu, mask, l);
-            else if (edge) weights<KT, STEP, SPLIT, true, false>(s_at, sc, fac, 0.f, Bu, mask, l);
-            else weights<KT, STEP, SPLIT, false, false>(s_at, sc, fac, 0.f, Bu, mask, l);
+            if constexpr (FAR) weights<KT, 16, SPLIT, true, true, true>(s_at, sc, fac, a.softcap, A, B, mask, l);
+            else if (a.softcap > 0.f) weights<KT, STEP, SPLIT, true, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
+            else if (edge) weights<KT, STEP, SPLIT, true, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
+            else weights<KT, STEP, SPLIT, false, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
             if (SPLIT && NT == 1) {
                 if (j > 0) { products_before(); take(shrinks[(j - 1) & 1][tid]); }
                 shrinks[j & 1][tid] = shrink;                        // for the other half's warps, who read it before PV of tile j + 1
@@ -491,17 +527,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             tmem_st_wait();
             ptx::tc_fence_before_sync();
             ptx::mbar_arrive(BAR(P_FULL + buf));
-        }
+            return true;
+        };
+        int j = 0;                                                   // two loops, the second in short code: a choice in one cost 6 % of a prompt's time
+        while (j < n && tile(std::false_type(), j)) j++;
+        for (; j < n; j++) tile(std::true_type(), j);
         // ---- the rows out ------------------------------------------------------------------------------------------------------------
         if (n > 0) {
             if (ok && !wait_warp(BAR(O_FULL + t), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 3u); ok = false; }
             ptx::tc_fence_after_sync();
             take(shrink);
         }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const float2 unit = attn::pow2_parts((int)fminf(fmaxf(B - A, -250.f), 250.f));
+        const float2 inv = make_float2((l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * unit.x, unit.y);
         if (SPLIT && NT == 1) {
             asm volatile("bar.sync 4, 256;" ::: "memory");           // the other half has read the last factor
-            shrinks[0][tid] = inv;
+            shrinks[0][tid] = inv.x;
+            shrinks[1][tid] = inv.y;
             asm volatile("bar.sync 3, 256;" ::: "memory");
         }
         // through shared memory, where Q was (every product is done): stored by its own thread a row took 16 bytes of each of 32 rows at a time
@@ -530,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             }
             rows_out<D, T>(rows_at, ROW, 0, dst, there, lane);
         }
-        if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (B + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
+        if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (A + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
         ptx::tc_fence_before_sync();
     } else if (SPLIT && NT == 1 && warp >= 4 && warp < 8) {
         // ---- dim 256, fp32 rows: the second half of O's columns ----------------------------------------------------------------------------
@@ -557,7 +599,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         asm volatile("bar.sync 4, 256;" ::: "memory");
         asm volatile("bar.sync 3, 256;" ::: "memory");
         const uint32_t rows_at = base + (tid & 96) * (D * sizeof(T));
-        stage<128, T>(rows_at + lane * (D * sizeof(T)), lane, 128, O, shrinks[0][lr]);
+        stage<128, T>(rows_at + lane * (D * sizeof(T)), lane, 128, O, make_float2(shrinks[0][lr], shrinks[1][lr]));
         rows_out<128, T>(rows_at, D * sizeof(T), 32, static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, rows - (row0 + (tid & 96)), lane);
         ptx::tc_fence_before_sync();
     } else if (warp >= 8 && warp < 12) {
@@ -615,6 +657,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         };
         int id = entry(0);
         float ks = 0.f, vs = 1.f;
+        bool far = false;
+        const float least = attn::pow2(-ORDINARY), most = attn::pow2(ORDINARY);
         if (id >= 0) { ks = a.ks[(size_t)id * a.Hkv + h]; vs = a.vs[(size_t)id * a.Hkv + h]; }
         for (int j = 0; j < n && ok; j++) {
             const int next = entry(j + 1);
@@ -622,12 +666,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             const int first = (tile0 + j) * KT + lane * piece;
             const size_t off = id >= 0 ? (((size_t)id * a.Hkv + h) * a.block + (first & (a.block - 1))) * D : 0;
             if (j > 0 && !wait_warp(BAR(RAW_EMPTY), (j - 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 6u); ok = false; break; }
+            far = far || __any_sync(0xffffffffu, !(vs >= least && vs < most));
+            const float4 x = scale_entry(ks, vs, far);
             // the slot's last reader was tile j - 4's rows, done before this K can be awaited (two stages and one tile of codes ahead)
             if (lane < pieces) {
-                const float none = vs == 0.f ? 1.f : 0.f, v1 = vs == 0.f ? 1.f : vs;
                 for (int u = 0; u < per; u++) {
                     const uint32_t to = scales + (j & (SCALE_SLOTS - 1)) * 128 + (lane * per + u) * 16;
-                    sts128(to, __float_as_uint(ks), __float_as_uint(lg2(v1)), __float_as_uint(1.f / v1), __float_as_uint(none));
+                    sts128(to, __float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w));
                 }
             }
             __syncwarp();

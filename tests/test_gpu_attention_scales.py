@@ -85,3 +85,19 @@ def not_a_number(w4a8, cuda, dtype, bad, D, news):
 @pytest.mark.parametrize("D,news", [(64, 3), (128, 5), (256, 2)])
 def test_scale_that_is_not_a_number(w4a8, cuda, dtype, bad, D, news):
     not_a_number(w4a8, cuda, dtype, bad, D, news)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("name", list(SCALES))
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scales_far_apart_in_prompts(w4a8, cuda, dtype, name, D):
+    """70 and 90 rows are tiles of rows, the three rows between them stream."""
+    for window in (0, 40):
+        compare(scaled(Case(w4a8, cuda, [100, 17, 300], [70, 3, 90], 8, 2, D, 16, dtype, window=window, seed=D), SCALES[name]))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("bad", ["v nan", "v inf", "k nan"])
+@pytest.mark.parametrize("D,news", [(64, 100), (128, 100), (256, 70)])
+def test_scale_that_is_not_a_number_in_prompts(w4a8, cuda, dtype, bad, D, news):
+    not_a_number(w4a8, cuda, dtype, bad, D, news)
