@@ -42,6 +42,7 @@ constexpr unsigned ERR_WAIT = 0xB00u;
 constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0, 1; 8-11: codes to fp16; 12: copies; 13: products
 constexpr int MAX_R = 2048;
 constexpr int SCALE_SLOTS = 4;
+enum { TILE_PLAIN, TILE_CAPPED, TILE_FAR };    // what a tile's scores need
 constexpr int ORDINARY = 40;                   // exponents of ordinary scales, either way
 constexpr float DEAD = -60.f;                  // log2 of a block's largest weight, in what B stands for, below which it is nothing to the products
 
@@ -129,6 +130,7 @@ __device__ __forceinline__ void unpack2(uint64_t x, float &a, float &b) {
     a = __uint_as_float(u); b = __uint_as_float(v);
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t mul2f(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 // Both passes over a tile's scores are loops over 32 columns whose code stays in the instruction cache nearest to the scheduler: written out
@@ -179,9 +181,9 @@ __device__ __forceinline__ float2 top_of(uint32_t s_at, uint32_t sc, float fac, 
                 m[e] = fmaxf(fmaxf(__uint_as_float(r[16 * u + e]), __uint_as_float(r[16 * u + 4 + e])), fmaxf(__uint_as_float(r[16 * u + 8 + e]), __uint_as_float(r[16 * u + 12 + e])));
             const float mm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), f = fac * k4[u].x;
             if (FAR) {
-                top_z = fmaxf(top_z, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap)) : mm * f);
+                top_z = fmaxf(top_z, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap, 0.f)) : mm * f);
             }
-            top = fmaxf(top, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap) + k4[u].y) : fmaf(mm, f, k4[u].y));
+            top = fmaxf(top, cap > 0.f ? (mm == -inf ? -inf : capped(mm * f, cap, k4[u].y)) : fmaf(mm, f, k4[u].y));
         }
     });
     return make_float2(top, top_z);
@@ -210,8 +212,31 @@ __device__ __forceinline__ void weights(uint32_t s_at, uint32_t sc, float fac, f
                 back[u] = dead[u] ? 1.f : -k4[u].w * ex2(d - k4[u].y);
             }
             if (CAP) {
+                float x[16], most = 0.f;
 #pragma unroll
-                for (int e = 16 * u; e < 16 * u + 16; e++) p[e] = ex2(!FAR || cap > 0.f ? capped(__uint_as_float(r[e]) * f, cap) + add : fmaf(__uint_as_float(r[e]), f, add));
+                for (int e = 0; e < 16; e++) {
+                    x[e] = __uint_as_float(r[16 * u + e]) * f;
+                    most = fmaxf(most, fabsf(x[e]));
+                }
+                if (FAR && !(cap > 0.f)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) p[16 * u + e] = ex2(fmaf(__uint_as_float(r[16 * u + e]), f, add));
+                } else if (__any_sync(0xffffffffu, most > attn::SMALL_X)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) p[16 * u + e] = ex2(capped(x[e], cap, add));
+                } else {                                                     // the same as capped, two at a time
+                    const uint64_t c3 = pack2(attn::TANH3, attn::TANH3), c5 = pack2(attn::TANH5, attn::TANH5), c7 = pack2(attn::TANH7, attn::TANH7), c9 = pack2(attn::TANH9, attn::TANH9),
+                                   by = pack2(cap * LOG2E, cap * LOG2E), a2 = pack2(add, add);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const uint64_t v = pack2(x[e], x[e + 1]), w = mul2f(v, v);
+                        const uint64_t t = fma2(mul2f(v, w), fma2(fma2(fma2(c9, w, c7), w, c5), w, c3), v);
+                        float y0, y1;
+                        unpack2(fma2(by, t, a2), y0, y1);
+                        p[16 * u + e] = ex2(y0);
+                        p[16 * u + e + 1] = ex2(y1);
+                    }
+                }
             } else {
                 const uint64_t f2 = pack2(f, f), a2 = pack2(add, add);
 #pragma unroll
@@ -476,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         };
         // One tile's scores to weights.  false, and nothing done, where it is the first with a scale that is not ordinary and `kind` does not know them.
         const auto tile = [&](auto kind, int j) {
-            constexpr bool FAR = decltype(kind)::value;
+            constexpr bool FAR = decltype(kind)::value == TILE_FAR, CAP = decltype(kind)::value == TILE_CAPPED;
             const int buf = NT == 2 ? t : j & 1;
             const uint32_t s_at = lanes + buf * S::S_COLS;
             if (ok && !wait_warp(BAR(S_FULL + buf), (NT == 2 ? j : j >> 1) & 1)) { if (lane == 0) dev_set_error(ERR_WAIT | 1u); ok = false; }
@@ -494,7 +519,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             const RowMask mask = {key0, hi, lo};
             float2 top;
             if constexpr (FAR) top = top_of<KT, 16, true, true>(s_at, sc, fac, a.softcap, mask);
-            else top = edge ? top_of<KT, STEP, true, false>(s_at, sc, fac, a.softcap, mask) : top_of<KT, STEP, false, false>(s_at, sc, fac, a.softcap, mask);
+            else {
+                const float cap = CAP ? a.softcap : 0.f;
+                top = edge ? top_of<KT, CAP ? 16 : STEP, true, false>(s_at, sc, fac, cap, mask) : top_of<KT, CAP ? 16 : STEP, false, false>(s_at, sc, fac, cap, mask);
+            }
             const bool again = top.x > B + 14.f || (FAR && top.y > A + 60.f);
             shrink = 1.f;
             if (__any_sync(0xffffffffu, again)) {
@@ -517,7 +545,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 }
             }
             if constexpr (FAR) weights<KT, 16, SPLIT, true, true, true>(s_at, sc, fac, a.softcap, A, B, mask, l);
-            else if (a.softcap > 0.f) weights<KT, STEP, SPLIT, true, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
+            else if constexpr (CAP) {
+                if (edge) weights<KT, 16, SPLIT, true, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
+                else weights<KT, 16, SPLIT, false, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
+            }
             else if (edge) weights<KT, STEP, SPLIT, true, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
             else weights<KT, STEP, SPLIT, false, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
             if (SPLIT && NT == 1) {
@@ -529,9 +560,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
             ptx::mbar_arrive(BAR(P_FULL + buf));
             return true;
         };
-        int j = 0;                                                   // two loops, the second in short code: a choice in one cost 6 % of a prompt's time
-        while (j < n && tile(std::false_type(), j)) j++;
-        for (; j < n; j++) tile(std::true_type(), j);
+        int j = 0;                                                   // loops of their own: a choice in one cost 6 % of a prompt's time, and more with caps
+        if (a.softcap > 0.f) while (j < n && tile(std::integral_constant<int, TILE_CAPPED>(), j)) j++;
+        else while (j < n && tile(std::integral_constant<int, TILE_PLAIN>(), j)) j++;
+        for (; j < n; j++) tile(std::integral_constant<int, TILE_FAR>(), j);
         // ---- the rows out ------------------------------------------------------------------------------------------------------------
         if (n > 0) {
             if (ok && !wait_warp(BAR(O_FULL + t), 0)) { if (lane == 0) dev_set_error(ERR_WAIT | 3u); ok = false; }
