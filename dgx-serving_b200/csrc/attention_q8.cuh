@@ -289,7 +289,8 @@ template <int D, int R_> struct Shape {
     static_assert(NP % 16 == 0 && 2 * N + 2 * OC <= 512 && FIXED + (MAX_R + 4) * 4 + 1024 + 4 * STAGE <= 226 * 1024, "shape");
 };
 
-template <typename T, int D, int R>
+// CAP: scores are capped.  (In one kernel their code cost the others 3 us of 54 with many rows.)
+template <typename T, int D, int R, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
     using S = Shape<D, R>;
     using L = Tile<D>;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     const float amax = __uint_as_float(mine), bad = mine >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.f;     // digits cannot tell infinities
                     const float p2 = row_factor(amax), f = amax > 0.f ? 127.f * 65536.f / (amax * p2) : 1.f;
                     if (lane >= r0 && lane < r0 + BATCH)
-                        rec[(k & 1) * R + lane] = make_float4(a.scale * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
+                        rec[(k & 1) * R + lane] = make_float4(a.scale * (CAP ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
                                                               __int_as_float(a.causal ? min(pos, s.x.seq - 1) : s.x.seq - 1),
                                                               __int_as_float(a.window > 0 ? max(0, pos - a.window + 1) : 0));
 #pragma unroll
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 ptx::tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(S_EMPTY + 8 * buf);
-                if (a.softcap > 0.f) {
+                if constexpr (CAP) {
 #pragma unroll
                     for (int r = 0; r < R; r++) y[r] = capped(y[r], a.softcap, 0.f);
                 }
@@ -960,10 +961,10 @@ inline void lay_out(Args &a, void *workspace, int dim) {
     a.part2 = a.part + ends() * MAX_ROWS * dim;
 }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, bool CAP>
 inline int launch_t(const Call &c, int rows, cudaStream_t st) {
     using S = Shape<D, R>;
-    auto kern = attention_q8_kernel<T, D, R>;
+    auto kern = attention_q8_kernel<T, D, R, CAP>;
     const uint64_t tokens = (uint64_t)c.a.num_blocks * c.a.Hkv * c.a.block;
     const uint32_t box = (uint32_t)(c.a.block < TK ? c.a.block : TK);
     CUtensorMap mk, mv;
@@ -1001,15 +1002,19 @@ inline int launch_t(const Call &c, int rows, cudaStream_t st) {
 }
 
 // The narrowest kernel that takes `rows` (queries x heads of a group of the request with most of them) at once.
-template <typename T, int D>
+template <typename T, int D, bool CAP>
 inline int launch_d(const Call &c, int rows, cudaStream_t st) {
-    if (rows <= 4) return launch_t<T, D, 4>(c, rows, st);
-    if (rows <= 8) return launch_t<T, D, 8>(c, rows, st);
-    return launch_t<T, D, 16>(c, rows, st);
+    if (rows <= 4) return launch_t<T, D, 4, CAP>(c, rows, st);
+    if (rows <= 8) return launch_t<T, D, 8, CAP>(c, rows, st);
+    return launch_t<T, D, 16, CAP>(c, rows, st);
 }
 
 inline int launch(const Call &c, int rows, cudaStream_t st) {
-    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) { return launch_d<decltype(t), decltype(d)::value>(c, rows, st); });
+    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        return c.a.softcap > 0.f ? launch_d<T, D, true>(c, rows, st) : launch_d<T, D, false>(c, rows, st);
+    });
 }
 
 }  // namespace attn
