@@ -114,7 +114,8 @@ W4A8_API int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *
     int rc = check_cache(cache, who);
     if (rc != W4A8_OK) return rc;
     if (heads_q <= 0 || heads_q % cache->heads != 0) return fail(W4A8_ERR_ARG, "%s: heads_q=%d is not a multiple of the cache's %d heads", who, heads_q, cache->heads);
-    if (window < 0 || !(softcap >= 0.f) || !(scale == scale)) return fail(W4A8_ERR_ARG, "%s: window=%d softcap=%g scale=%g", who, window, softcap, scale);
+    // (a cap whose quotients leave fp32 is none)
+    if (window < 0 || !(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f)) || !(scale == scale)) return fail(W4A8_ERR_ARG, "%s: window=%d softcap=%g scale=%g", who, window, softcap, scale);
     if (R == 0 || T == 0) return W4A8_OK;
     const int64_t columns = (int64_t)heads_q * cache->dim;
     if ((rc = check_rows(Q, ldq, columns, size, "Q", who)) != W4A8_OK || (rc = check_rows(O, ldo, columns, size, "O", who)) != W4A8_OK) return rc;

@@ -315,7 +315,7 @@ int w4a8_kv_read_q8(const w4a8_kv_cache *cache, const int32_t *block_table, int 
 
 /* O[t] = softmax(scale * q k^T) v for the rows Q[T][heads_q * dim]: rows cu_q[r] .. cu_q[r + 1) are the LAST tokens of request r, which holds
  * seq_len[r] tokens (the step's own are in the cache already).  Query head h reads kv head h / (heads_q / heads).  The query at position p
- * sees keys j <= p (causal; all j < seq_len without) with j > p - window (window > 0).  softcap > 0: scores become
+ * sees keys j <= p (causal; all j < seq_len without) with j > p - window (window > 0).  softcap > 0 (1e-30 to 1e30): scores become
  * softcap * tanh(score / softcap).  Rows that see nothing get zeros (and lse -inf); seq_len 0 is such a request.  lse[T][heads_q] (may be
  * NULL): log of the sum of exp(score).  Scales are not negative; where one is infinite or not a number, rows that see its block are not numbers
  * and the others as without it.  Scores, sums and weighted values are held in fp32 or exactly.  Rows of requests with few (rows * heads_q /
