@@ -54,12 +54,21 @@ class KVCache(ctypes.Structure):
                 raise ValueError("a KV cache's tensors are contiguous")
         if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
             raise ValueError("k, v: [num_blocks][heads][block][dim]; k_scale, v_scale: [num_blocks][heads]")
-        if (k.element_size(), v.element_size(), k_scale.element_size(), v_scale.element_size()) != (1, 1, 4, 4):
+        if [str(t.dtype) for t in (k, v, k_scale, v_scale)] != ["torch.int8", "torch.int8", "torch.float32", "torch.float32"]:
             raise ValueError("a KV cache holds int8 codes and fp32 scales")
+        if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
+            raise ValueError("a KV cache's tensors are on one device")
         c = cls(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
         c._tensors = (k, v, k_scale, v_scale)
-        c._ref = ctypes.byref(c)
+        c._host = not k.is_cuda
         return c
+
+
+def _on_gpu(cache):
+    """The cache, unless KVCache.of made it of tensors in host memory: a launch would follow their pointers."""
+    if getattr(cache, "_host", False):
+        raise ValueError("the KV cache's tensors are not on a GPU")
+    return cache
 
 
 DTYPES = {"fp32": 0, "fp16": 1, "bf16": 2}          # W4A8_F32, W4A8_F16, W4A8_BF16: rows of the attention operators
@@ -297,12 +306,12 @@ def kv_plan(kv_len, new_len, R, block, block_table, table_width, free_blocks, nu
 
 def launch_kv_append_q8(K, V, ld, slot, T, cache, dtype="fp32", stream=None):
     """Rows K, V [T][heads * dim] (pitch ld elements) into their slots of the 8-bit cache (w4a8_kv_append_q8)."""
-    _check(lib().w4a8_kv_append_q8(_ptr(K), _ptr(V), ld, _ptr(slot), T, cache, DTYPES.get(dtype, dtype), _stream(stream)))
+    _check(lib().w4a8_kv_append_q8(_ptr(K), _ptr(V), ld, _ptr(slot), T, _on_gpu(cache), DTYPES.get(dtype, dtype), _stream(stream)))
 
 
 def launch_kv_read_q8(cache, block_table, table_width, begin, cu, R, T, K, V, ld, dtype="fp32", stream=None):
     """The numbers that the cache holds for tokens begin[r] + i of each request, to rows cu[r] + i of K and V (w4a8_kv_read_q8)."""
-    _check(lib().w4a8_kv_read_q8(cache, _ptr(block_table), table_width, _ptr(begin), _ptr(cu), R, T, _ptr(K), _ptr(V), ld, DTYPES.get(dtype, dtype),
+    _check(lib().w4a8_kv_read_q8(_on_gpu(cache), _ptr(block_table), table_width, _ptr(begin), _ptr(cu), R, T, _ptr(K), _ptr(V), ld, DTYPES.get(dtype, dtype),
                                  _stream(stream)))
 
 
@@ -314,7 +323,7 @@ def launch_attention_q8(Q, ldq, cache, block_table, table_width, cu_q, seq_len, 
                         softcap=0.0, max_q=0, lse=None, stream=None):
     """Attention of the rows Q[T][heads_q * dim], the last tokens of R requests, over the 8-bit cache (w4a8_attention_q8).  workspace: a device
     tensor of attention_q8_workspace_bytes(...) bytes, zeroed once."""
-    _check(lib().w4a8_attention_q8(_ptr(Q), ldq, cache, _ptr(block_table), table_width, _ptr(cu_q), _ptr(seq_len), R, T, heads_q, _ptr(O), ldo, _ptr(lse),
+    _check(lib().w4a8_attention_q8(_ptr(Q), ldq, _on_gpu(cache), _ptr(block_table), table_width, _ptr(cu_q), _ptr(seq_len), R, T, heads_q, _ptr(O), ldo, _ptr(lse),
                                    scale, causal, window, softcap, max_q, DTYPES.get(dtype, dtype), _ptr(workspace),
                                    workspace.numel() * workspace.element_size(), _stream(stream)))
 
