@@ -20,14 +20,15 @@ w4a8 = importlib.import_module(__package__)
 
 
 class PagedTables:
-    """Which blocks the requests' tokens lie in: lengths, block tables and the free list of `num_blocks` blocks, on the GPU."""
+    """Which blocks the requests' tokens lie in: lengths, block tables and the free list of `num_blocks` blocks, on the GPU.  A step is step(),
+    the layers' calls, done(), and release() of the requests that have ended."""
 
     def __init__(self, requests, width, num_blocks, block, device="cuda"):
         i32 = dict(dtype=torch.int32, device=device)
         self.R, self.width, self.num_blocks, self.block = requests, width, num_blocks, block
         self.kv_len = torch.zeros(requests, **i32)
         self.table = torch.full((requests, width), -1, **i32)
-        self.free = torch.arange(num_blocks, **i32)
+        self.free = torch.arange(num_blocks + 1, **i32)      # the last is no block: where release puts what is none
         self.seq_len = torch.zeros(requests, **i32)
         self.cu = torch.zeros(requests + 1, **i32)
         self.status = torch.zeros(4, **i32)                  # [0]: the first free block of the next step
@@ -47,6 +48,17 @@ class PagedTables:
         """After the step's last layer: the tokens placed are the requests'; those that got no room keep what they had."""
         torch.where(self.seq_len > 0, self.seq_len, self.kv_len, out=self.kv_len)
         self.first.copy_(self.status[:1])
+
+    def release(self, ended):
+        """Between done() and the next step: the requests that `ended` marks (bool, on the GPU) hold nothing any more, their blocks go back to the
+        free list, in front of what is left of it."""
+        held = (self.kv_len + self.block - 1) // self.block
+        blocks = (torch.arange(self.width, device=held.device) < held[:, None]) & ended[:, None]
+        at = self.first - torch.cumsum(blocks.flatten(), 0)
+        self.free[torch.where(blocks.flatten(), at, self.num_blocks)] = self.table.flatten()
+        self.first -= blocks.sum()
+        self.table.masked_fill_(blocks, -1)
+        self.kv_len.masked_fill_(ended, 0)
 
 
 class AttentionBlock:
