@@ -79,6 +79,8 @@ __device__ __forceinline__ float2 pow2_parts(int d) { return make_float2(pow2(d 
 struct Request {
     int q0, n, seq, lo, tiles, groups;       // first row of Q, rows, tokens, first token that any row sees, tiles from its tile on, row groups
 };
+// The first key that the query at position `pos` sees.  (One in front of all tokens sees as much as the first; so no difference leaves 32 bits.)
+__device__ __forceinline__ int first_seen(int pos, int window) { return window > 0 ? max(0, max(pos, 0) - window + 1) : 0; }
 __device__ __forceinline__ Request request(const Args &a, int r, int rows_per_group) {
     Request x;
     x.q0 = max(0, min(a.cu_q[r], a.T));
@@ -86,7 +88,7 @@ __device__ __forceinline__ Request request(const Args &a, int r, int rows_per_gr
     x.seq = max(0, a.seq_len[r]);
     const long long most = (long long)a.width * a.block;
     if (x.seq > most) { x.seq = (int)most; dev_set_error(kv::ERR_LENGTH); }
-    x.lo = a.window > 0 ? max(0, x.seq - x.n - a.window + 1) : 0;
+    x.lo = first_seen(x.seq - x.n, a.window);
     // at least one tile, so that rows that see nothing are written too
     x.tiles = x.seq > x.lo ? (x.seq + TK - 1) / TK - x.lo / TK : 1;
     const int rows = x.n * a.G;
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                 w.tiles = more ? s.tiles : 0;
                 if (more) {
                     const int q0 = s.x.seq - s.x.n + s.rg * R / a.G, q1 = s.x.seq - s.x.n + min(s.rg * R + R - 1, s.x.n * a.G - 1) / a.G;
-                    w.min_hi = a.causal ? min(q0, s.x.seq - 1) : s.x.seq - 1; w.max_lo = a.window > 0 ? max(0, q1 - a.window + 1) : 0;
+                    w.min_hi = a.causal ? min(q0, s.x.seq - 1) : s.x.seq - 1; w.max_lo = first_seen(q1, a.window);
                     w.tile0 = s.x.lo / TK + s.tile; w.n = s.x.n; w.q0 = s.x.q0; w.rg = s.rg; w.h = s.h;
                     w.first = s.tile == 0; w.pair0 = s.pair0; w.pair_tiles = s.pair_tiles;
                 }
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_kernel(const __grid_c
                     if (lane >= r0 && lane < r0 + BATCH)
                         rec[(k & 1) * R + lane] = make_float4(a.scale * (CAP ? 1.f / a.softcap : LOG2E) / f / p2 + bad, -inf,
                                                               __int_as_float(a.causal ? min(pos, s.x.seq - 1) : s.x.seq - 1),
-                                                              __int_as_float(a.window > 0 ? max(0, pos - a.window + 1) : 0));
+                                                              __int_as_float(first_seen(pos, a.window)));
 #pragma unroll
                     for (int i = 0; i < TURNS; i++) {
                         const int r = r0 + i * RPW + sub;

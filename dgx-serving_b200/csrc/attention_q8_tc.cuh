@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
     const int nt = NT == 2 && row0 + 128 < rows ? 2 : 1;                          // row tiles with rows in them
     const int last_row = min(row0 + NT * 128, rows) - 1;
     const int first_q = row0 / a.G, last_q = last_row / a.G;
-    const int lo_all = a.window > 0 ? max(0, x.seq - x.n + first_q - a.window + 1) : 0;
+    const int lo_all = attn::first_seen(x.seq - x.n + first_q, a.window);
     const int hi_all = a.causal ? x.seq - x.n + last_q + 1 : x.seq;               // keys [lo_all, hi_all) for some row
     const int tile0 = lo_all / KT, n = hi_all > lo_all ? (hi_all + KT - 1) / KT - tile0 : 0;
 
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         const int t = warp >> 2, row = row0 + t * 128 + (tid & 127);
         const int query = min(row, rows - 1) / a.G, head = h * a.G + min(row, rows - 1) % a.G;
         const int at = x.seq - x.n + query;
-        const int hi = a.causal ? min(at, x.seq - 1) : x.seq - 1, lo = a.window > 0 ? at - a.window + 1 : 0;
+        const int hi = a.causal ? min(at, x.seq - 1) : x.seq - 1, lo = attn::first_seen(at, a.window);
         const int min_hi = __reduce_min_sync(0xffffffffu, hi), max_lo = __reduce_max_sync(0xffffffffu, lo);
         float fac = 0.f;
         if (n > 0) {
