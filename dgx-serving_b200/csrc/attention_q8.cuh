@@ -86,7 +86,7 @@ __device__ __forceinline__ Request request(const Args &a, int r, int rows_per_gr
     x.q0 = max(0, min(a.cu_q[r], a.T));
     x.n = max(0, min(a.cu_q[r + 1], a.T) - x.q0);
     x.seq = max(0, a.seq_len[r]);
-    const long long most = (long long)a.width * a.block;
+    const long long most = min((long long)a.width * a.block, (long long)kv::LONGEST);
     if (x.seq > most) { x.seq = (int)most; dev_set_error(kv::ERR_LENGTH); }
     x.lo = first_seen(x.seq - x.n, a.window);
     // at least one tile, so that rows that see nothing are written too

@@ -19,7 +19,7 @@ const char *kv_device_error_text(unsigned int v) {
     switch (v) {
         case kv::ERR_BLOCK_ID: return "a block table names a block that the cache does not have, for a token that was needed";
         case kv::ERR_SLOT: return "kv_append: a slot beyond the cache";
-        case kv::ERR_LENGTH: return "attention: a request has more tokens than its block table's row holds";
+        case kv::ERR_LENGTH: return "attention: a request has more tokens than its block table's row holds, or than 2^31 - 512";
         default: return "a kernel's bounded wait ran out";
     }
 }

@@ -9,6 +9,7 @@
 namespace w4a8 {
 namespace kv {
 
+constexpr int LONGEST = 0x7fffffff - 511;     // tokens of a request: positions a few tiles on are counted in 31 bits too
 enum { ERR_BLOCK_ID = 0x900u, ERR_SLOT = 0x901u, ERR_LENGTH = 0x902u };   // codes of the device-side error word
 
 // ---- element types of the rows outside the cache ---------------------------------------------------------------------------------
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(PlanArgs a) {
         if (r < a.R) {
             const int kv = max(0, a.kv_len[r]), nw = max(0, a.new_len[r]);
             const int want = ceil_div64((long long)kv + nw, a.block);
-            const int need = want <= a.width ? want - ceil_div64(kv, a.block) : 0;
+            const int need = want <= a.width && (long long)kv + nw <= LONGEST ? want - ceil_div64(kv, a.block) : 0;
             v = ((unsigned long long)(unsigned)nw << 32) | (unsigned)need;
         }
         unsigned long long s = v;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(PlanArgs a) {
     // served: the request's tokens fit its table row, and it needs no block or the free list reaches for it and all in front of it
     const auto served = [&](int r, int kv) {
         const int want = ceil_div64((long long)kv + (cu[r + 1] - cu[r]), a.block);
-        return want <= a.width && (before[r + 1] == before[r] || before[r + 1] <= avail);
+        return want <= a.width && (long long)kv + (cu[r + 1] - cu[r]) <= LONGEST && (before[r + 1] == before[r] || before[r + 1] <= avail);
     };
     const int gt = blockIdx.x * PLAN_THREADS + tid, gn = gridDim.x * PLAN_THREADS;
     if (blockIdx.x == 0) {

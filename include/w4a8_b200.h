@@ -276,7 +276,8 @@ int w4a8_moe_block_shard(const float *n2, const uint8_t *gu_wq, const void *gu_s
  * block = 16, 32, 64 or 128 tokens; dim = 64, 128 or 256.  A request's tokens lie in the blocks that its row of the block table names:
  * token p in block table[r][p / block], place p % block; slot = block * block_size + place.  num_blocks * block < 2^31.
  * Rows outside the cache (Q, K, V, O) are fp32, fp16 or bf16 (dtype), a token per row of `ld` elements, heads side by side in it, so that
- * columns of a fused QKV product can be passed as they are; pointers and pitches are multiples of 16 bytes.
+ * columns of a fused QKV product can be passed as they are; pointers and pitches are multiples of 16 bytes.  A request has at most 2^31 - 512
+ * tokens.
  * Table entries, slots and lengths are read on the device.  One that points outside the cache is not followed: it is left out (a slot) or
  * taken as block 0 (a table entry, whose request's result is then void), and w4a8_device_status reports it. */
 enum { W4A8_F32 = 0, W4A8_F16 = 1, W4A8_BF16 = 2 };
