@@ -34,8 +34,8 @@ static int check_cache(const w4a8_kv_cache *c, const char *who) {
     if (c->dim != 64 && c->dim != 128 && c->dim != 256) return fail(W4A8_ERR_ARG, "%s: dim=%d (64, 128 or 256)", who, c->dim);
     if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return fail(W4A8_ERR_ARG, "%s: block=%d (16, 32, 64 or 128 tokens)", who, c->block);
     if (c->heads <= 0 || c->heads > 65535 || c->num_blocks <= 0) return fail(W4A8_ERR_ARG, "%s: heads=%d num_blocks=%d", who, c->heads, c->num_blocks);
-    if ((int64_t)c->num_blocks * c->block > 0x7fffffff || (int64_t)c->num_blocks * c->heads * c->block > 0x7fffffffll * 2)
-        return fail(W4A8_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens: slots and rows have to fit 31 bits", who, c->num_blocks, c->block);
+    if ((int64_t)c->num_blocks * c->block > 0x7fffffff || (int64_t)c->num_blocks * c->heads * c->block > 0x7fffffff)
+        return fail(W4A8_ERR_UNSUPPORTED, "%s: %d blocks of %d heads and %d tokens: slots, and the rows of all heads, have to fit 31 bits", who, c->num_blocks, c->heads, c->block);
     if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(W4A8_ERR_ALIGN, "%s: k and v of the cache must be 16-byte aligned", who);
     return W4A8_OK;
 }

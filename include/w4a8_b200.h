@@ -274,7 +274,7 @@ int w4a8_moe_block_shard(const float *n2, const uint8_t *gu_wq, const void *gu_s
  *   k, v              [num_blocks][heads][block][dim] int8, contiguous, 16-byte aligned; element = code * scale
  *   k_scale, v_scale  [num_blocks][heads] fp32
  * block = 16, 32, 64 or 128 tokens; dim = 64, 128 or 256.  A request's tokens lie in the blocks that its row of the block table names:
- * token p in block table[r][p / block], place p % block; slot = block * block_size + place.  num_blocks * block < 2^31.
+ * token p in block table[r][p / block], place p % block; slot = block * block_size + place.  num_blocks * heads * block < 2^31.
  * Rows outside the cache (Q, K, V, O) are fp32, fp16 or bf16 (dtype), a token per row of `ld` elements, heads side by side in it, so that
  * columns of a fused QKV product can be passed as they are; pointers and pitches are multiples of 16 bytes.  A request has at most 2^31 - 512
  * tokens.
