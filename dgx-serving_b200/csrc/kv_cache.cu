@@ -59,7 +59,15 @@ W4A8_API int w4a8_kv_plan(const int32_t *kv_len, const int32_t *new_len, int R, 
     if (R > kv::PLAN_MAX_R) return fail(W4A8_ERR_UNSUPPORTED, "kv_plan: %d requests (at most %d)", R, kv::PLAN_MAX_R);
     if (!first_free || !cu_new || !status || (T && !slot) || (num_free && !free_blocks) || (R && (!kv_len || !new_len || !seq_len || (table_width && !block_table))))
         return fail(W4A8_ERR_ARG, "kv_plan: null pointer argument");
-    if (R && (seq_len == kv_len || seq_len == new_len)) return fail(W4A8_ERR_ARG, "kv_plan: seq_len must not be an input (a request that is not served keeps its kv_len)");
+    // every CTA reads the inputs to its end, and what is written early may be one of them (seq_len and kv_len, status and first_free)
+    const struct { const void *p; size_t n; const char *name; } in[] = {{kv_len, (size_t)R, "kv_len"}, {new_len, (size_t)R, "new_len"}, {free_blocks, (size_t)num_free, "free_blocks"},
+                                                                        {first_free, 1, "first_free"}},
+        out[] = {{seq_len, (size_t)R, "seq_len"}, {cu_new, (size_t)R + 1, "cu_new"}, {slot, (size_t)T, "slot"}, {position, (size_t)T, "position"}, {status, 4, "status"},
+                 {block_table, (size_t)R * table_width, "block_table"}};
+    for (const auto &i : in)
+        for (const auto &o : out)
+            if (i.p && o.p && i.n && o.n && (uintptr_t)i.p < (uintptr_t)o.p + o.n * 4 && (uintptr_t)o.p < (uintptr_t)i.p + i.n * 4)
+                return fail(W4A8_ERR_ARG, "kv_plan: %s overlaps %s, an input that is read to the end", o.name, i.name);
     int rc = require_sm100();
     if (rc != W4A8_OK) return rc;
     kv::PlanArgs a = {kv_len, new_len, free_blocks, first_free, block_table, seq_len, cu_new, slot, position, status, R, block, table_width, num_free, T};
