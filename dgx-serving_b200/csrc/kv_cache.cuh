@@ -165,7 +165,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(PlanArgs a) {
                 pos = kv + t - cu[r];
                 const int b = pos / a.block, have = ceil_div64(kv, a.block);
                 const int id = b < have ? a.table[(size_t)r * a.width + b] : a.free_blocks[first + before[r] + b - have];
-                slot = id * a.block + pos % a.block;
+                // no slot can be made of any id (its product may wrap to a slot of another request)
+                if ((unsigned)id < 0x80000000u / (unsigned)a.block) slot = id * a.block + pos % a.block;
+                else dev_set_error(ERR_BLOCK_ID);
             }
         }
         a.slot[t] = slot;

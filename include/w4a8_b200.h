@@ -294,7 +294,9 @@ typedef struct w4a8_kv_cache {
  *   A request is served if its tokens fit its table row and need[r] = 0 or the free list reaches for it and all requests in front of it
  *   (those that do not fit their row need nothing).  Others get no block: seq_len[r] = 0, slots -1; kv_len stays theirs for the next step.
  *   seq_len[r] = kv_len + new_len; cu_new[R + 1] = sums of new_len (the rows' starts, served or not)
- *   slot[t], position[t] (may be NULL) of row t < T: -1 where there is none (rows of requests not served, rows behind cu_new[R])
+ *   slot[t], position[t] (may be NULL) of row t < T: -1 where there is none (rows of requests not served, rows behind cu_new[R]).  An id of the table or
+ *   the free list that no slot can be made of gives slot -1, and w4a8_device_status reports it.  T is the step's rows, at least the sum of new_len:
+ *   tokens beyond T would count as held, without a slot.
  *   status[4] = index in free_blocks behind the last block taken; requests not served; blocks taken; tokens placed.
  * Outputs must not overlap inputs.  R <= 16384, sum of new_len < 2^31. */
 int w4a8_kv_plan(const int32_t *kv_len, const int32_t *new_len, int R, int block, int32_t *block_table, int table_width,
