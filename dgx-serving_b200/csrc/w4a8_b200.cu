@@ -120,17 +120,17 @@ W4A8_API int w4a8_device_status(uint32_t *detail) {
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
     e = cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(v));
     if (e != cudaSuccess) return cuda_fail(e, "read device error word");
-    if (v != 0) cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
-    unsigned int kv_error = 0;
-    e = kv_take_device_error(&kv_error);
-    if (e != cudaSuccess) return cuda_fail(e, "read device error word");
-    if (v == 0 && kv_error != 0) {
-        if (detail) *detail = kv_error;
-        return fail(W4A8_ERR_DEVICE, "%s (code 0x%x)", kv_device_error_text(kv_error), kv_error);
-    }
-    if (v != 0) {
+    if (v != 0) {                                       // the cache's word, if it is set too, is the next call's
+        e = cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
+        if (e != cudaSuccess) return cuda_fail(e, "clear device error word");
         if (detail) *detail = v;
         return fail(W4A8_ERR_DEVICE, "a kernel's bounded wait ran out (code 0x%x)", v);
+    }
+    e = kv_take_device_error(&v);
+    if (e != cudaSuccess) return cuda_fail(e, "read device error word");
+    if (v != 0) {
+        if (detail) *detail = v;
+        return fail(W4A8_ERR_DEVICE, "%s (code 0x%x)", kv_device_error_text(v), v);
     }
     if (detail) *detail = 0;
     return W4A8_OK;
