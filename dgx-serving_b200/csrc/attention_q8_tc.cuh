@@ -43,6 +43,7 @@ constexpr int THREADS = 512;                   // warps 0-3, 4-7: rows of tile 0
 constexpr int MAX_R = 2048;
 constexpr int SCALE_SLOTS = 4;
 enum { TILE_PLAIN, TILE_CAPPED, TILE_FAR };    // what a tile's scores need
+constexpr int LONG_KEYS = 32768;               // keys of an item beyond which 16-bit rows' sums leave the tensor core with every tile, as fp32 rows' do
 constexpr int ORDINARY = 40;                   // exponents of ordinary scales, either way
 constexpr float DEAD = -60.f;                  // log2 of a block's largest weight, in what B stands for, below which it is nothing to the products
 
@@ -378,13 +379,16 @@ __device__ __forceinline__ void add_columns(float (&O)[128], uint32_t at, float 
     }
 }
 
-template <typename T, int D>
+// The tensor core's sums lose up to a unit in the last place with every sixteen keys, toward zero: 16-bit rows over 131072 keys were off by 7.9e-4, over
+// 2^20 by 6.3e-3.  SUMS: they are one tile's, and the rows' sums over the tiles are held in registers (fp32 rows; 16-bit rows over more than LONG_KEYS keys, which
+// are LONG's; 32768 lose 1.9e-4, less than fp16's rounding).
+template <typename T, int D, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn::Args a, const int8_t *__restrict__ kc, const int8_t *__restrict__ vc) {
     using S = Shape<T, D>;
     constexpr int KT = S::KT, NT = S::NT, ST = S::ST, TERMS = S::TERMS;
-    constexpr bool SPLIT = S::SPLIT;
-    constexpr int STEP = SPLIT ? 16 : 32;          // columns of scores in work; fp32 rows' registers hold O
-    constexpr int OWN = D < 128 ? D : 128;         // columns of O that a thread sums itself (fp32 rows)
+    constexpr bool SPLIT = S::SPLIT, SUMS = SPLIT || LONG;
+    constexpr int STEP = SUMS ? 16 : 32;           // columns of scores in work; where the registers do not hold O, more
+    constexpr int OWN = D < 128 ? D : 128;         // columns of O that a thread sums itself (SUMS)
     extern __shared__ unsigned char smem_raw[];
     __shared__ unsigned wsum[THREADS / 32];
     __shared__ int item[4];                       // request, kv head, row tile
@@ -440,12 +444,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
     const int hi_all = a.causal ? x.seq - x.n + last_q + 1 : x.seq;               // keys [lo_all, hi_all) for some row
     const int tile0 = lo_all / KT, n = hi_all > lo_all ? (hi_all + KT - 1) / KT - tile0 : 0;
 
+    if (!SPLIT && (n * KT > LONG_KEYS) != LONG) return;                          // the other kernel's
+
     if (warp == 13) {
         ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
         ptx::tmem_relinquish();
     }
     if (tid == 0) {
-        constexpr int P_COUNT = SPLIT && NT == 1 ? 256 : 128;
+        constexpr int P_COUNT = SUMS && NT == 1 ? 256 : 128;
         const int counts[BARS] = {1, 1, 4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, P_COUNT, P_COUNT, 1, 1, 1};
         for (int i = 0; i < BARS; i++) ptx::mbar_init(BAR(i), counts[i]);
         ptx::mbar_fence_init();
@@ -479,16 +485,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         const float inf = __int_as_float(0x7f800000);
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
         const uint32_t o_at = lanes + S::O_COL + t * D;
-        // fp32 rows: the tensor core's sums lose up to a unit in the last place with every sixteen keys (toward zero), so O in tensor memory
-        // is one tile's and the rows' sums over the tiles are held here, in registers
-        float O[SPLIT ? OWN : 1];
-        if constexpr (SPLIT) {
+        // SUMS: O in tensor memory is one tile's
+        float O[SUMS ? OWN : 1];
+        if constexpr (SUMS) {
 #pragma unroll
             for (int e = 0; e < OWN; e++) O[e] = 0.f;
         }
         float A = NONE, B = NONE, l = 0.f, shrink = 1.f;             // A follows B until a tile is far
         const auto take = [&](float by) {                            // O of the tile before, complete in tensor memory, into the registers
-            if constexpr (SPLIT) {
+            if constexpr (SUMS) {
 #pragma unroll
                 for (int c = 0; c < OWN / 32; c++) {
                     uint32_t o[32];
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 ptx::tc_fence_after_sync();
             };
             bool waited = NT == 2 || j == 0;                         // two row tiles: S_t of this tile came after PV_t of the one before
-            if (SPLIT && NT == 2 && j > 0) take(shrink);
+            if (SUMS && NT == 2 && j > 0) take(shrink);
             const RowMask mask = {key0, hi, lo};
             float2 top;
             if constexpr (FAR) top = top_of<KT, 16, true, true>(s_at, sc, fac, a.softcap, mask);
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                 l *= ex2(A - An);
                 A = An;
                 B = Bn;
-                if (!SPLIT && j > 0) {
+                if (!SUMS && j > 0) {
                     if (!waited) { products_before(); waited = true; }
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
@@ -544,14 +549,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
                     }
                 }
             }
-            if constexpr (FAR) weights<KT, 16, SPLIT, true, true, true>(s_at, sc, fac, a.softcap, A, B, mask, l);
+            float sum = 0.f;                                         // of the tile: one addition for each tile to the row's, not one for sixteen keys
+            if constexpr (FAR) weights<KT, 16, SPLIT, true, true, true>(s_at, sc, fac, a.softcap, A, B, mask, sum);
             else if constexpr (CAP) {
-                if (edge) weights<KT, 16, SPLIT, true, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
-                else weights<KT, 16, SPLIT, false, true, false>(s_at, sc, fac, a.softcap, A, B, mask, l);
+                if (edge) weights<KT, 16, SPLIT, true, true, false>(s_at, sc, fac, a.softcap, A, B, mask, sum);
+                else weights<KT, 16, SPLIT, false, true, false>(s_at, sc, fac, a.softcap, A, B, mask, sum);
             }
-            else if (edge) weights<KT, STEP, SPLIT, true, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
-            else weights<KT, STEP, SPLIT, false, false, false>(s_at, sc, fac, 0.f, A, B, mask, l);
-            if (SPLIT && NT == 1) {
+            else if (edge) weights<KT, STEP, SPLIT, true, false, false>(s_at, sc, fac, 0.f, A, B, mask, sum);
+            else weights<KT, STEP, SPLIT, false, false, false>(s_at, sc, fac, 0.f, A, B, mask, sum);
+            l += sum;
+            if (SUMS && NT == 1) {
                 if (j > 0) { products_before(); take(shrinks[(j - 1) & 1][tid]); }
                 shrinks[j & 1][tid] = shrink;                        // for the other half's warps, who read it before PV of tile j + 1
             } else if (!waited) products_before();                   // every phase is awaited, so none is mistaken for another
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         }
         const float2 unit = attn::pow2_parts((int)fminf(fmaxf(B - A, -250.f), 250.f));
         const float2 inv = make_float2((l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * unit.x, unit.y);
-        if (SPLIT && NT == 1) {
+        if (SUMS && NT == 1) {
             asm volatile("bar.sync 4, 256;" ::: "memory");           // the other half has read the last factor
             shrinks[0][tid] = inv.x;
             shrinks[1][tid] = inv.y;
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         static_assert(sizeof(T) == 2 * TERMS, "a row of the output takes what its terms took");
         const uint32_t rows_at = base + t * TERMS * S::QT + (tid & 96) * ROW, row_at = rows_at + lane * ROW;
         const int there = rows - (row0 + t * 128 + (tid & 96));
-        if constexpr (SPLIT) {
+        if constexpr (SUMS) {
             stage<OWN, T>(row_at, lane, 0, O, inv);
             rows_out<OWN, T>(rows_at, ROW, 0, dst, there, lane);
         } else {
@@ -606,8 +613,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         }
         if (a.lse && row < rows) a.lse[(size_t)(x.q0 + query) * a.Hq + head] = l > 0.f ? (A + log2f(l)) * LN2 : (l == 0.f ? -inf : l);
         ptx::tc_fence_before_sync();
-    } else if (SPLIT && NT == 1 && warp >= 4 && warp < 8) {
-        // ---- dim 256, fp32 rows: the second half of O's columns ----------------------------------------------------------------------------
+    } else if (SUMS && NT == 1 && warp >= 4 && warp < 8) {
+        // ---- dim 256, SUMS: the second half of O's columns ----------------------------------------------------------------------------
         raise_registers<200>();
         const int lr = tid & 127, row = row0 + lr, query = min(row, rows - 1) / a.G, head = h * a.G + min(row, rows - 1) % a.G;
         const uint32_t o_at = tmem + ((uint32_t)(warp & 3) << 21) + S::O_COL + 128;
@@ -632,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
         asm volatile("bar.sync 3, 256;" ::: "memory");
         const uint32_t rows_at = base + (tid & 96) * (D * sizeof(T));
         stage<128, T>(rows_at + lane * (D * sizeof(T)), lane, 128, O, make_float2(shrinks[0][lr], shrinks[1][lr]));
-        rows_out<128, T>(rows_at, D * sizeof(T), 32, static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, rows - (row0 + (tid & 96)), lane);
+        rows_out<128, T>(rows_at, D * sizeof(T), 128 * (int)sizeof(T) / 16, static_cast<T *>(a.out) + (long long)(x.q0 + query) * a.ldo + (long long)head * D + 128, rows - (row0 + (tid & 96)), lane);
         ptx::tc_fence_before_sync();
     } else if (warp >= 8 && warp < 12) {
         // ---- codes to fp16 -------------------------------------------------------------------------------------------------------------
@@ -751,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
 #pragma unroll
                     for (int k = 0; k < KT / 16; k++)
                         umma_f16_ts(lead, tmem + S::O_COL + t * D, tmem + buf * S::S_COLS + 16 * k + 8 * term,
-                                    desc_mn_sw128(vb + k * 16 * 128, KT * 128), id_o, (!SPLIT && j > 0) || term > 0 || k > 0);
+                                    desc_mn_sw128(vb + k * 16 * 128, KT * 128), id_o, (!SUMS && j > 0) || term > 0 || k > 0);
             };
             wait(K_FULL, 0, 8u);
             if (ok) {
@@ -790,10 +797,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_q8_tc_kernel(const attn:
     if (warp == 13) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool LONG>
 inline int launch_t(const attn::Call &c, cudaStream_t st) {
     using S = Shape<T, D>;
-    auto kern = attention_q8_tc_kernel<T, D>;
+    auto kern = attention_q8_tc_kernel<T, D, LONG>;
     static PerDevice<bool> configured;
     if (!configured.get()) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -808,7 +815,14 @@ inline int launch_t(const attn::Call &c, cudaStream_t st) {
 }
 
 inline int launch(const attn::Call &c, cudaStream_t st) {
-    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) { return launch_t<decltype(t), decltype(d)::value>(c, st); });
+    return kv::by_type(c.dtype, c.dim, [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        const int rc = launch_t<T, D, false>(c, st);
+        if constexpr (!Shape<T, D>::SPLIT)                              // can a request be that long?
+            if (rc == W4A8_OK && (long long)c.a.width * c.a.block > LONG_KEYS) return launch_t<T, D, true>(c, st);
+        return rc;
+    });
 }
 
 }  // namespace attn_tc
