@@ -4,6 +4,7 @@ One step takes the new rows of any number of requests side by side (prompts, chu
 
     plan      block tables and slots of the step, from the lengths, on the GPU        w4a8_kv_plan
     qkv       the rows' queries, keys and values, one W4A8 product                    w4a8_linear
+    rotate    the caller's, if there is one: rotary positions, norms                  -
     append    keys and values into their blocks as int8 codes                         w4a8_kv_append_q8
     attend    every row over all tokens that its request holds                        w4a8_attention_q8
     out       the output product                                                      w4a8_linear
@@ -33,15 +34,17 @@ class PagedTables:
         self.cu = torch.zeros(requests + 1, **i32)
         self.status = torch.zeros(4, **i32)                  # [0]: the first free block of the next step
         self.first = torch.zeros(1, **i32)
-        self.slot = torch.empty(0, **i32)                    # of the step's rows
+        self.slot = torch.empty(0, **i32)                    # of the step's rows, and their places in their requests
+        self.position = torch.empty(0, **i32)
 
     def step(self, new_len, T):
         """Room for new_len[r] tokens of each request (int32, on the GPU), T rows in all; slots of the rows, -1 where there was none."""
         if new_len.dtype != torch.int32 or new_len.shape != (self.R,) or not new_len.is_contiguous() or new_len.device != self.table.device:
             raise ValueError("new_len: %d int32 numbers, contiguous, on %s" % (self.R, self.table.device))
         self.slot = torch.empty(T, dtype=torch.int32, device=new_len.device)
+        self.position = torch.empty_like(self.slot)
         w4a8.kv_plan(self.kv_len, new_len, self.R, self.block, self.table, self.width, self.free, self.num_blocks, self.first, self.seq_len, self.cu,
-                     self.slot, None, T, self.status)
+                     self.slot, self.position, T, self.status)
         return self.slot
 
     def done(self):
@@ -63,11 +66,12 @@ class PagedTables:
 
 class AttentionBlock:
     """One layer.  wqkv: (Wq, scales) of [(heads_q + 2 * heads) * dim][hidden] (queries, keys, values), wo: of [hidden][heads_q * dim]; both
-    packed int4 with fp32 scales of 32 elements."""
+    packed int4 with fp32 scales of 32 elements.  rotate(q, k, position), if there is one, is called between the QKV product and the append with the rows'
+    queries [T][heads_q][dim] and keys [T][heads][dim], to be changed in place (rotary positions, norms of queries and keys), and the rows' positions."""
 
-    def __init__(self, wqkv, wo, hidden, heads_q, heads, dim, tables, max_rows, scale=None, window=0, softcap=0.0):
+    def __init__(self, wqkv, wo, hidden, heads_q, heads, dim, tables, max_rows, scale=None, window=0, softcap=0.0, rotate=None):
         self.wqkv, self.wo, self.hidden, self.heads_q, self.heads, self.dim, self.tables = wqkv, wo, hidden, heads_q, heads, dim, tables
-        self.max_rows = max_rows
+        self.max_rows, self.rotate = max_rows, rotate
         self.scale, self.window, self.softcap = dim ** -0.5 if scale is None else scale, window, softcap
         dev = tables.table.device
         codes = (tables.num_blocks, heads, tables.block, dim)
@@ -105,6 +109,8 @@ class AttentionBlock:
         q, k, v = self.qkv, self.qkv[:, self.heads_q * self.dim:], self.qkv[:, (self.heads_q + self.heads) * self.dim:]
         self.mix[:T].zero_()                                 # rows behind the last request's (a padded step) are left as they are by the attention
         w4a8.linear(X, self.xq, self.xs, self.xsum, *self.wqkv, self.qkv, T, self.cols, self.hidden)
+        if self.rotate is not None:
+            self.rotate(q[:T, : self.heads_q * self.dim].view(T, self.heads_q, self.dim), k[:T, : self.heads * self.dim].view(T, self.heads, self.dim), t.position)
         w4a8.launch_kv_append_q8(k, v, self.cols, t.slot, T, self.cache)
         w4a8.launch_attention_q8(q, self.cols, self.cache, t.table, t.width, t.cu, t.seq_len, t.R, T, self.heads_q, self.mix, self.heads_q * self.dim,
                                  self.scale, "fp32", self.workspace, window=self.window, softcap=self.softcap, max_q=max_q)
