@@ -156,7 +156,7 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
 }
-// Power of two that brings a row whose largest magnitude is amax near 2^13, and its inverse times `scale`.
+// Power of two that brings a row whose largest magnitude is amax near 2^13; 1 for zeros and what is no number.
 __device__ __forceinline__ float row_factor(float amax) {
     if (!(amax > 0.f) || !(amax < __int_as_float(0x7f800000))) return 1.f;
     int e = 13 - (((__float_as_int(amax) >> 23) & 0xFF) - 127);

@@ -70,7 +70,7 @@ W4A8_API int w4a8_kv_plan(const int32_t *kv_len, const int32_t *new_len, int R, 
                 return fail(W4A8_ERR_ARG, "kv_plan: %s overlaps %s, an input that is read to the end", o.name, i.name);
     int rc = require_sm100();
     if (rc != W4A8_OK) return rc;
-    kv::PlanArgs a = {kv_len, new_len, free_blocks, first_free, block_table, seq_len, cu_new, slot, position, status, R, block, table_width, num_free, T};
+    kv::PlanArgs a = {kv_len, new_len, free_blocks, first_free, block_table, seq_len, cu_new, slot, position, status, R, block, table_width, num_free, T, 0x7fffffffu / (unsigned)block};
     return kv::launch_plan(a, (cudaStream_t)stream);
 }
 
