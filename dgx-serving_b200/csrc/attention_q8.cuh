@@ -11,20 +11,20 @@
 //  - Both products are tcgen05.mma kind::i8 with the keys' tile as the 128-row operand, so the codes go from HBM by TMA to shared memory (128-byte
 //    swizzle; along the block table, a block never has to be a whole tile) and no thread touches them: S^T [keys][rows] = K Q^T with K as it
 //    lies, O^T [dim][rows] += V^T P^T with V read as the transposed operand.  Widening the codes to fp16 for mma.sync cost 450 instructions for 16
-//    keys and bound the stream: two requests of 115k tokens 96 us, 64 ragged ones of up to 8192 tokens 128.  Now 84 us (5.9 TB/s) and 99 (5.5).
+//    keys and bound the stream: two requests of 115k tokens 96 us, 64 ragged ones of up to 8192 tokens 128.  Now 84 us (5.9 TB/s) and 101 (5.4).
 //  - A query row is a fixed-point number relative to its largest magnitude, three signed digits of base 256 (2^-23 of it): three columns.  A weight
 //    times its block's scale is a whole number too, x = exp(s) 2^-A * vs 2^-E * 2^25 up to 2^31, four columns of P.  All sums are whole numbers and
 //    exact; O stays in tensor memory over the tiles.  The row's reference A is such that its largest weight was in [1, 2) when it was chosen, E is the
 //    largest exponent of the scales of blocks that the row has seen of.  When a weight would pass 2^4.9 or E grows, O is read out, rescaled and summed in
 //    fp32.  So a weight times its scale is rounded to 2^-26 of the row's largest of either, or as fp32 is; A and E are whole numbers and rescaling is
 //    exact.  The sum of the weights, l = sum exp(s) 2^-A, knows nothing of the scales.  (One reference for the products, 2^28 for the largest, with l
-//    taken from them by 1 / vs, took 51.4, 40 and 98.9 us where few queries, a window and ragged tokens now take 55.4, 41.1 and 100.3; but l left fp32
+//    taken from them by 1 / vs, took 51.5, 40.4 and 98.9 us where few queries, a window and ragged tokens now take 53.5, 43 (two of it the caps) and 100.8; but l left fp32
 //    at scales above 2^62, and lost the weights of tokens whose scale is 2^-150 of another's.)
 //  - 128 threads have a key each, about thirty instructions for a row.  Two such groups take the tiles in turn, each with its own S, P, O, reference and
 //    sums, because a tile's chain of steps (1300 cycles with 4 rows, 3500 with 16) takes longer than its bytes do; they meet at the end of a pair, one
 //    handing over, the other writing.
 //  - What is left: 3 us before the first tile and 3 us for the last join, and for many rows the chain: 16 requests of up to 56 rows and 6000 tokens take
-//    52 us where their bytes take 9.
+//    54 us where their bytes take 9.
 #pragma once
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"

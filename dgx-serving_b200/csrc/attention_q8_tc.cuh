@@ -16,8 +16,8 @@
 //    own, A, and a block's x are taken back from B to A by powers of two, or, where they are less than 2^-60 of what B stands for, are the sum's alone.
 //    Both ways give the same bits where both can, so a row's result does not depend on scales that it does not see.
 //  - fp32 rows enter as two fp16 terms each, Q and P: twice the products, 22 bits.
-// One prompt of 4096 tokens, 32 heads of 128 over 8, causal: 208 us, 661 TFLOP/s of the 1633 that a large product reaches.  A step of two row
-// tiles and 128 keys takes about 4600 cycles where its products take 2100 and its exponentials 2050: the row's warps, two on a scheduler, are in
+// One prompt of 4096 tokens, 32 heads of 128 over 8, causal: 201 us, 684 TFLOP/s of the 1633 that a large product reaches.  A step of two row
+// tiles and 128 keys took about 4600 cycles, at 206 us, where its products take 2100 and its exponentials 2050: the row's warps, two on a scheduler, are in
 // the way, with the maximum (850), the wait for the scores (1450) and the weights (2500).  Steps of 64 keys with two buffers of scores for each row
 // tile hid the wait, and had every step's fixed costs twice: 240 us.
 #pragma once

@@ -325,9 +325,12 @@ int w4a8_kv_read_q8(const w4a8_kv_cache *cache, const int32_t *block_table, int 
  * heads <= 64) are whole numbers in units of 2^-23 of their largest magnitude, their weights times values' scales of 2^-25 of the row's largest
  * weight times the largest scale that it sees; rows of prompts and their weights enter the products in one fp16 term each, fp32 rows' in two (22
  * bits).
+ * fp32 rows' sums over the keys are rounded once for every 64 or 128 of them; 16-bit rows' with every sixteen, toward zero, up to 32768 keys (1.9e-4 of
+ * the result), and like fp32 rows' beyond.
  * max_q: no request has more rows (0: not known); it chooses the kernel, not the result's meaning.
  * The workspace (256-byte aligned, zeroed once by the caller, left zeroed where that matters) serves one stream at a time; its size holds
- * for any lengths.  Row order, requests side by side and the GPU's SM count decide how the key axis is cut, so a row's last bits can differ
+ * for any lengths (T and max_q do not change it).  After w4a8_device_status has reported a wait that ran out it has to be zeroed again: parts of
+ * requests may have been counted that nobody joined.  Row order, requests side by side and the GPU's SM count decide how the key axis is cut, so a row's last bits can differ
  * between batches; the same call gives the same bits. */
 size_t w4a8_attention_q8_workspace_bytes(const w4a8_kv_cache *cache, int heads_q, int T, int max_q);
 int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *cache, const int32_t *block_table, int table_width, const int32_t *cu_q,
