@@ -64,6 +64,84 @@ class KVCache(ctypes.Structure):
         return c
 
 
+def _fp32_vector(t, n, name):
+    """A contiguous fp32 tensor of n elements on a GPU, or None."""
+    if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != n or not t.is_contiguous() or not t.is_cuda):
+        raise ValueError("%s: %d contiguous fp32 numbers on a GPU" % (name, n))
+    return t
+
+
+class Norm(ctypes.Structure):
+    """Mirror of w4a8_norm: the weights and constants of one residual add with its norms."""
+    _fields_ = [("weight", ctypes.c_void_p), ("post_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("gate_ld", ctypes.c_int64), ("eps", ctypes.c_double),
+                ("alpha", ctypes.c_float), ("K", ctypes.c_int), ("variant", ctypes.c_int), ("post_variant", ctypes.c_int), ("dtype", ctypes.c_int), ("y_dtype", ctypes.c_int)]
+
+    @classmethod
+    def of(cls, K, weight=None, variant=0, eps=1e-6, post_weight=None, post_variant=-1, gate=None, alpha=1.0, dtype="fp32", y_dtype=None):
+        """weight, post_weight: fp32 [K] tensors, which the object keeps alive.  gate: fp32 [K], or [S][K] with a row for each token.  variant -1: no norm,
+        0: * weight, 1: * (1 + weight), 2: no weight.  y_dtype None: dtype."""
+        _fp32_vector(weight, K, "weight")
+        _fp32_vector(post_weight, K, "post_weight")
+        gate_ld = 0
+        if gate is not None:
+            if str(gate.dtype) != "torch.float32" or not gate.is_cuda or gate.dim() not in (1, 2) or gate.shape[-1] != K or (K > 1 and gate.stride(-1) != 1):
+                raise ValueError("gate: fp32 [%d] or [rows][%d] on a GPU" % (K, K))
+            gate_ld = gate.stride(0) if gate.dim() == 2 else 0
+            if gate.dim() == 2 and gate_ld < K:
+                raise ValueError("gate: rows that overlap")
+        n = cls(_ptr(weight), _ptr(post_weight), _ptr(gate), gate_ld, float(eps), float(alpha), K, variant, post_variant, DTYPES[dtype], DTYPES[dtype if y_dtype is None else y_dtype])
+        n._tensors = (weight, post_weight, gate)
+        return n
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4, "divisors": 5}
+
+
+def rope_table(rotary, base=10000.0, scaling="none", factor=1.0, original=0.0, low=0.0, high=0.0, divisors=None):
+    """The frequencies of rotary / 2 pairs in units of 2^-64 turn a token (a list of whole numbers), and what cosine and sine are multiplied by
+    (w4a8_rope_table)."""
+    n = max(0, rotary) // 2
+    if divisors is not None and len(divisors) != n:
+        raise ValueError("divisors: one for each of the %d pairs" % n)
+    turns, magnitude = (ctypes.c_uint64 * max(1, n))(), ctypes.c_float(0.0)
+    _check(lib().w4a8_rope_table(rotary, float(base), ROPE_SCALINGS[scaling], float(factor), float(original), float(low), float(high),
+                                 None if divisors is None else (ctypes.c_double * max(1, n))(*[float(d) for d in divisors]), turns, ctypes.byref(magnitude)))
+    return list(turns[:n]), magnitude.value
+
+
+class Rope(ctypes.Structure):
+    """Mirror of w4a8_rope: frequencies of rotary positions on the GPU, and the norms of queries and keys."""
+    _fields_ = [("turns", ctypes.c_void_p), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("eps", ctypes.c_double), ("magnitude", ctypes.c_float),
+                ("dim", ctypes.c_int), ("rotary", ctypes.c_int), ("interleaved", ctypes.c_int), ("variant", ctypes.c_int)]
+
+    @classmethod
+    def of(cls, dim, rotary, base=10000.0, scaling="none", interleaved=False, q_weight=None, k_weight=None, variant=-1, eps=1e-6, device="cuda", magnitude=None, **parameters):
+        """Heads of `dim` elements, the first `rotary` of them turned.  scaling and parameters: rope_table's; magnitude: instead of the scaling's own.
+        q_weight, k_weight: fp32 [dim], kept alive as the table is."""
+        import torch
+        _fp32_vector(q_weight, dim, "q_weight")
+        _fp32_vector(k_weight, dim, "k_weight")
+        turns, m = rope_table(rotary, base, scaling, **parameters)
+        table = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=device)
+        r = cls(_ptr(table) if turns else None, _ptr(q_weight), _ptr(k_weight), float(eps), float(m if magnitude is None else magnitude), dim, rotary, int(bool(interleaved)), variant)
+        r._tensors = (table, q_weight, k_weight)
+        return r
+
+
+class Router(ctypes.Structure):
+    """Mirror of w4a8_router: how experts are chosen."""
+    _fields_ = [("bias", ctypes.c_void_p), ("experts", ctypes.c_int), ("topk", ctypes.c_int), ("scoring", ctypes.c_int), ("groups", ctypes.c_int), ("topk_groups", ctypes.c_int),
+                ("group_score", ctypes.c_int), ("renormalise", ctypes.c_int), ("scale", ctypes.c_float)]
+
+    @classmethod
+    def of(cls, experts, topk, scoring="softmax", bias=None, groups=1, topk_groups=1, group_score="max", renormalise=True, scale=1.0):
+        """scoring: "softmax" or "sigmoid"; group_score: "max" or "sum2"; bias: fp32 [experts], kept alive."""
+        _fp32_vector(bias, experts, "bias")
+        r = cls(_ptr(bias), experts, topk, {"softmax": 0, "sigmoid": 1}[scoring], groups, topk_groups, {"max": 0, "sum2": 1}[group_score], int(bool(renormalise)), float(scale))
+        r._tensors = (bias,)
+        return r
+
+
 def _on_gpu(cache):
     """The cache, unless KVCache.of made it of tensors in host memory: a launch would follow their pointers."""
     if getattr(cache, "_host", False):
@@ -101,6 +179,13 @@ _SIGNATURES = {
     "w4a8_attention_q8_workspace_bytes": (_Z, [ctypes.POINTER(KVCache), _I, _I, _I]),
     "w4a8_attention_q8": (_I, [_P, _L, ctypes.POINTER(KVCache), _P, _I, _P, _P, _I, _I, _I, _P, _L, _P, ctypes.c_float, _I, _I, ctypes.c_float, _I, _I,
                                _P, _Z, _P]),
+    "w4a8_add_norm": (_I, [ctypes.POINTER(Norm), _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _I, _I, _P]),
+    "w4a8_rope_table": (_I, [_I, ctypes.c_double, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _P, _P, ctypes.POINTER(ctypes.c_float)]),
+    "w4a8_rope_qk": (_I, [ctypes.POINTER(Rope), _P, _L, _I, _P, _L, _I, _P, _I, _P, _L, _P, _L, _I, _P]),
+    "w4a8_moe_route": (_I, [ctypes.POINTER(Router), _P, _L, _I, _I, _P, _P, _P]),
+    "w4a8_quantize_rows_q8": (_I, [_P, _L, _I, _I, _I, _P, _P, _P]),
+    "w4a8_gemm_w8a8": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "w4a8_linear_w8a8": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P]),
     "w4a8_shard_rows": (_I, [_L, _I, _I, ctypes.POINTER(_L), ctypes.POINTER(_L)]),
     "w4a8_load_qmat_shard": (_I, [ctypes.c_char_p, ctypes.c_char_p, _L, _L, _I, _I, _I, ctypes.POINTER(QMat)]),
     "w4a8_upload_qmat_shard": (_I, [_P, _P, _L, _L, _I, _I, _I, ctypes.POINTER(QMat)]),
@@ -326,6 +411,43 @@ def launch_attention_q8(Q, ldq, cache, block_table, table_width, cu_q, seq_len, 
     _check(lib().w4a8_attention_q8(_ptr(Q), ldq, _on_gpu(cache), _ptr(block_table), table_width, _ptr(cu_q), _ptr(seq_len), R, T, heads_q, _ptr(O), ldo, _ptr(lse),
                                    scale, causal, window, softcap, max_q, DTYPES.get(dtype, dtype), _ptr(workspace),
                                    workspace.numel() * workspace.element_size(), _stream(stream)))
+
+
+def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=None, group=32, ldh=0, ldy=0, ldo=0, ldn=0, stream=None):
+    """h' = h + norm(y) * gate * alpha of S rows, to H_out, and its norm n, to N and / or quantized to xq, xs, xsum (w4a8_add_norm).  Y None: h' = h.
+    group 32: blocks of 32 elements, 0: one scale for a row.  Pitches of 0: K."""
+    K = norm.K
+    _check(lib().w4a8_add_norm(norm, _ptr(H), ldh or K, _ptr(Y), ldy or K, _ptr(H_out), ldo or K, _ptr(N), ldn or K, _ptr(xq), _ptr(xs), _ptr(xsum), group, S, _stream(stream)))
+
+
+def launch_rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out=None, ldqo=0, K_out=None, ldko=0, dtype="fp32", stream=None):
+    """Norms and rotary positions of queries Q[T][heads_q * dim] and keys K[T][heads_k * dim] (w4a8_rope_qk); outputs None: in place."""
+    if Q_out is None:
+        Q_out, ldqo = Q, ldq
+    if K_out is None:
+        K_out, ldko = K, ldk
+    _check(lib().w4a8_rope_qk(rope, _ptr(Q), ldq, heads_q, _ptr(K), ldk, heads_k, _ptr(position), T, _ptr(Q_out), ldqo, _ptr(K_out), ldko, DTYPES.get(dtype, dtype), _stream(stream)))
+
+
+def launch_moe_route(router, logits, ld, S, idx, weight, dtype="fp32", stream=None):
+    """The experts idx[S][topk] of S tokens and their weights, from logits[S][experts] (w4a8_moe_route): what moe_block takes."""
+    _check(lib().w4a8_moe_route(router, _ptr(logits), ld, S, DTYPES.get(dtype, dtype), _ptr(idx), _ptr(weight), _stream(stream)))
+
+
+def launch_quantize_rows_q8(X, ldx, S, K, xq, xs, dtype="fp32", stream=None):
+    """Rows to int8 with one scale each (w4a8_quantize_rows_q8): activations of the 8-bit products, or their weights, a channel per row."""
+    _check(lib().w4a8_quantize_rows_q8(_ptr(X), ldx, S, K, DTYPES.get(dtype, dtype), _ptr(xq), _ptr(xs), _stream(stream)))
+
+
+def launch_gemm_w8a8(xq, xs, wq, ws, Y, ldy, M, N, K, dtype="fp32", bias=None, stream=None):
+    """Y[M][N] = xq wq^T * xs[m] * ws[n] + bias[n], the sums exact (w4a8_gemm_w8a8)."""
+    _check(lib().w4a8_gemm_w8a8(_ptr(xq), _ptr(xs), _ptr(wq), _ptr(ws), _ptr(bias), _ptr(Y), ldy, M, N, K, DTYPES.get(dtype, dtype), _stream(stream)))
+
+
+def linear_w8a8(X, ldx, xq, xs, wq, ws, Y, ldy, S, N, K, x_dtype="fp32", y_dtype="fp32", bias=None, skip_quantize=0, stream=None):
+    """linear() for 8-bit weights with a scale for each output channel (w4a8_linear_w8a8)."""
+    _check(lib().w4a8_linear_w8a8(_ptr(X), ldx, _ptr(xq), _ptr(xs), _ptr(wq), _ptr(ws), _ptr(bias), _ptr(Y), ldy, S, N, K, DTYPES.get(x_dtype, x_dtype),
+                                  DTYPES.get(y_dtype, y_dtype), skip_quantize, _stream(stream)))
 
 
 def shard_rows(N, rank, world):

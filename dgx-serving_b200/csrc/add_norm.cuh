@@ -1,0 +1,231 @@
+// Residual add and norms of rows in one kernel, with the quantizer of the product that follows:
+//   p = norm(y) * gate * alpha,  h' = h + p,  n = norm(h'),  n -> its own type and / or int8 codes.
+// Each of these is a pass over the rows in the graphs (kernels/norm_fused.cuh, kernels/rmsnorm.cuh, kernels/quantize_x.cuh); together they read h and y
+// once and write h' and n once, which is what bounds the kernel for many rows.  A CTA has a row, its threads keep the row's elements in registers
+// between the passes over it: the sum of squares of y (if y is normed), the sum of squares of h', the largest magnitude of n (if a row has
+// one scale).
+//
+// Every element is computed by single fp32 operations in a stated order and the sums of squares in fp64, with one rounding of the factor
+// r to fp32: how many threads share a row then changes no bit of any output, and codes are the same wherever they are made.  The fp64
+// additions cost nothing where HBM is the bound (one conversion and one fma an element, against 16 bytes of traffic).
+#pragma once
+#include "common.cuh"
+#include "rows.cuh"
+
+namespace w4a8 {
+namespace addnorm {
+
+constexpr int MAX_K = 32768;
+
+struct Args {
+    const void *h, *y;
+    void *h_out, *n_out;
+    const float *w, *pw, *gate;
+    int64_t ldh, ldy, ldo, ldn, ldg;
+    int8_t *xq;
+    float *xs;
+    int32_t *xsum;
+    double inv_k, eps;
+    float alpha;
+    int K, variant, post, group;                  // group 32, or 0: one scale for the row
+};
+
+// The sum over the CTA, in every thread; the same bits in all of them.
+__device__ __forceinline__ double cta_sum(double v, double *sh) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (warps == 1) return v;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? sh[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float cta_max(float v, float *sh) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (warps == 1) return v;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? sh[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+template <int V>
+__device__ __forceinline__ double squares(const float (&x)[V], double ss) {
+#pragma unroll
+    for (int i = 0; i < V; i++) ss = fma((double)x[i], (double)x[i], ss);
+    return ss;
+}
+// x * r * w, x * r * (1 + w) or x * r, from left to right.
+template <int V>
+__device__ __forceinline__ void normed(float (&x)[V], float r, const float *w, int variant) {
+    float f[V];
+    if (variant != W4A8_NORM_NO_SCALE) load_row<float, V>(w, f);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        x[i] = __fmul_rn(x[i], r);
+        if (variant == W4A8_NORM_SCALE) x[i] = __fmul_rn(x[i], f[i]);
+        if (variant == W4A8_NORM_ONE_PLUS) x[i] = __fmul_rn(x[i], __fadd_rn(1.f, f[i]));
+    }
+}
+
+// Elements of one thread's vector: 16 bytes of rows where all are fp32, eight elements where some have 16 bits.
+template <typename TH, typename TY>
+constexpr int VEC = sizeof(TH) == 4 && sizeof(TY) == 4 ? 4 : 8;
+
+template <typename TH, typename TY, int EP, int MAXT>                  // EP elements a thread
+__global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
+    constexpr int V = VEC<TH, TY>, NV = EP / V;
+    __shared__ double sh_y[32], sh_h[32];
+    __shared__ float sh_max[32];
+    const int nt = blockDim.x, nvec = a.K / V;
+    const size_t row = blockIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    const TH *h = static_cast<const TH *>(a.h) + row * a.ldh;
+    float x[NV][V];
+#pragma unroll
+    for (int u = 0; u < NV; u++) {
+        const int j = threadIdx.x + u * nt;
+#pragma unroll
+        for (int i = 0; i < V; i++) x[u][i] = 0.f;
+        if (j < nvec) load_row<TH, V>(h + j * V, x[u]);
+    }
+    if (a.y) {
+        const TY *y = static_cast<const TY *>(a.y) + row * a.ldy;
+        float p[NV][V];
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int j = threadIdx.x + u * nt;
+#pragma unroll
+            for (int i = 0; i < V; i++) p[u][i] = 0.f;
+            if (j < nvec) load_row<TY, V>(y + j * V, p[u]);
+        }
+        float r = 1.f;
+        if (a.post != W4A8_NORM_NONE) {
+            double ss = 0.0;
+#pragma unroll
+            for (int u = 0; u < NV; u++) ss = squares(p[u], ss);
+            r = (float)rsqrt(fma(cta_sum(ss, sh_y), a.inv_k, a.eps));
+        }
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int j = threadIdx.x + u * nt;
+            if (j < nvec) {
+                if (a.post != W4A8_NORM_NONE) normed(p[u], r, a.pw + j * V, a.post);
+                if (a.gate) {
+                    float g[V];
+                    load_row<float, V>(a.gate + row * a.ldg + j * V, g);
+#pragma unroll
+                    for (int i = 0; i < V; i++) p[u][i] = __fmul_rn(p[u][i], g[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) x[u][i] = __fadd_rn(x[u][i], __fmul_rn(p[u][i], a.alpha));
+            }
+        }
+    }
+    if (a.h_out) {
+        TH *o = static_cast<TH *>(a.h_out) + row * a.ldo;
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int j = threadIdx.x + u * nt;
+            if (j < nvec) store_row<TH, V>(o + j * V, x[u]);
+        }
+    }
+    if (!a.n_out && !a.xq) return;
+    if (a.variant != W4A8_NORM_NONE) {
+        double ss = 0.0;
+#pragma unroll
+        for (int u = 0; u < NV; u++) ss = squares(x[u], ss);
+        const float r = (float)rsqrt(fma(cta_sum(ss, sh_h), a.inv_k, a.eps));
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int j = threadIdx.x + u * nt;
+            if (j < nvec) normed(x[u], r, a.w + j * V, a.variant);
+        }
+    }
+    if (a.n_out) {
+        TH *o = static_cast<TH *>(a.n_out) + row * a.ldn;
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int j = threadIdx.x + u * nt;
+            if (j < nvec) store_row<TH, V>(o + j * V, x[u]);
+        }
+    }
+    if (!a.xq) return;
+    float amax[NV], top = 0.f;
+#pragma unroll
+    for (int u = 0; u < NV; u++) {
+        amax[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; i++) amax[u] = fmaxf(amax[u], fabsf(x[u][i]));
+        top = fmaxf(top, amax[u]);
+    }
+    if (a.group == 0) top = cta_max(top, sh_max);
+#pragma unroll
+    for (int u = 0; u < NV; u++) {
+        const int j = threadIdx.x + u * nt;
+        float m = top;
+        if (a.group != 0) {                                            // the 32 / V lanes of a block: all of them have elements, or none
+            m = amax[u];
+#pragma unroll
+            for (int o = 1; o < 32 / V; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        const float d = quant_scale(m);
+        uint32_t q[V / 4];
+        int sum = 0;
+#pragma unroll
+        for (int c = 0; c < V / 4; c++) {
+            int s4 = 0;
+            q[c] = m != 0.f ? quantize4_pack(make_float4(x[u][4 * c], x[u][4 * c + 1], x[u][4 * c + 2], x[u][4 * c + 3]), d, s4) : 0u;
+            sum += s4;
+        }
+        if (a.group != 0 && a.xsum) {
+#pragma unroll
+            for (int o = 1; o < 32 / V; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        if (j < nvec) {
+            int8_t *dst = a.xq + row * a.K + j * V;
+            if constexpr (V == 4) *reinterpret_cast<uint32_t *>(dst) = q[0];
+            else *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0], q[1]);
+            if (a.group != 0) {
+                if (j % (32 / V) == 0) {
+                    const size_t b = row * (a.K / 32) + j / (32 / V);
+                    a.xs[b] = d;
+                    if (a.xsum) a.xsum[b] = sum;
+                }
+            } else if (j == 0) {
+                a.xs[row] = d;
+            }
+        }
+    }
+}
+
+template <typename TH, typename TY, int EP, int MAXT>
+inline int launch_ep(const Args &a, int S, cudaStream_t st) {
+    const int need = (a.K + EP - 1) / EP;
+    const cudaError_t e = launch_pdl(add_norm_kernel<TH, TY, EP, MAXT>, dim3(S), dim3((need + 31) / 32 * 32), 0, st, a);
+    if (e != cudaSuccess) return cuda_fail(e, "add_norm launch");
+    return launch_status("add_norm");
+}
+template <typename TH, typename TY>
+inline int launch_t(const Args &a, int S, cudaStream_t st) {
+    if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024>(a, S, st);
+    if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512>(a, S, st);
+    if (a.K <= 512 * 32) return launch_ep<TH, TY, 32, 512>(a, S, st);
+    return launch_ep<TH, TY, 32, 1024>(a, S, st);
+}
+inline int launch(const Args &a, int S, int dtype, int y_dtype, cudaStream_t st) {
+    if (dtype == W4A8_F32) return launch_t<float, float>(a, S, st);
+    if (dtype == W4A8_F16) return y_dtype == W4A8_F32 ? launch_t<__half, float>(a, S, st) : launch_t<__half, __half>(a, S, st);
+    return y_dtype == W4A8_F32 ? launch_t<__nv_bfloat16, float>(a, S, st) : launch_t<__nv_bfloat16, __nv_bfloat16>(a, S, st);
+}
+
+}  // namespace addnorm
+}  // namespace w4a8

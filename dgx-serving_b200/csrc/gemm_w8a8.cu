@@ -1,0 +1,51 @@
+// The 8-bit products' translation unit of libw4a8_b200.so.
+#include "common.cuh"
+#include "gemm_w8a8.cuh"
+
+namespace w4a8 {
+
+// The device-side error word of this translation unit, read and cleared (w4a8_device_status).
+cudaError_t w8a8_take_device_error(unsigned int *v) {
+    const unsigned int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(v, g_dev_error, sizeof(*v));
+    if (e == cudaSuccess && *v != 0) e = cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero));
+    return e;
+}
+
+}  // namespace w4a8
+
+using namespace w4a8;
+
+W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy, int M, int N, int K,
+                            int dtype, void *stream) {
+    const char *who = "gemm_w8a8";
+    const size_t size = row_size(dtype);
+    if (!size) return fail(W4A8_ERR_ARG, "%s: dtype=%d (0 fp32, 1 fp16, 2 bf16)", who, dtype);
+    if (M < 0 || N < 0 || K < 0 || K % QBLK != 0) return fail(W4A8_ERR_ARG, "%s: M=%d N=%d K=%d (K must be a multiple of %d)", who, M, N, K, QBLK);
+    if (K > w8a8::MAX_K) return fail(W4A8_ERR_UNSUPPORTED, "%s: K=%d (at most %d: sums have to fit 32 bits)", who, K, w8a8::MAX_K);
+    if (M == 0 || N == 0) return W4A8_OK;
+    if (K == 0) return fail(W4A8_ERR_ARG, "%s: K=0", who);
+    if (!xq || !xs || !wq || !ws || !Y) return fail(W4A8_ERR_ARG, "%s: null pointer argument", who);
+    if (ldy < N) return fail(W4A8_ERR_ARG, "%s: Y has rows of %d elements, a pitch of %lld", who, N, (long long)ldy);
+    if (!aligned(xq, 16) || !aligned(wq, 16)) return fail(W4A8_ERR_ALIGN, "%s: xq and wq must be 16-byte aligned", who);
+    if (!aligned(xs, 4) || !aligned(ws, 4) || (bias && !aligned(bias, 4)) || !aligned(Y, size)) return fail(W4A8_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+    const Rows y = {Y, ldy, N, M, size}, in[] = {{xq, K, K, M, 1}, {xs, M, M, 1, 4}, {wq, K, K, N, 1}, {ws, N, N, 1, 4}, {bias, N, N, 1, 4}};
+    static const char *const names[] = {"xq", "xs", "wq", "ws", "bias"};
+    for (int i = 0; i < 5; i++)
+        if (rows_overlap(y, in[i])) return fail(W4A8_ERR_ARG, "%s: Y overlaps %s", who, names[i]);
+    int rc = require_sm100();
+    if (rc != W4A8_OK) return rc;
+    w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0};
+    return w8a8::launch(xq, wq, a, w8a8::plan_for(M, N, K, sm_count()), dtype, (cudaStream_t)stream);
+}
+
+W4A8_API int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy,
+                              int S, int N, int K, int x_dtype, int y_dtype, int skip_quantize, void *stream) {
+    if (S < 0 || N < 0) return fail(W4A8_ERR_ARG, "linear_w8a8: negative size S=%d N=%d", S, N);
+    if (S == 0 || N == 0) return W4A8_OK;
+    if (!skip_quantize) {
+        const int rc = w4a8_quantize_rows_q8(x, ldx, S, K, x_dtype, xq, xs, stream);
+        if (rc != W4A8_OK) return rc;
+    }
+    return w4a8_gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, S, N, K, y_dtype, stream);
+}

@@ -3,60 +3,16 @@
 // Cache layout: codes k, v [num_blocks][heads][block][dim] int8 and scales [num_blocks][heads] fp32; a token's element is code * scale.
 // A block holds `block` consecutive tokens of one request; slot = block id * block + token's place in it.
 #pragma once
-#include <cuda_bf16.h>
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace w4a8 {
 namespace kv {
 
+using w4a8::Row;
+
 constexpr int LONGEST = 0x7fffffff - 511;     // tokens of a request: positions a few tiles on are counted in 31 bits too
 enum { ERR_BLOCK_ID = 0x900u, ERR_SLOT = 0x901u, ERR_LENGTH = 0x902u };   // codes of the device-side error word
-
-// ---- element types of the rows outside the cache ---------------------------------------------------------------------------------
-template <typename T> struct Row;   // 16 bytes of a row: N elements
-template <> struct Row<float> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void unpack(uint4 r, float (&x)[4]) {
-        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    }
-};
-template <> struct Row<__half> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void unpack(uint4 r, float (&x)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<__half2 *>(&w[i]) = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-template <> struct Row<__nv_bfloat16> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void unpack(uint4 r, float (&x)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<__nv_bfloat162 *>(&w[i]) = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
 
 // ---- block tables and slot maps ----------------------------------------------------------------------------------------------------
 // One launch.  Every CTA scans all requests (two sums at once, in the halves of a 64-bit number: new tokens and fresh blocks before each

@@ -1,4 +1,5 @@
-// The matmul path's translation unit of libw4a8_b200.so (the KV cache and attention are kv_cache.cu): includes its kernel
+// The matmul path's translation unit of libw4a8_b200.so (the KV cache and attention are kv_cache.cu, norms, rotary positions and routing layer_ops.cu,
+// products of 8-bit weights gemm_w8a8.cu): includes its kernel
 // files and defines their part of the C ABI declared in include/w4a8_b200.h.  Build (see dgx-serving_b200/build.py):
 //   nvcc -gencode arch=compute_100a,code=sm_100a -O3 -std=c++17 -lineinfo -Xcompiler -fPIC -shared
 #include <cerrno>
@@ -24,6 +25,7 @@ namespace w4a8 {
 
 cudaError_t kv_take_device_error(unsigned int *v);     // kv_cache.cu
 const char *kv_device_error_text(unsigned int v);
+cudaError_t w8a8_take_device_error(unsigned int *v);   // gemm_w8a8.cu
 
 char *err_buf() {
     static thread_local char buf[512] = {0};
@@ -131,6 +133,12 @@ W4A8_API int w4a8_device_status(uint32_t *detail) {
     if (v != 0) {
         if (detail) *detail = v;
         return fail(W4A8_ERR_DEVICE, "%s (code 0x%x)", kv_device_error_text(v), v);
+    }
+    e = w8a8_take_device_error(&v);
+    if (e != cudaSuccess) return cuda_fail(e, "read device error word");
+    if (v != 0) {
+        if (detail) *detail = v;
+        return fail(W4A8_ERR_DEVICE, "a kernel's bounded wait ran out (code 0x%x)", v);
     }
     if (detail) *detail = 0;
     return W4A8_OK;

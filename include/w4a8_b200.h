@@ -337,6 +337,93 @@ int w4a8_attention_q8(const void *Q, int64_t ldq, const w4a8_kv_cache *cache, co
                       const int32_t *seq_len, int R, int T, int heads_q, void *O, int64_t ldo, float *lse, float scale, int causal, int window,
                       float softcap, int max_q, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- between a block's output and the next block's input ----------------------------------------------------
+ * What a layer does around its products beside the cache: the residual stream and its norms, rotary positions, the choice of experts, and
+ * products whose weights stay at 8 bits.  (The reference has them as separate fp32 kernels: kernels/norm_fused.cuh, rmsnorm.cuh, rope.cuh,
+ * router_topk.cuh.)  Rows are fp32, fp16 or bf16 (W4A8_F32 ...), a token per row of `ld` elements; pointers to rows and vectors and pitches
+ * in bytes are multiples of 16 unless an entry says otherwise.  The structs are read on the host during the call; what they point to is
+ * device memory.  An output may be an input's own memory (same address, pitch and type) where an entry says so, and overlaps no input
+ * otherwise. */
+
+/* Norms of one kind: x * r * weight, x * r * (1 + weight), x * r, or x itself; r = 1 / sqrt(mean(x^2) + eps). */
+enum { W4A8_NORM_NONE = -1, W4A8_NORM_SCALE = 0, W4A8_NORM_ONE_PLUS = 1, W4A8_NORM_NO_SCALE = 2 };
+
+/* Residual add and norms in one launch, for S rows of K elements:
+ *   p = norm(y; post_weight, post_variant) * gate * alpha         h' = h + p         n = norm(h'; weight, variant)
+ * y NULL: h' = h.  gate NULL: none; gate_ld 0: one fp32 number for each channel, else rows of a token each, gate_ld apart.
+ * Outputs, each NULL if not wanted: h_out = h' (may be h's own memory), n_out = n (may be h's or y's), both rounded once to dtype; xq, xs, xsum = n
+ * quantized: group 32: w4a8_quantize_x_q8's form, the input of the W4A8 products (xq [S][K], xs, xsum [S][K / 32]); group 0: one scale for
+ * each row, the input of w4a8_gemm_w8a8 (xq [S][K], xs [S], no xsum).  What is normed and quantized is not rounded to dtype before.
+ * Every step is one fp32 operation in the order written (left to right); the sums of squares and r are taken in fp64 and r is rounded to fp32 once,
+ * so that the bits do not depend on how a row is cut.  h, h_out and n_out have type dtype, y has y_dtype: dtype or W4A8_F32.
+ * K a multiple of 32, at most 32768. */
+typedef struct w4a8_norm {
+    const float *weight, *post_weight;   /* [K]; NULL where the variant takes none */
+    const float *gate;
+    int64_t gate_ld;
+    double eps;
+    float alpha;
+    int K, variant, post_variant, dtype, y_dtype;
+} w4a8_norm;
+int w4a8_add_norm(const w4a8_norm *norm, const void *h, int64_t ldh, const void *y, int64_t ldy, void *h_out, int64_t ldo, void *n_out, int64_t ldn,
+                  int8_t *xq, float *xs, int32_t *xsum, int group, int S, void *stream);
+
+/* Rotary positions: the frequencies of the rotary / 2 pairs in units of 2^-64 turn a token, written to host memory (the caller copies them to
+ * the device once), and what cosine and sine are multiplied by.  frequency[i] = base^(-2 i / rotary) radians, and by `scaling`:
+ *   0 none; 1 linear: / factor; 2 ntk: the base times factor^(rotary / (rotary - 2));
+ *   3 yarn: pairs of more than `high` (default 32) turns in `original` tokens as they are, of less than `low` (default 1) / factor, a ramp over
+ *     the pairs' numbers between; magnitude 0.1 ln(factor) + 1 for factors above 1;
+ *   4 bands: the same with a ramp over the turns themselves, high default 4, magnitude 1;
+ *   5 divisors: / divisor[i] (host memory).
+ * low or high 0: the default.  rotary a multiple of 2, at most 1024. */
+enum { W4A8_ROPE_NONE = 0, W4A8_ROPE_LINEAR = 1, W4A8_ROPE_NTK = 2, W4A8_ROPE_YARN = 3, W4A8_ROPE_BANDS = 4, W4A8_ROPE_DIVISORS = 5 };
+int w4a8_rope_table(int rotary, double base, int scaling, double factor, double original, double low, double high, const double *divisor,
+                    uint64_t *turns_host, float *magnitude);
+
+/* Norms and rotary positions of a step's queries and keys in one launch: q[T][heads_q * dim], k[T][heads_k * dim], columns of a fused QKV product
+ * as they are.  Each head is normed (variant; q_weight, k_weight [dim]), and of its first `rotary` elements the pairs (i, i + rotary / 2), or
+ * (2 i, 2 i + 1) where interleaved, are turned by position[t] * frequency[i]: (a cos - b sin, b cos + a sin), times magnitude.  The product is
+ * taken modulo a turn in whole numbers, so angles are as exact at 2^31 tokens as at one.  Rows of a negative position (no request owns them)
+ * are left as they are in the outputs.  q_out, k_out may be q's, k's own memory.  heads_k 0: queries alone.  dim a multiple of 8, at most
+ * 256; rotary a multiple of 8, 0 to dim. */
+typedef struct w4a8_rope {
+    const uint64_t *turns;               /* [rotary / 2], device memory */
+    const float *q_weight, *k_weight;
+    double eps;
+    float magnitude;
+    int dim, rotary, interleaved, variant;
+} w4a8_rope;
+int w4a8_rope_qk(const w4a8_rope *rope, const void *q, int64_t ldq, int heads_q, const void *k, int64_t ldk, int heads_k, const int32_t *position, int T,
+                 void *q_out, int64_t ldqo, void *k_out, int64_t ldko, int dtype, void *stream);
+
+/* The experts of S tokens and their weights, idx and weight [S][topk] as w4a8_moe_block takes them, from logits[S][experts] (rows of any
+ * alignment): score = softmax over the experts, or sigmoid of each; choice = score + bias[e] (NULL: none).  With groups > 1 the experts
+ * [g * experts / groups, ...) are a group, its score the largest choice (group_score 0) or the sum of the two largest (1), and only the
+ * topk_groups best groups take part.  idx: the topk largest choices in falling order; equal ones, of groups too, by the lowest index.
+ * weight = the chosen scores (without bias), divided by their sum if renormalise, times scale.  Choices are compared in fp64.
+ * A logit that is not a number counts as -inf, +inf as the largest fp32 number; an expert of -inf has the score 0 and is chosen last, and
+ * where all are, the weights are 0.  The indices name different experts in every case.  experts <= 1024, topk <= 32, groups <= 32. */
+typedef struct w4a8_router {
+    const float *bias;
+    int experts, topk, scoring, groups, topk_groups, group_score, renormalise;   /* scoring 0 softmax, 1 sigmoid */
+    float scale;
+} w4a8_router;
+int w4a8_moe_route(const w4a8_router *router, const void *logits, int64_t ld, int S, int dtype, int32_t *idx, float *weight, void *stream);
+
+/* Products whose weights stay at 8 bits (the layers that lose too much at 4): wq[N][K] int8 with one fp32 scale for each output channel, xq[M][K]
+ * int8 with one for each row.
+ *   w4a8_quantize_rows_q8: xs = amax / 127, xq = rintf(x / xs) clamped to +-127, a row of zeros 0 (w4a8_quantize_x_q8's arithmetic over whole
+ *   rows; weights are quantized offline by the same call, a channel per row).  K a multiple of 32, at most 32768.
+ *   w4a8_gemm_w8a8: Y[m][n] = float(sum_k xq[m][k] * wq[n][k]) * xs[m] * ws[n] + bias[n] (NULL: none), rounded once to dtype; the sum is exact, so
+ *   a row's bits depend on neither M nor the way K is cut.  Y has any alignment and pitch; xq and wq are 16-byte aligned.  Any M, N; K a multiple
+ *   of 32, at most 131040.
+ *   w4a8_linear_w8a8: both, one after the other (skip_quantize: xq and xs are there already). */
+int w4a8_quantize_rows_q8(const void *x, int64_t ldx, int S, int K, int dtype, int8_t *xq, float *xs, void *stream);
+int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy, int M, int N, int K,
+                   int dtype, void *stream);
+int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy,
+                     int S, int N, int K, int x_dtype, int y_dtype, int skip_quantize, void *stream);
+
 /* ---- a15: N-sharded weight upload --------------------------------------------------------------------
  * Replaces QMat + load_dev()/mat() (runtime/weights_qwen.h:8, runtime/weights_qwen.cu:12-36,
  * runtime/weights_gemma4.cu:12-41): `<name>_q4.bin` holds N*K/2 bytes, `<name>_scale.bin` holds

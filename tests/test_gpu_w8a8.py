@@ -1,0 +1,128 @@
+"""8-bit products with scales for each row and channel: the sums are exact, so outputs are compared bit for bit with the definition's fp32 steps."""
+import pytest
+import torch
+
+from layer_plain import DTYPES, quantize
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(M, N, K, seed, bias=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    xq = torch.randint(-127, 128, (M, K), generator=g, device="cuda", dtype=torch.int8)
+    wq = torch.randint(-128, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    xs, ws = torch.rand(M, generator=g, device="cuda") * 0.1, torch.rand(N, generator=g, device="cuda") * 1e-3
+    return xq, xs, wq, ws, torch.randn(N, generator=g, device="cuda") if bias else None
+
+
+def _want(xq, xs, wq, ws, b, dtype):
+    y = (xq.double() @ wq.double().T).float() * xs[:, None] * ws           # whole numbers below 2^53: the double is exact, rounded once
+    return (y if b is None else y + b).to(DTYPES[dtype])
+
+
+def _run(w4a8, case, dtype, ld=0):
+    xq, xs, wq, ws, b = case
+    M, N, K = xq.shape[0], wq.shape[0], xq.shape[1]
+    Y = torch.full((M + 1, N + ld), 3.0, device=xq.device).to(DTYPES[dtype])
+    w4a8.launch_gemm_w8a8(xq, xs, wq, ws, Y, N + ld, M, N, K, dtype, bias=b)
+    assert (Y[M] == 3).all() and (Y[:, N:] == 3).all()
+    return Y[:M, :N]
+
+
+@pytest.mark.parametrize("K", [32, 96, 128, 416, 2048])
+@pytest.mark.parametrize("M,N", [(1, 1), (1, 128), (2, 300), (7, 5), (16, 129), (17, 1000), (33, 64), (64, 640), (65, 127), (100, 4091), (128, 256), (129, 700), (256, 130), (257, 1), (300, 999), (777, 257)])
+def test_products_are_exact(w4a8, cuda, M, N, K):
+    case = _case(M, N, K, M + N + K, bias=(M + N) % 2 == 0)
+    for dtype, ld in (("fp32", 0), ("bf16", 1), ("fp16", 5)):
+        assert torch.equal(_run(w4a8, case, dtype, ld), _want(*case, dtype)), dtype
+    w4a8.device_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 17408, 5120), (16, 3840, 15360), (5, 128, 32768), (40, 512, 16416), (2048, 1024, 512), (333, 4091, 3840), (8, 60000, 256), (1000, 3000, 1056), (64, 6144, 5120)])
+def test_larger_products(w4a8, cuda, M, N, K):
+    case = _case(M, N, K, K, bias=False)
+    assert torch.equal(_run(w4a8, case, "fp32"), _want(*case, "fp32"))
+    w4a8.device_status()
+
+
+def test_the_largest_sums_fit(w4a8, cuda):
+    K = 131040
+    xq, wq = torch.full((3, K), -128, dtype=torch.int8, device=cuda), torch.full((5, K), -128, dtype=torch.int8, device=cuda)
+    xq[1], wq[2] = 127, 127
+    one = torch.ones(5, device=cuda)
+    case = (xq, one[:3].clone(), wq, one, None)
+    assert torch.equal(_run(w4a8, case, "fp32"), _want(*case, "fp32"))
+
+
+def test_bits_do_not_depend_on_the_rows_of_a_call(w4a8, cuda):
+    case = _case(300, 520, 1312, 3)
+    whole = _run(w4a8, case, "fp32").clone()
+    for lo, n in ((0, 1), (5, 16), (100, 33), (7, 64), (3, 290)):
+        part = (case[0][lo:lo + n], case[1][lo:lo + n]) + case[2:]
+        assert torch.equal(_run(w4a8, part, "fp32"), whole[lo:lo + n])
+
+
+def test_outputs_of_odd_address_and_pitch(w4a8, cuda):
+    case = _case(21, 77, 224, 8)
+    for dtype in DTYPES:
+        Y = torch.zeros(21 * 81 + 1, device=cuda).to(DTYPES[dtype])[1:].view(21, 81)
+        w4a8.launch_gemm_w8a8(*case[:4], Y, 81, 21, 77, 224, dtype, bias=case[4])
+        assert torch.equal(Y[:, :77], _want(*case, dtype)) and (Y[:, 77:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("S,K", [(1, 32), (3, 5120), (200, 416), (2, 32768), (150, 8224), (17, 16384)])
+def test_rows_are_quantized_by_the_definition(w4a8, cuda, S, K, dtype):
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = (torch.randn(S, K + 8, generator=g, device=cuda) * torch.exp(2 * torch.randn(S, 1, generator=g, device=cuda))).to(DTYPES[dtype])
+    x[S // 2] = 0
+    xq, xs = torch.full((S + 1, K), 9, dtype=torch.int8, device=cuda), torch.full((S + 1,), 9.0, device=cuda)
+    w4a8.launch_quantize_rows_q8(x, K + 8, S, K, xq, xs, dtype)
+    q, scale, _ = quantize(x[:, :K].float(), 0)
+    assert torch.equal(xq[:S], q) and torch.equal(xs[:S], scale[:, 0]) and (xq[S] == 9).all() and xs[S] == 9
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 640, 512), (16, 3000, 2048), (70, 128, 1024), (300, 600, 512)])
+def test_weights_quantized_just_before_their_product(w4a8, cuda, M, N, K):
+    """Rows and weights quantized on the same stream directly in front of the product, in both orders, many times over: what is fetched early is not stale."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    xq, xs = torch.empty(M, K, dtype=torch.int8, device=cuda), torch.empty(M, device=cuda)
+    wq, ws = torch.empty(N, K, dtype=torch.int8, device=cuda), torch.empty(N, device=cuda)
+    xw = [(torch.randn(M, K, generator=g, device=cuda), torch.randn(N, K, generator=g, device=cuda)) for _ in range(6)]
+    Y = [torch.empty(M, N, device=cuda) for _ in xw]
+    for i, ((x, w), y) in enumerate(zip(xw, Y)):
+        if i % 2:
+            w4a8.launch_quantize_rows_q8(w, K, N, K, wq, ws)
+            w4a8.linear_w8a8(x, K, xq, xs, wq, ws, y, N, M, N, K)
+        else:
+            w4a8.launch_quantize_rows_q8(x, K, M, K, xq, xs)
+            w4a8.launch_quantize_rows_q8(w, K, N, K, wq, ws)
+            w4a8.linear_w8a8(None, K, xq, xs, wq, ws, y, N, M, N, K, skip_quantize=1)
+    for (x, w), y in zip(xw, Y):
+        (q, s, _), (p, t, _) = quantize(x, 0), quantize(w, 0)
+        assert torch.equal(y, _want(q, s[:, 0], p, t[:, 0], None, "fp32"))
+
+
+def test_two_streams_and_a_graph(w4a8, cuda):
+    cases = [_case(40, 1000, 2048, 1), _case(500, 1000, 512, 2)]
+    Y = [torch.empty(c[0].shape[0], 1000, device=cuda) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for c, y, st in zip(cases, Y, streams):
+            w4a8.launch_gemm_w8a8(*c[:4], y, 1000, c[0].shape[0], 1000, c[0].shape[1], bias=c[4], stream=st)
+    torch.cuda.synchronize()
+    for c, y in zip(cases, Y):
+        assert torch.equal(y, _want(*c, "fp32"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c, y in zip(cases, Y):
+            w4a8.launch_gemm_w8a8(*c[:4], y, 1000, c[0].shape[0], 1000, c[0].shape[1], bias=c[4])
+    for c in cases:
+        c[0].neg_()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for c, y in zip(cases, Y):
+        assert torch.equal(y, _want(*c, "fp32"))
+    w4a8.device_status()
