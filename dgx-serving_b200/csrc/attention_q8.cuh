@@ -239,20 +239,9 @@ template <int W> __device__ __forceinline__ uint64_t desc_p(uint32_t addr) {
 }
 // D = int32, A and B signed bytes, 128 rows, N columns; bits 15 and 16: A and B are MN-major.
 __host__ __device__ constexpr uint32_t idesc_s8(int N, int mn) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(mn * 3) << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24); }
-// The whole warp comes here and the elected lane issues: addresses and descriptors then stay in uniform registers.
-__device__ __forceinline__ uint32_t elected() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e;
-}
-__device__ __forceinline__ void umma_s8(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t lead, uint32_t bar) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
-}
+using ptx::elected;
+using ptx::umma_commit;
+using ptx::umma_s8;
 __device__ __forceinline__ float out_round(float, float v) { return v; }
 __device__ __forceinline__ __half out_round(__half, float v) { return __float2half_rn(v); }
 __device__ __forceinline__ __nv_bfloat16 out_round(__nv_bfloat16, float v) { return __float2bfloat16_rn(v); }

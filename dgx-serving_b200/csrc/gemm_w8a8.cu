@@ -35,7 +35,7 @@ W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq,
         if (rows_overlap(y, in[i])) return fail(W4A8_ERR_ARG, "%s: Y overlaps %s", who, names[i]);
     int rc = require_sm100();
     if (rc != W4A8_OK) return rc;
-    w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0};
+    w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0, 0, 0};
     return w8a8::launch(xq, wq, a, w8a8::plan_for(M, N, K, sm_count()), dtype, (cudaStream_t)stream);
 }
 

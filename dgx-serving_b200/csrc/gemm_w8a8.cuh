@@ -22,18 +22,18 @@ namespace w4a8 {
 namespace w8a8 {
 
 constexpr int MAX_K = 131040;
-constexpr int BW = 128, KT = 128;              // channels of a tile; bytes of K in a stage
-constexpr int A_STAGE = BW * KT;
+constexpr int LANES = 128, KT = 128;           // channels of an MMA; bytes of K in a row of a swizzled tile
+constexpr int A_STAGE = LANES * KT;
 constexpr int MAX_STAGES = 12, EPI_WARPS = 4, THREADS = (2 + EPI_WARPS) * 32;
 constexpr int SMEM_MAX = 227 * 1024, SMEM_FIXED = 1024 /* alignment */ + 512 /* barriers */;
-constexpr int SPLIT_MAX = 8, SPLIT_BT = 64;    // CTAs that share a tile, and the widest tile that they share
-enum : unsigned { ERR_PRODUCER = 0xA10u, ERR_MMA = 0xA20u, ERR_EPILOGUE = 0xA30u };
+constexpr int SPLIT_MAX = 8, SPLIT_BT = 128;   // CTAs that share a tile, and the widest tile that they share
+enum : unsigned { ERR_PRODUCER = 0xA10u, ERR_MMA = 0xA20u, ERR_EPILOGUE = 0xA30u, ERR_SUMS = 0xA40u };
 
 struct Args {
     const float *xs, *ws, *bias;
     void *y;
     int64_t ldy;
-    int M, N, K, bt, stages, split, t_tiles, tiles, tmem_cols;
+    int M, N, K, bw, bt, kp, stages, split, t_tiles, tiles, tmem_cols;
 };
 
 // The slot of a ring, and how often it came round.
@@ -53,7 +53,11 @@ __device__ __forceinline__ uint32_t remote(uint32_t smem, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void st_remote(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// `bytes` of this CTA's shared memory to another one's of the cluster, where they count on an mbarrier.
+__device__ __forceinline__ void send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 __device__ __forceinline__ void prefetch_l2_2d(const void *tmap, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y) : "memory");
@@ -68,22 +72,29 @@ template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Args a) {
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t raw = ptx::smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
-    const uint32_t stage_bytes = A_STAGE + (uint32_t)a.bt * KT;
+    const uint32_t part_bytes = A_STAGE + (uint32_t)a.bt * KT, stage_bytes = part_bytes * a.kp;
     const uint32_t bars = base + (uint32_t)a.stages * stage_bytes, recv = bars + 512;
     const auto FULL = [&](int s) { return bars + 8u * s; };
     const auto EMPTY = [&](int s) { return bars + 8u * (MAX_STAGES + s); };
     const auto T_FULL = [&](int s) { return bars + 8u * (2 * MAX_STAGES + s); };
     const auto T_EMPTY = [&](int s) { return bars + 8u * (2 * MAX_STAGES + 2 + s); };
-    const uint32_t slot_addr = bars + 8u * (2 * MAX_STAGES + 4);
+    const uint32_t sums_full = bars + 8u * (2 * MAX_STAGES + 4), slot_addr = bars + 8u * (2 * MAX_STAGES + 5);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = SPLIT ? blockIdx.x % a.split : 0;
     const int nkt = (a.K + KT - 1) / KT;
     const int k_lo = SPLIT ? (int)((long)nkt * rank / a.split) : 0, k_hi = SPLIT ? (int)((long)nkt * (rank + 1) / a.split) : nkt;
     const int first = SPLIT ? blockIdx.x / a.split : blockIdx.x, step = SPLIT ? a.tiles : gridDim.x;
+    // SPLIT: rows [r * own, (r + 1) * own) of the tile are the r-th CTA's to finish
+    const int own = SPLIT ? (a.bt + a.split - 1) / a.split : 0, tile_rows = min(a.bt, a.M - first % a.t_tiles * a.bt);
+    const auto rows_of = [&](int r) { return max(0, min(own, tile_rows - r * own)); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; i++) { ptx::mbar_init(FULL(i), 1); ptx::mbar_init(EMPTY(i), 1); }
         for (int i = 0; i < 2; i++) { ptx::mbar_init(T_FULL(i), 1); ptx::mbar_init(T_EMPTY(i), EPI_WARPS); }
+        if constexpr (SPLIT) {
+            ptx::mbar_init(sums_full, 1);
+            ptx::mbar_arrive_expect_tx(sums_full, (uint32_t)((a.split - 1) * rows_of(rank) * LANES * 4));
+        }
         ptx::mbar_fence_init();
         ptx::tma_prefetch_desc(&tmW);
         ptx::tma_prefetch_desc(&tmX);
@@ -100,83 +111,126 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot_addr));
 
     if (warp == 0) {
-        if (lane == 0) {
-            Turn ring;
-            bool ok = true;
-            // while the kernel in front drains, the first stages' weights are brought to L2: whatever it writes, L2 has it
-            const int early = min(a.stages, k_hi - k_lo);
-            for (int i = 0; i < early; i++) prefetch_l2_2d(&tmW, (k_lo + i) * KT, first / a.t_tiles * BW);
-            pdl_wait();
-            pdl_launch_dependents();
-            for (int tile = first; tile < a.tiles && ok; tile += step)
-                for (int kt = k_lo; kt < k_hi; kt++) {
-                    if (!ptx::mbar_wait(EMPTY(ring.slot), ring.phase ^ 1u)) { dev_set_error(ERR_PRODUCER); ok = false; break; }
-                    const uint32_t at = base + ring.slot * stage_bytes;
-                    ptx::mbar_arrive_expect_tx(FULL(ring.slot), stage_bytes);
-                    ptx::tma_load_2d(at, &tmW, kt * KT, tile / a.t_tiles * BW, FULL(ring.slot));
-                    ptx::tma_load_2d(at + A_STAGE, &tmX, kt * KT, tile % a.t_tiles * a.bt, FULL(ring.slot));
-                    ring.next(a.stages);
+        const uint32_t lead = ptx::elected();
+        Turn ring;
+        // while the kernel in front drains, the first stages' weights are brought to L2: whatever it writes, L2 has it
+        const int early = min(a.stages * a.kp, k_hi - k_lo);
+        if (lead)
+            for (int i = 0; i < early; i++) prefetch_l2_2d(&tmW, (k_lo + i) * KT, first / a.t_tiles * a.bw);
+        pdl_wait();
+        pdl_launch_dependents();
+        bool ok = true;
+        for (int tile = first; tile < a.tiles && ok; tile += step) {
+            const int w_row = tile / a.t_tiles * a.bw, x_row = tile % a.t_tiles * a.bt;
+            for (int kt = k_lo; kt < k_hi; kt += a.kp) {
+                if (!ptx::mbar_wait_warp(EMPTY(ring.slot), ring.phase ^ 1u)) { dev_set_error(ERR_PRODUCER); ok = false; break; }
+                const int parts = min(a.kp, k_hi - kt);
+                uint32_t at = base + ring.slot * stage_bytes;
+                const uint32_t bar = FULL(ring.slot);
+                ptx::mbar_arrive_expect_tx(lead, bar, (uint32_t)(a.bw + a.bt) * KT * parts);
+                for (int p = 0; p < parts; p++, at += part_bytes) {
+                    ptx::tma_load_2d(lead, at, &tmW, (kt + p) * KT, w_row, bar);
+                    ptx::tma_load_2d(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
                 }
-            if (!ok) {                             // copies in flight land before the CTA's shared memory goes away
-                const long long t0 = clock64();
-                while (clock64() - t0 < (1ll << 21)) { }
+                ring.next(a.stages);
             }
         }
+        if (!ok) {                                             // copies in flight land before the CTA's shared memory goes away
+            const long long t0 = clock64();
+            while (clock64() - t0 < (1ll << 21)) { }
+        }
     } else if (warp == 1) {
-        if (lane == 0) {
-            pdl_wait();                            // before the first bounded wait: the kernel in front may take longer than any of them
-            Turn ring, buf;
-            const uint32_t idesc = ptx::umma_idesc_s8(BW, a.bt);
-            bool ok = true;
-            for (int tile = first; tile < a.tiles && ok; tile += step) {
-                if (!ptx::mbar_wait(T_EMPTY(buf.slot), buf.phase ^ 1u)) { dev_set_error(ERR_MMA | 1); ok = false; break; }
+        pdl_wait();                                            // before the first bounded wait: the kernel in front may take longer than any of them
+        const uint32_t lead = ptx::elected(), idesc = ptx::umma_idesc_s8(LANES, a.bt);
+        Turn ring, buf;
+        bool ok = true;
+        for (int tile = first; tile < a.tiles && ok; tile += step) {
+            if (!ptx::mbar_wait_warp(T_EMPTY(buf.slot), buf.phase ^ 1u)) { dev_set_error(ERR_MMA | 1); ok = false; break; }
+            ptx::tc_fence_after_sync();
+            const uint32_t acc = tmem + buf.slot * (a.tmem_cols / 2);
+            for (int kt = k_lo; kt < k_hi; kt += a.kp) {
+                if (!ptx::mbar_wait_warp(FULL(ring.slot), ring.phase)) { dev_set_error(ERR_MMA | 2); ok = false; break; }
                 ptx::tc_fence_after_sync();
-                for (int kt = k_lo; kt < k_hi; kt++) {
-                    if (!ptx::mbar_wait(FULL(ring.slot), ring.phase)) { dev_set_error(ERR_MMA | 2); ok = false; break; }
-                    ptx::tc_fence_after_sync();
-                    const uint64_t w = ptx::umma_desc_k_sw128(base + ring.slot * stage_bytes), x = ptx::umma_desc_k_sw128(base + ring.slot * stage_bytes + A_STAGE);
-                    const int parts = min(KT, a.K - kt * KT) / 32;
-                    for (int p = 0; p < parts; p++) ptx::umma_i8(tmem + buf.slot * (a.tmem_cols / 2), w + 2 * p, x + 2 * p, idesc, kt > k_lo || p > 0);
-                    ptx::umma_commit(EMPTY(ring.slot));
-                    ring.next(a.stages);
+                uint32_t at = base + ring.slot * stage_bytes;
+                for (int q = kt; q < min(kt + a.kp, k_hi); q++, at += part_bytes) {
+                    const uint64_t w = ptx::umma_desc_k_sw128(at), x = ptx::umma_desc_k_sw128(at + A_STAGE);
+                    const int parts = min(KT, a.K - q * KT) / 32;
+#pragma unroll
+                    for (int p = 0; p < KT / 32; p++)
+                        if (p < parts) ptx::umma_s8(lead, acc, w + 2 * p, x + 2 * p, idesc, q > k_lo || p > 0);
                 }
-                if (ok) ptx::umma_commit(T_FULL(buf.slot));
-                buf.next(2);
+                ptx::umma_commit(lead, EMPTY(ring.slot));
+                ring.next(a.stages);
             }
-            if (!ok) {                             // products in flight end before TMEM is given back
-                const long long t0 = clock64();
-                while (clock64() - t0 < (1ll << 21)) { }
-            }
+            if (ok) ptx::umma_commit(lead, T_FULL(buf.slot));
+            buf.next(2);
+        }
+        if (!ok) {                                             // products in flight end before TMEM is given back
+            const long long t0 = clock64();
+            while (clock64() - t0 < (1ll << 21)) { }
         }
     } else {
         pdl_wait();
-        const int quad = warp & 3;                 // TMEM lanes [32 * quad, 32 * quad + 32) are this warp's
+        const int quad = warp & 3, row = quad * 32 + lane;     // TMEM lanes [32 * quad, 32 * quad + 32) are this warp's
         Turn buf;
         for (int tile = first; tile < a.tiles; tile += step) {
-            const int t0 = tile % a.t_tiles * a.bt, n = tile / a.t_tiles * BW + quad * 32 + lane, cols = min(a.bt, a.M - t0);
-            const bool live = n < a.N;
+            // what the outputs need besides the sums, while these are on their way: lane l has the scales of rows l, l + 32, ...
+            const int n = tile / a.t_tiles * a.bw + row, t0 = tile % a.t_tiles * a.bt + rank * own, rows = SPLIT ? rows_of(rank) : min(a.bt, a.M - t0);
+            const bool live = row < a.bw && n < a.N;
+            constexpr int XR = SPLIT ? SPLIT_BT / 2 / 32 : 8;
+            float x[XR];
+#pragma unroll
+            for (int i = 0; i < XR; i++) x[i] = 32 * i + lane < rows ? a.xs[t0 + 32 * i + lane] : 0.f;
             const float w = live ? a.ws[n] : 0.f, b = live && a.bias ? a.bias[n] : 0.f;
             T *y = static_cast<T *>(a.y) + (size_t)t0 * a.ldy + n;
             if (!ptx::mbar_wait_warp(T_FULL(buf.slot), buf.phase)) { dev_set_error(ERR_EPILOGUE); break; }
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf.slot * (a.tmem_cols / 2);
-            for (int c0 = 0; c0 < cols; c0 += 16) {
-                uint32_t d[16];
-                ptx::tmem_ld(acc + c0, d);
+            const int columns = SPLIT ? tile_rows : rows;
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? SPLIT_BT / 32 : 8); i++) {
+                if (32 * i >= columns) break;
+                uint32_t d[32];
+                if (32 * i + 16 < a.bt) ptx::tmem_ld(acc + 32 * i, d);
+                else {                                         // an odd number of sixteens: the last one alone
+                    uint32_t half[16];
+                    ptx::tmem_ld(acc + 32 * i, half);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) d[j] = half[j];
+                }
                 ptx::tmem_ld_wait();
-                if constexpr (SPLIT) {
-                    const int own = (a.bt + a.split - 1) / a.split;    // columns [r * own, (r + 1) * own) are the r-th CTA's
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int c = c0 + j, r = c / own;
-                        if (c < cols) st_remote(remote(recv + 4u * (((uint32_t)(rank * own + c - r * own) * BW) + quad * 32 + lane), r), d[j]);
+                for (int j = 0; j < 32; j++) {
+                    if constexpr (SPLIT) {                     // every product has been read: the stages' memory is free
+                        if (32 * i + j < columns) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + 4u * ((32 * i + j) * LANES + row)), "r"(d[j]) : "memory");
+                    } else {
+                        const float v = scaled((int)d[j], __shfl_sync(0xffffffffu, x[i], j), w, b);
+                        if (live && 32 * i + j < columns) put(y, v);
+                        y += a.ldy;
                     }
-                } else {
-                    const float xv = c0 + lane < cols ? a.xs[t0 + c0 + lane] : 0.f;
+                }
+            }
+            if constexpr (SPLIT) {
+                ptx::fence_proxy_async_smem();
+                epilogue_sync();
+                if (warp == 2 && lane < a.split && lane != rank && rows_of(lane) > 0)
+                    send(remote(recv + (uint32_t)(rank * own * LANES * 4), lane), base + (uint32_t)(lane * own * LANES * 4), (uint32_t)(rows_of(lane) * LANES * 4), remote(sums_full, lane));
+                if (!ptx::mbar_wait_warp(sums_full, 0)) { dev_set_error(ERR_SUMS); break; }
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const float v = scaled((int)d[j], __shfl_sync(0xffffffffu, xv, j), w, b);
-                        if (live && c0 + j < cols) put(y + (size_t)(c0 + j) * a.ldy, v);
+                for (int i = 0; i < XR; i++) {
+#pragma unroll 4
+                    for (int j = 0; j < 32; j++) {
+                        const int c = 32 * i + j;
+                        if (c >= rows) break;
+                        int sum = 0;
+                        for (int r = 0; r < a.split; r++) {
+                            int v;
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"((r == rank ? base : recv) + 4u * ((r * own + c) * LANES + row)));
+                            sum += v;
+                        }
+                        const float v = scaled(sum, __shfl_sync(0xffffffffu, x[i], j), w, b);
+                        if (live) put(y, v);
+                        y += a.ldy;
                     }
                 }
             }
@@ -186,26 +240,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
             buf.next(2);
         }
     }
-    if constexpr (SPLIT) {
+    if constexpr (SPLIT) {                                     // nobody leaves while sums are on their way from it or to it
         __syncwarp();
-        cluster_sync();                            // every sum has arrived; and nobody leaves while another one's are on their way
-        if (warp >= 2) {
-            const int quad = warp & 3, t0 = first % a.t_tiles * a.bt, n = first / a.t_tiles * BW + quad * 32 + lane, cols = min(a.bt, a.M - t0);
-            const int own = (a.bt + a.split - 1) / a.split, c_hi = min(cols, (rank + 1) * own);
-            const bool live = n < a.N;
-            const float w = live ? a.ws[n] : 0.f, b = live && a.bias ? a.bias[n] : 0.f;
-            T *y = static_cast<T *>(a.y) + (size_t)t0 * a.ldy + n;
-            for (int c = rank * own; c < c_hi; c++) {
-                int sum = 0;
-                for (int r = 0; r < a.split; r++) {
-                    int v;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(recv + 4u * (((uint32_t)(r * own + c - rank * own) * BW) + quad * 32 + lane)));
-                    sum += v;
-                }
-                const float v = scaled(sum, a.xs[t0 + c], w, b);
-                if (live) put(y + (size_t)c * a.ldy, v);
-            }
-        }
+        cluster_sync();
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
@@ -217,18 +254,25 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-struct Plan { int bt, split; };
+// How the outputs are cut: tiles of bw channels and bt rows, split CTAs to a tile.
+struct Plan { int bw, bt, split, kp; };
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
+inline int split_receive(int bt, int split) { return split > 1 ? split * ceil_div(bt, split) * LANES * 4 : 0; }
+inline int stages_for(int bt, int split, int kp) {
+    const int n = (SMEM_MAX - SMEM_FIXED - split_receive(bt, split)) / ((A_STAGE + bt * KT) * kp);
+    return n > MAX_STAGES ? MAX_STAGES : n;
+}
+
 inline Plan plan_for(int M, int N, int K, int sms) {
-    const int w_tiles = ceil_div(N, BW), nkt = ceil_div(K, KT);
-    if (M <= SPLIT_BT) {
+    const int nkt = ceil_div(K, KT), w_tiles = ceil_div(N, LANES);
+    if (M <= 64) {
         int split = sms / w_tiles;
-        split = split < 1 ? 1 : split > SPLIT_MAX ? SPLIT_MAX : split;
-        while (split > 1 && nkt / split < 4) split--;
-        return {ceil_div(M, 16) * 16, split};
+        split = split < 1 ? 1 : split > 4 ? 4 : split == 3 ? 2 : split;
+        while (split > 1 && nkt / split < 4) split /= 2;
+        return {LANES, ceil_div(M, 16) * 16, split, 2};
     }
-    Plan best = {256, 1};
+    Plan best = {LANES, 256, 1, 1};
     double least = 1e30;
     for (int bt = 64; bt <= 256; bt += 16) {
         const long tiles = (long)w_tiles * ceil_div(M, bt);
@@ -248,11 +292,8 @@ inline int launch_t(Args a, const CUtensorMap &tmW, const CUtensorMap &tmX, cuda
         if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 smem opt-in");
         configured = true;
     }
-    const int own = ceil_div(a.bt, a.split), recv = SPLIT ? a.split * own * BW * 4 : 0;
-    const int stage = A_STAGE + a.bt * KT;
-    int stages = (SMEM_MAX - SMEM_FIXED - recv) / stage;
-    a.stages = stages > MAX_STAGES ? MAX_STAGES : stages;
-    const int smem = a.stages * stage + SMEM_FIXED + recv, sms = sm_count();
+    a.stages = stages_for(a.bt, a.split, a.kp);
+    const int smem = a.stages * a.kp * (A_STAGE + a.bt * KT) + SMEM_FIXED + split_receive(a.bt, a.split), sms = sm_count();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(SPLIT ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms));
     cfg.blockDim = dim3(THREADS);
@@ -278,16 +319,18 @@ inline int launch_t(Args a, const CUtensorMap &tmW, const CUtensorMap &tmX, cuda
 }
 
 inline int launch(const int8_t *xq, const int8_t *wq, Args a, Plan p, int dtype, cudaStream_t st) {
+    a.bw = p.bw;
     a.bt = p.bt;
+    a.kp = p.kp;
     a.split = p.split;
     a.t_tiles = ceil_div(a.M, p.bt);
-    const long tiles = (long)a.t_tiles * ceil_div(a.N, BW);
+    const long tiles = (long)a.t_tiles * ceil_div(a.N, p.bw);
     if (tiles > 0x3fffffff) return fail(W4A8_ERR_UNSUPPORTED, "gemm_w8a8: %d x %d outputs", a.M, a.N);
     a.tiles = (int)tiles;
     a.tmem_cols = 32;
-    while (a.tmem_cols < 2 * a.bt) a.tmem_cols *= 2;
+    while (a.tmem_cols < (p.split > 1 ? 1 : 2) * a.bt) a.tmem_cols *= 2;
     CUtensorMap tmW, tmX;
-    int rc = tmap_cached(&tmW, wq, (uint64_t)a.K, (uint64_t)a.N, KT, BW, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    int rc = tmap_cached(&tmW, wq, (uint64_t)a.K, (uint64_t)a.N, KT, (uint32_t)a.bw, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (rc != W4A8_OK) return rc;
     rc = tmap_cached(&tmX, xq, (uint64_t)a.K, (uint64_t)a.M, KT, (uint32_t)a.bt, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != W4A8_OK) return rc;
