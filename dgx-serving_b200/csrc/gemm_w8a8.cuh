@@ -7,7 +7,11 @@
 // 256, chosen on the host.  A step of one token then pads 16 columns and not 128 rows, and the epilogue's lanes hold neighbouring channels:
 // what a warp stores of a row is contiguous.
 //
-// One CTA per SM, warp-specialised: warp 0 starts copies, warp 1 the MMAs, warps 2 to 5 convert, scale and store one tile while the next one
+// Large products run on pairs of CTAs (cta_group::2): 256 channels by bt rows, each CTA holding its 128 channels and half of the rows, one thread of the
+// first CTA issuing the MMAs of both.  A byte in shared memory then serves twice the products: what fills shared memory bounds these products, and
+// under the power cap what it costs to move.
+//
+// One CTA per SM, warp-specialised: warp 0 starts copies, warp 1 the MMAs, warps 2 to 9 convert, scale and store one tile while the next one
 // accumulates in the other half of TMEM.  Where there are fewer tiles than SMs, the CTAs of a cluster share a tile's K (`split` of them), send
 // their int32 sums to the CTA that owns the columns through distributed shared memory, and that one adds them: no workspace, no second
 // launch, and the same bits, since integers add in any order.
@@ -24,7 +28,7 @@ namespace w8a8 {
 constexpr int MAX_K = 131040;
 constexpr int LANES = 128, KT = 128;           // channels of an MMA; bytes of K in a row of a swizzled tile
 constexpr int A_STAGE = LANES * KT;
-constexpr int MAX_STAGES = 12, EPI_WARPS = 4, THREADS = (2 + EPI_WARPS) * 32;
+constexpr int MAX_STAGES = 12, EPI_WARPS = 8, THREADS = (2 + EPI_WARPS) * 32;
 constexpr int SMEM_MAX = 227 * 1024, SMEM_FIXED = 1024 /* alignment */ + 512 /* barriers */;
 constexpr int SPLIT_MAX = 8, SPLIT_BT = 128;   // CTAs that share a tile, and the widest tile that they share
 enum : unsigned { ERR_PRODUCER = 0xA10u, ERR_MMA = 0xA20u, ERR_EPILOGUE = 0xA30u, ERR_SUMS = 0xA40u };
@@ -57,7 +61,32 @@ __device__ __forceinline__ uint32_t remote(uint32_t smem, int rank) {
 __device__ __forceinline__ void send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory"); }
+
+// ---- two CTAs of a cluster as a pair (cta_group::2): ranks 0 and 1 ---------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t columns) {          // a warp of each CTA
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t tmem, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+// Into this CTA's memory; the bytes count on an mbarrier of either CTA.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t lead, uint32_t dst_smem, const void *tmap, int x, int y, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}"
+                 ::"r"(dst_smem), "l"(tmap), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_s8_pair(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+// Arrives on the barrier at this place in both CTAs.
+__device__ __forceinline__ void umma_commit_pair(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 __device__ __forceinline__ void prefetch_l2_2d(const void *tmap, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y) : "memory");
@@ -68,11 +97,13 @@ __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T, bool SPLIT>
+enum Mode { ONE, SPLIT, PAIR };                // a tile is one CTA's; several share its K; two share its channels
+
+template <typename T, Mode MODE>
 __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Args a) {
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t raw = ptx::smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
-    const uint32_t part_bytes = A_STAGE + (uint32_t)a.bt * KT, stage_bytes = part_bytes * a.kp;
+    const uint32_t x_rows = MODE == PAIR ? a.bt / 2 : a.bt, part_bytes = A_STAGE + x_rows * KT, stage_bytes = part_bytes * a.kp;
     const uint32_t bars = base + (uint32_t)a.stages * stage_bytes, recv = bars + 512;
     const auto FULL = [&](int s) { return bars + 8u * s; };
     const auto EMPTY = [&](int s) { return bars + 8u * (MAX_STAGES + s); };
@@ -80,18 +111,19 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
     const auto T_EMPTY = [&](int s) { return bars + 8u * (2 * MAX_STAGES + 2 + s); };
     const uint32_t sums_full = bars + 8u * (2 * MAX_STAGES + 4), slot_addr = bars + 8u * (2 * MAX_STAGES + 5);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = SPLIT ? blockIdx.x % a.split : 0;
+    const int rank = MODE == ONE ? 0 : blockIdx.x % a.split;   // in the cluster
     const int nkt = (a.K + KT - 1) / KT;
-    const int k_lo = SPLIT ? (int)((long)nkt * rank / a.split) : 0, k_hi = SPLIT ? (int)((long)nkt * (rank + 1) / a.split) : nkt;
-    const int first = SPLIT ? blockIdx.x / a.split : blockIdx.x, step = SPLIT ? a.tiles : gridDim.x;
+    const int k_lo = MODE == SPLIT ? (int)((long)nkt * rank / a.split) : 0, k_hi = MODE == SPLIT ? (int)((long)nkt * (rank + 1) / a.split) : nkt;
+    const int first = MODE == ONE ? blockIdx.x : blockIdx.x / a.split, step = MODE == SPLIT ? a.tiles : MODE == PAIR ? gridDim.x / 2 : gridDim.x;
+    const int my_row = MODE == PAIR ? rank * LANES : 0;        // this CTA's channels in a tile
     // SPLIT: rows [r * own, (r + 1) * own) of the tile are the r-th CTA's to finish
-    const int own = SPLIT ? (a.bt + a.split - 1) / a.split : 0, tile_rows = min(a.bt, a.M - first % a.t_tiles * a.bt);
+    const int own = MODE == SPLIT ? (a.bt + a.split - 1) / a.split : 0, tile_rows = min(a.bt, a.M - first % a.t_tiles * a.bt);
     const auto rows_of = [&](int r) { return max(0, min(own, tile_rows - r * own)); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; i++) { ptx::mbar_init(FULL(i), 1); ptx::mbar_init(EMPTY(i), 1); }
-        for (int i = 0; i < 2; i++) { ptx::mbar_init(T_FULL(i), 1); ptx::mbar_init(T_EMPTY(i), EPI_WARPS); }
-        if constexpr (SPLIT) {
+        for (int i = 0; i < 2; i++) { ptx::mbar_init(T_FULL(i), 1); ptx::mbar_init(T_EMPTY(i), MODE == PAIR ? 2 * EPI_WARPS : EPI_WARPS); }
+        if constexpr (MODE == SPLIT) {
             ptx::mbar_init(sums_full, 1);
             ptx::mbar_arrive_expect_tx(sums_full, (uint32_t)((a.split - 1) * rows_of(rank) * LANES * 4));
         }
@@ -100,12 +132,15 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
         ptx::tma_prefetch_desc(&tmX);
     }
     if (warp == 1) {
-        ptx::tmem_alloc(slot_addr, a.tmem_cols);
-        ptx::tmem_relinquish();
+        if constexpr (MODE == PAIR) tmem_alloc_pair(slot_addr, a.tmem_cols);
+        else {
+            ptx::tmem_alloc(slot_addr, a.tmem_cols);
+            ptx::tmem_relinquish();
+        }
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
-    if constexpr (SPLIT) cluster_sync();           // sums are sent to CTAs that have begun
+    if constexpr (MODE != ONE) cluster_sync();                 // others' memory and barriers are used once they have begun
     ptx::tc_fence_after_sync();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot_addr));
@@ -116,21 +151,26 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
         // while the kernel in front drains, the first stages' weights are brought to L2: whatever it writes, L2 has it
         const int early = min(a.stages * a.kp, k_hi - k_lo);
         if (lead)
-            for (int i = 0; i < early; i++) prefetch_l2_2d(&tmW, (k_lo + i) * KT, first / a.t_tiles * a.bw);
+            for (int i = 0; i < early; i++) prefetch_l2_2d(&tmW, (k_lo + i) * KT, first / a.t_tiles * a.bw + my_row);
         pdl_wait();
         pdl_launch_dependents();
         bool ok = true;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
-            const int w_row = tile / a.t_tiles * a.bw, x_row = tile % a.t_tiles * a.bt;
+            const int w_row = tile / a.t_tiles * a.bw + my_row, x_row = tile % a.t_tiles * a.bt + (MODE == PAIR ? rank * x_rows : 0);
             for (int kt = k_lo; kt < k_hi; kt += a.kp) {
                 if (!ptx::mbar_wait_warp(EMPTY(ring.slot), ring.phase ^ 1u)) { dev_set_error(ERR_PRODUCER); ok = false; break; }
                 const int parts = min(a.kp, k_hi - kt);
                 uint32_t at = base + ring.slot * stage_bytes;
-                const uint32_t bar = FULL(ring.slot);
-                ptx::mbar_arrive_expect_tx(lead, bar, (uint32_t)(a.bw + a.bt) * KT * parts);
+                const uint32_t bar = MODE == PAIR ? remote(FULL(ring.slot), 0) : FULL(ring.slot);      // a pair's bytes count where its MMAs are issued
+                if (MODE != PAIR || rank == 0) ptx::mbar_arrive_expect_tx(lead, FULL(ring.slot), (uint32_t)(a.bw + a.bt) * KT * parts);
                 for (int p = 0; p < parts; p++, at += part_bytes) {
-                    ptx::tma_load_2d(lead, at, &tmW, (kt + p) * KT, w_row, bar);
-                    ptx::tma_load_2d(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
+                    if constexpr (MODE == PAIR) {
+                        tma_load_2d_pair(lead, at, &tmW, (kt + p) * KT, w_row, bar);
+                        tma_load_2d_pair(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
+                    } else {
+                        ptx::tma_load_2d(lead, at, &tmW, (kt + p) * KT, w_row, bar);
+                        ptx::tma_load_2d(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
+                    }
                 }
                 ring.next(a.stages);
             }
@@ -139,9 +179,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
             const long long t0 = clock64();
             while (clock64() - t0 < (1ll << 21)) { }
         }
+    } else if (warp == 1 && rank != 0 && MODE == PAIR) {
+        pdl_wait();                                            // the first CTA issues for both
     } else if (warp == 1) {
         pdl_wait();                                            // before the first bounded wait: the kernel in front may take longer than any of them
-        const uint32_t lead = ptx::elected(), idesc = ptx::umma_idesc_s8(LANES, a.bt);
+        const uint32_t lead = ptx::elected(), idesc = ptx::umma_idesc_s8(MODE == PAIR ? 2 * LANES : LANES, a.bt);
         Turn ring, buf;
         bool ok = true;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
@@ -157,12 +199,19 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                     const int parts = min(KT, a.K - q * KT) / 32;
 #pragma unroll
                     for (int p = 0; p < KT / 32; p++)
-                        if (p < parts) ptx::umma_s8(lead, acc, w + 2 * p, x + 2 * p, idesc, q > k_lo || p > 0);
+                        if (p < parts) {
+                            if constexpr (MODE == PAIR) umma_s8_pair(lead, acc, w + 2 * p, x + 2 * p, idesc, q > k_lo || p > 0);
+                            else ptx::umma_s8(lead, acc, w + 2 * p, x + 2 * p, idesc, q > k_lo || p > 0);
+                        }
                 }
-                ptx::umma_commit(lead, EMPTY(ring.slot));
+                if constexpr (MODE == PAIR) umma_commit_pair(lead, EMPTY(ring.slot));
+                else ptx::umma_commit(lead, EMPTY(ring.slot));
                 ring.next(a.stages);
             }
-            if (ok) ptx::umma_commit(lead, T_FULL(buf.slot));
+            if (ok) {
+                if constexpr (MODE == PAIR) umma_commit_pair(lead, T_FULL(buf.slot));
+                else ptx::umma_commit(lead, T_FULL(buf.slot));
+            }
             buf.next(2);
         }
         if (!ok) {                                             // products in flight end before TMEM is given back
@@ -171,56 +220,62 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
         }
     } else {
         pdl_wait();
-        const int quad = warp & 3, row = quad * 32 + lane;     // TMEM lanes [32 * quad, 32 * quad + 32) are this warp's
+        // TMEM lanes [32 * quad, 32 * quad + 32) are this warp's, and of their columns every second 32
+        const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 2) >> 2;
         Turn buf;
         for (int tile = first; tile < a.tiles; tile += step) {
-            // what the outputs need besides the sums, while these are on their way: lane l has the scales of rows l, l + 32, ...
-            const int n = tile / a.t_tiles * a.bw + row, t0 = tile % a.t_tiles * a.bt + rank * own, rows = SPLIT ? rows_of(rank) : min(a.bt, a.M - t0);
-            const bool live = row < a.bw && n < a.N;
-            constexpr int XR = SPLIT ? SPLIT_BT / 2 / 32 : 8;
+            // what the outputs need besides the sums, while these are on their way: lane l has the scales of rows l, l + 32, ... of its columns
+            const int n = tile / a.t_tiles * a.bw + my_row + row, t0 = tile % a.t_tiles * a.bt + (MODE == SPLIT ? rank * own : 0), rows = MODE == SPLIT ? rows_of(rank) : min(a.bt, a.M - t0);
+            const bool live = my_row + row < a.bw && n < a.N;
+            constexpr int XR = MODE == SPLIT ? SPLIT_BT / 2 / 64 : 4;
             float x[XR];
 #pragma unroll
-            for (int i = 0; i < XR; i++) x[i] = 32 * i + lane < rows ? a.xs[t0 + 32 * i + lane] : 0.f;
+            for (int i = 0; i < XR; i++) {
+                const int c = MODE == SPLIT ? 2 * (32 * i + lane) + side : 64 * i + 32 * side + lane;
+                x[i] = c < rows ? a.xs[t0 + c] : 0.f;
+            }
             const float w = live ? a.ws[n] : 0.f, b = live && a.bias ? a.bias[n] : 0.f;
             T *y = static_cast<T *>(a.y) + (size_t)t0 * a.ldy + n;
             if (!ptx::mbar_wait_warp(T_FULL(buf.slot), buf.phase)) { dev_set_error(ERR_EPILOGUE); break; }
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf.slot * (a.tmem_cols / 2);
-            const int columns = SPLIT ? tile_rows : rows;
+            const int columns = MODE == SPLIT ? tile_rows : rows;
 #pragma unroll
-            for (int i = 0; i < (SPLIT ? SPLIT_BT / 32 : 8); i++) {
-                if (32 * i >= columns) break;
+            for (int i = 0; i < (MODE == SPLIT ? SPLIT_BT / 64 : 4); i++) {
+                const int c0 = 64 * i + 32 * side;
+                if (c0 >= columns) break;
                 uint32_t d[32];
-                if (32 * i + 16 < a.bt) ptx::tmem_ld(acc + 32 * i, d);
+                if (c0 + 16 < a.bt) ptx::tmem_ld(acc + c0, d);
                 else {                                         // an odd number of sixteens: the last one alone
                     uint32_t half[16];
-                    ptx::tmem_ld(acc + 32 * i, half);
+                    ptx::tmem_ld(acc + c0, half);
 #pragma unroll
                     for (int j = 0; j < 16; j++) d[j] = half[j];
                 }
                 ptx::tmem_ld_wait();
+                T *p = y + (size_t)c0 * a.ldy;
 #pragma unroll
                 for (int j = 0; j < 32; j++) {
-                    if constexpr (SPLIT) {                     // every product has been read: the stages' memory is free
-                        if (32 * i + j < columns) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + 4u * ((32 * i + j) * LANES + row)), "r"(d[j]) : "memory");
+                    if constexpr (MODE == SPLIT) {             // every product has been read: the stages' memory is free
+                        if (c0 + j < columns) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + 4u * ((c0 + j) * LANES + row)), "r"(d[j]) : "memory");
                     } else {
                         const float v = scaled((int)d[j], __shfl_sync(0xffffffffu, x[i], j), w, b);
-                        if (live && 32 * i + j < columns) put(y, v);
-                        y += a.ldy;
+                        if (live && c0 + j < columns) put(p, v);
+                        p += a.ldy;
                     }
                 }
             }
-            if constexpr (SPLIT) {
+            if constexpr (MODE == SPLIT) {
                 ptx::fence_proxy_async_smem();
                 epilogue_sync();
                 if (warp == 2 && lane < a.split && lane != rank && rows_of(lane) > 0)
                     send(remote(recv + (uint32_t)(rank * own * LANES * 4), lane), base + (uint32_t)(lane * own * LANES * 4), (uint32_t)(rows_of(lane) * LANES * 4), remote(sums_full, lane));
                 if (!ptx::mbar_wait_warp(sums_full, 0)) { dev_set_error(ERR_SUMS); break; }
 #pragma unroll
-                for (int i = 0; i < XR; i++) {
+                for (int i = 0; i < XR; i++) {                 // every second row
 #pragma unroll 4
                     for (int j = 0; j < 32; j++) {
-                        const int c = 32 * i + j;
+                        const int c = 2 * (32 * i + j) + side;
                         if (c >= rows) break;
                         int sum = 0;
                         for (int r = 0; r < a.split; r++) {
@@ -229,18 +284,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                             sum += v;
                         }
                         const float v = scaled(sum, __shfl_sync(0xffffffffu, x[i], j), w, b);
-                        if (live) put(y, v);
-                        y += a.ldy;
+                        if (live) put(y + (size_t)c * a.ldy, v);
                     }
                 }
             }
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(T_EMPTY(buf.slot));
+            if (lane == 0) {
+                if constexpr (MODE == PAIR) arrive_remote(remote(T_EMPTY(buf.slot), 0));
+                else ptx::mbar_arrive(T_EMPTY(buf.slot));
+            }
             buf.next(2);
         }
     }
-    if constexpr (SPLIT) {                                     // nobody leaves while sums are on their way from it or to it
+    if constexpr (MODE != ONE) {                               // nobody leaves while another CTA reads or writes its memory
         __syncwarp();
         cluster_sync();
     }
@@ -249,18 +306,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
     if (warp == 1) {
         __syncwarp();
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc(tmem, a.tmem_cols);
+        if constexpr (MODE == PAIR) tmem_dealloc_pair(tmem, a.tmem_cols);
+        else ptx::tmem_dealloc(tmem, a.tmem_cols);
     }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 // How the outputs are cut: tiles of bw channels and bt rows, split CTAs to a tile.
-struct Plan { int bw, bt, split, kp; };
+// pair: two CTAs to a tile, of 256 channels.
+struct Plan { int bw, bt, split, kp, pair; };
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 inline int split_receive(int bt, int split) { return split > 1 ? split * ceil_div(bt, split) * LANES * 4 : 0; }
-inline int stages_for(int bt, int split, int kp) {
-    const int n = (SMEM_MAX - SMEM_FIXED - split_receive(bt, split)) / ((A_STAGE + bt * KT) * kp);
+inline int stages_for(const Plan &p) {
+    const int n = (SMEM_MAX - SMEM_FIXED - split_receive(p.bt, p.split)) / ((A_STAGE + (p.pair ? p.bt / 2 : p.bt) * KT) * p.kp);
     return n > MAX_STAGES ? MAX_STAGES : n;
 }
 
@@ -270,9 +329,9 @@ inline Plan plan_for(int M, int N, int K, int sms) {
         int split = sms / w_tiles;
         split = split < 1 ? 1 : split > 4 ? 4 : split == 3 ? 2 : split;
         while (split > 1 && nkt / split < 4) split /= 2;
-        return {LANES, ceil_div(M, 16) * 16, split, 2};
+        return {LANES, ceil_div(M, 16) * 16, split, 2, 0};
     }
-    Plan best = {LANES, 256, 1, 1};
+    Plan best = {LANES, 256, 1, 1, 0};
     double least = 1e30;
     for (int bt = 64; bt <= 256; bt += 16) {
         const long tiles = (long)w_tiles * ceil_div(M, bt);
@@ -282,9 +341,9 @@ inline Plan plan_for(int M, int N, int K, int sms) {
     return best;
 }
 
-template <typename T, bool SPLIT>
-inline int launch_t(Args a, const CUtensorMap &tmW, const CUtensorMap &tmX, cudaStream_t st) {
-    auto kern = gemm_w8a8_kernel<T, SPLIT>;
+template <typename T, Mode MODE>
+inline int launch_t(Args a, const Plan &p, const CUtensorMap &tmW, const CUtensorMap &tmX, cudaStream_t st) {
+    auto kern = gemm_w8a8_kernel<T, MODE>;
     static PerDevice<bool> configured_dev;
     bool &configured = configured_dev.get();
     if (!configured) {
@@ -292,16 +351,16 @@ inline int launch_t(Args a, const CUtensorMap &tmW, const CUtensorMap &tmX, cuda
         if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 smem opt-in");
         configured = true;
     }
-    a.stages = stages_for(a.bt, a.split, a.kp);
-    const int smem = a.stages * a.kp * (A_STAGE + a.bt * KT) + SMEM_FIXED + split_receive(a.bt, a.split), sms = sm_count();
+    a.stages = stages_for(p);
+    const int smem = a.stages * a.kp * (A_STAGE + (MODE == PAIR ? a.bt / 2 : a.bt) * KT) + SMEM_FIXED + split_receive(p.bt, p.split), sms = sm_count();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(SPLIT ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms));
+    cfg.gridDim = dim3(MODE == SPLIT ? a.tiles * a.split : MODE == PAIR ? 2 * (a.tiles < sms / 2 ? a.tiles : sms / 2) : (a.tiles < sms ? a.tiles : sms));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int n = 0;
-    if (SPLIT) {
+    if (MODE != ONE) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
         attr[n].val.clusterDim.x = a.split; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
         n++;
@@ -322,7 +381,7 @@ inline int launch(const int8_t *xq, const int8_t *wq, Args a, Plan p, int dtype,
     a.bw = p.bw;
     a.bt = p.bt;
     a.kp = p.kp;
-    a.split = p.split;
+    a.split = p.pair ? 2 : p.split;                // CTAs of a cluster
     a.t_tiles = ceil_div(a.M, p.bt);
     const long tiles = (long)a.t_tiles * ceil_div(a.N, p.bw);
     if (tiles > 0x3fffffff) return fail(W4A8_ERR_UNSUPPORTED, "gemm_w8a8: %d x %d outputs", a.M, a.N);
@@ -330,12 +389,13 @@ inline int launch(const int8_t *xq, const int8_t *wq, Args a, Plan p, int dtype,
     a.tmem_cols = 32;
     while (a.tmem_cols < (p.split > 1 ? 1 : 2) * a.bt) a.tmem_cols *= 2;
     CUtensorMap tmW, tmX;
-    int rc = tmap_cached(&tmW, wq, (uint64_t)a.K, (uint64_t)a.N, KT, (uint32_t)a.bw, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    int rc = tmap_cached(&tmW, wq, (uint64_t)a.K, (uint64_t)a.N, KT, (uint32_t)(p.pair ? LANES : a.bw), CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (rc != W4A8_OK) return rc;
-    rc = tmap_cached(&tmX, xq, (uint64_t)a.K, (uint64_t)a.M, KT, (uint32_t)a.bt, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    rc = tmap_cached(&tmX, xq, (uint64_t)a.K, (uint64_t)a.M, KT, (uint32_t)(p.pair ? a.bt / 2 : a.bt), CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != W4A8_OK) return rc;
     const auto by_split = [&](auto t) {
-        return p.split > 1 ? launch_t<decltype(t), true>(a, tmW, tmX, st) : launch_t<decltype(t), false>(a, tmW, tmX, st);
+        if (p.pair) return launch_t<decltype(t), PAIR>(a, p, tmW, tmX, st);
+        return p.split > 1 ? launch_t<decltype(t), SPLIT>(a, p, tmW, tmX, st) : launch_t<decltype(t), ONE>(a, p, tmW, tmX, st);
     };
     if (dtype == W4A8_F32) return by_split(float());
     return dtype == W4A8_F16 ? by_split(__half()) : by_split(__nv_bfloat16());
