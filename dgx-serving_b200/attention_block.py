@@ -1,13 +1,13 @@
-"""A decoder layer's attention block: W4A8 projections around the 8-bit paged KV cache.
+"""A decoder layer's attention block: projections of 4- or 8-bit weights around the 8-bit paged KV cache.
 
 One step takes the new rows of any number of requests side by side (prompts, chunks of prompts and single tokens mixed):
 
     plan      block tables and slots of the step, from the lengths, on the GPU        w4a8_kv_plan
-    qkv       the rows' queries, keys and values, one W4A8 product                    w4a8_linear
-    rotate    the caller's, if there is one: rotary positions, norms                  -
+    qkv       the rows' queries, keys and values, one product                         w4a8_linear, w4a8_linear_w8a8
+    rotate    rotary positions and norms of queries and keys, or the caller's code    w4a8_rope_qk
     append    keys and values into their blocks as int8 codes                         w4a8_kv_append_q8
     attend    every row over all tokens that its request holds                        w4a8_attention_q8
-    out       the output product                                                      w4a8_linear
+    out       the output product                                                      w4a8_linear, w4a8_linear_w8a8
 
 The plan belongs to the step, not to the layer: PagedTables is shared by all layers, each of which has a cache of its own under the same
 block ids.  Nothing here waits for the GPU; lengths, tables and the free list stay on it.  The graphs whose place this takes keep an fp32 or
@@ -64,10 +64,20 @@ class PagedTables:
         self.kv_len.masked_fill_(ended, 0)
 
 
+def check_matrix(matrix, n, k, name):
+    """(Wq, scales) of [n][k]: packed int4 with fp32 scales of 32 elements, or int8 with one fp32 scale for each row.  True: int8."""
+    wq, sc = matrix
+    wide = wq.dtype == torch.int8 and wq.numel() == n * k
+    if wq.numel() * wq.element_size() != (n * k if wide else n * k // 2) or sc.dtype != torch.float32 or sc.numel() != (n if wide else n * k // 32) or not (wq.is_contiguous() and sc.is_contiguous()):
+        raise ValueError("%s: %d rows of %d packed int4 and %d fp32 scales, or int8 and one scale a row, contiguous" % (name, n, k, k // 32))
+    return wide
+
+
 class AttentionBlock:
-    """One layer.  wqkv: (Wq, scales) of [(heads_q + 2 * heads) * dim][hidden] (queries, keys, values), wo: of [hidden][heads_q * dim]; both
-    packed int4 with fp32 scales of 32 elements.  rotate(q, k, position), if there is one, is called between the QKV product and the append with the rows'
-    queries [T][heads_q][dim] and keys [T][heads][dim], to be changed in place (rotary positions, norms of queries and keys), and the rows' positions."""
+    """One layer.  wqkv: (Wq, scales) of [(heads_q + 2 * heads) * dim][hidden] (queries, keys, values), wo: of [hidden][heads_q * dim]; each
+    packed int4 (uint8) with fp32 scales of 32 elements, or int8 with one fp32 scale for each output channel.  rotate: a Rope, whose norms and rotary positions the
+    queries and keys get between the QKV product and the append; or the caller's rotate(q, k, position), called there with the rows' queries
+    [T][heads_q][dim] and keys [T][heads][dim], to be changed in place, and the rows' positions."""
 
     def __init__(self, wqkv, wo, hidden, heads_q, heads, dim, tables, max_rows, scale=None, window=0, softcap=0.0, rotate=None):
         self.wqkv, self.wo, self.hidden, self.heads_q, self.heads, self.dim, self.tables = wqkv, wo, hidden, heads_q, heads, dim, tables
@@ -78,9 +88,10 @@ class AttentionBlock:
         self.cache = w4a8.KVCache.of(torch.zeros(codes, dtype=torch.int8, device=dev), torch.zeros(codes, dtype=torch.int8, device=dev),
                                      torch.zeros(codes[:2], device=dev), torch.zeros(codes[:2], device=dev))
         self.cols = (heads_q + 2 * heads) * dim
-        for (wq, sc), n, k, name in ((wqkv, self.cols, hidden, "wqkv"), (wo, hidden, heads_q * dim, "wo")):
-            if wq.numel() * wq.element_size() != n * k // 2 or sc.dtype != torch.float32 or sc.numel() != n * k // 32 or not (wq.is_contiguous() and sc.is_contiguous()):
-                raise ValueError("%s: %d rows of %d packed int4 and %d fp32 scales, contiguous" % (name, n, k, k // 32))
+        self.wide_qkv = check_matrix(wqkv, self.cols, hidden, "wqkv")
+        self.wide_o = check_matrix(wo, hidden, heads_q * dim, "wo")
+        if isinstance(rotate, w4a8.Rope) and rotate.dim != dim:
+            raise ValueError("rotate: heads of %d elements, the block's have %d" % (rotate.dim, dim))
         self.qkv = torch.empty(max_rows, self.cols, device=dev)
         self.mix = torch.empty(max_rows, heads_q * dim, device=dev)
         widest = max(hidden, heads_q * dim)
@@ -100,6 +111,12 @@ class AttentionBlock:
         if not X.is_cuda or X.device != self.qkv.device:
             raise ValueError("X is on %s, the block on %s" % (X.device, self.qkv.device))
 
+    def _product(self, X, matrix, wide, Y, T, n, k):
+        if wide:
+            w4a8.linear_w8a8(X, k, self.xq, self.xs, *matrix, Y, n, T, n, k)
+        else:
+            w4a8.linear(X, self.xq, self.xs, self.xsum, *matrix, Y, T, n, k)
+
     def __call__(self, X, max_q=0):
         """X[T][hidden] fp32, the step's rows in the order of the requests -> the block's output [T][hidden], zeros in rows that no request
         owns (a padded step).  max_q: no request has more rows."""
@@ -108,11 +125,13 @@ class AttentionBlock:
         Y = torch.empty_like(X)
         q, k, v = self.qkv, self.qkv[:, self.heads_q * self.dim:], self.qkv[:, (self.heads_q + self.heads) * self.dim:]
         self.mix[:T].zero_()                                 # rows behind the last request's (a padded step) are left as they are by the attention
-        w4a8.linear(X, self.xq, self.xs, self.xsum, *self.wqkv, self.qkv, T, self.cols, self.hidden)
-        if self.rotate is not None:
+        self._product(X, self.wqkv, self.wide_qkv, self.qkv, T, self.cols, self.hidden)
+        if isinstance(self.rotate, w4a8.Rope):
+            w4a8.launch_rope_qk(self.rotate, q, self.cols, self.heads_q, k, self.cols, self.heads, t.position, T)
+        elif self.rotate is not None:
             self.rotate(q[:T, : self.heads_q * self.dim].view(T, self.heads_q, self.dim), k[:T, : self.heads * self.dim].view(T, self.heads, self.dim), t.position)
         w4a8.launch_kv_append_q8(k, v, self.cols, t.slot, T, self.cache)
         w4a8.launch_attention_q8(q, self.cols, self.cache, t.table, t.width, t.cu, t.seq_len, t.R, T, self.heads_q, self.mix, self.heads_q * self.dim,
                                  self.scale, "fp32", self.workspace, window=self.window, softcap=self.softcap, max_q=max_q)
-        w4a8.linear(self.mix, self.xq, self.xs, self.xsum, *self.wo, Y, T, self.hidden, self.heads_q * self.dim)
+        self._product(self.mix, self.wo, self.wide_o, Y, T, self.hidden, self.heads_q * self.dim)
         return Y

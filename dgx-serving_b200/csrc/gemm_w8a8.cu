@@ -36,7 +36,9 @@ W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq,
     int rc = require_sm100();
     if (rc != W4A8_OK) return rc;
     w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0, 0, 0};
-    return w8a8::launch(xq, wq, a, w8a8::plan_for(M, N, K, sm_count()), dtype, (cudaStream_t)stream);
+    w8a8::Plan plan;
+    if ((rc = w8a8::plan_cached(M, N, K, &plan)) != W4A8_OK) return rc;
+    return w8a8::launch(xq, wq, a, plan, dtype, (cudaStream_t)stream);
 }
 
 W4A8_API int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy,

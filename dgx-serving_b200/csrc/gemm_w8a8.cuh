@@ -19,18 +19,13 @@
 #include <cuda.h>
 #include "common.cuh"
 #include "ptx_sm100.cuh"
+#include "gemm_w8a8_plan.cuh"
 #include "rows.cuh"
 #include "tmap_cache.cuh"
 
 namespace w4a8 {
 namespace w8a8 {
 
-constexpr int MAX_K = 131040;
-constexpr int LANES = 128, KT = 128;           // channels of an MMA; bytes of K in a row of a swizzled tile
-constexpr int A_STAGE = LANES * KT;
-constexpr int MAX_STAGES = 12, EPI_WARPS = 8, THREADS = (2 + EPI_WARPS) * 32;
-constexpr int SMEM_MAX = 227 * 1024, SMEM_FIXED = 1024 /* alignment */ + 512 /* barriers */;
-constexpr int SPLIT_MAX = 8, SPLIT_BT = 128;   // CTAs that share a tile, and the widest tile that they share
 enum : unsigned { ERR_PRODUCER = 0xA10u, ERR_MMA = 0xA20u, ERR_EPILOGUE = 0xA30u, ERR_SUMS = 0xA40u };
 
 struct Args {
@@ -312,49 +307,67 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-// How the outputs are cut: tiles of bw channels and bt rows, split CTAs to a tile.
-// pair: two CTAs to a tile, of 256 channels.
-struct Plan { int bw, bt, split, kp, pair; };
-inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
-
-inline int split_receive(int bt, int split) { return split > 1 ? split * ceil_div(bt, split) * LANES * 4 : 0; }
-inline int stages_for(const Plan &p) {
-    const int n = (SMEM_MAX - SMEM_FIXED - split_receive(p.bt, p.split)) / ((A_STAGE + (p.pair ? p.bt / 2 : p.bt) * KT) * p.kp);
-    return n > MAX_STAGES ? MAX_STAGES : n;
+template <typename T, Mode MODE>
+inline int opt_in() {                                                  // a per-device function attribute
+    static PerDevice<bool> configured_dev;
+    bool &configured = configured_dev.get();
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(gemm_w8a8_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 smem opt-in");
+        configured = true;
+    }
+    return W4A8_OK;
 }
 
-inline Plan plan_for(int M, int N, int K, int sms) {
-    const int nkt = ceil_div(K, KT), w_tiles = ceil_div(N, LANES);
-    if (M <= 64) {
-        int split = sms / w_tiles;
-        split = split < 1 ? 1 : split > 4 ? 4 : split == 3 ? 2 : split;
-        while (split > 1 && nkt / split < 4) split /= 2;
-        return {LANES, ceil_div(M, 16) * 16, split, 2, 0};
+// How many clusters fit depends on how the GPU's SMs are grouped: asked of the driver once a device.
+inline int caps_of(Caps *out) {
+    static PerDevice<Caps> caps_dev;
+    Caps &caps = caps_dev.get();
+    if (caps.sms == 0) {
+        Caps c = {};
+        int rc = opt_in<float, SPLIT>();
+        if (rc != W4A8_OK) return rc;
+        for (int n = 2; n <= SPLIT_MAX; n++) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = n; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+            cfg.gridDim = dim3(n); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_MAX; cfg.attrs = &attr; cfg.numAttrs = 1;
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&c.clusters[n], gemm_w8a8_kernel<float, SPLIT>, &cfg);
+            if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 clusters");
+        }
+        c.sms = sm_count();
+        caps = c;
     }
-    Plan best = {LANES, 256, 1, 1, 0};
-    double least = 1e30;
-    for (int bt = 64; bt <= 256; bt += 16) {
-        const long tiles = (long)w_tiles * ceil_div(M, bt);
-        const double cost = (double)ceil_div(tiles, sms) * (bt < 128 ? 128 : bt);
-        if (cost <= least) { least = cost; best.bt = bt; }
+    *out = caps;
+    return W4A8_OK;
+}
+// The plan of a shape, kept for the shapes called last (a decode loop has a few; finding one takes some microseconds).
+inline int plan_cached(int M, int N, int K, Plan *out) {
+    struct Slot { int M, N, K, dev; Plan plan; };
+    static Slot slots[256] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+    Slot &s = slots[((uint32_t)M * 2654435761u ^ (uint32_t)N * 2246822519u ^ (uint32_t)K * 3266489917u) >> 24];
+    if (s.M != M || s.N != N || s.K != K || s.dev != dev) {
+        Caps caps;
+        const int rc = caps_of(&caps);
+        if (rc != W4A8_OK) return rc;
+        s = {M, N, K, dev, plan_for(M, N, K, caps)};
     }
-    return best;
+    *out = s.plan;
+    return W4A8_OK;
 }
 
 template <typename T, Mode MODE>
 inline int launch_t(Args a, const Plan &p, const CUtensorMap &tmW, const CUtensorMap &tmX, cudaStream_t st) {
     auto kern = gemm_w8a8_kernel<T, MODE>;
-    static PerDevice<bool> configured_dev;
-    bool &configured = configured_dev.get();
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
-        if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 smem opt-in");
-        configured = true;
-    }
+    const int rc = opt_in<T, MODE>();
+    if (rc != W4A8_OK) return rc;
     a.stages = stages_for(p);
-    const int smem = a.stages * a.kp * (A_STAGE + (MODE == PAIR ? a.bt / 2 : a.bt) * KT) + SMEM_FIXED + split_receive(p.bt, p.split), sms = sm_count();
+    const int smem = smem_for(p), sms = sm_count();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(MODE == SPLIT ? a.tiles * a.split : MODE == PAIR ? 2 * (a.tiles < sms / 2 ? a.tiles : sms / 2) : (a.tiles < sms ? a.tiles : sms));
+    cfg.gridDim = dim3(MODE == SPLIT ? a.tiles * a.split : MODE == PAIR ? 2 * (a.tiles < p.at_once ? a.tiles : p.at_once) : (a.tiles < sms ? a.tiles : sms));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;

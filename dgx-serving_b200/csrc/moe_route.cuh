@@ -2,13 +2,14 @@
 // a bias for balance, groups of experts, the topk largest choices, renormalised weights.
 //
 // A warp has a token.  Its lanes hold the token's experts in registers, a group's experts in 32 / G neighbouring lanes (G the power of two at
-// or above the groups), so that all groups find their best by the same few shuffles.  Choices are compared as 64-bit whole numbers that have
-// the order of fp64 scores; the topk largest are taken one after the other by the warp's integer maximum (three redux instructions: upper and
-// lower half, then the lowest index among equals).  Memory is a few hundred bytes a token: what bounds the kernel are its instructions, and
-// the chain of topk maxima for a few tokens.
+// or above the groups), so that all groups find their best by the same few shuffles.  The topk largest choices are taken one after the other by the
+// warp's integer maximum of numbers in the order of the choices, and the lowest index among equals.  Memory is a few hundred bytes a token: what
+// bounds the kernel are its instructions, and the chain of topk maxima for a few tokens.
 //
-// Scores are fp64 because choices lie close to one another: with 256 experts and 4096 tokens some fp32 scores are within a rounding of the next one,
-// and which expert a token gets must not depend on the exponential's last bit.
+// Choices lie close to one another: with 256 experts and 4096 tokens some fp32 scores are within a rounding of the next one, and which expert a
+// token gets must not depend on the exponential's last bit.  They are compared in fp64, then; but a token whose fp32 choices are further apart
+// than fp32 can be wrong (all but a few in a thousand) has the same order in both and is done with 32-bit maxima.  4096 tokens of 256 experts in 8 groups,
+// sigmoid and bias: 16.6 us all in fp64.
 #pragma once
 #include "common.cuh"
 #include "rows.cuh"
@@ -47,6 +48,95 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
+// The same for fp32.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const int b = __float_as_int(v + 0.f);
+    return (uint32_t)(b < 0 ? ~b : b | (1 << 31));
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __int_as_float((int)k < 0 ? (int)k & 0x7fffffff : (int)~k); }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {                // of numbers that are not negative
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+// The warp's largest key, and the lowest expert that has it.
+__device__ __forceinline__ uint32_t take(uint32_t best, int e, uint32_t &top) {
+    top = __reduce_max_sync(0xffffffffu, best);
+    return __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)e : 0xffffffffu);
+}
+__device__ __forceinline__ uint32_t take(uint64_t best, int e, uint64_t &top) {
+    const uint32_t hi = (uint32_t)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t lo = hi == top_hi ? (uint32_t)best : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
+    top = (uint64_t)top_hi << 32 | top_lo;
+    return __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)e : 0xffffffffu);
+}
+__device__ __forceinline__ double number(uint64_t k) { return unordered(k); }
+__device__ __forceinline__ float number(uint32_t k) { return unordered(k); }
+
+// The topk largest of the warp's keys (0: no expert there); lane k gets the k-th expert.  slack: what the difference of two choices may be wrong
+// by; < 0: nothing, equal keys are equal choices.  False: the keys do not decide.
+template <typename KEY, int EPL>
+__device__ __forceinline__ bool select(const Args &a, KEY (&key)[EPL], int group, int lane, int e_first, int lanes, float slack, int &mine) {
+    const bool loose = slack >= 0.f;
+    bool sure = true;
+    if (a.topk_groups < a.groups) {
+        KEY best = 0, second = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            second = max(second, min(best, key[i]));
+            best = max(best, key[i]);
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+            const KEY b2 = __shfl_xor_sync(0xffffffffu, best, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+            second = max(max(second, s2), min(best, b2));
+            best = max(best, b2);
+        }
+        const KEY score = group >= a.groups ? 0 : a.sum2 ? ordered(number(best) + number(second)) : best;
+        int ahead = 0;                             // groups in front of this one
+        bool close = false;
+        for (int g = 0; g < a.groups; g++) {
+            const KEY other = __shfl_sync(0xffffffffu, score, g << a.lanes_log2);
+            ahead += other > score || (other == score && g < group);
+            if (loose) close |= g != group && !(fabsf((float)number(other) - (float)number(score)) > 2.f * slack);
+        }
+        // (a group next to another one matters where one of the two is taken and the other is not: looked at for all that are next to the border)
+        if (loose) sure = !__any_sync(0xffffffffu, close && group < a.groups && (ahead == a.topk_groups || ahead == a.topk_groups - 1));
+        if (ahead >= a.topk_groups) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) key[i] = 0;
+        }
+    }
+    KEY best = 0;
+    int at = 0;
+    auto find = [&]() {
+        best = key[0]; at = 0;
+#pragma unroll
+        for (int i = 1; i < EPL; i++)
+            if (key[i] > best) { best = key[i]; at = i; }
+    };
+    find();
+    KEY before = 0;
+    for (int k = 0; k < a.topk + (loose ? 1 : 0); k++) {
+        const int e = e_first + at * lanes;
+        KEY top;
+        const int winner = (int)take(best, e, top);
+        if (loose && k > 0 && top != 0 && !(number(before) - number(top) > slack)) sure = false;
+        before = top;
+        if (k == a.topk) break;
+        if (lane == k) mine = winner;
+        if (e == winner) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++)
+                if (i == at) key[i] = 0;
+            find();
+        }
+    }
+    return sure;
+}
+
 constexpr int WARPS = 4;
 
 template <typename T, int EPL>                     // EPL experts a lane
@@ -59,100 +149,70 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     const T *row = static_cast<const T *>(a.logits) + t * a.ld;
     const int lanes = 1 << a.lanes_log2, group = lane >> a.lanes_log2, sub = lane & (lanes - 1);
     const int e0 = group * a.members;              // expert i of this lane is e0 + sub + i * lanes
+    const auto there = [&](int i) { return group < a.groups && sub + i * lanes < a.members; };
     const bool by_logit = !a.sigmoid && !a.bias && !a.sum2;
     float x[EPL];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
-        const int m = sub + i * lanes;
-        x[i] = group < a.groups && m < a.members ? logit(widen(row[e0 + m])) : -INFINITY;
+        x[i] = there(i) ? logit(widen(row[e0 + sub + i * lanes])) : -INFINITY;
         top = fmaxf(top, x[i]);
     }
     if (!a.sigmoid) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
         if (top == -INFINITY) top = 0.f;           // then every exponential is 0
     }
-    double total = 0.0;
-    uint64_t key[EPL];
-    if (by_logit) {                                // the order of the logits is that of the scores
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            if (!a.renormalise) total += exp((double)x[i] - (double)top);
-            key[i] = ordered((double)x[i]);
-        }
-        if (!a.renormalise) total = warp_sum(total);
-    } else {
-        double s[EPL];
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            s[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
-            total += s[i];
-        }
-        if (!a.sigmoid) {
-            total = warp_sum(total);
-            if (total > 0.0) {
-#pragma unroll
-                for (int i = 0; i < EPL; i++) s[i] = s[i] / total;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            const int m = sub + i * lanes;
-            const double b = a.bias && group < a.groups && m < a.members ? (double)a.bias[e0 + m] : 0.0;
-            key[i] = ordered(s[i] + b);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < EPL; i++)                  // places that hold no expert come after all others
-        if (group >= a.groups || sub + i * lanes >= a.members) key[i] = 0;
-
-    if (a.topk_groups < a.groups) {
-        uint64_t best = 0, second = 0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            second = max(second, min(best, key[i]));
-            best = max(best, key[i]);
-        }
-        for (int o = 1; o < lanes; o <<= 1) {
-            const uint64_t b2 = __shfl_xor_sync(0xffffffffu, best, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
-            second = max(max(second, s2), min(best, b2));
-            best = max(best, b2);
-        }
-        const uint64_t score = group >= a.groups ? 0 : a.sum2 ? ordered(unordered(best) + unordered(second)) : best;
-        int ahead = 0;                             // groups in front of this one
-        for (int g = 0; g < a.groups; g++) {
-            const uint64_t other = __shfl_sync(0xffffffffu, score, g << a.lanes_log2);
-            ahead += other > score || (other == score && g < group);
-        }
-        if (ahead >= a.topk_groups) {
-#pragma unroll
-            for (int i = 0; i < EPL; i++) key[i] = 0;
-        }
-    }
-
     int mine = 0;                                  // lane k: the k-th expert
-    uint64_t best = 0;
-    int at = 0;
-    auto find = [&]() {
-        best = key[0]; at = 0;
+    bool sure;
+    {
+        uint32_t key[EPL];
+        float slack = -1.f;
+        if (by_logit) {                            // the order of the logits is that of the scores
 #pragma unroll
-        for (int i = 1; i < EPL; i++)
-            if (key[i] > best) { best = key[i]; at = i; }
-    };
-    find();
-    for (int k = 0; k < a.topk; k++) {
-        const uint32_t hi = (uint32_t)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
-        const uint32_t lo = hi == top_hi ? (uint32_t)best : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
-        const int e = e0 + sub + at * lanes;
-        const int winner = (int)__reduce_min_sync(0xffffffffu, hi == top_hi && lo == top_lo ? (unsigned)e : 0xffffffffu);
-        if (lane == k) mine = winner;
-        if (e == winner) {
+            for (int i = 0; i < EPL; i++) key[i] = there(i) ? ordered(x[i]) : 0u;
+        } else {
+            float s[EPL], sum = 0.f, largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (i == at) key[i] = 0;
-            find();
+            for (int i = 0; i < EPL; i++) {
+                s[i] = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - top);
+                sum += s[i];
+            }
+            if (!a.sigmoid) {
+                sum = warp_sum(sum);
+                const float inv = sum > 0.f ? 1.f / sum : 1.f;
+#pragma unroll
+                for (int i = 0; i < EPL; i++) s[i] *= inv;
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const float b = a.bias && there(i) ? a.bias[e0 + sub + i * lanes] : 0.f;
+                largest = fmaxf(largest, s[i] + fabsf(b));
+                s[i] += b;
+                largest = s[i] == s[i] && fabsf(s[i]) < INFINITY ? largest : INFINITY;
+                key[i] = there(i) ? ordered(s[i]) : 0u;
+            }
+            // A score is off by at most 64 * 2^-24 of itself (the exponential 2 ulp, a sum of up to 1024 terms by 64 + 5 roundings of halves, a reciprocal and
+            // a product), a choice by one rounding more, and two of them by twice that.
+            slack = warp_max(largest) * 0x1p-16f;
         }
+        sure = select(a, key, group, lane, e0 + sub, lanes, slack, mine);
+        if (!by_logit && !(slack < INFINITY)) sure = false;
+    }
+    double total = 0.0;
+    if (!a.sigmoid && (!sure || !a.renormalise)) {
+#pragma unroll
+        for (int i = 0; i < EPL; i++) total += exp((double)x[i] - (double)top);
+        total = warp_sum(total);
+    }
+    if (!sure) {
+        uint64_t key[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            double s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
+            if (!a.sigmoid && total > 0.0) s /= total;
+            key[i] = there(i) ? ordered(s + (a.bias ? (double)a.bias[e0 + sub + i * lanes] : 0.0)) : 0ull;
+        }
+        select(a, key, group, lane, e0 + sub, lanes, -1.f, mine);
     }
     double w = 0.0;
     if (lane < a.topk) {
@@ -160,7 +220,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         if (a.sigmoid) w = 1.0 / (1.0 + exp(-v));
         else {
             w = exp(v - (double)top);
-            if (total > 0.0) w /= total;           // (0: none was taken, because weights are renormalised)
+            if (total > 0.0) w /= total;           // (0: not taken, because weights are renormalised)
         }
     }
     if (a.renormalise) {

@@ -26,47 +26,50 @@ struct Args {
     int skip_q, skip_k;                                                   // elements that are not turned already lie where they belong
 };
 
-// A group of LPH lanes has a head, a lane 8 elements of it: two runs of four at `a` and `b`, which hold four whole pairs where the head is
-// rotated (i and i + rotary / 2 side by side in one lane) and eight neighbours elsewhere.  A CTA has one token's heads, so that
-// cosines and sines are computed once for all of them.
-constexpr int THREADS = 128, BATCH = 4;                                   // BATCH heads' loads of a lane in flight
+// A group of LPH lanes has a head, a lane two runs of V of its elements, at `ia` and `ib`: V whole pairs where the head is rotated (i and
+// i + rotary / 2 in one lane) and neighbours elsewhere.  A run is 16 bytes (V 4 of fp32, 8 of 16 bits; 4 there too where rotary / 2 is no
+// multiple of 8, or dim none of 16).  A CTA has one token's heads, so that cosines and sines are computed once for all of them.
+//
+// Many tokens: bytes in flight are the bound, since each CTA waits for its position, then its rows, then stores.  Rows are asked for at once, before the
+// position is known, BATCH heads a lane.  8000 tokens of 40 heads of 128 in bf16, half of them turned: see launch_l.
+constexpr int THREADS = 128;
 
-template <typename T, int LPH>
+template <typename T, int V, int LPH, int BATCH>                         // BATCH heads' loads of a lane in flight
 __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
     __shared__ float2 turn[MAX_DIM / 2];
     const int t = blockIdx.x, half = a.rotary / 2;
-    pdl_wait();
-    pdl_launch_dependents();
-    const int pos = a.position[t];
-    if (pos < 0) return;
     const int group = threadIdx.x / LPH, j = threadIdx.x % LPH;
     constexpr int GROUPS = THREADS / LPH;
-    const bool turned = 8 * j < a.rotary, live = 8 * j < a.dim;
-    const int ia = turned && !a.interleaved ? 4 * j : 8 * j, ib = turned && !a.interleaved ? 4 * j + half : 8 * j + 4;
+    const bool turned = 2 * V * j < a.rotary, live = 2 * V * j < a.dim;
+    const int ia = turned && !a.interleaved ? V * j : 2 * V * j, ib = turned && !a.interleaved ? V * j + half : 2 * V * j + V;
     const int first = blockIdx.y * a.per_cta, last = min(first + a.per_cta, a.heads);
     const T *q = static_cast<const T *>(a.q) + (size_t)t * a.ldq, *k = static_cast<const T *>(a.k) + (size_t)t * a.ldk;
     T *qo = static_cast<T *>(a.q_out) + (size_t)t * a.ldqo, *ko = static_cast<T *>(a.k_out) + (size_t)t * a.ldko;
-    float x[BATCH][8];
+    pdl_wait();
+    pdl_launch_dependents();
+    float x[BATCH][2 * V];
     auto fetch = [&](int h0) {
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
             const int h = h0 + b * GROUPS;
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[b][i] = 0.f;
+            for (int i = 0; i < 2 * V; i++) x[b][i] = 0.f;
             if (h < last && live) {
                 const bool is_q = h < a.heads_q;
                 const T *src = is_q ? q + (size_t)h * a.dim : k + (size_t)(h - a.heads_q) * a.dim;
                 if (turned || !(is_q ? a.skip_q : a.skip_k)) {
-                    float lo[4], hi[4];
-                    load_row<T, 4>(src + ia, lo);
-                    load_row<T, 4>(src + ib, hi);
+                    float lo[V], hi[V];
+                    load_row<T, V>(src + ia, lo);
+                    load_row<T, V>(src + ib, hi);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) { x[b][i] = lo[i]; x[b][4 + i] = hi[i]; }
+                    for (int i = 0; i < V; i++) { x[b][i] = lo[i]; x[b][V + i] = hi[i]; }
                 }
             }
         }
     };
     fetch(first + group);
+    const int pos = a.position[t];
+    if (pos < 0) return;
     for (int i = threadIdx.x; i < half; i += THREADS) {
         const uint64_t angle = (uint64_t)(uint32_t)pos * a.turns[i];
         float s, c;
@@ -74,12 +77,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
         turn[i] = make_float2(c * a.magnitude, s * a.magnitude);
     }
     __syncthreads();
-    float c[4], s[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 cs = turned ? turn[4 * j + i] : make_float2(1.f, 0.f);
-        c[i] = cs.x; s[i] = cs.y;
-    }
+    const float2 *mine = turn + V * j;                                    // this lane's pairs
     for (int h0 = first + group; h0 - group < last; h0 += BATCH * GROUPS) {
         if (h0 != first + group) fetch(h0);
 #pragma unroll
@@ -90,48 +88,53 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
             if (a.variant != W4A8_NORM_NONE) {
                 float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[b][i], x[b][i], ss);
+                for (int i = 0; i < 2 * V; i++) ss = fmaf(x[b][i], x[b][i], ss);
 #pragma unroll
                 for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 const float r = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
-                float lo[4] = {1.f, 1.f, 1.f, 1.f}, hi[4] = {1.f, 1.f, 1.f, 1.f};
                 if (a.variant != W4A8_NORM_NO_SCALE && live) {
                     const float *w = is_q ? a.qw : a.kw;
-                    load_row<float, 4>(w + ia, lo);
-                    load_row<float, 4>(w + ib, hi);
-                }
-                const float one = a.variant == W4A8_NORM_ONE_PLUS ? 1.f : 0.f;
+                    const float one = a.variant == W4A8_NORM_ONE_PLUS ? 1.f : 0.f;
+                    float lo[V], hi[V];
+                    load_row<float, V>(w + ia, lo);
+                    load_row<float, V>(w + ib, hi);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[b][i] = x[b][i] * r * (one + lo[i]);
-                    x[b][4 + i] = x[b][4 + i] * r * (one + hi[i]);
+                    for (int i = 0; i < V; i++) { x[b][i] *= r * (one + lo[i]); x[b][V + i] *= r * (one + hi[i]); }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2 * V; i++) x[b][i] *= r;
                 }
             }
             if (h < last && live && (turned || !(is_q ? a.skip_q : a.skip_k))) {
-                float lo[4], hi[4];
-                if (!turned || !a.interleaved) {                          // c = 1, s = 0 where nothing is turned
+                float lo[V], hi[V];
+                if (!turned) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        lo[i] = turned ? x[b][i] * c[i] - x[b][4 + i] * s[i] : x[b][i];
-                        hi[i] = turned ? x[b][4 + i] * c[i] + x[b][i] * s[i] : x[b][4 + i];
+                    for (int i = 0; i < V; i++) { lo[i] = x[b][i]; hi[i] = x[b][V + i]; }
+                } else if (!a.interleaved) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float2 cs = mine[i];
+                        lo[i] = x[b][i] * cs.x - x[b][V + i] * cs.y;
+                        hi[i] = x[b][V + i] * cs.x + x[b][i] * cs.y;
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float u = x[b][2 * i] * c[i] - x[b][2 * i + 1] * s[i], v = x[b][2 * i + 1] * c[i] + x[b][2 * i] * s[i];
-                        (i < 2 ? lo : hi)[2 * i & 3] = u;
-                        (i < 2 ? lo : hi)[(2 * i & 3) + 1] = v;
+                    for (int i = 0; i < V; i++) {
+                        const float2 cs = mine[i];
+                        const float u = x[b][2 * i] * cs.x - x[b][2 * i + 1] * cs.y, v = x[b][2 * i + 1] * cs.x + x[b][2 * i] * cs.y;
+                        if (i < V / 2) { lo[2 * i] = u; lo[2 * i + 1] = v; }
+                        else { hi[2 * i - V] = u; hi[2 * i - V + 1] = v; }
                     }
                 }
                 T *dst = is_q ? qo + (size_t)h * a.dim : ko + (size_t)(h - a.heads_q) * a.dim;
-                store_row<T, 4>(dst + ia, lo);
-                store_row<T, 4>(dst + ib, hi);
+                store_row<T, V>(dst + ia, lo);
+                store_row<T, V>(dst + ib, hi);
             }
         }
     }
 }
 
-template <typename T, int LPH>
+template <typename T, int V, int LPH>
 inline int launch_l(Args a, int T_rows, cudaStream_t st) {
     constexpr int GROUPS = THREADS / LPH;
     // a CTA takes one head a group while that leaves SMs idle, up to all of a token's heads where there are tokens enough for every SM
@@ -139,19 +142,27 @@ inline int launch_l(Args a, int T_rows, cudaStream_t st) {
     int per = 1;
     while (per < passes && (long)T_rows * ((passes + per - 1) / per) > 8L * sm_count()) per++;
     a.per_cta = per * GROUPS;
-    const cudaError_t e = launch_pdl(rope_kernel<T, LPH>, dim3(T_rows, (a.heads + a.per_cta - 1) / a.per_cta), dim3(THREADS), 0, st, a);
+    const dim3 grid(T_rows, (a.heads + a.per_cta - 1) / a.per_cta);
+    constexpr int MOST = V == 8 ? 3 : 5;
+    const cudaError_t e = per == 1 ? launch_pdl(rope_kernel<T, V, LPH, 1>, grid, dim3(THREADS), 0, st, a)
+                                   : launch_pdl(rope_kernel<T, V, LPH, MOST>, grid, dim3(THREADS), 0, st, a);
     if (e != cudaSuccess) return cuda_fail(e, "rope launch");
     return launch_status("rope");
 }
+template <typename T, int V>
+inline int launch_v(const Args &a, int T_rows, cudaStream_t st) {
+    if (a.dim <= 8 * V) return launch_l<T, V, 4>(a, T_rows, st);
+    if (a.dim <= 16 * V) return launch_l<T, V, 8>(a, T_rows, st);
+    if (a.dim <= 32 * V || V == 8) return launch_l<T, V, 16>(a, T_rows, st);
+    return launch_l<T, V, V == 4 ? 32 : 16>(a, T_rows, st);
+}
 template <typename T>
-inline int launch_t(const Args &a, int T_rows, cudaStream_t st) {
-    if (a.dim <= 64) return launch_l<T, 8>(a, T_rows, st);
-    if (a.dim <= 128) return launch_l<T, 16>(a, T_rows, st);
-    return launch_l<T, 32>(a, T_rows, st);
+inline int launch_16(const Args &a, int T_rows, cudaStream_t st) {
+    return a.dim % 16 == 0 && a.rotary % 16 == 0 ? launch_v<T, 8>(a, T_rows, st) : launch_v<T, 4>(a, T_rows, st);
 }
 inline int launch(const Args &a, int T_rows, int dtype, cudaStream_t st) {
-    if (dtype == W4A8_F32) return launch_t<float>(a, T_rows, st);
-    return dtype == W4A8_F16 ? launch_t<__half>(a, T_rows, st) : launch_t<__nv_bfloat16>(a, T_rows, st);
+    if (dtype == W4A8_F32) return launch_v<float, 4>(a, T_rows, st);
+    return dtype == W4A8_F16 ? launch_16<__half>(a, T_rows, st) : launch_16<__nv_bfloat16>(a, T_rows, st);
 }
 
 // Frequencies in units of 2^-64 turn.  long double has the 64 bits that they are kept in.
