@@ -140,6 +140,6 @@ W4A8_API int w4a8_moe_route(const w4a8_router *r, const void *logits, int64_t ld
     static const char *const names[] = {"logits", "bias", "idx", "weight"};
     int rc = check_apart(who, rows, names, 4, 2, [](int, int) { return false; });
     if (rc != W4A8_OK || (rc = require_sm100()) != W4A8_OK) return rc;
-    route::Args a = {logits, r->bias, idx, weight, ld, S, r->experts, r->topk, r->scoring, r->groups, r->topk_groups, r->group_score == 1 && r->topk_groups < r->groups, r->renormalise != 0, 0, 0, r->scale};
+    route::Args a = {logits, r->bias, idx, weight, ld, S, r->experts, r->topk, r->scoring, r->groups, r->topk_groups, r->group_score == 1 && r->topk_groups < r->groups, r->renormalise != 0, 0, 0, 0, r->scale};
     return route::launch(a, dtype, (cudaStream_t)stream);
 }

@@ -2,14 +2,15 @@
 // a bias for balance, groups of experts, the topk largest choices, renormalised weights.
 //
 // A warp has a token.  Its lanes hold the token's experts in registers, a group's experts in 32 / G neighbouring lanes (G the power of two at
-// or above the groups), so that all groups find their best by the same few shuffles.  The topk largest choices are taken one after the other by the
-// warp's integer maximum of numbers in the order of the choices, and the lowest index among equals.  Memory is a few hundred bytes a token: what
-// bounds the kernel are its instructions, and the chain of topk maxima for a few tokens.
+// or above the groups) and neighbours in a lane, so that all groups find their best by the same few shuffles and a lane's logits come by 16-byte loads.
+// Each lane sorts what it holds, and the topk largest are taken
+// from the lanes' heads one after the other, by two integer maxima over the warp: the fp32 choice in an order that whole numbers have, then the
+// lowest index among equals.  Memory is a few hundred bytes a token: what bounds the kernel are its instructions, and for a few tokens the chain of maxima.
 //
 // Choices lie close to one another: with 256 experts and 4096 tokens some fp32 scores are within a rounding of the next one, and which expert a
-// token gets must not depend on the exponential's last bit.  They are compared in fp64, then; but a token whose fp32 choices are further apart
-// than fp32 can be wrong (all but a few in a thousand) has the same order in both and is done with 32-bit maxima.  4096 tokens of 256 experts in 8 groups,
-// sigmoid and bias: 16.6 us all in fp64.
+// token gets must not depend on the exponential's last bit.  So four candidates more than topk are taken; where neighbours among them are closer than
+// fp32 can be wrong (4 tokens in 100), the candidates are put in order by their choices in fp64, one a lane, and where that does not decide either
+// (a border of groups, more near values than candidates) the whole token is done again in fp64.
 #pragma once
 #include "common.cuh"
 #include "rows.cuh"
@@ -27,6 +28,7 @@ struct Args {
     int64_t ld;
     int S, experts, topk, sigmoid, groups, topk_groups, sum2, renormalise;
     int members, lanes_log2;                       // experts of a group; log2 of the lanes that hold them
+    int wide;                                      // lanes are full, and what they hold is aligned to 16 bytes
     float scale;
 };
 
@@ -54,6 +56,21 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return (uint32_t)(b < 0 ? ~b : b | (1 << 31));
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __int_as_float((int)k < 0 ? (int)k & 0x7fffffff : (int)~k); }
+// e^v = 2^(v log2 e), the exponent as a sum of two numbers: within 6 * 2^-24 of itself where it is normal (ex2.approx 2^-22, a product, the second number's
+// part of the result), without expf's cases.  The sigmoids of 4096 tokens by expf and an IEEE division: 14.6 us as above, 13.4 by __expf.
+__device__ __forceinline__ float exp_close(float v) {
+    constexpr float L = 1.44269502f, L2 = 1.92596299e-8f;             // log2 e = L + L2
+    v = fminf(fmaxf(v, -200.f), 100.f);                                // 0 and infinity
+    const float p = v * L, q = fmaf(v, L2, fmaf(v, L, -p));
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
+    return e * fmaf(q, 0.693147181f, 1.f);
+}
+__device__ __forceinline__ float reciprocal(float v) {                 // 1 ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -62,82 +79,108 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float warp_max(float v) {                // of numbers that are not negative
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
-// The warp's largest key, and the lowest expert that has it.
-__device__ __forceinline__ uint32_t take(uint32_t best, int e, uint32_t &top) {
-    top = __reduce_max_sync(0xffffffffu, best);
-    return __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)e : 0xffffffffu);
-}
+// The topk largest fp64 choices (0: no expert there); equal ones by the lowest index.  Lane k gets the k-th expert.
 __device__ __forceinline__ uint32_t take(uint64_t best, int e, uint64_t &top) {
     const uint32_t hi = (uint32_t)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
     const uint32_t lo = hi == top_hi ? (uint32_t)best : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
     top = (uint64_t)top_hi << 32 | top_lo;
     return __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)e : 0xffffffffu);
 }
-__device__ __forceinline__ double number(uint64_t k) { return unordered(k); }
-__device__ __forceinline__ float number(uint32_t k) { return unordered(k); }
-
-// The topk largest of the warp's keys (0: no expert there); lane k gets the k-th expert.  slack: what the difference of two choices may be wrong
-// by; < 0: nothing, equal keys are equal choices.  False: the keys do not decide.
-template <typename KEY, int EPL>
-__device__ __forceinline__ bool select(const Args &a, KEY (&key)[EPL], int group, int lane, int e_first, int lanes, float slack, int &mine) {
-    const bool loose = slack >= 0.f;
-    bool sure = true;
+template <int EPL>
+__device__ __noinline__ int select_double(const Args &a, uint64_t (&key)[EPL], int group, int lane, int e0, int lanes) {
+    uint64_t top;
     if (a.topk_groups < a.groups) {
-        KEY best = 0, second = 0;
+        uint64_t best = 0, second = 0;
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
             second = max(second, min(best, key[i]));
             best = max(best, key[i]);
         }
         for (int o = 1; o < lanes; o <<= 1) {
-            const KEY b2 = __shfl_xor_sync(0xffffffffu, best, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+            const uint64_t b2 = __shfl_xor_sync(0xffffffffu, best, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
             second = max(max(second, s2), min(best, b2));
             best = max(best, b2);
         }
-        const KEY score = group >= a.groups ? 0 : a.sum2 ? ordered(number(best) + number(second)) : best;
-        int ahead = 0;                             // groups in front of this one
-        bool close = false;
-        for (int g = 0; g < a.groups; g++) {
-            const KEY other = __shfl_sync(0xffffffffu, score, g << a.lanes_log2);
-            ahead += other > score || (other == score && g < group);
-            if (loose) close |= g != group && !(fabsf((float)number(other) - (float)number(score)) > 2.f * slack);
-        }
-        // (a group next to another one matters where one of the two is taken and the other is not: looked at for all that are next to the border)
-        if (loose) sure = !__any_sync(0xffffffffu, close && group < a.groups && (ahead == a.topk_groups || ahead == a.topk_groups - 1));
-        if (ahead >= a.topk_groups) {
+        uint64_t score = group >= a.groups ? 0 : a.sum2 ? ordered(unordered(best) + unordered(second)) : best;
+        bool open = false;
+        for (int k = 0; k < a.topk_groups; k++)
+            if ((int)take(score, group, top) == group) { open = true; score = 0; }
+        if (!open) {
 #pragma unroll
             for (int i = 0; i < EPL; i++) key[i] = 0;
         }
     }
-    KEY best = 0;
-    int at = 0;
-    auto find = [&]() {
-        best = key[0]; at = 0;
+    int mine = 0;
+    for (int k = 0; k < a.topk; k++) {
+        uint64_t best = key[0];
+        int at = 0;
 #pragma unroll
         for (int i = 1; i < EPL; i++)
             if (key[i] > best) { best = key[i]; at = i; }
-    };
-    find();
-    KEY before = 0;
-    for (int k = 0; k < a.topk + (loose ? 1 : 0); k++) {
-        const int e = e_first + at * lanes;
-        KEY top;
-        const int winner = (int)take(best, e, top);
-        if (loose && k > 0 && top != 0 && !(number(before) - number(top) > slack)) sure = false;
-        before = top;
-        if (k == a.topk) break;
+        const int e = e0 + at, winner = (int)take(best, e, top);
         if (lane == k) mine = winner;
-        if (e == winner) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (i == at) key[i] = 0;
-            find();
-        }
+        for (int i = 0; i < EPL; i++)
+            if (e == winner && i == at) key[i] = 0;
     }
-    return sure;
+    return mine;
 }
 
-constexpr int WARPS = 4;
+// What a lane holds, as fp32 choice and index in one number (the index inverted, so that of equal choices the first is the largest), no two
+// alike; 0 where there is none.  Up to eight are sorted once and then move up; more are looked
+// through each time (4096 tokens of 512 experts, sixteen a lane, topk 8: 12.2 us so, 18.7 sorted).
+template <int N>
+struct Held {
+    static constexpr bool SORTED = N <= 8;
+    uint64_t key[N];
+    __device__ __forceinline__ void settle() {
+        if constexpr (SORTED) {                    // odd-even merge sort, largest first
+#pragma unroll
+            for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+                for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+                    for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                        for (int i = 0; i < k; i++)
+                            if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                                const uint64_t u = key[i + j], v = key[i + j + k];
+                                key[i + j] = max(u, v);
+                                key[i + j + k] = min(u, v);
+                            }
+        }
+    }
+    __device__ __forceinline__ uint64_t best() const {
+        if constexpr (SORTED) return key[0];
+        uint64_t m[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < N; i++) m[i & 3] = max(m[i & 3], key[i]);
+        return max(max(m[0], m[1]), max(m[2], m[3]));
+    }
+    __device__ __forceinline__ uint32_t second(uint64_t first) const {           // the second choice, 0 if there is none
+        if constexpr (SORTED) return N > 1 ? (uint32_t)(key[N > 1] >> 32) : 0u;
+        uint64_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) m = key[i] != first ? max(m, key[i]) : m;
+        return (uint32_t)(m >> 32);
+    }
+    __device__ __forceinline__ void drop(uint64_t first, bool yes) {
+        if constexpr (SORTED) {
+#pragma unroll
+            for (int i = 0; i + 1 < N; i++) key[i] = yes ? key[i + 1] : key[i];
+            key[N - 1] = yes ? 0 : key[N - 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) key[i] = yes && key[i] == first ? 0 : key[i];
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; i++) key[i] = 0;
+    }
+};
+
+constexpr int WARPS = 4, SPARE = 4;
 
 template <typename T, int EPL>                     // EPL experts a lane
 __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
@@ -148,94 +191,173 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     if (t >= a.S) return;
     const T *row = static_cast<const T *>(a.logits) + t * a.ld;
     const int lanes = 1 << a.lanes_log2, group = lane >> a.lanes_log2, sub = lane & (lanes - 1);
-    const int e0 = group * a.members;              // expert i of this lane is e0 + sub + i * lanes
-    const auto there = [&](int i) { return group < a.groups && sub + i * lanes < a.members; };
-    const bool by_logit = !a.sigmoid && !a.bias && !a.sum2;
-    float x[EPL];
+    const int e0 = group * a.members + sub * EPL;  // the first expert of this lane
+    const auto there = [&](int i) { return group < a.groups && sub * EPL + i < a.members; };
+    const bool by_logit = !a.sigmoid && !a.bias && !a.sum2;            // the order of the logits is that of the scores
+    // every load at once: places that hold no expert read the row's first
+    float x[EPL], b[EPL];
+    bool loaded = false;
+    if constexpr (EPL % Row<T>::N == 0) {
+        if (a.wide) {
+            load_row<T, EPL>(row + (group < a.groups ? e0 : 0), x);
+#pragma unroll
+            for (int i = 0; i < EPL; i++) b[i] = 0.f;
+            if (a.bias) load_row<float, EPL>(a.bias + (group < a.groups ? e0 : 0), b);
+            loaded = true;
+        }
+    }
+    if (!loaded) {
+#pragma unroll
+        for (int i = 0; i < EPL; i++) x[i] = widen(row[there(i) ? e0 + i : 0]);
+#pragma unroll
+        for (int i = 0; i < EPL; i++) b[i] = a.bias ? a.bias[there(i) ? e0 + i : 0] : 0.f;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
-        x[i] = there(i) ? logit(widen(row[e0 + sub + i * lanes])) : -INFINITY;
+        x[i] = there(i) ? logit(x[i]) : -INFINITY;
         top = fmaxf(top, x[i]);
     }
     if (!a.sigmoid) {
         top = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
         if (top == -INFINITY) top = 0.f;           // then every exponential is 0
     }
-    int mine = 0;                                  // lane k: the k-th expert
-    bool sure;
-    {
-        uint32_t key[EPL];
-        float slack = -1.f;
-        if (by_logit) {                            // the order of the logits is that of the scores
+    Held<EPL> held;
+    const auto hold = [&](int i, float c) { held.key[i] = there(i) ? (uint64_t)ordered(c) << 32 | ~(uint32_t)(e0 + i) : 0ull; };
+    float slack = 0.f;
+    if (by_logit) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) key[i] = there(i) ? ordered(x[i]) : 0u;
-        } else {
-            float s[EPL], sum = 0.f, largest = 0.f;
+        for (int i = 0; i < EPL; i++) hold(i, x[i]);
+    } else {
+        float s[EPL], sum = 0.f, largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                s[i] = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - top);
-                sum += s[i];
-            }
-            if (!a.sigmoid) {
-                sum = warp_sum(sum);
-                const float inv = sum > 0.f ? 1.f / sum : 1.f;
-#pragma unroll
-                for (int i = 0; i < EPL; i++) s[i] *= inv;
-            }
-#pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                const float b = a.bias && there(i) ? a.bias[e0 + sub + i * lanes] : 0.f;
-                largest = fmaxf(largest, s[i] + fabsf(b));
-                s[i] += b;
-                largest = s[i] == s[i] && fabsf(s[i]) < INFINITY ? largest : INFINITY;
-                key[i] = there(i) ? ordered(s[i]) : 0u;
-            }
-            // A score is off by at most 64 * 2^-24 of itself (the exponential 2 ulp, a sum of up to 1024 terms by 64 + 5 roundings of halves, a reciprocal and
-            // a product), a choice by one rounding more, and two of them by twice that.
-            slack = warp_max(largest) * 0x1p-16f;
+        for (int i = 0; i < EPL; i++) {
+            s[i] = a.sigmoid ? reciprocal(1.f + exp_close(-x[i])) : exp_close(x[i] - top);
+            sum += s[i];
         }
-        sure = select(a, key, group, lane, e0 + sub, lanes, slack, mine);
-        if (!by_logit && !(slack < INFINITY)) sure = false;
-    }
-    double total = 0.0;
-    if (!a.sigmoid && (!sure || !a.renormalise)) {
+        if (!a.sigmoid) {
+            sum = warp_sum(sum);
+            const float inv = sum > 0.f ? reciprocal(sum) : 1.f;
 #pragma unroll
-        for (int i = 0; i < EPL; i++) total += exp((double)x[i] - (double)top);
-        total = warp_sum(total);
+            for (int i = 0; i < EPL; i++) s[i] *= inv;
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            if (there(i)) largest = fmaxf(largest, s[i] + fabsf(b[i]));
+            s[i] += b[i];
+            largest = fabsf(s[i]) < INFINITY ? largest : INFINITY;
+            hold(i, s[i]);
+        }
+        // How far a choice may be off, in units of 2^-24 of the largest score and bias together.  Sigmoid: exp_close 6, the sum 1, the reciprocal 2, the
+        // bias 1: two choices 20, and 2^-19 is 32.  Softmax: exp_close 6 and its argument's rounding, |v| e^v < 0.4; a sum of up to 1024 terms 64 + 5; the
+        // reciprocal 2; the product and the sum with the bias 2: two 160, and 2^-16 is 256.
+        slack = warp_max(largest) * (a.sigmoid ? 0x1p-19f : 0x1p-16f);
     }
-    if (!sure) {
+    held.settle();
+    bool whole = !(slack < INFINITY);              // again in fp64
+    if (a.topk_groups < a.groups) {
+        const uint64_t first = held.best();
+        uint32_t best = (uint32_t)(first >> 32), second = held.second(first);
+        for (int o = 1; o < lanes; o <<= 1) {
+            const uint32_t b2 = __shfl_xor_sync(0xffffffffu, best, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+            second = max(max(second, s2), min(best, b2));
+            best = max(best, b2);
+        }
+        uint32_t score = group >= a.groups ? 0 : a.sum2 ? ordered(unordered(best) + unordered(second)) : best, before = 0;
+        bool open = false;
+        for (int k = 0; k < a.topk_groups + (by_logit ? 0 : 1); k++) { // the best group of those that are left, and of equal ones the first
+            const uint32_t most = __reduce_max_sync(0xffffffffu, score), g = __reduce_min_sync(0xffffffffu, score == most ? (uint32_t)group : 0xffffffffu);
+            if (k == a.topk_groups) whole |= !(unordered(before) - unordered(most) > 2.f * slack);      // the last group taken and the first that is not
+            else if ((int)g == group) { open = true; score = 0; }
+            before = most;
+        }
+        if (!open) held.clear();
+    }
+    const int wanted = by_logit ? a.topk : min(32, a.topk + SPARE);
+    int mine = 0, found = 0;                       // lane k: the k-th candidate
+    float choice = 0.f;
+    for (int k = 0; k < wanted; k++) {
+        const uint64_t best = held.best();
+        const uint32_t hi = (uint32_t)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
+        if (top_hi == 0) break;
+        const uint32_t top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? (uint32_t)best : 0u);
+        if (lane == k) { mine = (int)~top_lo; choice = unordered(top_hi); }
+        held.drop(best, hi == top_hi && (uint32_t)best == top_lo);
+        found = k + 1;
+    }
+    if (!by_logit && !whole) {
+        const float next = __shfl_down_sync(0xffffffffu, choice, 1);
+        if (__any_sync(0xffffffffu, lane < a.topk && lane + 1 < found && !(choice - next > slack))) {
+            // candidates that were not taken are further away than fp32 can be wrong, or there are none
+            const float last = __shfl_sync(0xffffffffu, choice, found - 1), end = __shfl_sync(0xffffffffu, choice, a.topk - 1);
+            if (found < wanted || end - last > slack) {
+                double total = 1.0;
+                if (!a.sigmoid) {
+                    total = 0.0;
+#pragma unroll
+                    for (int i = 0; i < EPL; i++) total += exp((double)x[i] - (double)top);
+                    total = warp_sum(total);
+                }
+                const double v = (double)logit(widen(row[mine]));
+                double c = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top);
+                if (!a.sigmoid && total > 0.0) c /= total;
+                if (a.bias) c += (double)a.bias[mine];
+                int ahead = 0, placed = 0;
+                for (int k = 0; k < found; k++) {
+                    const double other = __shfl_sync(0xffffffffu, c, k);
+                    const int e = __shfl_sync(0xffffffffu, mine, k);
+                    ahead += other > c || (other == c && e < mine);
+                }
+                for (int k = 0; k < found; k++) {
+                    const int place = __shfl_sync(0xffffffffu, ahead, k), e = __shfl_sync(0xffffffffu, mine, k);
+                    if (place == lane) placed = e;
+                }
+                mine = placed;
+            } else whole = true;
+        }
+    }
+    if (whole) {
+        double total = 0.0;
+        if (!a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) total += exp((double)x[i] - (double)top);
+            total = warp_sum(total);
+        }
         uint64_t key[EPL];
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
             double s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
             if (!a.sigmoid && total > 0.0) s /= total;
-            key[i] = there(i) ? ordered(s + (a.bias ? (double)a.bias[e0 + sub + i * lanes] : 0.0)) : 0ull;
+            key[i] = there(i) ? ordered(s + (double)b[i]) : 0ull;
         }
-        select(a, key, group, lane, e0 + sub, lanes, -1.f, mine);
+        mine = select_double(a, key, group, lane, e0, lanes);
     }
-    double w = 0.0;
+    float w = 0.f;
     if (lane < a.topk) {
-        const double v = (double)logit(widen(row[mine]));
-        if (a.sigmoid) w = 1.0 / (1.0 + exp(-v));
-        else {
-            w = exp(v - (double)top);
-            if (total > 0.0) w /= total;           // (0: not taken, because weights are renormalised)
+        const float v = logit(widen(row[mine]));
+        w = a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top);
+    }
+    float sum = warp_sum(w);
+    if (!a.renormalise) {                          // softmax over all experts, the sum in fp32 as the weights are
+        sum = 0.f;
+        if (!a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) sum += expf(x[i] - top);
+            sum = warp_sum(sum);
         }
     }
-    if (a.renormalise) {
-        const double sum = warp_sum(w);
-        if (sum > 0.0) w /= sum;
-    }
+    if (sum > 0.f) w /= sum;
     if (lane < a.topk) {
         a.idx[t * a.topk + lane] = mine;
-        a.weight[t * a.topk + lane] = (float)(w * (double)a.scale);
+        a.weight[t * a.topk + lane] = w * a.scale;
     }
 }
 
 template <typename T>
-inline int launch_t(const Args &a, cudaStream_t st) {
-    const int epl = (a.members + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
+inline int launch_t(Args a, cudaStream_t st) {
+    int epl = 1;
+    while ((epl << a.lanes_log2) < a.members) epl *= 2;
+    a.wide = a.members == epl << a.lanes_log2 && aligned(a.logits, 16) && a.ld * sizeof(T) % 16 == 0 && (!a.bias || aligned(a.bias, 16));
     const dim3 grid((unsigned)((a.S + (long)WARPS - 1) / WARPS)), block(WARPS * 32);
     cudaError_t e;
     if (epl <= 1) e = launch_pdl(route_kernel<T, 1>, grid, block, 0, st, a);

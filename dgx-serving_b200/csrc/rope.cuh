@@ -47,22 +47,19 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
     T *qo = static_cast<T *>(a.q_out) + (size_t)t * a.ldqo, *ko = static_cast<T *>(a.k_out) + (size_t)t * a.ldko;
     pdl_wait();
     pdl_launch_dependents();
-    float x[BATCH][2 * V];
+    Packed<T, V> raw[BATCH][2];
     auto fetch = [&](int h0) {
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
             const int h = h0 + b * GROUPS;
-#pragma unroll
-            for (int i = 0; i < 2 * V; i++) x[b][i] = 0.f;
+            raw[b][0].clear();
+            raw[b][1].clear();
             if (h < last && live) {
                 const bool is_q = h < a.heads_q;
                 const T *src = is_q ? q + (size_t)h * a.dim : k + (size_t)(h - a.heads_q) * a.dim;
                 if (turned || !(is_q ? a.skip_q : a.skip_k)) {
-                    float lo[V], hi[V];
-                    load_row<T, V>(src + ia, lo);
-                    load_row<T, V>(src + ib, hi);
-#pragma unroll
-                    for (int i = 0; i < V; i++) { x[b][i] = lo[i]; x[b][V + i] = hi[i]; }
+                    raw[b][0].load(src + ia);
+                    raw[b][1].load(src + ib);
                 }
             }
         }
@@ -85,10 +82,13 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
             const int h = h0 + b * GROUPS;
             if (h - group >= last) break;                                 // the same for the whole CTA: lanes of a group meet in the sums below
             const bool is_q = h < a.heads_q;
+            float u[V], v[V];                                             // the two runs
+            raw[b][0].unpack(u);
+            raw[b][1].unpack(v);
             if (a.variant != W4A8_NORM_NONE) {
                 float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < 2 * V; i++) ss = fmaf(x[b][i], x[b][i], ss);
+                for (int i = 0; i < V; i++) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
 #pragma unroll
                 for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 const float r = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
@@ -99,36 +99,35 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
                     load_row<float, V>(w + ia, lo);
                     load_row<float, V>(w + ib, hi);
 #pragma unroll
-                    for (int i = 0; i < V; i++) { x[b][i] *= r * (one + lo[i]); x[b][V + i] *= r * (one + hi[i]); }
+                    for (int i = 0; i < V; i++) { u[i] *= r * (one + lo[i]); v[i] *= r * (one + hi[i]); }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) x[b][i] *= r;
+                    for (int i = 0; i < V; i++) { u[i] *= r; v[i] *= r; }
                 }
             }
             if (h < last && live && (turned || !(is_q ? a.skip_q : a.skip_k))) {
-                float lo[V], hi[V];
-                if (!turned) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) { lo[i] = x[b][i]; hi[i] = x[b][V + i]; }
-                } else if (!a.interleaved) {
+                if (turned && !a.interleaved) {
 #pragma unroll
                     for (int i = 0; i < V; i++) {
                         const float2 cs = mine[i];
-                        lo[i] = x[b][i] * cs.x - x[b][V + i] * cs.y;
-                        hi[i] = x[b][V + i] * cs.x + x[b][i] * cs.y;
+                        const float w = u[i] * cs.x - v[i] * cs.y;
+                        v[i] = v[i] * cs.x + u[i] * cs.y;
+                        u[i] = w;
                     }
-                } else {
+                } else if (turned) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        const float2 cs = mine[i];
-                        const float u = x[b][2 * i] * cs.x - x[b][2 * i + 1] * cs.y, v = x[b][2 * i + 1] * cs.x + x[b][2 * i] * cs.y;
-                        if (i < V / 2) { lo[2 * i] = u; lo[2 * i + 1] = v; }
-                        else { hi[2 * i - V] = u; hi[2 * i - V + 1] = v; }
+                    for (int i = 0; i < V; i += 2) {
+                        const float2 cs = mine[i / 2], ds = mine[(V + i) / 2];
+                        const float w = u[i] * cs.x - u[i + 1] * cs.y, z = v[i] * ds.x - v[i + 1] * ds.y;
+                        u[i + 1] = u[i + 1] * cs.x + u[i] * cs.y;
+                        v[i + 1] = v[i + 1] * ds.x + v[i] * ds.y;
+                        u[i] = w;
+                        v[i] = z;
                     }
                 }
                 T *dst = is_q ? qo + (size_t)h * a.dim : ko + (size_t)(h - a.heads_q) * a.dim;
-                store_row<T, V>(dst + ia, lo);
-                store_row<T, V>(dst + ib, hi);
+                store_row<T, V>(dst + ia, u);
+                store_row<T, V>(dst + ib, v);
             }
         }
     }

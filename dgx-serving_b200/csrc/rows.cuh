@@ -70,6 +70,33 @@ __device__ __forceinline__ void load_row(const T *p, float (&x)[V]) {
         }
     }
 }
+// The same as it lies in memory, widened later: 16 bits an element while a load is in flight.
+template <typename T, int V>
+struct Packed {
+    uint4 r[V < Row<T>::N ? 1 : V / Row<T>::N];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (V < Row<T>::N) {
+            const uint2 h = *reinterpret_cast<const uint2 *>(p);
+            r[0] = make_uint4(h.x, h.y, 0u, 0u);
+        } else {
+#pragma unroll
+            for (int c = 0; c < V / Row<T>::N; c++) r[c] = reinterpret_cast<const uint4 *>(p)[c];
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (auto &v : r) v = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void unpack(float (&x)[V]) const {
+#pragma unroll
+        for (int c = 0; c < V; c += Row<T>::N) {
+            float t[Row<T>::N];
+            Row<T>::unpack(r[c / Row<T>::N], t);
+#pragma unroll
+            for (int i = 0; i < Row<T>::N && c + i < V; i++) x[c + i] = t[i];
+        }
+    }
+};
 template <typename T, int V>
 __device__ __forceinline__ void store_row(T *p, const float (&x)[V]) {
     if constexpr (V < Row<T>::N) {

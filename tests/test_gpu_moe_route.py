@@ -41,8 +41,8 @@ def check(w4a8, logits, topk, dtype="fp32", **how):
     w4a8.launch_moe_route(router, logits, logits.stride(0), S, idx, weight, dtype)
     want_idx, want = plain(logits, topk, **how)
     assert np.array_equal(idx[:S].cpu().numpy(), want_idx)
-    # fp64 until one rounding to fp32
-    assert np.allclose(weight[:S].cpu().numpy(), want, rtol=2 ** -23, atol=1e-44)
+    # fp32: the exponential 2 ulp and, of its argument's rounding, |v| e^v < 0.4 of the largest weight; the sum of 32 (1024) terms 6 (38) roundings, two quotients, the scale
+    assert np.allclose(weight[:S].cpu().numpy(), want, rtol=(54 if how.get("renormalise", True) is False else 22) * 2.0 ** -24, atol=2.0 ** -24 * 2.5)
     assert (idx[S] == -7).all() and (weight[S] == -7).all()
 
 
@@ -102,7 +102,7 @@ def test_many_tokens_two_streams_and_a_graph(w4a8, cuda):
     torch.cuda.synchronize()
     for l, o in zip(logits, out):
         want_idx, want = plain(l, 8)
-        assert np.array_equal(o[0].cpu().numpy(), want_idx) and np.allclose(o[1].cpu().numpy(), want, rtol=2 ** -23)
+        assert np.array_equal(o[0].cpu().numpy(), want_idx) and np.allclose(o[1].cpu().numpy(), want, rtol=22 * 2.0 ** -24, atol=2.0 ** -24)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         w4a8.launch_moe_route(router, logits[0], E, S, *out[0])
