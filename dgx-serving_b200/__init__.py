@@ -11,6 +11,8 @@ Function names and argument order mirror the reference launchers
 kernels/gemm_mmq.cuh:230, kernels/gemm_mmq_raster.cuh:115).
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -222,6 +224,25 @@ def lib():
     return _lib
 
 
+_native = None
+_NATIVE_ENTRIES = ("add_norm", "rope_qk", "moe_route", "quantize_rows_q8", "gemm_w8a8", "linear_w8a8")
+
+
+def _binding():
+    """csrc/binding.c: the layer operators' entries without ctypes, whose conversions take longer than their smallest kernels."""
+    global _native
+    if _native is None:
+        path = os.path.join(_HERE, "_binding.so")
+        if not os.path.exists(path):
+            raise RuntimeError("%s not built; run python dgx-serving_b200/build.py" % path)
+        loader = importlib.machinery.ExtensionFileLoader("_binding", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+        loader.exec_module(module)
+        module.bind(*[ctypes.cast(getattr(lib(), "w4a8_" + n), ctypes.c_void_p).value for n in _NATIVE_ENTRIES])
+        _native = module
+    return _native
+
+
 def _check(rc):
     if rc != OK:
         raise W4A8Error(rc, lib().w4a8_last_error().decode())
@@ -417,7 +438,9 @@ def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=No
     """h' = h + norm(y) * gate * alpha of S rows, to H_out, and its norm n, to N and / or quantized to xq, xs, xsum (w4a8_add_norm).  Y None: h' = h.
     group 32: blocks of 32 elements, 0: one scale for a row.  Pitches of 0: K."""
     K = norm.K
-    _check(lib().w4a8_add_norm(norm, _ptr(H), ldh or K, _ptr(Y), ldy or K, _ptr(H_out), ldo or K, _ptr(N), ldn or K, _ptr(xq), _ptr(xs), _ptr(xsum), group, S, _stream(stream)))
+    rc = (_native or _binding()).add_norm(norm, H, ldh or K, Y, ldy or K, H_out, ldo or K, N, ldn or K, xq, xs, xsum, group, S, _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def launch_rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out=None, ldqo=0, K_out=None, ldko=0, dtype="fp32", stream=None):
@@ -426,28 +449,37 @@ def launch_rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out=No
         Q_out, ldqo = Q, ldq
     if K_out is None:
         K_out, ldko = K, ldk
-    _check(lib().w4a8_rope_qk(rope, _ptr(Q), ldq, heads_q, _ptr(K), ldk, heads_k, _ptr(position), T, _ptr(Q_out), ldqo, _ptr(K_out), ldko, DTYPES.get(dtype, dtype), _stream(stream)))
+    rc = (_native or _binding()).rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out, ldqo, K_out, ldko, DTYPES.get(dtype, dtype), _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def launch_moe_route(router, logits, ld, S, idx, weight, dtype="fp32", stream=None):
     """The experts idx[S][topk] of S tokens and their weights, from logits[S][experts] (w4a8_moe_route): what moe_block takes."""
-    _check(lib().w4a8_moe_route(router, _ptr(logits), ld, S, DTYPES.get(dtype, dtype), _ptr(idx), _ptr(weight), _stream(stream)))
+    rc = (_native or _binding()).moe_route(router, logits, ld, S, DTYPES.get(dtype, dtype), idx, weight, _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def launch_quantize_rows_q8(X, ldx, S, K, xq, xs, dtype="fp32", stream=None):
     """Rows to int8 with one scale each (w4a8_quantize_rows_q8): activations of the 8-bit products, or their weights, a channel per row."""
-    _check(lib().w4a8_quantize_rows_q8(_ptr(X), ldx, S, K, DTYPES.get(dtype, dtype), _ptr(xq), _ptr(xs), _stream(stream)))
+    rc = (_native or _binding()).quantize_rows_q8(X, ldx, S, K, DTYPES.get(dtype, dtype), xq, xs, _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def launch_gemm_w8a8(xq, xs, wq, ws, Y, ldy, M, N, K, dtype="fp32", bias=None, stream=None):
     """Y[M][N] = xq wq^T * xs[m] * ws[n] + bias[n], the sums exact (w4a8_gemm_w8a8)."""
-    _check(lib().w4a8_gemm_w8a8(_ptr(xq), _ptr(xs), _ptr(wq), _ptr(ws), _ptr(bias), _ptr(Y), ldy, M, N, K, DTYPES.get(dtype, dtype), _stream(stream)))
+    rc = (_native or _binding()).gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, M, N, K, DTYPES.get(dtype, dtype), _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def linear_w8a8(X, ldx, xq, xs, wq, ws, Y, ldy, S, N, K, x_dtype="fp32", y_dtype="fp32", bias=None, skip_quantize=0, stream=None):
     """linear() for 8-bit weights with a scale for each output channel (w4a8_linear_w8a8)."""
-    _check(lib().w4a8_linear_w8a8(_ptr(X), ldx, _ptr(xq), _ptr(xs), _ptr(wq), _ptr(ws), _ptr(bias), _ptr(Y), ldy, S, N, K, DTYPES.get(x_dtype, x_dtype),
-                                  DTYPES.get(y_dtype, y_dtype), skip_quantize, _stream(stream)))
+    rc = (_native or _binding()).linear_w8a8(X, ldx, xq, xs, wq, ws, bias, Y, ldy, S, N, K, DTYPES.get(x_dtype, x_dtype), DTYPES.get(y_dtype, y_dtype), skip_quantize, _stream(stream))
+    if rc:
+        _check(rc)
 
 
 def shard_rows(N, rank, world):

@@ -124,3 +124,35 @@ def test_structs_of_tensors(w4a8):
         w4a8.Router.of(64, 8, bias=torch.zeros(63))
     with pytest.raises(KeyError):
         w4a8.Router.of(64, 8, scoring="sparse")
+
+
+def test_the_binding_without_ctypes(w4a8):
+    """The launchers' own way into the library: what it cannot convert is an exception, what the library refuses is its error."""
+    t = torch.zeros(4, 64)
+    n = norm_of(w4a8, K=48)
+    with pytest.raises(w4a8.W4A8Error, match="multiple of 32") as e:
+        w4a8.launch_add_norm(n, t, t, 4, N=t, stream=0)
+    assert e.value.code == w4a8.ERR_ARG
+    with pytest.raises(w4a8.W4A8Error, match="no output"):
+        w4a8.launch_add_norm(norm_of(w4a8), t, None, 4, stream=0)
+    with pytest.raises(w4a8.W4A8Error, match="pitch"):
+        w4a8.launch_gemm_w8a8(t, t, t, t, t, 39, 8, 40, 64, stream=0)
+    with pytest.raises(w4a8.W4A8Error, match="null"):
+        w4a8.linear_w8a8(None, 64, t, t, t, t, t, 40, 8, 40, 64, stream=0)
+    with pytest.raises(w4a8.W4A8Error, match="null"):
+        w4a8.launch_quantize_rows_q8(t, 64, 4, 64, t, None, stream=0)
+    with pytest.raises(w4a8.W4A8Error, match="experts"):
+        w4a8.launch_moe_route(w4a8.Router.of(64, 40), t, 64, 4, t, t, stream=0)
+    with pytest.raises(w4a8.W4A8Error, match="dtype"):
+        w4a8.launch_rope_qk(w4a8.Rope(), t, 64, 1, t, 64, 1, t, 4, dtype=7, stream=0)
+    w4a8.launch_add_norm(norm_of(w4a8), None, None, 0, stream=0)                     # nothing to do
+    with pytest.raises(OverflowError):
+        w4a8.launch_add_norm(norm_of(w4a8), t, t, 1 << 40, N=t, stream=0)
+    with pytest.raises(TypeError):
+        w4a8.launch_add_norm(norm_of(w4a8), t, t, 4.0, N=t, stream=0)
+    with pytest.raises(AttributeError):
+        w4a8.launch_add_norm(norm_of(w4a8), "h", t, 4, N=t, stream=0)
+    with pytest.raises(TypeError, match="a struct of"):
+        w4a8._binding().add_norm(w4a8.Rope(), t, 64, t, 64, None, 64, t, 64, None, None, None, 32, 4, 0)
+    with pytest.raises(TypeError, match="15 expected"):
+        w4a8._binding().add_norm(norm_of(w4a8), t)
