@@ -62,11 +62,10 @@ __device__ __forceinline__ double squares(const float (&x)[V], double ss) {
     for (int i = 0; i < V; i++) ss = fma((double)x[i], (double)x[i], ss);
     return ss;
 }
-// x * r * w, x * r * (1 + w) or x * r, from left to right.
+__device__ __forceinline__ bool takes_weight(int variant) { return variant == W4A8_NORM_SCALE || variant == W4A8_NORM_ONE_PLUS; }
+// x * r * f, x * r * (1 + f) or x * r, from left to right.
 template <int V>
-__device__ __forceinline__ void normed(float (&x)[V], float r, const float *w, int variant) {
-    float f[V];
-    if (variant != W4A8_NORM_NO_SCALE) load_row<float, V>(w, f);
+__device__ __forceinline__ void normed(float (&x)[V], float r, const float (&f)[V], int variant) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         x[i] = __fmul_rn(x[i], r);
@@ -79,8 +78,10 @@ __device__ __forceinline__ void normed(float (&x)[V], float r, const float *w, i
 template <typename TH, typename TY>
 constexpr int VEC = sizeof(TH) == 4 && sizeof(TY) == 4 ? 4 : 8;
 
-template <typename TH, typename TY, int EP, int MAXT>                  // EP elements a thread
-__global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
+// EP elements a thread.  EARLY: weights are asked for together with the rows and not behind the sums that they do not depend on: a
+// trip to L2 less for each norm where a few rows are bound by latency (64 rows of 5120 with codes 3.3 -> 2.8 us), registers that cost CTAs where there are many.  SUM: there is a y.
+template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM>
+__global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
     constexpr int V = VEC<TH, TY>, NV = EP / V;
     __shared__ double sh_y[32], sh_h[32];
     __shared__ float sh_max[32];
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
     pdl_wait();
     pdl_launch_dependents();
     const TH *h = static_cast<const TH *>(a.h) + row * a.ldh;
-    float x[NV][V];
+    float x[NV][V], f[EARLY ? NV : 1][V];
 #pragma unroll
     for (int u = 0; u < NV; u++) {
         const int j = threadIdx.x + u * nt;
@@ -97,15 +98,23 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
         for (int i = 0; i < V; i++) x[u][i] = 0.f;
         if (j < nvec) load_row<TH, V>(h + j * V, x[u]);
     }
-    if (a.y) {
+    const auto fetch = [&](float (&to)[V], const float *from, int j) { if (j < nvec) load_row<float, V>(from + j * V, to); };
+    if constexpr (SUM) {
         const TY *y = static_cast<const TY *>(a.y) + row * a.ldy;
-        float p[NV][V];
+        float p[NV][V], pf[EARLY ? NV : 1][V];
 #pragma unroll
         for (int u = 0; u < NV; u++) {
             const int j = threadIdx.x + u * nt;
 #pragma unroll
             for (int i = 0; i < V; i++) p[u][i] = 0.f;
             if (j < nvec) load_row<TY, V>(y + j * V, p[u]);
+        }
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int u = 0; u < NV; u++) {
+                if (takes_weight(a.post)) fetch(pf[u], a.pw, threadIdx.x + u * nt);
+                if (takes_weight(a.variant)) fetch(f[u], a.w, threadIdx.x + u * nt);
+            }
         }
         float r = 1.f;
         if (a.post != W4A8_NORM_NONE) {
@@ -118,7 +127,10 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
         for (int u = 0; u < NV; u++) {
             const int j = threadIdx.x + u * nt;
             if (j < nvec) {
-                if (a.post != W4A8_NORM_NONE) normed(p[u], r, a.pw + j * V, a.post);
+                if (a.post != W4A8_NORM_NONE) {
+                    if (!EARLY && takes_weight(a.post)) fetch(pf[0], a.pw, j);
+                    normed(p[u], r, pf[EARLY ? u : 0], a.post);
+                }
                 if (a.gate) {
                     float g[V];
                     load_row<float, V>(a.gate + row * a.ldg + j * V, g);
@@ -129,6 +141,10 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
                 for (int i = 0; i < V; i++) x[u][i] = __fadd_rn(x[u][i], __fmul_rn(p[u][i], a.alpha));
             }
         }
+    } else if constexpr (EARLY) {
+#pragma unroll
+        for (int u = 0; u < NV; u++)
+            if (takes_weight(a.variant)) fetch(f[u], a.w, threadIdx.x + u * nt);
     }
     if (a.h_out) {
         TH *o = static_cast<TH *>(a.h_out) + row * a.ldo;
@@ -147,7 +163,10 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
 #pragma unroll
         for (int u = 0; u < NV; u++) {
             const int j = threadIdx.x + u * nt;
-            if (j < nvec) normed(x[u], r, a.w + j * V, a.variant);
+            if (j < nvec) {
+                if (!EARLY && takes_weight(a.variant)) fetch(f[0], a.w, j);
+                normed(x[u], r, f[EARLY ? u : 0], a.variant);
+            }
         }
     }
     if (a.n_out) {
@@ -207,24 +226,28 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const Args a) {
     }
 }
 
-template <typename TH, typename TY, int EP, int MAXT>
+template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM>
 inline int launch_ep(const Args &a, int S, cudaStream_t st) {
     const int need = (a.K + EP - 1) / EP;
-    const cudaError_t e = launch_pdl(add_norm_kernel<TH, TY, EP, MAXT>, dim3(S), dim3((need + 31) / 32 * 32), 0, st, a);
+    const cudaError_t e = launch_pdl(add_norm_kernel<TH, TY, EP, MAXT, EARLY, SUM>, dim3(S), dim3((need + 31) / 32 * 32), 0, st, a);
     if (e != cudaSuccess) return cuda_fail(e, "add_norm launch");
     return launch_status("add_norm");
 }
-template <typename TH, typename TY>
+template <typename TH, typename TY, bool SUM>
 inline int launch_t(const Args &a, int S, cudaStream_t st) {
-    if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024>(a, S, st);
-    if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512>(a, S, st);
-    if (a.K <= 512 * 32) return launch_ep<TH, TY, 32, 512>(a, S, st);
-    return launch_ep<TH, TY, 32, 1024>(a, S, st);
+    if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024, true, SUM>(a, S, st);
+    if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512, false, SUM>(a, S, st);
+    if (a.K <= 512 * 32) return launch_ep<TH, TY, 32, 512, false, SUM>(a, S, st);
+    return launch_ep<TH, TY, 32, 1024, false, SUM>(a, S, st);
+}
+template <typename TH>
+inline int launch_y(const Args &a, int S, int dtype, int y_dtype, cudaStream_t st) {
+    if (!a.y) return launch_t<TH, TH, false>(a, S, st);
+    return y_dtype == dtype ? launch_t<TH, TH, true>(a, S, st) : launch_t<TH, float, true>(a, S, st);
 }
 inline int launch(const Args &a, int S, int dtype, int y_dtype, cudaStream_t st) {
-    if (dtype == W4A8_F32) return launch_t<float, float>(a, S, st);
-    if (dtype == W4A8_F16) return y_dtype == W4A8_F32 ? launch_t<__half, float>(a, S, st) : launch_t<__half, __half>(a, S, st);
-    return y_dtype == W4A8_F32 ? launch_t<__nv_bfloat16, float>(a, S, st) : launch_t<__nv_bfloat16, __nv_bfloat16>(a, S, st);
+    if (dtype == W4A8_F32) return launch_y<float>(a, S, dtype, W4A8_F32, st);
+    return dtype == W4A8_F16 ? launch_y<__half>(a, S, dtype, y_dtype, st) : launch_y<__nv_bfloat16>(a, S, dtype, y_dtype, st);
 }
 
 }  // namespace addnorm

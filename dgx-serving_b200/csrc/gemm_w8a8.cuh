@@ -266,20 +266,21 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                 if (warp == 2 && lane < a.split && lane != rank && rows_of(lane) > 0)
                     send(remote(recv + (uint32_t)(rank * own * LANES * 4), lane), base + (uint32_t)(lane * own * LANES * 4), (uint32_t)(rows_of(lane) * LANES * 4), remote(sums_full, lane));
                 if (!ptx::mbar_wait_warp(sums_full, 0)) { dev_set_error(ERR_SUMS); break; }
+                static_assert(XR == 1);
+                const int *mine = reinterpret_cast<const int *>(smem_dyn + (base - raw)) + row, *theirs = reinterpret_cast<const int *>(smem_dyn + (recv - raw)) + row;
+                for (int j = 0; 2 * j + side < rows; j += 4) {             // every second row, four of them at a time
+                    int sum[4] = {};
+                    for (int r = 0; r < a.split; r++) {
+                        const int *from = (r == rank ? mine : theirs) + (r * own + 2 * j + side) * LANES;
 #pragma unroll
-                for (int i = 0; i < XR; i++) {                 // every second row
-#pragma unroll 4
-                    for (int j = 0; j < 32; j++) {
-                        const int c = 2 * (32 * i + j) + side;
-                        if (c >= rows) break;
-                        int sum = 0;
-                        for (int r = 0; r < a.split; r++) {
-                            int v;
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"((r == rank ? base : recv) + 4u * ((r * own + c) * LANES + row)));
-                            sum += v;
-                        }
-                        const float v = scaled(sum, __shfl_sync(0xffffffffu, x[i], j), w, b);
-                        if (live) put(y + (size_t)c * a.ldy, v);
+                        for (int q = 0; q < 4; q++)
+                            if (2 * (j + q) + side < rows) sum[q] += from[2 * q * LANES];
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int c = 2 * (j + q) + side;
+                        const float v = scaled(sum[q], __shfl_sync(0xffffffffu, x[0], j + q), w, b);
+                        if (live && c < rows) put(y + (size_t)c * a.ldy, v);
                     }
                 }
             }

@@ -22,10 +22,10 @@ inline int stages_for(const Plan &p) {
     return n > MAX_STAGES ? MAX_STAGES : n;
 }
 
-// What a plan takes, in us: a launch; for each wave of tiles the K-tiles' copies (1.47 ns a row of 128 bytes, both operands'; shared memory fills at 90 bytes a
-// ns), MMAs (pairs: 1.8 ns a row) or hand-offs (0.11 a K-tile and 0.18 a stage), whichever is most, or the outputs of the tile before; the weights from HBM;
-// and what sums between CTAs and pairs cost.  Fitted to 1900 shapes (M 1 to 3000, N 256 to 20000, K 256 to 16384), each timed behind its quantizer with some 30 to
-// 150 plans on a B200: the plan that it picks is 2.5 % slower than the best of them on average, 8 % at the 90th percentile.
+// What a plan takes, in us: a launch; for each wave of tiles the K-tiles' copies (1.5 ns a row of 128 bytes, both operands'; shared memory fills at 85 bytes a
+// ns), MMAs (pairs) or hand-offs (0.12 a K-tile and 0.16 a stage), whichever is most, or the outputs of the tile before; the weights from HBM; and what sums
+// between CTAs and pairs cost.  Fitted to 1600 shapes (M 1 to 3000, N 256 to 20000, K 256 to 16384), each timed behind its quantizer with some 30 to
+// 150 plans on a B200: the plan that it picks is 2.2 % slower than the best of them on average, 6.5 % at the 90th percentile, 25 % at most.
 struct Caps { int sms, clusters[SPLIT_MAX + 1]; };                     // clusters of n CTAs that fit the GPU at once
 inline int k_parts(int bt, int split, bool pair) {                     // fewer hand-offs, as long as three stages fit
     if (pair) return bt <= 160 ? 2 : 1;
@@ -36,11 +36,11 @@ inline float cost_of(const Plan &p, int M, int N, int K, const Caps &caps) {
     const int at_once = p.pair ? caps.clusters[2] : p.split > 1 ? caps.clusters[p.split] : caps.sms;
     if (at_once <= 0 || (p.split > 1 && tiles > at_once)) return 1e30f;
     const float waves = (float)((tiles + at_once - 1) / at_once), k_tiles = (float)ceil_div(ceil_div(K, KT), p.split);
-    const float mma = p.pair ? 1.8e-3f * (p.bt > 90 ? p.bt : 90) : 0.f, fill = 1.47e-3f * (p.pair ? LANES + p.bt / 2 : p.bw + p.bt), hand = 0.112f + 0.18f / p.kp;
+    const float mma = p.pair ? 0.134f + 1.23e-3f * p.bt : 0.f, fill = 1.5e-3f * (p.pair ? LANES + p.bt / 2 : p.bw + p.bt), hand = 0.124f + 0.156f / p.kp;
     const float per = k_tiles * (mma > fill ? (mma > hand ? mma : hand) : fill > hand ? fill : hand);
-    const float out = 0.0128f * p.bt * (p.pair ? 1.38f : 1.f) + 1.06f;
-    const float body = (waves - 1.f) * (per > out ? per : out) + per + out, mem = (float)N * (float)K / 12.1e6f;
-    return 2.5f + (body > mem ? body + 0.35f * mem : mem + 0.35f * body) + (p.split > 1 ? 0.37f + 0.049f * p.bt : 0.f) + (p.pair ? 0.5f : 0.f);
+    const float out = 0.0123f * p.bt * (p.pair ? 1.39f : 1.f) + 1.19f;
+    const float body = (waves - 1.f) * (per > out ? per : out) + per + out, mem = (float)N * (float)K / 16.1e6f;
+    return 2.4f + (body > mem ? body + 0.35f * mem : mem + 0.35f * body) + (p.split > 1 ? 0.53f + 0.029f * p.bt : 0.f) + (p.pair ? 0.5f : 0.f);
 }
 inline Plan plan_for(int M, int N, int K, const Caps &caps) {
     Plan best = {LANES, 256, 1, 1, 0, caps.sms};
@@ -60,7 +60,7 @@ inline Plan plan_for(int M, int N, int K, const Caps &caps) {
         last = bt;
         for (int bw = 64; bw <= LANES; bw += 32) {
             try_plan({bw, bt, 1, 0, 0, 0});
-            for (int split = 2; split <= SPLIT_MAX; split += split < 4 ? 1 : 2)
+            for (int split = 2; split <= SPLIT_MAX; split *= 2)         // (with threes and sixes the best plans are 0.2 % faster on average)
                 if (bt <= SPLIT_BT && nkt / split >= 2) try_plan({bw, bt, split, 0, 0, 0});
         }
         try_plan({2 * LANES, ceil_div(bt, 32) * 32, 1, 0, 1, 0});
