@@ -239,6 +239,13 @@ def _binding():
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
         loader.exec_module(module)
         module.bind(*[ctypes.cast(getattr(lib(), "w4a8_" + n), ctypes.c_void_p).value for n in _NATIVE_ENTRIES])
+        import torch
+        device, raw = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if device is None or raw is None:
+            device, raw = torch.cuda.current_device, lambda d: torch.cuda.current_stream(d).cuda_stream
+        if torch.cuda.is_available():
+            torch.cuda.init()                                         # the two functions above expect it
+        module.streams(device, raw)
         _native = module
     return _native
 
@@ -438,7 +445,7 @@ def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=No
     """h' = h + norm(y) * gate * alpha of S rows, to H_out, and its norm n, to N and / or quantized to xq, xs, xsum (w4a8_add_norm).  Y None: h' = h.
     group 32: blocks of 32 elements, 0: one scale for a row.  Pitches of 0: K."""
     K = norm.K
-    rc = (_native or _binding()).add_norm(norm, H, ldh or K, Y, ldy or K, H_out, ldo or K, N, ldn or K, xq, xs, xsum, group, S, _stream(stream))
+    rc = (_native or _binding()).add_norm(norm, H, ldh or K, Y, ldy or K, H_out, ldo or K, N, ldn or K, xq, xs, xsum, group, S, stream)
     if rc:
         _check(rc)
 
@@ -449,35 +456,35 @@ def launch_rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out=No
         Q_out, ldqo = Q, ldq
     if K_out is None:
         K_out, ldko = K, ldk
-    rc = (_native or _binding()).rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out, ldqo, K_out, ldko, DTYPES.get(dtype, dtype), _stream(stream))
+    rc = (_native or _binding()).rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out, ldqo, K_out, ldko, DTYPES.get(dtype, dtype), stream)
     if rc:
         _check(rc)
 
 
 def launch_moe_route(router, logits, ld, S, idx, weight, dtype="fp32", stream=None):
     """The experts idx[S][topk] of S tokens and their weights, from logits[S][experts] (w4a8_moe_route): what moe_block takes."""
-    rc = (_native or _binding()).moe_route(router, logits, ld, S, DTYPES.get(dtype, dtype), idx, weight, _stream(stream))
+    rc = (_native or _binding()).moe_route(router, logits, ld, S, DTYPES.get(dtype, dtype), idx, weight, stream)
     if rc:
         _check(rc)
 
 
 def launch_quantize_rows_q8(X, ldx, S, K, xq, xs, dtype="fp32", stream=None):
     """Rows to int8 with one scale each (w4a8_quantize_rows_q8): activations of the 8-bit products, or their weights, a channel per row."""
-    rc = (_native or _binding()).quantize_rows_q8(X, ldx, S, K, DTYPES.get(dtype, dtype), xq, xs, _stream(stream))
+    rc = (_native or _binding()).quantize_rows_q8(X, ldx, S, K, DTYPES.get(dtype, dtype), xq, xs, stream)
     if rc:
         _check(rc)
 
 
 def launch_gemm_w8a8(xq, xs, wq, ws, Y, ldy, M, N, K, dtype="fp32", bias=None, stream=None):
     """Y[M][N] = xq wq^T * xs[m] * ws[n] + bias[n], the sums exact (w4a8_gemm_w8a8)."""
-    rc = (_native or _binding()).gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, M, N, K, DTYPES.get(dtype, dtype), _stream(stream))
+    rc = (_native or _binding()).gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, M, N, K, DTYPES.get(dtype, dtype), stream)
     if rc:
         _check(rc)
 
 
 def linear_w8a8(X, ldx, xq, xs, wq, ws, Y, ldy, S, N, K, x_dtype="fp32", y_dtype="fp32", bias=None, skip_quantize=0, stream=None):
     """linear() for 8-bit weights with a scale for each output channel (w4a8_linear_w8a8)."""
-    rc = (_native or _binding()).linear_w8a8(X, ldx, xq, xs, wq, ws, bias, Y, ldy, S, N, K, DTYPES.get(x_dtype, x_dtype), DTYPES.get(y_dtype, y_dtype), skip_quantize, _stream(stream))
+    rc = (_native or _binding()).linear_w8a8(X, ldx, xq, xs, wq, ws, bias, Y, ldy, S, N, K, DTYPES.get(x_dtype, x_dtype), DTYPES.get(y_dtype, y_dtype), skip_quantize, stream)
     if rc:
         _check(rc)
 

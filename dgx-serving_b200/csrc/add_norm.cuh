@@ -236,6 +236,7 @@ inline int launch_ep(const Args &a, int S, cudaStream_t st) {
 template <typename TH, typename TY, bool SUM>
 inline int launch_t(const Args &a, int S, cudaStream_t st) {
     if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024, true, SUM>(a, S, st);
+    if (!SUM && a.K <= 1024 * 16 && S <= sm_count()) return launch_ep<TH, TY, 16, 1024, false, SUM>(a, S, st);
     if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512, false, SUM>(a, S, st);
     if (a.K <= 512 * 32) return launch_ep<TH, TY, 32, 512, false, SUM>(a, S, st);
     return launch_ep<TH, TY, 32, 1024, false, SUM>(a, S, st);

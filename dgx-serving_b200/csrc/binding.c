@@ -1,13 +1,15 @@
 /* The layer operators for Python without ctypes: a call costs about 0.5 us in place of 3, which is what a decode step's smallest operators
  * take on the GPU.  The functions are the C ABI's (include/w4a8_b200.h), found in the library that the package has loaded (bind); arguments in its order.  A
- * pointer is a number, None, or a tensor (its data_ptr()); a struct is a ctypes Structure.  Each returns the status code. */
+ * pointer is a number, None, or a tensor (its data_ptr()); a struct is a ctypes Structure; a stream is a number, an object with a cuda_stream, or None: what
+ * the two functions given to streams() say is torch's current one.  Each returns the status code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <limits.h>
 typedef struct w4a8_arena w4a8_arena;
 #include "../../include/w4a8_b200.h"
 
-static PyObject *data_ptr_name;
+static PyObject *data_ptr_name, *cuda_stream_name;
+static PyObject *current_device, *current_stream;         /* of torch: device(), raw stream(device) */
 
 /* Each conversion does nothing once one before it has failed. */
 static void *as_pointer(PyObject *o, int *ok) {
@@ -18,6 +20,25 @@ static void *as_pointer(PyObject *o, int *ok) {
         return p;
     }
     PyObject *n = PyObject_CallMethodNoArgs(o, data_ptr_name);
+    if (!n) { *ok = 0; return NULL; }
+    void *p = PyLong_AsVoidPtr(n);
+    if (!p && PyErr_Occurred()) *ok = 0;
+    Py_DECREF(n);
+    return p;
+}
+static void *as_stream(PyObject *o, int *ok) {
+    if (!*ok) return NULL;
+    if (PyLong_Check(o)) return as_pointer(o, ok);
+    PyObject *n = NULL;
+    if (o != Py_None) n = PyObject_GetAttr(o, cuda_stream_name);
+    else if (!current_stream) PyErr_SetString(PyExc_RuntimeError, "no current stream: streams() has not been called");
+    else {
+        PyObject *device = PyObject_CallNoArgs(current_device);
+        if (device) {
+            n = PyObject_CallOneArg(current_stream, device);
+            Py_DECREF(device);
+        }
+    }
     if (!n) { *ok = 0; return NULL; }
     void *p = PyLong_AsVoidPtr(n);
     if (!p && PyErr_Occurred()) *ok = 0;
@@ -80,27 +101,27 @@ static __typeof__(&w4a8_linear_w8a8) f_linear_w8a8;
 ENTRY(add_norm, 15)
         const w4a8_norm *norm = as_struct(a[0], sizeof(w4a8_norm), &ok); const void *h = P(1); const int64_t ldh = L(2); const void *y = P(3); const int64_t ldy = L(4);
         void *ho = P(5); const int64_t ldo = L(6); void *no = P(7); const int64_t ldn = L(8); int8_t *xq = P(9); float *xs = P(10); int32_t *xsum = P(11);
-        const int group = I(12), S = I(13); void *stream = P(14);
+        const int group = I(12), S = I(13); void *stream = as_stream(a[14], &ok);
     CALL(add_norm, norm, h, ldh, y, ldy, ho, ldo, no, ldn, xq, xs, xsum, group, S, stream)
 ENTRY(rope_qk, 15)
         const w4a8_rope *rope = as_struct(a[0], sizeof(w4a8_rope), &ok); const void *q = P(1); const int64_t ldq = L(2); const int hq = I(3); const void *k = P(4);
         const int64_t ldk = L(5); const int hk = I(6); const int32_t *position = P(7); const int T = I(8); void *qo = P(9); const int64_t ldqo = L(10); void *ko = P(11);
-        const int64_t ldko = L(12); const int dtype = I(13); void *stream = P(14);
+        const int64_t ldko = L(12); const int dtype = I(13); void *stream = as_stream(a[14], &ok);
     CALL(rope_qk, rope, q, ldq, hq, k, ldk, hk, position, T, qo, ldqo, ko, ldko, dtype, stream)
 ENTRY(moe_route, 8)
         const w4a8_router *router = as_struct(a[0], sizeof(w4a8_router), &ok); const void *logits = P(1); const int64_t ld = L(2); const int S = I(3), dtype = I(4);
-        int32_t *idx = P(5); float *weight = P(6); void *stream = P(7);
+        int32_t *idx = P(5); float *weight = P(6); void *stream = as_stream(a[7], &ok);
     CALL(moe_route, router, logits, ld, S, dtype, idx, weight, stream)
 ENTRY(quantize_rows_q8, 8)
-        const void *x = P(0); const int64_t ldx = L(1); const int S = I(2), K = I(3), dtype = I(4); int8_t *xq = P(5); float *xs = P(6); void *stream = P(7);
+        const void *x = P(0); const int64_t ldx = L(1); const int S = I(2), K = I(3), dtype = I(4); int8_t *xq = P(5); float *xs = P(6); void *stream = as_stream(a[7], &ok);
     CALL(quantize_rows_q8, x, ldx, S, K, dtype, xq, xs, stream)
 ENTRY(gemm_w8a8, 12)
         const int8_t *xq = P(0); const float *xs = P(1); const int8_t *wq = P(2); const float *ws = P(3); const float *bias = P(4); void *Y = P(5); const int64_t ldy = L(6);
-        const int M = I(7), N = I(8), K = I(9), dtype = I(10); void *stream = P(11);
+        const int M = I(7), N = I(8), K = I(9), dtype = I(10); void *stream = as_stream(a[11], &ok);
     CALL(gemm_w8a8, xq, xs, wq, ws, bias, Y, ldy, M, N, K, dtype, stream)
 ENTRY(linear_w8a8, 16)
         const void *x = P(0); const int64_t ldx = L(1); int8_t *xq = P(2); float *xs = P(3); const int8_t *wq = P(4); const float *ws = P(5); const float *bias = P(6);
-        void *Y = P(7); const int64_t ldy = L(8); const int S = I(9), N = I(10), K = I(11), xd = I(12), yd = I(13), skip = I(14); void *stream = P(15);
+        void *Y = P(7); const int64_t ldy = L(8); const int S = I(9), N = I(10), K = I(11), xd = I(12), yd = I(13), skip = I(14); void *stream = as_stream(a[15], &ok);
     CALL(linear_w8a8, x, ldx, xq, xs, wq, ws, bias, Y, ldy, S, N, K, xd, yd, skip, stream)
 
 /* bind(addresses of the six functions, in the order of the table below) */
@@ -119,10 +140,21 @@ static PyObject *bind(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+/* streams(device(), stream(device)) */
+static PyObject *streams(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+    if (!count(n, 2)) return NULL;
+    Py_INCREF(a[0]);
+    Py_INCREF(a[1]);
+    Py_XSETREF(current_device, a[0]);
+    Py_XSETREF(current_stream, a[1]);
+    Py_RETURN_NONE;
+}
+
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, NULL}
-static PyMethodDef methods[] = {METHOD(bind), METHOD(add_norm), METHOD(rope_qk), METHOD(moe_route), METHOD(quantize_rows_q8), METHOD(gemm_w8a8), METHOD(linear_w8a8), {NULL, NULL, 0, NULL}};
+static PyMethodDef methods[] = {METHOD(bind), METHOD(streams), METHOD(add_norm), METHOD(rope_qk), METHOD(moe_route), METHOD(quantize_rows_q8), METHOD(gemm_w8a8), METHOD(linear_w8a8), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", NULL, -1, methods};
 PyMODINIT_FUNC PyInit__binding(void) {
     data_ptr_name = PyUnicode_InternFromString("data_ptr");
-    return data_ptr_name ? PyModule_Create(&module) : NULL;
+    cuda_stream_name = PyUnicode_InternFromString("cuda_stream");
+    return data_ptr_name && cuda_stream_name ? PyModule_Create(&module) : NULL;
 }

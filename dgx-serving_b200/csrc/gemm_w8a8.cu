@@ -16,14 +16,15 @@ cudaError_t w8a8_take_device_error(unsigned int *v) {
 
 using namespace w4a8;
 
-W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy, int M, int N, int K,
-                            int dtype, void *stream) {
-    const char *who = "gemm_w8a8";
+// What a product's arguments have to be; *empty: there is nothing to do.
+static int check_product(const char *who, const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, const void *Y, int64_t ldy, int M, int N, int K,
+                         int dtype, bool *empty) {
     const size_t size = row_size(dtype);
     if (!size) return fail(W4A8_ERR_ARG, "%s: dtype=%d (0 fp32, 1 fp16, 2 bf16)", who, dtype);
     if (M < 0 || N < 0 || K < 0 || K % QBLK != 0) return fail(W4A8_ERR_ARG, "%s: M=%d N=%d K=%d (K must be a multiple of %d)", who, M, N, K, QBLK);
     if (K > w8a8::MAX_K) return fail(W4A8_ERR_UNSUPPORTED, "%s: K=%d (at most %d: sums have to fit 32 bits)", who, K, w8a8::MAX_K);
-    if (M == 0 || N == 0) return W4A8_OK;
+    *empty = M == 0 || N == 0;
+    if (*empty) return W4A8_OK;
     if (K == 0) return fail(W4A8_ERR_ARG, "%s: K=0", who);
     if (!xq || !xs || !wq || !ws || !Y) return fail(W4A8_ERR_ARG, "%s: null pointer argument", who);
     if (ldy < N) return fail(W4A8_ERR_ARG, "%s: Y has rows of %d elements, a pitch of %lld", who, N, (long long)ldy);
@@ -33,8 +34,14 @@ W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq,
     static const char *const names[] = {"xq", "xs", "wq", "ws", "bias"};
     for (int i = 0; i < 5; i++)
         if (rows_overlap(y, in[i])) return fail(W4A8_ERR_ARG, "%s: Y overlaps %s", who, names[i]);
-    int rc = require_sm100();
-    if (rc != W4A8_OK) return rc;
+    return W4A8_OK;
+}
+
+W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy, int M, int N, int K,
+                            int dtype, void *stream) {
+    bool empty;
+    int rc = check_product("gemm_w8a8", xq, xs, wq, ws, bias, Y, ldy, M, N, K, dtype, &empty);
+    if (rc != W4A8_OK || empty || (rc = require_sm100()) != W4A8_OK) return rc;
     w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0, 0, 0};
     w8a8::Plan plan;
     if ((rc = w8a8::plan_cached(M, N, K, &plan)) != W4A8_OK) return rc;
@@ -43,11 +50,10 @@ W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq,
 
 W4A8_API int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy,
                               int S, int N, int K, int x_dtype, int y_dtype, int skip_quantize, void *stream) {
-    if (S < 0 || N < 0) return fail(W4A8_ERR_ARG, "linear_w8a8: negative size S=%d N=%d", S, N);
-    if (S == 0 || N == 0) return W4A8_OK;
-    if (!skip_quantize) {
-        const int rc = w4a8_quantize_rows_q8(x, ldx, S, K, x_dtype, xq, xs, stream);
-        if (rc != W4A8_OK) return rc;
-    }
+    if (S > 0 && N > 0 && !skip_quantize && !x) return fail(W4A8_ERR_ARG, "linear_w8a8: null pointer argument");
+    bool empty;
+    int rc = check_product("linear_w8a8", xq, xs, wq, ws, bias, Y, ldy, S, N, K, y_dtype, &empty);      // before the first of the two launches
+    if (rc != W4A8_OK || empty) return rc;
+    if (!skip_quantize && (rc = w4a8_quantize_rows_q8(x, ldx, S, K, x_dtype, xq, xs, stream)) != W4A8_OK) return rc;
     return w4a8_gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, S, N, K, y_dtype, stream);
 }
