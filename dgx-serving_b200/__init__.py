@@ -78,6 +78,8 @@ class Norm(ctypes.Structure):
     _fields_ = [("weight", ctypes.c_void_p), ("post_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("gate_ld", ctypes.c_int64), ("eps", ctypes.c_double),
                 ("alpha", ctypes.c_float), ("K", ctypes.c_int), ("variant", ctypes.c_int), ("post_variant", ctypes.c_int), ("dtype", ctypes.c_int), ("y_dtype", ctypes.c_int)]
 
+    _gate_rows = 1 << 63
+
     @classmethod
     def of(cls, K, weight=None, variant=0, eps=1e-6, post_weight=None, post_variant=-1, gate=None, alpha=1.0, dtype="fp32", y_dtype=None):
         """weight, post_weight: fp32 [K] tensors, which the object keeps alive.  gate: fp32 [K], or [S][K] with a row for each token.  variant -1: no norm,
@@ -85,6 +87,8 @@ class Norm(ctypes.Structure):
         _fp32_vector(weight, K, "weight")
         _fp32_vector(post_weight, K, "post_weight")
         gate_ld = 0
+        if gate is not None and gate.dim() == 2 and gate.shape[0] == 1:
+            gate = gate[0]
         if gate is not None:
             if str(gate.dtype) != "torch.float32" or not gate.is_cuda or gate.dim() not in (1, 2) or gate.shape[-1] != K or (K > 1 and gate.stride(-1) != 1):
                 raise ValueError("gate: fp32 [%d] or [rows][%d] on a GPU" % (K, K))
@@ -93,6 +97,8 @@ class Norm(ctypes.Structure):
                 raise ValueError("gate: rows that overlap")
         n = cls(_ptr(weight), _ptr(post_weight), _ptr(gate), gate_ld, float(eps), float(alpha), K, variant, post_variant, DTYPES[dtype], DTYPES[dtype if y_dtype is None else y_dtype])
         n._tensors = (weight, post_weight, gate)
+        if gate_ld:
+            n._gate_rows = gate.shape[0]
         return n
 
 
@@ -445,6 +451,8 @@ def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=No
     """h' = h + norm(y) * gate * alpha of S rows, to H_out, and its norm n, to N and / or quantized to xq, xs, xsum (w4a8_add_norm).  Y None: h' = h.
     group 32: blocks of 32 elements, 0: one scale for a row.  Pitches of 0: K."""
     K = norm.K
+    if S > norm._gate_rows:
+        raise ValueError("%d rows, a gate of %d" % (S, norm._gate_rows))
     rc = (_native or _binding()).add_norm(norm, H, ldh or K, Y, ldy or K, H_out, ldo or K, N, ldn or K, xq, xs, xsum, group, S, stream)
     if rc:
         _check(rc)

@@ -23,6 +23,7 @@ static int check_product(const char *who, const int8_t *xq, const float *xs, con
     if (!size) return fail(W4A8_ERR_ARG, "%s: dtype=%d (0 fp32, 1 fp16, 2 bf16)", who, dtype);
     if (M < 0 || N < 0 || K < 0 || K % QBLK != 0) return fail(W4A8_ERR_ARG, "%s: M=%d N=%d K=%d (K must be a multiple of %d)", who, M, N, K, QBLK);
     if (K > w8a8::MAX_K) return fail(W4A8_ERR_UNSUPPORTED, "%s: K=%d (at most %d: sums have to fit 32 bits)", who, K, w8a8::MAX_K);
+    if (M > w8a8::MAX_ROWS || N > w8a8::MAX_ROWS) return fail(W4A8_ERR_UNSUPPORTED, "%s: M=%d N=%d (at most %d: places in the last tiles are counted in 31 bits)", who, M, N, w8a8::MAX_ROWS);
     *empty = M == 0 || N == 0;
     if (*empty) return W4A8_OK;
     if (K == 0) return fail(W4A8_ERR_ARG, "%s: K=0", who);

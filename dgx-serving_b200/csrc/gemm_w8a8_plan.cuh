@@ -4,7 +4,7 @@
 namespace w4a8 {
 namespace w8a8 {
 
-constexpr int MAX_K = 131040;
+constexpr int MAX_K = 131040, MAX_ROWS = 0x7fffffff - 1023;
 constexpr int LANES = 128, KT = 128;           // channels of an MMA; bytes of K in a row of a swizzled tile
 constexpr int A_STAGE = LANES * KT;
 constexpr int MAX_STAGES = 12, EPI_WARPS = 8, THREADS = (2 + EPI_WARPS) * 32;

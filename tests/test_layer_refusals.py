@@ -108,6 +108,7 @@ def test_gemm_w8a8(w4a8):
                  dict(Y=BASE << 1), dict(bias=(BASE << 4) + 4)):
         assert call(**args) == A, args
     assert call(K=131072) == w4a8.ERR_UNSUPPORTED
+    assert call(M=2 ** 31 - 1023) == w4a8.ERR_UNSUPPORTED and call(N=2 ** 31 - 1, ldy=2 ** 31) == w4a8.ERR_UNSUPPORTED
     for args in (dict(xq=BASE + 8), dict(wq=(BASE << 2) + 4), dict(Y=(BASE << 4) + 2)):
         assert call(**args) == w4a8.ERR_ALIGN, args
     assert call(M=0, xq=None) == w4a8.OK and call(N=0, ldy=0, Y=None) == w4a8.OK
@@ -154,5 +155,9 @@ def test_the_binding_without_ctypes(w4a8):
         w4a8.launch_add_norm(norm_of(w4a8), "h", t, 4, N=t, stream=0)
     with pytest.raises(TypeError, match="a struct of"):
         w4a8._binding().add_norm(w4a8.Rope(), t, 64, t, 64, None, 64, t, 64, None, None, None, 32, 4, 0)
+    n = norm_of(w4a8)
+    n._gate_rows = 3                                         # what Norm.of notes of a gate with a row for each token
+    with pytest.raises(ValueError, match="4 rows, a gate of 3"):
+        w4a8.launch_add_norm(n, t, t, 4, N=t, stream=0)
     with pytest.raises(TypeError, match="15 expected"):
         w4a8._binding().add_norm(norm_of(w4a8), t)

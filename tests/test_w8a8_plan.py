@@ -13,8 +13,8 @@ int main() {
     int bad = 0, kinds[3] = {};
     const Caps whole = {148, {0, 0, 74, 45, 33, 0, 22, 0, 15}}, small = {132, {0, 0, 60, 0, 14, 0, 0, 0, 3}};
     for (const Caps &caps : {whole, small})
-        for (int M : {1, 2, 15, 16, 17, 31, 33, 48, 49, 64, 65, 100, 128, 129, 200, 255, 256, 257, 300, 333, 512, 777, 1000, 2048, 5000, 100000, 2147483647})
-            for (int N : {1, 5, 63, 64, 65, 127, 128, 129, 255, 300, 1024, 3840, 4091, 6144, 17408, 151936, 2147483647})
+        for (int M : {1, 2, 15, 16, 17, 31, 33, 48, 49, 64, 65, 100, 128, 129, 200, 255, 256, 257, 300, 333, 512, 777, 1000, 2048, 5000, 100000, MAX_ROWS})
+            for (int N : {1, 5, 63, 64, 65, 127, 128, 129, 255, 300, 1024, 3840, 4091, 6144, 17408, 151936, MAX_ROWS})
                 for (int K : {32, 96, 128, 160, 256, 512, 1056, 4096, 5120, 15360, 32768, 131040}) {
                     const Plan p = plan_for(M, N, K, caps);
                     const long tiles = (long)ceil_div(N, p.bw) * ceil_div(M, p.bt);
