@@ -28,18 +28,21 @@ struct Args {
 
 // A group of LPH lanes has a head, a lane two runs of V of its elements, at `ia` and `ib`: V whole pairs where the head is rotated (i and
 // i + rotary / 2 in one lane) and neighbours elsewhere.  A run is 16 bytes (V 4 of fp32, 8 of 16 bits; 4 there too where rotary / 2 is no
-// multiple of 8, or dim none of 16).  A CTA has one token's heads, so that cosines and sines are computed once for all of them.
+// multiple of 8, dim none of 16, or weights come with it).  A CTA has one token's heads, so that cosines and sines are computed once for all of them.
 //
 // Many tokens: bytes in flight are the bound, since each CTA waits for its position, then its rows, then stores.  Rows are asked for at once, before the
-// position is known, BATCH heads a lane.  8000 tokens of 40 heads of 128 in bf16, half of them turned: see launch_l.
-constexpr int THREADS = 128;
+// position is known, BATCH heads a lane.  8000 tokens of 40 heads of 128 in bf16, half of them turned, 28 us: 5.8 TB/s; rows held widened while in
+// flight, and so fewer CTAs, 46.
+// Threads of a CTA: 40 heads divide into groups of eight and not of sixteen, and smaller CTAs wait for less at their barrier (8000 tokens in bf16, 128 threads / 64: 29.3 / 28.0 us,
+// with norms 38.6 / 36.4); fp32 rows, whose loads fill the registers, lose by it (52.2 / 55.1).
+template <typename T> constexpr int CTA = sizeof(T) == 4 ? 128 : 64;
 
 template <typename T, int V, int LPH, int BATCH>                         // BATCH heads' loads of a lane in flight
-__global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
+__global__ void __launch_bounds__(CTA<T>) rope_kernel(const Args a) {
     __shared__ float2 turn[MAX_DIM / 2];
     const int t = blockIdx.x, half = a.rotary / 2;
     const int group = threadIdx.x / LPH, j = threadIdx.x % LPH;
-    constexpr int GROUPS = THREADS / LPH;
+    constexpr int THREADS = CTA<T>, GROUPS = THREADS / LPH;
     const bool turned = 2 * V * j < a.rotary, live = 2 * V * j < a.dim;
     const int ia = turned && !a.interleaved ? V * j : 2 * V * j, ib = turned && !a.interleaved ? V * j + half : 2 * V * j + V;
     const int first = blockIdx.y * a.per_cta, last = min(first + a.per_cta, a.heads);
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
 
 template <typename T, int V, int LPH>
 inline int launch_l(Args a, int T_rows, cudaStream_t st) {
-    constexpr int GROUPS = THREADS / LPH;
+    constexpr int THREADS = CTA<T>, GROUPS = THREADS / LPH;
     // a CTA takes one head a group while that leaves SMs idle, up to all of a token's heads where there are tokens enough for every SM
     const int passes = (a.heads + GROUPS - 1) / GROUPS;
     int per = 1;
@@ -157,7 +160,10 @@ inline int launch_v(const Args &a, int T_rows, cudaStream_t st) {
 }
 template <typename T>
 inline int launch_16(const Args &a, int T_rows, cudaStream_t st) {
-    return a.dim % 16 == 0 && a.rotary % 16 == 0 ? launch_v<T, 8>(a, T_rows, st) : launch_v<T, 4>(a, T_rows, st);
+    // Runs of 8 where pairs and heads allow, but with weights, which are read for each head and twice as wide as the elements, 4: 8000 tokens of 40 heads of 128
+    // with weighted norms 43.9 us in runs of 8, 38.7 in runs of 4 (interleaved 57.4 and 41.1); without weights 36.0 and more.
+    const bool weighted = a.variant == W4A8_NORM_SCALE || a.variant == W4A8_NORM_ONE_PLUS;
+    return a.dim % 16 == 0 && a.rotary % 16 == 0 && !weighted ? launch_v<T, 8>(a, T_rows, st) : launch_v<T, 4>(a, T_rows, st);
 }
 inline int launch(const Args &a, int T_rows, int dtype, cudaStream_t st) {
     if (dtype == W4A8_F32) return launch_v<float, 4>(a, T_rows, st);
