@@ -43,7 +43,7 @@ W4A8_API int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq,
     bool empty;
     int rc = check_product("gemm_w8a8", xq, xs, wq, ws, bias, Y, ldy, M, N, K, dtype, &empty);
     if (rc != W4A8_OK || empty || (rc = require_sm100()) != W4A8_OK) return rc;
-    w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K, 0, 0, 0, 0, 0, 0, 0, 0};
+    w8a8::Args a = {xs, ws, bias, Y, ldy, M, N, K};
     w8a8::Plan plan;
     if ((rc = w8a8::plan_cached(M, N, K, &plan)) != W4A8_OK) return rc;
     return w8a8::launch(xq, wq, a, plan, dtype, (cudaStream_t)stream);
@@ -55,6 +55,19 @@ W4A8_API int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs,
     bool empty;
     int rc = check_product("linear_w8a8", xq, xs, wq, ws, bias, Y, ldy, S, N, K, y_dtype, &empty);      // before the first of the two launches
     if (rc != W4A8_OK || empty) return rc;
-    if (!skip_quantize && (rc = w4a8_quantize_rows_q8(x, ldx, S, K, x_dtype, xq, xs, stream)) != W4A8_OK) return rc;
+    if (!skip_quantize) {
+        const size_t size = row_size(x_dtype);
+        w8a8::Plan plan;
+        const Rows in = {x, ldx, K, S, size}, codes = {xq, K, K, S, 1}, scales = {xs, S, S, 1, 4}, y = {Y, ldy, N, S, row_size(y_dtype)};
+        // a row or two by the product itself (what is not right with x is the quantizer's to say; an output in x's place needs x read first)
+        if (S <= w8a8::ROWS_MAX && size && K <= 32768 && ldx >= K && aligned(x, 16) && ldx * size % 16 == 0 && !rows_overlap(y, in) && !rows_overlap(codes, in) &&
+            !rows_overlap(scales, in) && !rows_overlap(scales, codes) && (rc = require_sm100()) == W4A8_OK && (rc = w8a8::plan_cached(S, N, K, &plan)) == W4A8_OK &&
+            w8a8::row_plan(plan, S, K)) {
+            w8a8::Args a = {xs, ws, bias, Y, ldy, S, N, K};
+            a.x = x; a.ldx = ldx; a.x_dtype = x_dtype; a.xq_out = xq; a.xs_out = xs;
+            return w8a8::launch(xq, wq, a, plan, y_dtype, (cudaStream_t)stream);
+        }
+        if (rc != W4A8_OK || (rc = w4a8_quantize_rows_q8(x, ldx, S, K, x_dtype, xq, xs, stream)) != W4A8_OK) return rc;
+    }
     return w4a8_gemm_w8a8(xq, xs, wq, ws, bias, Y, ldy, S, N, K, y_dtype, stream);
 }

@@ -11,6 +11,10 @@
 // first CTA issuing the MMAs of both.  A byte in shared memory then serves twice the products: what fills shared memory bounds these products, and
 // under the power cap what it costs to move.
 //
+// A row or two (ROWS) are quantized where they are used: every CTA takes the row's largest magnitude and writes its own part of K into the shared memory that the
+// MMA reads, while the weights are on their way.  That saves the quantizer's launch, in which HBM is idle, and costs a read of the row from L2 for each SM
+// (row_plan has what both take).
+//
 // One CTA per SM, warp-specialised: warp 0 starts copies, warp 1 the MMAs, warps 2 to 9 convert, scale and store one tile while the next one
 // accumulates in the other half of TMEM.  Where there are fewer tiles than SMs, the CTAs of a cluster share a tile's K (`split` of them), send
 // their int32 sums to the CTA that owns the columns through distributed shared memory, and that one adds them: no workspace, no second
@@ -33,6 +37,11 @@ struct Args {
     void *y;
     int64_t ldy;
     int M, N, K, bw, bt, kp, stages, split, t_tiles, tiles, tmem_cols;
+    const void *x;                             // ROWS: rows to quantize, their type, and where codes and scales go besides
+    int64_t ldx;
+    int8_t *xq_out;
+    float *xs_out;
+    int x_dtype;
 };
 
 // The slot of a ring, and how often it came round.
@@ -92,19 +101,27 @@ __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Eight elements of a row of any type.
+__device__ __forceinline__ void load8(const void *row, int64_t at, int dtype, float (&v)[8]) {
+    if (dtype == W4A8_F32) load_row<float, 8>(static_cast<const float *>(row) + at, v);
+    else if (dtype == W4A8_F16) load_row<__half, 8>(static_cast<const __half *>(row) + at, v);
+    else load_row<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16 *>(row) + at, v);
+}
+
 enum Mode { ONE, SPLIT, PAIR };                // a tile is one CTA's; several share its K; two share its channels
 
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool ROWS>
 __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Args a) {
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t raw = ptx::smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
-    const uint32_t x_rows = MODE == PAIR ? a.bt / 2 : a.bt, part_bytes = A_STAGE + x_rows * KT, stage_bytes = part_bytes * a.kp;
-    const uint32_t bars = base + (uint32_t)a.stages * stage_bytes, recv = bars + 512;
+    const uint32_t x_rows = MODE == PAIR ? a.bt / 2 : a.bt, part_bytes = A_STAGE + (ROWS ? 0 : x_rows * KT), stage_bytes = part_bytes * a.kp;
+    const uint32_t bars = base + (uint32_t)a.stages * stage_bytes, recv = bars + 512, x_at = recv + (MODE == SPLIT ? (uint32_t)(a.split * ((a.bt + a.split - 1) / a.split) * LANES * 4) : 0u) + 512;   // (x_at: a multiple of 1024)
     const auto FULL = [&](int s) { return bars + 8u * s; };
     const auto EMPTY = [&](int s) { return bars + 8u * (MAX_STAGES + s); };
     const auto T_FULL = [&](int s) { return bars + 8u * (2 * MAX_STAGES + s); };
     const auto T_EMPTY = [&](int s) { return bars + 8u * (2 * MAX_STAGES + 2 + s); };
-    const uint32_t sums_full = bars + 8u * (2 * MAX_STAGES + 4), slot_addr = bars + 8u * (2 * MAX_STAGES + 5);
+    const uint32_t sums_full = bars + 8u * (2 * MAX_STAGES + 4), slot_addr = bars + 8u * (2 * MAX_STAGES + 5), x_full = bars + 8u * (2 * MAX_STAGES + 6);
+    float *row_max = reinterpret_cast<float *>(smem_dyn + (bars - raw) + 256), *row_scale = row_max + EPI_WARPS;       // ROWS
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = MODE == ONE ? 0 : blockIdx.x % a.split;   // in the cluster
     const int nkt = (a.K + KT - 1) / KT;
@@ -118,6 +135,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; i++) { ptx::mbar_init(FULL(i), 1); ptx::mbar_init(EMPTY(i), 1); }
         for (int i = 0; i < 2; i++) { ptx::mbar_init(T_FULL(i), 1); ptx::mbar_init(T_EMPTY(i), MODE == PAIR ? 2 * EPI_WARPS : EPI_WARPS); }
+        if constexpr (ROWS) ptx::mbar_init(x_full, EPI_WARPS * 32);
         if constexpr (MODE == SPLIT) {
             ptx::mbar_init(sums_full, 1);
             ptx::mbar_arrive_expect_tx(sums_full, (uint32_t)((a.split - 1) * rows_of(rank) * LANES * 4));
@@ -157,14 +175,14 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                 const int parts = min(a.kp, k_hi - kt);
                 uint32_t at = base + ring.slot * stage_bytes;
                 const uint32_t bar = MODE == PAIR ? remote(FULL(ring.slot), 0) : FULL(ring.slot);      // a pair's bytes count where its MMAs are issued
-                if (MODE != PAIR || rank == 0) ptx::mbar_arrive_expect_tx(lead, FULL(ring.slot), (uint32_t)(a.bw + a.bt) * KT * parts);
+                if (MODE != PAIR || rank == 0) ptx::mbar_arrive_expect_tx(lead, FULL(ring.slot), (uint32_t)(a.bw + (ROWS ? 0 : a.bt)) * KT * parts);
                 for (int p = 0; p < parts; p++, at += part_bytes) {
                     if constexpr (MODE == PAIR) {
                         tma_load_2d_pair(lead, at, &tmW, (kt + p) * KT, w_row, bar);
                         tma_load_2d_pair(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
                     } else {
                         ptx::tma_load_2d(lead, at, &tmW, (kt + p) * KT, w_row, bar);
-                        ptx::tma_load_2d(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
+                        if constexpr (!ROWS) ptx::tma_load_2d(lead, at + A_STAGE, &tmX, (kt + p) * KT, x_row, bar);
                     }
                 }
                 ring.next(a.stages);
@@ -181,6 +199,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
         const uint32_t lead = ptx::elected(), idesc = ptx::umma_idesc_s8(MODE == PAIR ? 2 * LANES : LANES, a.bt);
         Turn ring, buf;
         bool ok = true;
+        if (ROWS && !ptx::mbar_wait_warp(x_full, 0)) { dev_set_error(ERR_MMA | 3); ok = false; }
         for (int tile = first; tile < a.tiles && ok; tile += step) {
             if (!ptx::mbar_wait_warp(T_EMPTY(buf.slot), buf.phase ^ 1u)) { dev_set_error(ERR_MMA | 1); ok = false; break; }
             ptx::tc_fence_after_sync();
@@ -190,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                 ptx::tc_fence_after_sync();
                 uint32_t at = base + ring.slot * stage_bytes;
                 for (int q = kt; q < min(kt + a.kp, k_hi); q++, at += part_bytes) {
-                    const uint64_t w = ptx::umma_desc_k_sw128(at), x = ptx::umma_desc_k_sw128(at + A_STAGE);
+                    const uint64_t w = ptx::umma_desc_k_sw128(at), x = ptx::umma_desc_k_sw128(ROWS ? x_at + (uint32_t)(q - k_lo) * a.bt * KT : at + A_STAGE);
                     const int parts = min(KT, a.K - q * KT) / 32;
 #pragma unroll
                     for (int p = 0; p < KT / 32; p++)
@@ -218,6 +237,65 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
         // TMEM lanes [32 * quad, 32 * quad + 32) are this warp's, and of their columns every second 32
         const int quad = warp & 3, row = quad * 32 + lane, side = (warp - 2) >> 2;
         Turn buf;
+        if constexpr (ROWS) {
+            const int t = threadIdx.x - 64, vectors = a.K / 8;
+            const bool keep = first == 0;                      // the first tile's CTAs also store what the caller gets
+            constexpr int KEPT = 4, TURN = EPI_WARPS * 32;     // vectors of eight that a thread keeps between the two passes, all loaded at once
+            const int lo = k_lo * (KT / 8), hi = min(k_hi * (KT / 8), vectors);
+            for (int m = 0; m < a.M; m++) {
+                const char *src = static_cast<const char *>(a.x) + (size_t)m * a.ldx * (a.x_dtype == W4A8_F32 ? 4 : 2);
+                float kept[KEPT][8], top = 0.f;
+#pragma unroll
+                for (int u = 0; u < KEPT; u++) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) kept[u][i] = 0.f;
+                    if (t + u * TURN < vectors) load8(src, 8 * (t + u * TURN), a.x_dtype, kept[u]);
+                }
+                const auto largest = [&](const float (&v)[8]) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]));
+                };
+#pragma unroll
+                for (int u = 0; u < KEPT; u++) largest(kept[u]);
+                for (int j = t + KEPT * TURN; j < vectors; j += TURN) {
+                    float v[8];
+                    load8(src, 8 * j, a.x_dtype, v);
+                    largest(v);
+                }
+                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                if (lane == 0) row_max[warp - 2] = top;
+                epilogue_sync();
+#pragma unroll
+                for (int i = 0; i < EPI_WARPS; i++) top = fmaxf(top, row_max[i]);
+                const float d = quant_scale(top);
+                if (t == 0) {
+                    row_scale[m] = d;
+                    if (keep && rank == 0) a.xs_out[m] = d;
+                }
+                const auto codes = [&](int j, const float (&v)[8]) {
+                    if (j < lo || j >= hi) return;
+                    int sum;
+                    uint32_t q0 = 0, q1 = 0;
+                    if (top != 0.f) {
+                        q0 = quantize4_pack(make_float4(v[0], v[1], v[2], v[3]), d, sum);
+                        q1 = quantize4_pack(make_float4(v[4], v[5], v[6], v[7]), d, sum);
+                    }
+                    const int kt = j / (KT / 8) - k_lo, chunk = j % (KT / 8) / 2;          // m < 8: rows of one group of eight, swizzled by their number
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(x_at + (uint32_t)kt * a.bt * KT + m * KT + ((chunk ^ m) << 4) + (j & 1) * 8), "r"(q0), "r"(q1) : "memory");
+                    if (keep) *reinterpret_cast<uint2 *>(a.xq_out + (size_t)m * a.K + 8 * j) = make_uint2(q0, q1);
+                };
+#pragma unroll
+                for (int u = 0; u < KEPT; u++) codes(t + u * TURN, kept[u]);
+                for (int j = t + KEPT * TURN; j < hi; j += TURN) {
+                    float v[8];
+                    load8(src, 8 * j, a.x_dtype, v);
+                    codes(j, v);
+                }
+                epilogue_sync();                               // row_max is read, row_scale is there
+            }
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(x_full);
+        }
         for (int tile = first; tile < a.tiles; tile += step) {
             // what the outputs need besides the sums, while these are on their way: lane l has the scales of rows l, l + 32, ... of its columns
             const int n = tile / a.t_tiles * a.bw + my_row + row, t0 = tile % a.t_tiles * a.bt + (MODE == SPLIT ? rank * own : 0), rows = MODE == SPLIT ? rows_of(rank) : min(a.bt, a.M - t0);
@@ -227,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < XR; i++) {
                 const int c = MODE == SPLIT ? 2 * (32 * i + lane) + side : 64 * i + 32 * side + lane;
-                x[i] = c < rows ? a.xs[t0 + c] : 0.f;
+                x[i] = c < rows ? (ROWS ? row_scale[t0 + c] : a.xs[t0 + c]) : 0.f;
             }
             const float w = live ? a.ws[n] : 0.f, b = live && a.bias ? a.bias[n] : 0.f;
             T *y = static_cast<T *>(a.y) + (size_t)t0 * a.ldy + n;
@@ -308,12 +386,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool ROWS = false>
 inline int opt_in() {                                                  // a per-device function attribute
     static PerDevice<bool> configured_dev;
     bool &configured = configured_dev.get();
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(gemm_w8a8_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        const cudaError_t e = cudaFuncSetAttribute(gemm_w8a8_kernel<T, MODE, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
         if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 smem opt-in");
         configured = true;
     }
@@ -334,7 +412,7 @@ inline int caps_of(Caps *out) {
             attr.id = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = n; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
             cfg.gridDim = dim3(n); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_MAX; cfg.attrs = &attr; cfg.numAttrs = 1;
-            const cudaError_t e = cudaOccupancyMaxActiveClusters(&c.clusters[n], gemm_w8a8_kernel<float, SPLIT>, &cfg);
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&c.clusters[n], gemm_w8a8_kernel<float, SPLIT, false>, &cfg);
             if (e != cudaSuccess) return cuda_fail(e, "gemm_w8a8 clusters");
         }
         c.sms = sm_count();
@@ -360,13 +438,13 @@ inline int plan_cached(int M, int N, int K, Plan *out) {
     return W4A8_OK;
 }
 
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool ROWS>
 inline int launch_t(Args a, const Plan &p, const CUtensorMap &tmW, const CUtensorMap &tmX, cudaStream_t st) {
-    auto kern = gemm_w8a8_kernel<T, MODE>;
-    const int rc = opt_in<T, MODE>();
+    auto kern = gemm_w8a8_kernel<T, MODE, ROWS>;
+    const int rc = opt_in<T, MODE, ROWS>();
     if (rc != W4A8_OK) return rc;
-    a.stages = stages_for(p);
-    const int smem = smem_for(p), sms = sm_count();
+    a.stages = ROWS ? row_stages_for(p, a.K) : stages_for(p);
+    const int smem = ROWS ? row_smem_for(p, a.K) : smem_for(p), sms = sm_count();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(MODE == SPLIT ? a.tiles * a.split : MODE == PAIR ? 2 * (a.tiles < p.at_once ? a.tiles : p.at_once) : (a.tiles < sms ? a.tiles : sms));
     cfg.blockDim = dim3(THREADS);
@@ -408,8 +486,10 @@ inline int launch(const int8_t *xq, const int8_t *wq, Args a, Plan p, int dtype,
     rc = tmap_cached(&tmX, xq, (uint64_t)a.K, (uint64_t)a.M, KT, (uint32_t)(p.pair ? a.bt / 2 : a.bt), CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != W4A8_OK) return rc;
     const auto by_split = [&](auto t) {
-        if (p.pair) return launch_t<decltype(t), PAIR>(a, p, tmW, tmX, st);
-        return p.split > 1 ? launch_t<decltype(t), SPLIT>(a, p, tmW, tmX, st) : launch_t<decltype(t), ONE>(a, p, tmW, tmX, st);
+        using O = decltype(t);
+        if (a.x) return p.split > 1 ? launch_t<O, SPLIT, true>(a, p, tmW, tmX, st) : launch_t<O, ONE, true>(a, p, tmW, tmX, st);
+        if (p.pair) return launch_t<O, PAIR, false>(a, p, tmW, tmX, st);
+        return p.split > 1 ? launch_t<O, SPLIT, false>(a, p, tmW, tmX, st) : launch_t<O, ONE, false>(a, p, tmW, tmX, st);
     };
     if (dtype == W4A8_F32) return by_split(float());
     return dtype == W4A8_F16 ? by_split(__half()) : by_split(__nv_bfloat16());

@@ -1,5 +1,6 @@
 // How an 8-bit product (gemm_w8a8.cuh) is cut into tiles: sizes alone, no CUDA construct, so that the CPU can go through it for all of them.
 #pragma once
+#include <initializer_list>
 
 namespace w4a8 {
 namespace w8a8 {
@@ -34,7 +35,8 @@ inline int k_parts(int bt, int split, bool pair) {                     // fewer 
 inline float cost_of(const Plan &p, int M, int N, int K, const Caps &caps) {
     const long tiles = (long)ceil_div(N, p.bw) * ceil_div(M, p.bt);
     const int at_once = p.pair ? caps.clusters[2] : p.split > 1 ? caps.clusters[p.split] : caps.sms;
-    if (at_once <= 0 || (p.split > 1 && tiles > at_once)) return 1e30f;
+    // clusters of one wave; of threes the last two that should fit were seen to wait for others (44 and 45 of 45 took 1.2 times as long)
+    if (at_once <= 0 || (p.split > 1 && tiles > at_once - (p.split == 3 ? 2 : 0))) return 1e30f;
     const float waves = (float)((tiles + at_once - 1) / at_once), k_tiles = (float)ceil_div(ceil_div(K, KT), p.split);
     const float mma = p.pair ? 0.134f + 1.23e-3f * p.bt : 0.f, fill = 1.5e-3f * (p.pair ? LANES + p.bt / 2 : p.bw + p.bt), hand = 0.124f + 0.156f / p.kp;
     const float per = k_tiles * (mma > fill ? (mma > hand ? mma : hand) : fill > hand ? fill : hand);
@@ -60,7 +62,7 @@ inline Plan plan_for(int M, int N, int K, const Caps &caps) {
         last = bt;
         for (int bw = 64; bw <= LANES; bw += 32) {
             try_plan({bw, bt, 1, 0, 0, 0});
-            for (int split = 2; split <= SPLIT_MAX; split *= 2)         // (with threes and sixes the best plans are 0.2 % faster on average)
+            for (const int split : {2, 3, 4, 8})
                 if (bt <= SPLIT_BT && nkt / split >= 2) try_plan({bw, bt, split, 0, 0, 0});
         }
         try_plan({2 * LANES, ceil_div(bt, 32) * 32, 1, 0, 1, 0});
@@ -70,6 +72,23 @@ inline Plan plan_for(int M, int N, int K, const Caps &caps) {
 }
 inline int stage_bytes_for(const Plan &p) { return (A_STAGE + (p.pair ? p.bt / 2 : p.bt) * KT) * p.kp; }
 inline int smem_for(const Plan &p) { return stages_for(p) * stage_bytes_for(p) + SMEM_FIXED + split_receive(p.bt, p.split); }
+
+// Rows that the product quantizes itself stay in shared memory, a CTA's part of K of sixteen rows (the MMA's narrowest), and the stages hold weights alone.
+constexpr int ROWS_MAX = 2;
+inline int row_bytes(const Plan &p, int K) { return (ceil_div(ceil_div(K, KT), p.split) + (p.split > 1)) * 16 * KT; }
+inline int row_stages_for(const Plan &p, int K) {
+    const int n = (SMEM_MAX - SMEM_FIXED - 1024 - split_receive(p.bt, p.split) - row_bytes(p, K)) / (A_STAGE * p.kp);
+    return n > MAX_STAGES ? MAX_STAGES : n;
+}
+inline int row_smem_for(const Plan &p, int K) { return row_stages_for(p, K) * A_STAGE * p.kp + SMEM_FIXED + 1024 + split_receive(p.bt, p.split) + row_bytes(p, K); }
+// Whether a product of M rows quantizes them itself, and how: a single row wherever it fits beside stages of 96 KB (5120 x 17408 beside 64 KB: 20.1 / 27.0), two of up to 8192 elements, which the threads
+// keep between their two looks.  us in a graph, two launches / one, 17408 x 5120 18.5 / 16.8, 8192 x 3840 11.0 / 8.3, 4096 x 4096 8.3 / 6.1, 3840 x 15360 14.4 / 13.8;
+// two rows 18.6 / 17.8, 11.1 / 8.5, 8.4 / 7.0, 14.5 / 16.4; three 18.3 / 19.5, 11.2 / 9.4, 8.4 / 8.1, 14.4 / 18.8.
+inline bool row_plan(Plan &p, int M, int K) {
+    if (M > ROWS_MAX || (M > 1 && K > 8192) || p.pair || p.bt != 16) return false;
+    p.kp = 2;
+    return row_stages_for(p, K) >= 3;
+}
 
 }  // namespace w8a8
 }  // namespace w4a8

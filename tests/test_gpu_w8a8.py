@@ -126,3 +126,64 @@ def test_two_streams_and_a_graph(w4a8, cuda):
     for c, y in zip(cases, Y):
         assert torch.equal(y, _want(*c, "fp32"))
     w4a8.device_status()
+
+
+@pytest.mark.parametrize("x_dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(1, 640, 32), (1, 17408, 5120), (2, 300, 416), (2, 4096, 4096), (1, 1000, 15360), (1, 129, 32768), (2, 5000, 1312), (3, 512, 1024), (1, 60000, 256), (2, 1, 96), (1, 40000, 6144)])
+def test_a_row_or_two_in_one_call(w4a8, cuda, M, N, K, x_dtype):
+    """linear_w8a8 of few rows, which the product may quantize itself: codes, scales and outputs are those of the two calls, for the caller's pitch, with nothing behind them."""
+    g = torch.Generator(device="cuda").manual_seed(N + K)
+    x = (torch.randn(M, K + 8, generator=g, device=cuda) * 3).to(DTYPES[x_dtype])
+    if M > 1:
+        x[1] = 0                                                          # a row of zeros
+    _, _, wq, ws, b = _case(1, N, K, N)
+    xq, xs = torch.full((M + 1, K), 99, dtype=torch.int8, device=cuda), torch.full((M + 1,), 7.0, device=cuda)
+    q, scale, _ = quantize(x[:, :K].float(), 0)
+    for y_dtype in ("fp32", "bf16"):
+        Y = torch.full((M + 1, N + 3), 3.0, device=cuda).to(DTYPES[y_dtype])
+        w4a8.linear_w8a8(x, K + 8, xq, xs, wq, ws, Y, N + 3, M, N, K, x_dtype, y_dtype, bias=b)
+        assert torch.equal(xq[:M], q) and torch.equal(xs[:M], scale[:, 0]) and (xq[M] == 99).all() and xs[M] == 7
+        assert torch.equal(Y[:M, :N], _want(q, scale[:, 0], wq, ws, b, y_dtype)) and (Y[M] == 3).all() and (Y[:, N:] == 3).all()
+    w4a8.device_status()
+
+
+def test_an_output_in_the_place_of_its_row(w4a8, cuda):
+    """Y may be x's own memory: the row has been read before the outputs are written."""
+    K = N = 2048
+    x = torch.randn(1, K, device=cuda)
+    _, _, wq, ws, _ = _case(1, N, K, 4, bias=False)
+    q, scale, _ = quantize(x, 0)
+    want = _want(q, scale[:, 0], wq, ws, None, "fp32")
+    w4a8.linear_w8a8(x, K, torch.empty_like(q), torch.empty(1, device=cuda), wq, ws, x, N, 1, N, K)
+    assert torch.equal(x, want)
+
+
+def test_single_rows_in_a_chain_and_a_graph(w4a8, cuda):
+    """Row after row through two matrices, each the next one's input: what a launch leaves is what the next one reads, also in a graph."""
+    K = 1024
+    mats = [_case(1, K, K, 20 + i, bias=False)[2:4] for i in range(2)]
+    x = torch.randn(1, K, device=cuda)
+    xq, xs = torch.empty(1, K, dtype=torch.int8, device=cuda), torch.empty(1, device=cuda)
+    a, b = torch.empty(1, K, device=cuda), torch.empty(1, K, device=cuda)
+
+    def chain():
+        w4a8.linear_w8a8(x, K, xq, xs, *mats[0], a, K, 1, K, K)
+        for _ in range(4):
+            w4a8.linear_w8a8(a, K, xq, xs, *mats[1], b, K, 1, K, K)
+            w4a8.linear_w8a8(b, K, xq, xs, *mats[0], a, K, 1, K, K)
+
+    def plain(v):
+        for m in [mats[0]] + [mats[1], mats[0]] * 4:
+            q, s, _ = quantize(v, 0)
+            v = _want(q, s[:, 0], *m, None, "fp32")
+        return v
+    chain()
+    assert torch.equal(a, plain(x))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain()
+    for seed in range(3):
+        x.copy_(torch.randn(1, K, device=cuda))
+        graph.replay()
+        assert torch.equal(a, plain(x))
+    w4a8.device_status()
