@@ -19,6 +19,10 @@
 // accumulates in the other half of TMEM.  Where there are fewer tiles than SMs, the CTAs of a cluster share a tile's K (`split` of them), send
 // their int32 sums to the CTA that owns the columns through distributed shared memory, and that one adds them: no workspace, no second
 // launch, and the same bits, since integers add in any order.
+//
+// Bounds and figures (us, in a graph): 2048 x 17408 x 5120 128 (2.85 POP/s; tensor pipe and L2 at three quarters each), 4096^3 52, 333 x 4091 x 3840 9.8 (what an SM takes from
+// L2, 64 bytes a cycle), 16 x 3840 x 15360 13.2 (4.5 TB/s; clusters' start and sums are 4 of it), 1 x 17408 x 5120 15.4 (5.8 TB/s).  The issuing warps stay converged and an elected
+// lane issues: a lane that branches off alone took 300 cycles a K-tile for waits, descriptors and commits, and the first of these shapes 217 us.
 #pragma once
 #include <cuda.h>
 #include "common.cuh"
