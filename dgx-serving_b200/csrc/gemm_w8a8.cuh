@@ -313,7 +313,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
             }
             const float w = live ? a.ws[n] : 0.f, b = live && a.bias ? a.bias[n] : 0.f;
             T *y = static_cast<T *>(a.y) + (size_t)t0 * a.ldy + n;
-            if (!ptx::mbar_wait_warp(T_FULL(buf.slot), buf.phase)) { dev_set_error(ERR_EPILOGUE); break; }
+            bool ok = ptx::mbar_wait_warp(T_FULL(buf.slot), buf.phase);
+            if (!ok) dev_set_error(ERR_EPILOGUE);
+            if (MODE != SPLIT && !ok) break;               // (SPLIT: its warps meet below, whatever each one's wait came to)
             ptx::tc_fence_after_sync();
             const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf.slot * (a.tmem_cols / 2);
             const int columns = MODE == SPLIT ? tile_rows : rows;
@@ -347,7 +349,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_w8a8_kernel(const __grid_cons
                 epilogue_sync();
                 if (warp == 2 && lane < a.split && lane != rank && rows_of(lane) > 0)
                     send(remote(recv + (uint32_t)(rank * own * LANES * 4), lane), base + (uint32_t)(lane * own * LANES * 4), (uint32_t)(rows_of(lane) * LANES * 4), remote(sums_full, lane));
-                if (!ptx::mbar_wait_warp(sums_full, 0)) { dev_set_error(ERR_SUMS); break; }
+                if (!ptx::mbar_wait_warp(sums_full, 0)) { dev_set_error(ERR_SUMS); ok = false; }
+                if (!ok) {                                     // sums on their way land before the cluster's memory goes away
+                    const long long since = clock64();
+                    while (clock64() - since < (1ll << 21)) { }
+                    break;
+                }
                 static_assert(XR == 1);
                 const int *mine = reinterpret_cast<const int *>(smem_dyn + (base - raw)) + row, *theirs = reinterpret_cast<const int *>(smem_dyn + (recv - raw)) + row;
                 for (int j = 0; 2 * j + side < rows; j += 4) {             // every second row, four of them at a time

@@ -147,6 +147,23 @@ def test_a_row_or_two_in_one_call(w4a8, cuda, M, N, K, x_dtype):
     w4a8.device_status()
 
 
+def test_single_rows_at_the_ends_of_fp32(w4a8, cuda):
+    """A row quantized by its product, of subnormal, huge, infinite elements and NaN, and of zeros: the two calls' bits."""
+    N, K = 200, 512
+    g = torch.Generator(device="cuda").manual_seed(6)
+    base = torch.randn(1, K, generator=g, device=cuda)
+    _, _, wq, ws, b = _case(1, N, K, 7)
+    rows = [base * 1e-42, base * 1e-37, base * 1e37, base * 0, base.clone(), base.clone()]
+    rows[4][0, 100], rows[5][0, 511] = float("inf"), float("nan")
+    xq, xs, Y = torch.empty(1, K, dtype=torch.int8, device=cuda), torch.empty(1, device=cuda), torch.empty(1, N, device=cuda)
+    xq2, xs2, Y2 = torch.empty_like(xq), torch.empty_like(xs), torch.empty_like(Y)
+    for x in rows:
+        w4a8.linear_w8a8(x, K, xq, xs, wq, ws, Y, N, 1, N, K, bias=b)
+        w4a8.launch_quantize_rows_q8(x, K, 1, K, xq2, xs2)
+        w4a8.launch_gemm_w8a8(xq2, xs2, wq, ws, Y2, N, 1, N, K, bias=b)
+        assert torch.equal(xq, xq2) and torch.equal(xs.view(torch.int32), xs2.view(torch.int32)) and torch.equal(Y.isnan(), Y2.isnan()) and torch.equal(Y.nan_to_num(), Y2.nan_to_num())
+
+
 def test_an_output_in_the_place_of_its_row(w4a8, cuda):
     """Y may be x's own memory: the row has been read before the outputs are written."""
     K = N = 2048
