@@ -28,11 +28,13 @@ struct Args {
     double inv_k, eps;
     float alpha;
     int K, variant, post, group;                  // group 32, or 0: one scale for the row
+    int S;
 };
 
-// The sum over the CTA, in every thread; the same bits in all of them.
+// The sum over the CTA (WARP: over the warp), in every thread; the same bits in all of them.
+template <bool WARP>
 __device__ __forceinline__ double cta_sum(double v, double *sh) {
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int lane = threadIdx.x & 31, warps = WARP ? 1 : blockDim.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (warps == 1) return v;
@@ -43,8 +45,9 @@ __device__ __forceinline__ double cta_sum(double v, double *sh) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+template <bool WARP>
 __device__ __forceinline__ float cta_max(float v, float *sh) {
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int lane = threadIdx.x & 31, warps = WARP ? 1 : blockDim.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (warps == 1) return v;
@@ -80,20 +83,24 @@ constexpr int VEC = sizeof(TH) == 4 && sizeof(TY) == 4 ? 4 : 8;
 
 // EP elements a thread.  EARLY: weights are asked for together with the rows and not behind the sums that they do not depend on: a
 // trip to L2 less for each norm where a few rows are bound by latency (64 rows of 5120 with codes 3.3 -> 2.8 us), registers that cost CTAs where there are many.  SUM: there is a y.
-template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM>
+// WARP: a row is one warp's, several rows a CTA's, and nothing is waited for: short rows in great number are otherwise bound by the rate at which CTAs start
+// (8192 rows of 256 elements 8.9 us whatever is done to them, 4.5 to 5.6 so; above 512 elements sums of two rows are faster by CTAs, 8192 x 1024 20.4 and 21.3,
+// and quantizers by warps, 8.9 and 8.2).
+template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM, bool WARP>
 __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
     constexpr int V = VEC<TH, TY>, NV = EP / V;
     __shared__ double sh_y[32], sh_h[32];
     __shared__ float sh_max[32];
-    const int nt = blockDim.x, nvec = a.K / V;
-    const size_t row = blockIdx.x;
+    const int nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x, nvec = a.K / V;
+    const size_t row = WARP ? (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     pdl_wait();
     pdl_launch_dependents();
+    if (WARP && row >= (size_t)a.S) return;
     const TH *h = static_cast<const TH *>(a.h) + row * a.ldh;
     float x[NV][V], f[EARLY ? NV : 1][V];
 #pragma unroll
     for (int u = 0; u < NV; u++) {
-        const int j = threadIdx.x + u * nt;
+        const int j = tid + u * nt;
 #pragma unroll
         for (int i = 0; i < V; i++) x[u][i] = 0.f;
         if (j < nvec) load_row<TH, V>(h + j * V, x[u]);
@@ -104,7 +111,7 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
         float p[NV][V], pf[EARLY ? NV : 1][V];
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int j = threadIdx.x + u * nt;
+            const int j = tid + u * nt;
 #pragma unroll
             for (int i = 0; i < V; i++) p[u][i] = 0.f;
             if (j < nvec) load_row<TY, V>(y + j * V, p[u]);
@@ -112,8 +119,8 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
         if constexpr (EARLY) {
 #pragma unroll
             for (int u = 0; u < NV; u++) {
-                if (takes_weight(a.post)) fetch(pf[u], a.pw, threadIdx.x + u * nt);
-                if (takes_weight(a.variant)) fetch(f[u], a.w, threadIdx.x + u * nt);
+                if (takes_weight(a.post)) fetch(pf[u], a.pw, tid + u * nt);
+                if (takes_weight(a.variant)) fetch(f[u], a.w, tid + u * nt);
             }
         }
         float r = 1.f;
@@ -121,11 +128,11 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
             double ss = 0.0;
 #pragma unroll
             for (int u = 0; u < NV; u++) ss = squares(p[u], ss);
-            r = (float)rsqrt(fma(cta_sum(ss, sh_y), a.inv_k, a.eps));
+            r = (float)rsqrt(fma(cta_sum<WARP>(ss, sh_y), a.inv_k, a.eps));
         }
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int j = threadIdx.x + u * nt;
+            const int j = tid + u * nt;
             if (j < nvec) {
                 if (a.post != W4A8_NORM_NONE) {
                     if (!EARLY && takes_weight(a.post)) fetch(pf[0], a.pw, j);
@@ -144,13 +151,13 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
     } else if constexpr (EARLY) {
 #pragma unroll
         for (int u = 0; u < NV; u++)
-            if (takes_weight(a.variant)) fetch(f[u], a.w, threadIdx.x + u * nt);
+            if (takes_weight(a.variant)) fetch(f[u], a.w, tid + u * nt);
     }
     if (a.h_out) {
         TH *o = static_cast<TH *>(a.h_out) + row * a.ldo;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int j = threadIdx.x + u * nt;
+            const int j = tid + u * nt;
             if (j < nvec) store_row<TH, V>(o + j * V, x[u]);
         }
     }
@@ -159,10 +166,10 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
         double ss = 0.0;
 #pragma unroll
         for (int u = 0; u < NV; u++) ss = squares(x[u], ss);
-        const float r = (float)rsqrt(fma(cta_sum(ss, sh_h), a.inv_k, a.eps));
+        const float r = (float)rsqrt(fma(cta_sum<WARP>(ss, sh_h), a.inv_k, a.eps));
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int j = threadIdx.x + u * nt;
+            const int j = tid + u * nt;
             if (j < nvec) {
                 if (!EARLY && takes_weight(a.variant)) fetch(f[0], a.w, j);
                 normed(x[u], r, f[EARLY ? u : 0], a.variant);
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
         TH *o = static_cast<TH *>(a.n_out) + row * a.ldn;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int j = threadIdx.x + u * nt;
+            const int j = tid + u * nt;
             if (j < nvec) store_row<TH, V>(o + j * V, x[u]);
         }
     }
@@ -186,10 +193,10 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
         for (int i = 0; i < V; i++) amax[u] = fmaxf(amax[u], fabsf(x[u][i]));
         top = fmaxf(top, amax[u]);
     }
-    if (a.group == 0) top = cta_max(top, sh_max);
+    if (a.group == 0) top = cta_max<WARP>(top, sh_max);
 #pragma unroll
     for (int u = 0; u < NV; u++) {
-        const int j = threadIdx.x + u * nt;
+        const int j = tid + u * nt;
         float m = top;
         if (a.group != 0) {                                            // the 32 / V lanes of a block: all of them have elements, or none
             m = amax[u];
@@ -226,19 +233,24 @@ __global__ void __launch_bounds__(MAXT, 1) add_norm_kernel(const Args a) {
     }
 }
 
-template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM>
-inline int launch_ep(const Args &a, int S, cudaStream_t st) {
+template <typename TH, typename TY, int EP, int MAXT, bool EARLY, bool SUM, bool WARP = false>
+inline int launch_ep(Args a, int S, cudaStream_t st) {
+    constexpr int WARP_ROWS = 4;
+    a.S = S;
     const int need = (a.K + EP - 1) / EP;
-    const cudaError_t e = launch_pdl(add_norm_kernel<TH, TY, EP, MAXT, EARLY, SUM>, dim3(S), dim3((need + 31) / 32 * 32), 0, st, a);
+    const dim3 grid(WARP ? (unsigned)(((long)S + WARP_ROWS - 1) / WARP_ROWS) : (unsigned)S), block(WARP ? WARP_ROWS * 32 : (need + 31) / 32 * 32);
+    const cudaError_t e = launch_pdl(add_norm_kernel<TH, TY, EP, MAXT, EARLY, SUM, WARP>, grid, block, 0, st, a);
     if (e != cudaSuccess) return cuda_fail(e, "add_norm launch");
     return launch_status("add_norm");
 }
 template <typename TH, typename TY, bool SUM>
 inline int launch_t(const Args &a, int S, cudaStream_t st) {
     if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024, true, SUM>(a, S, st);
-    if (!SUM && a.K <= 1024 * 16 && S <= sm_count()) return launch_ep<TH, TY, 16, 1024, false, SUM>(a, S, st);
+    if (a.K <= 32 * 16 && S > 4 * sm_count()) return launch_ep<TH, TY, 16, 128, false, SUM, true>(a, S, st);
+    if constexpr (!SUM)
+        if (a.K <= 32 * 32 && S > 4 * sm_count()) return launch_ep<TH, TY, 32, 128, false, SUM, true>(a, S, st);
     if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512, false, SUM>(a, S, st);
-    if (a.K <= 512 * 32) return launch_ep<TH, TY, 32, 512, false, SUM>(a, S, st);
+    if (a.K <= 1024 * 16) return launch_ep<TH, TY, 16, 1024, false, SUM>(a, S, st);
     return launch_ep<TH, TY, 32, 1024, false, SUM>(a, S, st);
 }
 template <typename TH>

@@ -164,3 +164,30 @@ def test_the_largest_products_of_a_serving_step(w4a8, cuda):
     want = (xq.double() @ wq[at].double().T).float() * xs[:, None] * ws[at]
     assert torch.equal(Y[:, at], want)
     w4a8.device_status()
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [("fp32", "fp32"), ("bf16", "fp32"), ("fp16", "fp16")])
+@pytest.mark.parametrize("S,K", [(593, 32), (601, 96), (1203, 256), (602, 512), (700, 544), (605, 1024)])
+def test_short_rows_in_great_number(w4a8, cuda, S, K, dtype, y_dtype):
+    """Rows that a warp has to itself: the definition's bits in every output, nothing behind the last row, and the same bits as a row by itself."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    r = lambda *s: torch.randn(s, generator=g, device=cuda)
+    h, y, w, pw = r(S + 1, K).to(DTYPES[dtype]), r(S + 1, K).to(DTYPES[y_dtype]), r(K) * 0.1 + 1, r(K) * 0.1
+    for yy, post, group in ((y, 1, 32), (y, -1, 0), (None, -1, 0), (None, -1, 32)):
+        n = w4a8.Norm.of(K, w, 0, 1e-6, pw, post, None, 0.7, dtype, y_dtype)
+        blocks = 1 if group == 0 else K // 32
+        s_out, out = (torch.full((S + 1, K), 3.0, device=cuda).to(h.dtype) for _ in range(2))
+        xq, xs = torch.full((S + 1, K), 99, dtype=torch.int8, device=cuda), torch.full((S + 1, blocks), 7.0, device=cuda)
+        w4a8.launch_add_norm(n, h, yy, S, H_out=s_out, N=out, xq=xq, xs=xs, group=group)
+        want_s, want = add_norm32(h, yy, w, 0, pw, post, None, 0.7, 1e-6)
+        q, scale, _ = quantize(want, group)
+        assert torch.equal(s_out[:S], want_s[:S].to(h.dtype)) and torch.equal(out[:S], want[:S].to(h.dtype))
+        assert torch.equal(xq[:S], q[:S]) and torch.equal(xs[:S], scale[:S])
+        assert (s_out[S] == 3).all() and (out[S] == 3).all() and (xq[S] == 99).all() and (xs[S] == 7).all()
+        one = torch.empty(1, K, device=cuda).to(h.dtype)
+        w4a8.launch_add_norm(n, h[17:], None if yy is None else yy[17:], 1, N=one)
+        assert torch.equal(one[0], out[17])
+    xq, xs = torch.empty(S, K, dtype=torch.int8, device=cuda), torch.empty(S, device=cuda)
+    w4a8.launch_quantize_rows_q8(h, K, S, K, xq, xs, dtype)
+    q, scale, _ = quantize(h[:S].float(), 0)
+    assert torch.equal(xq, q) and torch.equal(xs, scale[:, 0])
