@@ -245,10 +245,13 @@ inline int launch_ep(Args a, int S, cudaStream_t st) {
 }
 template <typename TH, typename TY, bool SUM>
 inline int launch_t(const Args &a, int S, cudaStream_t st) {
-    if (a.K <= 1024 * 8 && S <= sm_count()) return launch_ep<TH, TY, 8, 1024, true, SUM>(a, S, st);
     if (a.K <= 32 * 16 && S > 4 * sm_count()) return launch_ep<TH, TY, 16, 128, false, SUM, true>(a, S, st);
     if constexpr (!SUM)
         if (a.K <= 32 * 32 && S > 4 * sm_count()) return launch_ep<TH, TY, 32, 128, false, SUM, true>(a, S, st);
+    // Eight elements a thread while all rows run at once (some 56 registers a thread with a sum, 32 without), sixteen where they come in waves: us, sixteen / eight, norms of
+    // 150 x 3840 3.7 / 3.0, 300 x 1024 3.1 / 2.2, 500 x 2048 3.9 / 3.1, but 300 x 5120 5.0 / 6.4; quantizers 200 x 5120 2.7 / 2.5, 590 x 4096 4.2 / 3.2.
+    const int threads = (a.K / 8 + 31) / 32 * 32, at_once = (SUM ? 1152 : 2048) / threads;
+    if (a.K <= 1024 * 8 && S <= sm_count() * (at_once < 1 ? 1 : at_once)) return launch_ep<TH, TY, 8, 1024, true, SUM>(a, S, st);
     if (a.K <= 512 * 16) return launch_ep<TH, TY, 16, 512, false, SUM>(a, S, st);
     if (a.K <= 1024 * 16) return launch_ep<TH, TY, 16, 1024, false, SUM>(a, S, st);
     return launch_ep<TH, TY, 32, 1024, false, SUM>(a, S, st);
