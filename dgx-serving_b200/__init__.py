@@ -122,6 +122,8 @@ class Rope(ctypes.Structure):
     _fields_ = [("turns", ctypes.c_void_p), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("eps", ctypes.c_double), ("magnitude", ctypes.c_float),
                 ("dim", ctypes.c_int), ("rotary", ctypes.c_int), ("interleaved", ctypes.c_int), ("variant", ctypes.c_int)]
 
+    _host = False
+
     @classmethod
     def of(cls, dim, rotary, base=10000.0, scaling="none", interleaved=False, q_weight=None, k_weight=None, variant=-1, eps=1e-6, device="cuda", magnitude=None, **parameters):
         """Heads of `dim` elements, the first `rotary` of them turned.  scaling and parameters: rope_table's; magnitude: instead of the scaling's own.
@@ -133,6 +135,7 @@ class Rope(ctypes.Structure):
         table = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=device)
         r = cls(_ptr(table) if turns else None, _ptr(q_weight), _ptr(k_weight), float(eps), float(m if magnitude is None else magnitude), dim, rotary, int(bool(interleaved)), variant)
         r._tensors = (table, q_weight, k_weight)
+        r._host = bool(turns) and not table.is_cuda
         return r
 
 
@@ -249,9 +252,10 @@ def _binding():
         device, raw = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if device is None or raw is None:
             device, raw = torch.cuda.current_device, lambda d: torch.cuda.current_stream(d).cuda_stream
-        if torch.cuda.is_available():
+        there = torch.cuda.is_available()
+        if there:
             torch.cuda.init()                                         # the two functions above expect it
-        module.streams(device, raw)
+        module.streams(device, raw, torch.cuda.device_count() if there else 0)
         _native = module
     return _native
 
@@ -460,6 +464,8 @@ def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=No
 
 def launch_rope_qk(rope, Q, ldq, heads_q, K, ldk, heads_k, position, T, Q_out=None, ldqo=0, K_out=None, ldko=0, dtype="fp32", stream=None):
     """Norms and rotary positions of queries Q[T][heads_q * dim] and keys K[T][heads_k * dim] (w4a8_rope_qk); outputs None: in place."""
+    if rope._host:
+        raise ValueError("the rope's table is not on a GPU")
     if Q_out is None:
         Q_out, ldqo = Q, ldq
     if K_out is None:

@@ -1,16 +1,37 @@
 /* The layer operators for Python without ctypes: a call costs about 0.5 us in place of 3, which is what a decode step's smallest operators
  * take on the GPU.  The functions are the C ABI's (include/w4a8_b200.h), found in the library that the package has loaded (bind); arguments in its order.  A
- * pointer is a number, None, or a tensor (its data_ptr()); a struct is a ctypes Structure; a stream is a number, an object with a cuda_stream, or None: what
- * the two functions given to streams() say is torch's current one.  Each returns the status code. */
+ * pointer is a number, None, or a tensor (its data_ptr()), which has to lie on the current GPU: a kernel would follow a pointer to host memory, or to another
+ * GPU's, to a fault.  A struct is a ctypes Structure; a stream is a number, an object with a cuda_stream, or None: what the two functions given to
+ * streams() say is torch's current one.  Each returns the status code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <limits.h>
 typedef struct w4a8_arena w4a8_arena;
 #include "../../include/w4a8_b200.h"
 
-static PyObject *data_ptr_name, *cuda_stream_name;
+static PyObject *data_ptr_name, *cuda_stream_name, *is_cuda_name, *get_device_name;
 static PyObject *current_device, *current_stream;         /* of torch: device(), raw stream(device) */
+static int gpus;                                          /* 0: nothing can be launched, and tensors may lie anywhere */
 
+/* Whether a tensor lies on the current GPU; which one that is, is asked for only where there are several. */
+static int on_gpu(PyObject *o) {
+    if (gpus == 0) return 1;
+    PyObject *there = PyObject_GetAttr(o, is_cuda_name);
+    if (!there) return 0;
+    const int yes = there == Py_True;
+    Py_DECREF(there);
+    if (!yes) {
+        PyErr_SetString(PyExc_ValueError, "a tensor that is not on a GPU");
+        return 0;
+    }
+    if (gpus == 1) return 1;
+    PyObject *its = PyObject_CallMethodNoArgs(o, get_device_name), *now = its ? PyObject_CallNoArgs(current_device) : NULL;
+    const int same = now ? PyObject_RichCompareBool(its, now, Py_EQ) : -1;
+    if (same == 0) PyErr_Format(PyExc_ValueError, "a tensor on GPU %S, the current one is %S", its, now);
+    Py_XDECREF(its);
+    Py_XDECREF(now);
+    return same == 1;
+}
 /* Each conversion does nothing once one before it has failed. */
 static void *as_pointer(PyObject *o, int *ok) {
     if (!*ok || o == Py_None) return NULL;
@@ -19,7 +40,7 @@ static void *as_pointer(PyObject *o, int *ok) {
         if (!p && PyErr_Occurred()) *ok = 0;
         return p;
     }
-    PyObject *n = PyObject_CallMethodNoArgs(o, data_ptr_name);
+    PyObject *n = on_gpu(o) ? PyObject_CallMethodNoArgs(o, data_ptr_name) : NULL;
     if (!n) { *ok = 0; return NULL; }
     void *p = PyLong_AsVoidPtr(n);
     if (!p && PyErr_Occurred()) *ok = 0;
@@ -140,9 +161,13 @@ static PyObject *bind(PyObject *self, PyObject *const *a, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-/* streams(device(), stream(device)) */
+/* streams(device(), stream(device), number of GPUs) */
 static PyObject *streams(PyObject *self, PyObject *const *a, Py_ssize_t n) {
-    if (!count(n, 2)) return NULL;
+    int ok = 1;
+    if (!count(n, 3)) return NULL;
+    const int there = I(2);
+    if (!ok) return NULL;
+    gpus = there;
     Py_INCREF(a[0]);
     Py_INCREF(a[1]);
     Py_XSETREF(current_device, a[0]);
@@ -156,5 +181,7 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", NULL, -1,
 PyMODINIT_FUNC PyInit__binding(void) {
     data_ptr_name = PyUnicode_InternFromString("data_ptr");
     cuda_stream_name = PyUnicode_InternFromString("cuda_stream");
-    return data_ptr_name && cuda_stream_name ? PyModule_Create(&module) : NULL;
+    is_cuda_name = PyUnicode_InternFromString("is_cuda");
+    get_device_name = PyUnicode_InternFromString("get_device");
+    return data_ptr_name && cuda_stream_name && is_cuda_name && get_device_name ? PyModule_Create(&module) : NULL;
 }

@@ -129,7 +129,7 @@ def test_structs_of_tensors(w4a8):
 
 def test_the_binding_without_ctypes(w4a8):
     """The launchers' own way into the library: what it cannot convert is an exception, what the library refuses is its error."""
-    t = torch.zeros(4, 64)
+    t = torch.zeros(4, 64, device="cuda" if GPU else "cpu")
     n = norm_of(w4a8, K=48)
     with pytest.raises(w4a8.W4A8Error, match="multiple of 32") as e:
         w4a8.launch_add_norm(n, t, t, 4, N=t, stream=0)
@@ -161,3 +161,40 @@ def test_the_binding_without_ctypes(w4a8):
         w4a8.launch_add_norm(n, t, t, 4, N=t, stream=0)
     with pytest.raises(TypeError, match="15 expected"):
         w4a8._binding().add_norm(norm_of(w4a8), t)
+
+
+class Elsewhere:
+    """What the binding looks at of a tensor on another GPU than the current one, which is 0 here."""
+    is_cuda = True
+
+    def __init__(self, gpu):
+        self.gpu = gpu
+
+    def get_device(self):
+        return self.gpu
+
+    def data_ptr(self):
+        return BASE
+
+
+def test_tensors_that_are_not_on_the_current_gpu(w4a8):
+    """A kernel would follow their pointers; where there is no GPU at all, nothing is launched.  The calls here have no rows."""
+    b, t = w4a8._binding(), torch.zeros(4, 64)
+    n = norm_of(w4a8)
+    try:
+        for gpus in (1, 2):
+            b.streams(lambda: 0, lambda device: 0, gpus)
+            with pytest.raises(ValueError, match="not on a GPU"):
+                w4a8.launch_add_norm(n, t, None, 0, N=None, stream=0)
+            with pytest.raises(ValueError, match="not on a GPU"):
+                w4a8.launch_gemm_w8a8(None, None, t, None, None, 64, 0, 64, 64, stream=0)
+            w4a8.launch_add_norm(n, Elsewhere(0), None, 0, stream=0)
+            w4a8.launch_add_norm(n, BASE, None, 0, stream=0)                          # a number is the caller's word
+        with pytest.raises(ValueError, match="on GPU 1, the current one is 0"):
+            w4a8.launch_add_norm(n, Elsewhere(1), None, 0, stream=0)
+        with pytest.raises(AttributeError):
+            w4a8.launch_add_norm(n, "h", None, 0, stream=0)
+    finally:
+        w4a8._native = None                                  # bound anew with torch's own functions
+    with pytest.raises(ValueError, match="table is not on a GPU"):
+        w4a8.launch_rope_qk(w4a8.Rope.of(64, 64, device="cpu"), BASE, 64, 1, BASE << 1, 64, 1, BASE << 2, 0, stream=0)
