@@ -35,6 +35,8 @@ class DecoderLayer:
             raise ValueError("router_w: int8")
         size = 2 if scale_dtype else 4
         for (wq, sc), n, kk, name in ((gate_up, 2 * inner, H, "gate_up"), (down, H, inner, "down")):
+            if wq.device != dev or sc.device != dev or router_w[0].device != dev or router_w[1].device != dev:
+                raise ValueError("%s, router_w: on %s, as the attention is" % (name, dev))
             if wq.numel() * wq.element_size() != E * n * kk // 2 or sc.numel() * sc.element_size() != E * n * kk // 32 * size or not (wq.is_contiguous() and sc.is_contiguous()):
                 raise ValueError("%s: packed int4 of %d experts, [%d][%d], and scales of 32 elements, contiguous" % (name, E, n, kk))
         self.normed = torch.empty(rows, H, device=dev)
@@ -52,6 +54,8 @@ class DecoderLayer:
                 raise ValueError("%s: contiguous fp32 rows of %d on %s" % (name, H, self.normed.device))
         if T > self.normed.shape[0]:
             raise ValueError("%d rows: this layer has room for %d" % (T, self.normed.shape[0]))
+        if not h.is_cuda or h.device.index != torch.cuda.current_device():
+            raise ValueError("h is on %s, which is not the current GPU" % h.device)
         n = self.normed[:T]
         w4a8.launch_add_norm(self.norm_in, h, y, T, H_out=None if y is None else h, N=n)
         a = self.attention(n, max_q=max_q)

@@ -49,5 +49,11 @@ def test_layers(w4a8, parts):
     for h, why in ((torch.zeros(4, H + 32), "h:"), (torch.zeros(4, H).half(), "h:"), (torch.zeros(4, 2 * H)[:, :H], "h:"), (torch.zeros(ROWS + 1, H), "room for")):
         with pytest.raises(ValueError, match=why):
             layer(h)
+    with pytest.raises(ValueError, match="not the current GPU"):
+        layer(torch.zeros(4, H))                             # a layer in host memory
+    meta = lambda n, k: tuple(x.to("meta") for x in four(n, k))
+    for bad in (dict(gate_up=meta(E * 2 * INNER, H)), dict(down=meta(E * H, INNER)), dict(router_w=tuple(x.to("meta") for x in eight(E, H)))):
+        with pytest.raises(ValueError, match="on cpu, as the attention"):
+            make(**bad)
     with pytest.raises(ValueError, match="y:"):
         layer(torch.zeros(4, H), torch.zeros(5, H))

@@ -143,3 +143,12 @@ def test_a_layer_in_a_graph(w4a8, oracle, cuda):
         want = plain(h2, y, max_q=1)
         assert torch.equal(out, want) and torch.equal(h, h2)
     w4a8.device_status()
+
+
+def test_a_step_without_rows(w4a8, oracle, cuda):
+    tables, layer = layer_of(w4a8, oracle, cuda, weights_of_norms(cuda))
+    tables.step(torch.zeros(R, dtype=torch.int32, device=cuda), 0)
+    empty = torch.empty(0, HIDDEN, device=cuda)
+    assert layer(empty).shape == (0, HIDDEN) and layer(empty, empty.clone()).shape == (0, HIDDEN)
+    tables.done()
+    assert (tables.kv_len == 0).all() and w4a8.device_status() is None
