@@ -59,12 +59,13 @@ __device__ __forceinline__ float unordered(uint32_t k) { return __int_as_float((
 // e^v = 2^(v log2 e), the exponent as a sum of two numbers: within 6 * 2^-24 of itself where it is normal (ex2.approx 2^-22, a product, the second number's
 // part of the result), without expf's cases.  The sigmoids of 4096 tokens by expf and an IEEE division: 14.6 us as above, 13.4 by __expf.
 __device__ __forceinline__ float exp_close(float v) {
-    constexpr float L = 1.44269502f, L2 = 1.92596299e-8f;             // log2 e = L + L2
+    constexpr double LOG2_E = 1.4426950408889634;
+    constexpr float L = (float)LOG2_E, L2 = (float)(LOG2_E - (double)L);
     v = fminf(fmaxf(v, -200.f), 100.f);                                // 0 and infinity
     const float p = v * L, q = fmaf(v, L2, fmaf(v, L, -p));
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p));
-    return e * fmaf(q, 0.693147181f, 1.f);
+    return e * fmaf(q, (float)(1.0 / LOG2_E), 1.f);
 }
 __device__ __forceinline__ float reciprocal(float v) {                 // 1 ulp
     float r;
