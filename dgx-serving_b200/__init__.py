@@ -255,7 +255,7 @@ def _binding():
         there = torch.cuda.is_available()
         if there:
             torch.cuda.init()                                         # the two functions above expect it
-        module.streams(device, raw, torch.cuda.device_count() if there else 0)
+        module.streams(device, raw, torch.cuda.device_count() if there else 0, torch.Tensor)
         _native = module
     return _native
 

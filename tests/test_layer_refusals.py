@@ -182,8 +182,8 @@ def test_tensors_that_are_not_on_the_current_gpu(w4a8):
     b, t = w4a8._binding(), torch.zeros(4, 64)
     n = norm_of(w4a8)
     try:
-        for gpus in (1, 2):
-            b.streams(lambda: 0, lambda device: 0, gpus)
+        for gpus, kind in ((1, torch.Tensor), (2, torch.Tensor), (1, Elsewhere), (2, None)):          # the tensors' type as torch's and as anybody's
+            b.streams(lambda: 0, lambda device: 0, gpus, kind)
             with pytest.raises(ValueError, match="not on a GPU"):
                 w4a8.launch_add_norm(n, t, None, 0, N=None, stream=0)
             with pytest.raises(ValueError, match="not on a GPU"):
