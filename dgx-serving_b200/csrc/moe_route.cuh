@@ -10,7 +10,7 @@
 // Choices lie close to one another: with 256 experts and 4096 tokens some fp32 scores are within a rounding of the next one, and which expert a
 // token gets must not depend on the exponential's last bit.  So four candidates more than topk are taken; where neighbours among them are closer than
 // fp32 can be wrong (4 tokens in 100), the candidates are put in order by their choices in fp64, one a lane, and where that does not decide either
-// (a border of groups, more near values than candidates) the whole token is done again in fp64.
+// (a border of groups, more near values than candidates, topk 32, which has none to spare) the whole token is done again in fp64.
 #pragma once
 #include "common.cuh"
 #include "rows.cuh"
@@ -287,8 +287,13 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         found = k + 1;
     }
     if (!by_logit && !whole) {
-        const float next = __shfl_down_sync(0xffffffffu, choice, 1);
-        if (__any_sync(0xffffffffu, lane < a.topk && lane + 1 < found && !(choice - next > slack))) {
+        float next = __shfl_down_sync(0xffffffffu, choice, 1);
+        bool behind = lane + 1 < found;                // whether `next` is a choice
+        if (a.topk == 32 && found == 32) {             // no lane is left for a candidate to spare: the best of what has not been taken stands in its place
+            const uint32_t left = __reduce_max_sync(0xffffffffu, (uint32_t)(held.best() >> 32));
+            if (lane == 31) { next = unordered(left); behind = left != 0; }
+        }
+        if (__any_sync(0xffffffffu, lane < a.topk && behind && !(choice - next > slack))) {
             // candidates that were not taken are further away than fp32 can be wrong, or there are none
             const float last = __shfl_sync(0xffffffffu, choice, found - 1), end = __shfl_sync(0xffffffffu, choice, a.topk - 1);
             if (found < wanted || end - last > slack) {
