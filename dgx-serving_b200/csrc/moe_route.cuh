@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         }
         // How far a choice may be off, in units of 2^-24 of the largest score and bias together.  Sigmoid: exp_close 6, the sum 1, the reciprocal 2, the
         // bias 1: two choices 20, and 2^-19 is 32.  Softmax: exp_close 6 and its argument's rounding, |v| e^v < 0.4; a sum of up to 1024 terms 64 + 5; the
-        // reciprocal 2; the product and the sum with the bias 2: two 160, and 2^-16 is 256.
-        slack = warp_max(largest) * (a.sigmoid ? 0x1p-19f : 0x1p-16f);
+        // reciprocal 2; the product and the sum with the bias 2: two 160, and 2^-16 is 256.  And scores below 2^-126 are 0: four of them, in two sums of two, 2^-124.
+        slack = warp_max(largest) * (a.sigmoid ? 0x1p-19f : 0x1p-16f) + 0x1p-124f;
     }
     held.settle();
     bool whole = !(slack < INFINITY);              // again in fp64
