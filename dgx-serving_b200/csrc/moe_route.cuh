@@ -338,11 +338,19 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         }
         mine = select_double(a, key, group, lane, e0, lanes);
     }
-    float w = 0.f;
-    if (lane < a.topk) {
-        const float v = logit(widen(row[mine]));
-        w = a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top);
+    // Weights in fp32.  Renormalised ones need the chosen scores up to a common factor alone, so the exponentials are of distances to the largest chosen logit:
+    // the largest of all may belong to an expert that a bias or its group keeps out, and fp32 ends 104 below it.  Sigmoids below e^-64 are e^v to
+    // 2^-92 of themselves, and get the same factor where all of the chosen are that small.  Scores below e^-745, which fp64 does not hold, are 0.
+    constexpr float BARE = -64.f, LEAST = -745.f;
+    const float v = lane < a.topk ? logit(widen(row[mine])) : -INFINITY;
+    float from = a.sigmoid ? 0.f : top, w = 0.f;
+    const bool held_in_64 = v - from > LEAST;
+    if (a.renormalise) {
+        const float most = unordered(__reduce_max_sync(0xffffffffu, ordered(v)));
+        if (!a.sigmoid || most < BARE) from = most;
     }
+    if (a.sigmoid && v >= BARE) w = 1.f / (1.f + expf(-v));
+    else if (held_in_64) w = expf(v - from);
     float sum = warp_sum(w);
     if (!a.renormalise) {                          // softmax over all experts, the sum in fp32 as the weights are
         sum = 0.f;

@@ -400,7 +400,9 @@ int w4a8_rope_qk(const w4a8_rope *rope, const void *q, int64_t ldq, int heads_q,
  * alignment): score = softmax over the experts, or sigmoid of each; choice = score + bias[e] (NULL: none).  With groups > 1 the experts
  * [g * experts / groups, ...) are a group, its score the largest choice (group_score 0) or the sum of the two largest (1), and only the
  * topk_groups best groups take part.  idx: the topk largest choices in falling order; equal ones, of groups too, by the lowest index.
- * weight = the chosen scores (without bias), divided by their sum if renormalise, times scale.  Choices are compared in fp64.
+ * weight = the chosen scores (without bias), divided by their sum if renormalise, times scale.  Choices are compared in fp64 (of a softmax without a bias whose groups
+ * are not added up, the logits themselves, which have the same order).  Weights are taken in fp32: renormalised ones within 25 * 2^-24 of the token's largest; scores that fp64
+ * does not hold (a sigmoid below e^-745, a softmax that far below its largest) are 0.
  * A logit that is not a number counts as -inf, +inf as the largest fp32 number; an expert of -inf has the score 0 (and without a bias is chosen last;
  * a bias of -inf shuts an expert out as long as there are others), and where all are, the weights are 0.  The indices name different experts in every case.  experts <= 1024, topk <= 32, groups <= 32. */
 typedef struct w4a8_router {
