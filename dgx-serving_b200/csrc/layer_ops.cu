@@ -115,7 +115,7 @@ W4A8_API int w4a8_rope_qk(const w4a8_rope *r, const void *q, int64_t ldq, int he
     if ((rc = check_apart(who, rows, names, 8, 6, [](int o, int i) { return (o == 6 && i == 0) || (o == 7 && i == 1); })) != W4A8_OK) return rc;
     if ((rc = require_sm100()) != W4A8_OK) return rc;
     const bool bare = r->variant == W4A8_NORM_NONE;
-    rope::Args a = {r->turns, r->q_weight, r->k_weight, position, q, k, q_out, k_out, ldq, ldk, ldqo, ldko, r->magnitude, 1.f / r->dim, (float)r->eps,
+    rope::Args a = {r->turns, r->q_weight, r->k_weight, position, q, k, q_out, k_out, ldq, ldk, ldqo, ldko, r->eps, r->magnitude, 1.f / r->dim, (float)r->eps,
                     heads_q, heads_q + heads_k, r->dim, r->rotary, r->interleaved != 0, r->variant, 0, bare && q == q_out, bare && k == k_out};
     return rope::launch(a, T, dtype, (cudaStream_t)stream);
 }

@@ -6,6 +6,7 @@
 // half turns whatever the position.  In fp32 the angle of token 131072 would have lost all bits below 2^-7.
 #pragma once
 #include <cmath>
+#include <type_traits>
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -21,6 +22,7 @@ struct Args {
     const void *q, *k;
     void *q_out, *k_out;
     int64_t ldq, ldk, ldqo, ldko;
+    double eps64;
     float magnitude, inv_dim, eps;
     int heads_q, heads, dim, rotary, interleaved, variant, per_cta;       // heads: of queries and keys; per_cta of them to a CTA
     int skip_q, skip_k;                                                   // elements that are not turned already lie where they belong
@@ -37,8 +39,15 @@ struct Args {
 // with norms 38.6 / 36.4); fp32 rows, whose loads fill the registers, lose by it (52.2 / 55.1).
 template <typename T> constexpr int CTA = sizeof(T) == 4 ? 128 : 64;
 
+// A head's factor comes from a sum of up to 256 squares in fp32, eps rounded to it and a reciprocal root within 2 ulp: within 2^-20 of itself where fp32 holds the squares, which it does
+// for factors between these two (2^-60, 2^40) and always for fp16 elements.  Heads of elements around 2e18 and above, or of tiny ones beside no eps, are summed again in fp64 before anything of their batch is stored, since
+// outputs may lie on inputs.  All sums of a batch first: looked at head by head, in between the stores, 8000 tokens with weighted norms took 5 to 11 % longer.
+constexpr uint32_t FACTOR_MIN = 0x21800000u, FACTOR_MAX = 0x53800000u;
+__device__ __forceinline__ uint32_t outside(float r) { return __float_as_uint(r) - FACTOR_MIN; }          // above FACTOR_MAX - FACTOR_MIN: outside, infinite or not a number
+
 template <typename T, int V, int LPH, int BATCH>                         // BATCH heads' loads of a lane in flight
 __global__ void __launch_bounds__(CTA<T>) rope_kernel(const Args a) {
+    constexpr bool WIDE = !std::is_same<T, __half>::value;
     __shared__ float2 turn[MAX_DIM / 2];
     const int t = blockIdx.x, half = a.rotary / 2;
     const int group = threadIdx.x / LPH, j = threadIdx.x % LPH;
@@ -78,23 +87,55 @@ __global__ void __launch_bounds__(CTA<T>) rope_kernel(const Args a) {
     }
     __syncthreads();
     const float2 *mine = turn + V * j;                                    // this lane's pairs
+    const auto factor = [&](const float (&u)[V], const float (&v)[V]) {   // lanes of a group meet here
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; i++) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        return rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+    };
     for (int h0 = first + group; h0 - group < last; h0 += BATCH * GROUPS) {
         if (h0 != first + group) fetch(h0);
+        float r[BATCH];
+        if (WIDE && a.variant != W4A8_NORM_NONE) {
+            uint32_t worst = 0;
+#pragma unroll
+            for (int b = 0; b < BATCH; b++) {
+                float u[V], v[V];
+                raw[b][0].unpack(u);
+                raw[b][1].unpack(v);
+                r[b] = factor(u, v);
+                if (h0 + b * GROUPS < last) worst = max(worst, outside(r[b]));
+            }
+            if (__any_sync(0xffffffffu, worst > FACTOR_MAX - FACTOR_MIN)) {
+#pragma unroll
+                for (int b = 0; b < BATCH; b++) {
+                    const int h = h0 + b * GROUPS;
+                    const bool is_q = h < a.heads_q;
+                    const T *src = is_q ? q + (size_t)h * a.dim : k + (size_t)(h - a.heads_q) * a.dim;
+                    double ss = 0.0;
+#pragma unroll 1
+                    for (int i = 0; i < 2 * V && h < last && live; i++) {
+                        const double x = (double)(float)src[i < V ? ia + i : ib + i - V];
+                        ss = fma(x, x, ss);
+                    }
+#pragma unroll 1
+                    for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    if (outside(r[b]) > FACTOR_MAX - FACTOR_MIN) r[b] = (float)rsqrt(ss / a.dim + a.eps64);
+                }
+            }
+        }
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
             const int h = h0 + b * GROUPS;
-            if (h - group >= last) break;                                 // the same for the whole CTA: lanes of a group meet in the sums below
+            if (h - group >= last) break;                                 // the same for the whole CTA
             const bool is_q = h < a.heads_q;
             float u[V], v[V];                                             // the two runs
             raw[b][0].unpack(u);
             raw[b][1].unpack(v);
             if (a.variant != W4A8_NORM_NONE) {
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; i++) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
-#pragma unroll
-                for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float r = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+                if (!WIDE) r[b] = factor(u, v);
                 if (a.variant != W4A8_NORM_NO_SCALE && live) {
                     const float *w = is_q ? a.qw : a.kw;
                     const float one = a.variant == W4A8_NORM_ONE_PLUS ? 1.f : 0.f;
@@ -102,10 +143,10 @@ __global__ void __launch_bounds__(CTA<T>) rope_kernel(const Args a) {
                     load_row<float, V>(w + ia, lo);
                     load_row<float, V>(w + ib, hi);
 #pragma unroll
-                    for (int i = 0; i < V; i++) { u[i] *= r * (one + lo[i]); v[i] *= r * (one + hi[i]); }
+                    for (int i = 0; i < V; i++) { u[i] = u[i] * r[b] * (one + lo[i]); v[i] = v[i] * r[b] * (one + hi[i]); }     // r may be near an end of fp32, where r * w is not one
                 } else {
 #pragma unroll
-                    for (int i = 0; i < V; i++) { u[i] *= r; v[i] *= r; }
+                    for (int i = 0; i < V; i++) { u[i] *= r[b]; v[i] *= r[b]; }
                 }
             }
             if (h < last && live && (turned || !(is_q ? a.skip_q : a.skip_k))) {

@@ -381,7 +381,7 @@ int w4a8_rope_table(int rotary, double base, int scaling, double factor, double 
                     uint64_t *turns_host, float *magnitude);
 
 /* Norms and rotary positions of a step's queries and keys in one launch: q[T][heads_q * dim], k[T][heads_k * dim], columns of a fused QKV product
- * as they are.  Each head is normed (variant; q_weight, k_weight [dim]), and of its first `rotary` elements the pairs (i, i + rotary / 2), or
+ * as they are.  Each head is normed (variant; q_weight, k_weight [dim]; sums and factor in fp32, in fp64 where fp32 does not hold the squares), and of its first `rotary` elements the pairs (i, i + rotary / 2), or
  * (2 i, 2 i + 1) where interleaved, are turned by position[t] * frequency[i]: (a cos - b sin, b cos + a sin), times magnitude.  The product is
  * taken modulo a turn in whole numbers, so angles are as exact at 2^31 tokens as at one.  Rows of a negative position (no request owns them)
  * are left as they are in the outputs.  q_out, k_out may be q's, k's own memory.  heads_k 0: queries alone.  dim a multiple of 8, at most
