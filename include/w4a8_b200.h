@@ -355,7 +355,8 @@ enum { W4A8_NORM_NONE = -1, W4A8_NORM_SCALE = 0, W4A8_NORM_ONE_PLUS = 1, W4A8_NO
  * quantized: group 32: w4a8_quantize_x_q8's form, the input of the W4A8 products (xq [S][K], xs, xsum [S][K / 32]); group 0: one scale for
  * each row, the input of w4a8_gemm_w8a8 (xq [S][K], xs [S], no xsum).  What is normed and quantized is not rounded to dtype before.
  * Every step is one fp32 operation in the order written (left to right); the sums of squares and r are taken in fp64 and r is rounded to fp32 once,
- * so that the bits do not depend on how a row is cut.  h, h_out and n_out have type dtype, y has y_dtype: dtype or W4A8_F32.
+ * so that a row's bits hardly ever depend on S: the last bits of the fp64 sum do, and where r lies that near to the middle of two fp32 numbers (one row in 10^8), it may be either.
+ * h, h_out and n_out have type dtype, y has y_dtype: dtype or W4A8_F32.
  * K a multiple of 32, at most 32768. */
 typedef struct w4a8_norm {
     const float *weight, *post_weight;   /* [K]; NULL where the variant takes none */
