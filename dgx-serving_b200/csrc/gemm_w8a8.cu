@@ -58,10 +58,16 @@ W4A8_API int w4a8_linear_w8a8(const void *x, int64_t ldx, int8_t *xq, float *xs,
     if (!skip_quantize) {
         const size_t size = row_size(x_dtype);
         w8a8::Plan plan;
-        const Rows in = {x, ldx, K, S, size}, codes = {xq, K, K, S, 1}, scales = {xs, S, S, 1, 4}, y = {Y, ldy, N, S, row_size(y_dtype)};
+        const Rows in = {size && ldx >= K ? x : nullptr, ldx, K, S, size}, codes = {xq, K, K, S, 1}, scales = {xs, S, S, 1, 4}, y = {Y, ldy, N, S, row_size(y_dtype)};
+        // codes and scales are written while CTAs still read weights (one launch) or before they do (two)
+        const Rows read[] = {in, {wq, K, K, N, 1}, {ws, N, N, 1, 4}, {bias, N, N, 1, 4}, codes};
+        static const char *const names[] = {"x", "wq", "ws", "bias", "xq"};
+        for (int i = 0; i < 5; i++) {
+            if (i < 4 && rows_overlap(codes, read[i])) return fail(W4A8_ERR_ARG, "linear_w8a8: xq overlaps %s", names[i]);
+            if (rows_overlap(scales, read[i])) return fail(W4A8_ERR_ARG, "linear_w8a8: xs overlaps %s", names[i]);
+        }
         // a row or two by the product itself (what is not right with x is the quantizer's to say; an output in x's place needs x read first)
-        if (S <= w8a8::ROWS_MAX && size && K <= 32768 && ldx >= K && aligned(x, 16) && ldx * size % 16 == 0 && !rows_overlap(y, in) && !rows_overlap(codes, in) &&
-            !rows_overlap(scales, in) && !rows_overlap(scales, codes) && (rc = require_sm100()) == W4A8_OK && (rc = w8a8::plan_cached(S, N, K, &plan)) == W4A8_OK &&
+        if (S <= w8a8::ROWS_MAX && in.p && K <= 32768 && aligned(x, 16) && ldx * size % 16 == 0 && !rows_overlap(y, in) && (rc = require_sm100()) == W4A8_OK && (rc = w8a8::plan_cached(S, N, K, &plan)) == W4A8_OK &&
             w8a8::row_plan(plan, S, K)) {
             w8a8::Args a = {xs, ws, bias, Y, ldy, S, N, K};
             a.x = x; a.ldx = ldx; a.x_dtype = x_dtype; a.xq_out = xq; a.xs_out = xs;

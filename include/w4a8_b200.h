@@ -421,7 +421,8 @@ int w4a8_moe_route(const w4a8_router *router, const void *logits, int64_t ld, in
  *   a row's bits depend on neither M nor the way K is cut.  Y has any alignment and pitch; xq and wq are 16-byte aligned.  Any M, N up to
  *   2^31 - 1024; K a multiple of 32, at most 131040.
  *   w4a8_linear_w8a8: both, one after the other (skip_quantize: xq and xs are there already); a row, or two of up to 8192 elements, in one launch where their
- *   codes fit beside the weights.  xq, xs and Y get the same bits either way, and Y may be x's own memory. */
+ *   codes fit beside the weights.  xq, xs and Y get the same bits either way, and Y may be x's own memory; xq and xs, where they are
+ *   written, overlap nothing else. */
 int w4a8_quantize_rows_q8(const void *x, int64_t ldx, int S, int K, int dtype, int8_t *xq, float *xs, void *stream);
 int w4a8_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, const float *bias, void *Y, int64_t ldy, int M, int N, int K,
                    int dtype, void *stream);
