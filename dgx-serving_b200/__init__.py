@@ -73,12 +73,27 @@ def _fp32_vector(t, n, name):
     return t
 
 
+def _gpu_of(tensors, name):
+    """The GPU that all tensors of a struct lie on (-1: host memory), None without any."""
+    at = {t.get_device() for t in tensors if t is not None}
+    if len(at) > 1:
+        raise ValueError("%s: tensors that are not on one GPU" % name)
+    return at.pop() if at else None
+
+
+def struct_on(struct, device, name):
+    """Refuses a Norm, Rope or Router whose tensors are not on `device`."""
+    if struct._gpu is not None and struct._gpu != (device.index if device.type == "cuda" else -1):
+        raise ValueError("%s: tensors that are not on %s" % (name, device))
+
+
 class Norm(ctypes.Structure):
     """Mirror of w4a8_norm: the weights and constants of one residual add with its norms."""
     _fields_ = [("weight", ctypes.c_void_p), ("post_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("gate_ld", ctypes.c_int64), ("eps", ctypes.c_double),
                 ("alpha", ctypes.c_float), ("K", ctypes.c_int), ("variant", ctypes.c_int), ("post_variant", ctypes.c_int), ("dtype", ctypes.c_int), ("y_dtype", ctypes.c_int)]
 
     _gate_rows = 1 << 63
+    _gpu = None
 
     @classmethod
     def of(cls, K, weight=None, variant=0, eps=1e-6, post_weight=None, post_variant=-1, gate=None, alpha=1.0, dtype="fp32", y_dtype=None):
@@ -97,6 +112,7 @@ class Norm(ctypes.Structure):
                 raise ValueError("gate: rows that overlap")
         n = cls(_ptr(weight), _ptr(post_weight), _ptr(gate), gate_ld, float(eps), float(alpha), K, variant, post_variant, DTYPES[dtype], DTYPES[dtype if y_dtype is None else y_dtype])
         n._tensors = (weight, post_weight, gate)
+        n._gpu = _gpu_of(n._tensors, "Norm")
         if gate_ld:
             n._gate_rows = gate.shape[0]
         return n
@@ -123,6 +139,7 @@ class Rope(ctypes.Structure):
                 ("dim", ctypes.c_int), ("rotary", ctypes.c_int), ("interleaved", ctypes.c_int), ("variant", ctypes.c_int)]
 
     _host = False
+    _gpu = None
 
     @classmethod
     def of(cls, dim, rotary, base=10000.0, scaling="none", interleaved=False, q_weight=None, k_weight=None, variant=-1, eps=1e-6, device="cuda", magnitude=None, **parameters):
@@ -136,6 +153,7 @@ class Rope(ctypes.Structure):
         r = cls(_ptr(table) if turns else None, _ptr(q_weight), _ptr(k_weight), float(eps), float(m if magnitude is None else magnitude), dim, rotary, int(bool(interleaved)), variant)
         r._tensors = (table, q_weight, k_weight)
         r._host = bool(turns) and not table.is_cuda
+        r._gpu = _gpu_of((table if turns else None, q_weight, k_weight), "Rope")
         return r
 
 
@@ -144,12 +162,15 @@ class Router(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("experts", ctypes.c_int), ("topk", ctypes.c_int), ("scoring", ctypes.c_int), ("groups", ctypes.c_int), ("topk_groups", ctypes.c_int),
                 ("group_score", ctypes.c_int), ("renormalise", ctypes.c_int), ("scale", ctypes.c_float)]
 
+    _gpu = None
+
     @classmethod
     def of(cls, experts, topk, scoring="softmax", bias=None, groups=1, topk_groups=1, group_score="max", renormalise=True, scale=1.0):
         """scoring: "softmax" or "sigmoid"; group_score: "max" or "sum2"; bias: fp32 [experts], kept alive."""
         _fp32_vector(bias, experts, "bias")
         r = cls(_ptr(bias), experts, topk, {"softmax": 0, "sigmoid": 1}[scoring], groups, topk_groups, {"max": 0, "sum2": 1}[group_score], int(bool(renormalise)), float(scale))
         r._tensors = (bias,)
+        r._gpu = _gpu_of(r._tensors, "Router")
         return r
 
 

@@ -90,8 +90,13 @@ class AttentionBlock:
         self.cols = (heads_q + 2 * heads) * dim
         self.wide_qkv = check_matrix(wqkv, self.cols, hidden, "wqkv")
         self.wide_o = check_matrix(wo, hidden, heads_q * dim, "wo")
-        if isinstance(rotate, w4a8.Rope) and rotate.dim != dim:
-            raise ValueError("rotate: heads of %d elements, the block's have %d" % (rotate.dim, dim))
+        for name, matrix in (("wqkv", wqkv), ("wo", wo)):
+            if any(t.device != dev for t in matrix):
+                raise ValueError("%s: on %s, as the tables are" % (name, dev))
+        if isinstance(rotate, w4a8.Rope):
+            if rotate.dim != dim:
+                raise ValueError("rotate: heads of %d elements, the block's have %d" % (rotate.dim, dim))
+            w4a8.struct_on(rotate, dev, "rotate")
         self.qkv = torch.empty(max_rows, self.cols, device=dev)
         self.mix = torch.empty(max_rows, heads_q * dim, device=dev)
         widest = max(hidden, heads_q * dim)
@@ -110,6 +115,8 @@ class AttentionBlock:
             raise ValueError("%d rows: the step was planned for %d" % (X.shape[0], self.tables.slot.numel()))
         if not X.is_cuda or X.device != self.qkv.device:
             raise ValueError("X is on %s, the block on %s" % (X.device, self.qkv.device))
+        if X.device.index != torch.cuda.current_device():
+            raise ValueError("X is on %s, which is not the current GPU" % X.device)
 
     def _product(self, X, matrix, wide, Y, T, n, k):
         if wide:

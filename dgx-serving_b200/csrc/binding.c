@@ -1,7 +1,7 @@
 /* The layer operators for Python without ctypes: a call costs about 0.5 us in place of 3, which is what a decode step's smallest operators
  * take on the GPU.  The functions are the C ABI's (include/w4a8_b200.h), found in the library that the package has loaded (bind); arguments in its order.  A
  * pointer is a number, None, or a tensor (its data_ptr()), which has to lie on the current GPU: a kernel would follow a pointer to host memory, or to another
- * GPU's, to a fault.  A struct is a ctypes Structure; a stream is a number, an object with a cuda_stream, or None: what the two functions given to
+ * GPU's, to a fault.  A struct is a ctypes Structure, whose _gpu says where the tensors behind it lie; a stream is a number, an object with a cuda_stream, or None: what the two functions given to
  * streams() say is torch's current one.  Each returns the status code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -9,7 +9,7 @@
 typedef struct w4a8_arena w4a8_arena;
 #include "../../include/w4a8_b200.h"
 
-static PyObject *data_ptr_name, *cuda_stream_name, *is_cuda_name, *get_device_name;
+static PyObject *data_ptr_name, *cuda_stream_name, *is_cuda_name, *get_device_name, *gpu_name;
 static PyObject *current_device, *current_stream;         /* of torch: device(), raw stream(device) */
 static int gpus;                                          /* 0: nothing can be launched, and tensors may lie anywhere */
 /* The tensor type's own C functions behind is_cuda and data_ptr(), called without a look-up: 0.1 us less for a call of five tensors. */
@@ -85,10 +85,29 @@ static int as_int(PyObject *o, int *ok) {
     }
     return (int)v;
 }
+/* Whether what a struct points to lies on the current GPU: its _gpu, if it has one that is not None. */
+static int struct_on_gpu(PyObject *o) {
+    PyObject *its = PyObject_GetAttr(o, gpu_name);
+    if (!its) {
+        if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return 0;
+        PyErr_Clear();
+        return 1;
+    }
+    int same = its == Py_None;
+    if (!same) {
+        PyObject *now = PyObject_CallNoArgs(current_device);
+        same = now ? PyObject_RichCompareBool(its, now, Py_EQ) : -1;
+        if (same == 0) PyErr_Format(PyExc_ValueError, "a struct of tensors on GPU %S, the current one is %S", its, now);
+        Py_XDECREF(now);
+    }
+    Py_DECREF(its);
+    return same == 1;
+}
 /* A struct's memory: it outlives the call, in which the library reads it. */
 static const void *as_struct(PyObject *o, size_t size, int *ok) {
     Py_buffer view;
     if (!*ok) return NULL;
+    if (gpus > 1 && !struct_on_gpu(o)) { *ok = 0; return NULL; }
     if (PyObject_GetBuffer(o, &view, PyBUF_SIMPLE) != 0) { *ok = 0; return NULL; }
     const void *p = view.buf;
     if ((size_t)view.len != size) {
@@ -207,5 +226,6 @@ PyMODINIT_FUNC PyInit__binding(void) {
     cuda_stream_name = PyUnicode_InternFromString("cuda_stream");
     is_cuda_name = PyUnicode_InternFromString("is_cuda");
     get_device_name = PyUnicode_InternFromString("get_device");
-    return data_ptr_name && cuda_stream_name && is_cuda_name && get_device_name ? PyModule_Create(&module) : NULL;
+    gpu_name = PyUnicode_InternFromString("_gpu");
+    return data_ptr_name && cuda_stream_name && is_cuda_name && get_device_name && gpu_name ? PyModule_Create(&module) : NULL;
 }

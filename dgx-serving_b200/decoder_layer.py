@@ -31,6 +31,8 @@ class DecoderLayer:
         for n, name in ((norm_in, "norm_in"), (norm_mlp, "norm_mlp")):
             if n.K != H or n.dtype != w4a8.DTYPES["fp32"] or n.y_dtype != w4a8.DTYPES["fp32"] or n.gate_ld != 0:
                 raise ValueError("%s: fp32 rows of %d, no gate of single tokens" % (name, H))
+        for part, name in ((norm_in, "norm_in"), (norm_mlp, "norm_mlp"), (router, "router")):
+            w4a8.struct_on(part, dev, name)
         if not attention_block.check_matrix(router_w, E, H, "router_w"):
             raise ValueError("router_w: int8")
         size = 2 if scale_dtype else 4
