@@ -472,6 +472,27 @@ def launch_attention_q8(Q, ldq, cache, block_table, table_width, cu_q, seq_len, 
                                    workspace.numel() * workspace.element_size(), _stream(stream)))
 
 
+# What the launches refuse of their parameters alone: calls without rows, which launch nothing and follow no pointer.
+def check_norm(norm):
+    _check(lib().w4a8_add_norm(norm, None, 0, None, 0, None, 0, None, 0, None, None, None, 32, 0, None))
+
+
+def check_rope(rope, heads_q, heads_k):
+    _check(lib().w4a8_rope_qk(rope, None, 0, heads_q, None, 0, heads_k, None, 0, None, 0, None, 0, 0, None))
+
+
+def check_router(router):
+    _check(lib().w4a8_moe_route(router, None, router.experts, 0, 0, None, None, None))
+
+
+def check_moe(topk, H, MI, num_experts, scale_dtype, act):
+    _check(lib().w4a8_moe_block(None, None, None, None, None, None, None, None, 0, topk, H, MI, num_experts, scale_dtype, act, None, 0, None))
+
+
+def check_attention(cache, heads_q, scale, window, softcap):
+    _check(lib().w4a8_attention_q8(None, 0, cache, None, 0, None, None, 0, 0, heads_q, None, 0, None, scale, 1, window, softcap, 0, 0, None, 0, None))
+
+
 def launch_add_norm(norm, H, Y, S, H_out=None, N=None, xq=None, xs=None, xsum=None, group=32, ldh=0, ldy=0, ldo=0, ldn=0, stream=None):
     """h' = h + norm(y) * gate * alpha of S rows, to H_out, and its norm n, to N and / or quantized to xq, xs, xsum (w4a8_add_norm).  Y None: h' = h.
     group 32: blocks of 32 elements, 0: one scale for a row.  Pitches of 0: K."""

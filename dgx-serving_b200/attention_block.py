@@ -70,6 +70,8 @@ def check_matrix(matrix, n, k, name):
     wide = wq.dtype == torch.int8 and wq.numel() == n * k
     if wq.numel() * wq.element_size() != (n * k if wide else n * k // 2) or sc.dtype != torch.float32 or sc.numel() != (n if wide else n * k // 32) or not (wq.is_contiguous() and sc.is_contiguous()):
         raise ValueError("%s: %d rows of %d packed int4 and %d fp32 scales, or int8 and one scale a row, contiguous" % (name, n, k, k // 32))
+    if wide and wq.data_ptr() % 16:
+        raise ValueError("%s: int8 rows must be 16-byte aligned" % name)
     return wide
 
 
@@ -97,6 +99,10 @@ class AttentionBlock:
             if rotate.dim != dim:
                 raise ValueError("rotate: heads of %d elements, the block's have %d" % (rotate.dim, dim))
             w4a8.struct_on(rotate, dev, "rotate")
+            if rotate.variant in (0, 1) and not (rotate.q_weight and rotate.k_weight):
+                raise ValueError("rotate: norms without their weights")
+            w4a8.check_rope(rotate, heads_q, heads)
+        w4a8.check_attention(self.cache, heads_q, self.scale, window, softcap)      # what a launch would refuse after the rows have been appended
         self.qkv = torch.empty(max_rows, self.cols, device=dev)
         self.mix = torch.empty(max_rows, heads_q * dim, device=dev)
         widest = max(hidden, heads_q * dim)

@@ -31,8 +31,15 @@ class DecoderLayer:
         for n, name in ((norm_in, "norm_in"), (norm_mlp, "norm_mlp")):
             if n.K != H or n.dtype != w4a8.DTYPES["fp32"] or n.y_dtype != w4a8.DTYPES["fp32"] or n.gate_ld != 0:
                 raise ValueError("%s: fp32 rows of %d, no gate of single tokens" % (name, H))
-        for part, name in ((norm_in, "norm_in"), (norm_mlp, "norm_mlp"), (router, "router")):
-            w4a8.struct_on(part, dev, name)
+            w4a8.struct_on(n, dev, name)
+            # what a launch in the middle of the layer would refuse
+            if (n.variant in (0, 1) and not n.weight) or (n is norm_mlp and n.post_variant in (0, 1) and not n.post_weight):
+                raise ValueError("%s: a norm without its weight" % name)
+            if any((p or 0) % 16 for p in (n.weight, n.post_weight, n.gate)):
+                raise ValueError("%s: weights and gate must be 16-byte aligned" % name)
+            w4a8.check_norm(n)
+        w4a8.struct_on(router, dev, "router")
+        w4a8.check_router(router)
         if not attention_block.check_matrix(router_w, E, H, "router_w"):
             raise ValueError("router_w: int8")
         size = 2 if scale_dtype else 4
@@ -41,6 +48,9 @@ class DecoderLayer:
                 raise ValueError("%s, router_w: on %s, as the attention is" % (name, dev))
             if wq.numel() * wq.element_size() != E * n * kk // 2 or sc.numel() * sc.element_size() != E * n * kk // 32 * size or not (wq.is_contiguous() and sc.is_contiguous()):
                 raise ValueError("%s: packed int4 of %d experts, [%d][%d], and scales of 32 elements, contiguous" % (name, E, n, kk))
+            if wq.data_ptr() % 16 or sc.data_ptr() % 16:
+                raise ValueError("%s: weights and scales must be 16-byte aligned" % name)
+        w4a8.check_moe(k, H, inner, E, scale_dtype, act)
         self.normed = torch.empty(rows, H, device=dev)
         self.xq, self.xs = torch.empty(rows, H, dtype=torch.int8, device=dev), torch.empty(rows, device=dev)
         self.logits = torch.empty(rows, E, device=dev)
@@ -58,7 +68,10 @@ class DecoderLayer:
             raise ValueError("%d rows: this layer has room for %d" % (T, self.normed.shape[0]))
         if not h.is_cuda or h.device.index != torch.cuda.current_device():
             raise ValueError("h is on %s, which is not the current GPU" % h.device)
+        if max_q < 0 or T * self.router.topk > 1 << 24:
+            raise ValueError("max_q=%d, %d rows of %d experts (at most 2^24)" % (max_q, T, self.router.topk))
         n = self.normed[:T]
+        self.attention._check(n)                              # nothing is launched, and h not changed, for a call that is refused
         w4a8.launch_add_norm(self.norm_in, h, y, T, H_out=None if y is None else h, N=n)
         a = self.attention(n, max_q=max_q)
         w4a8.launch_add_norm(self.norm_mlp, h, a, T, H_out=h, N=n, xq=self.xq, xs=self.xs, group=0)
