@@ -435,10 +435,10 @@ inline int caps_of(Caps *out) {
 // The plan of a shape, kept for the shapes called last (a decode loop has a few; finding one takes some microseconds).
 inline int plan_cached(int M, int N, int K, Plan *out) {
     struct Slot { int M, N, K, dev; Plan plan; };
-    static Slot slots[256] = {};
+    static Slot slots[PLAN_SLOTS] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
-    Slot &s = slots[((uint32_t)M * 2654435761u ^ (uint32_t)N * 2246822519u ^ (uint32_t)K * 3266489917u) >> 24];
+    Slot &s = slots[plan_slot(M, N, K, dev)];
     if (s.M != M || s.N != N || s.K != K || s.dev != dev) {
         Caps caps;
         const int rc = caps_of(&caps);

@@ -70,6 +70,9 @@ inline Plan plan_for(int M, int N, int K, const Caps &caps) {
     }
     return best;
 }
+// Where the plan of a shape is kept: the GPU turns the place, so that the same layers on several GPUs do not put one another out.
+constexpr int PLAN_SLOTS = 256;
+inline int plan_slot(int M, int N, int K, int dev) { return (((unsigned)M * 2654435761u ^ (unsigned)N * 2246822519u ^ (unsigned)K * 3266489917u) + (unsigned)dev * 2654435769u) >> 24; }
 inline int stage_bytes_for(const Plan &p) { return (A_STAGE + (p.pair ? p.bt / 2 : p.bt) * KT) * p.kp; }
 inline int smem_for(const Plan &p) { return stages_for(p) * stage_bytes_for(p) + SMEM_FIXED + split_receive(p.bt, p.split); }
 
