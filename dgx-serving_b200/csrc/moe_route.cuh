@@ -10,8 +10,9 @@
 // Choices lie close to one another: with 256 experts and 4096 tokens some fp32 scores are within a rounding of the next one, and which expert a
 // token gets must not depend on the exponential's last bit.  So four candidates more than topk are taken; where neighbours among them are closer than
 // fp32 can be wrong (4 tokens in 100), the candidates are put in order by their choices in fp64, one a lane, and where that does not decide either
-// (a border of groups, more near values than candidates, topk 32, which has none to spare) the whole token is done again in fp64.
+// (a border of groups, more near values than candidates) the whole token is done again in fp64.  There is a lane for 32 candidates, and of the next one its choice.
 #pragma once
+#include <type_traits>
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -183,7 +184,9 @@ struct Held {
 
 constexpr int WARPS = 4, SPARE = 4;
 
-template <typename T, int EPL>                     // EPL experts a lane
+// EPL experts a lane.  BY_LOGIT: a softmax without a bias whose groups are not added up, where the order of the logits is that of the scores: nothing to
+// be decided in fp64, and without that code 4096 tokens of 128 experts take 3.8 us and not 5.3.
+template <typename T, int EPL, bool BY_LOGIT>
 __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     const int lane = threadIdx.x & 31;
     const long t = (long)blockIdx.x * WARPS + (threadIdx.x >> 5);
@@ -194,7 +197,6 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     const int lanes = 1 << a.lanes_log2, group = lane >> a.lanes_log2, sub = lane & (lanes - 1);
     const int e0 = group * a.members + sub * EPL;  // the first expert of this lane
     const auto there = [&](int i) { return group < a.groups && sub * EPL + i < a.members; };
-    const bool by_logit = !a.sigmoid && !a.bias && !a.sum2;            // the order of the logits is that of the scores
     // every load at once: places that hold no expert read the row's first
     float x[EPL], b[EPL];
     bool loaded = false;
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     Held<EPL> held;
     const auto hold = [&](int i, float c) { held.key[i] = there(i) ? (uint64_t)ordered(c) << 32 | ~(uint32_t)(e0 + i) : 0ull; };
     float slack = 0.f;
-    if (by_logit) {
+    if constexpr (BY_LOGIT) {
 #pragma unroll
         for (int i = 0; i < EPL; i++) hold(i, x[i]);
     } else {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         }
         uint32_t score = group >= a.groups ? 0 : a.sum2 ? ordered(unordered(best) + unordered(second)) : best, before = 0;
         bool open = false;
-        for (int k = 0; k < a.topk_groups + (by_logit ? 0 : 1); k++) { // the best group of those that are left, and of equal ones the first
+        for (int k = 0; k < a.topk_groups + (BY_LOGIT ? 0 : 1); k++) { // the best group of those that are left, and of equal ones the first
             const uint32_t most = __reduce_max_sync(0xffffffffu, score), g = __reduce_min_sync(0xffffffffu, score == most ? (uint32_t)group : 0xffffffffu);
             if (k == a.topk_groups) whole |= !(unordered(before) - unordered(most) > 2.f * slack);      // the last group taken and the first that is not
             else if ((int)g == group) { open = true; score = 0; }
@@ -274,29 +276,27 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
         }
         if (!open) held.clear();
     }
-    const int wanted = by_logit ? a.topk : min(32, a.topk + SPARE);
+    const int wanted = BY_LOGIT ? a.topk : min(33, a.topk + SPARE);       // the 33rd has no lane, it is the best of those that are not taken
     int mine = 0, found = 0;                       // lane k: the k-th candidate
+    uint32_t lowest = 0;
     float choice = 0.f;
     for (int k = 0; k < wanted; k++) {
         const uint64_t best = held.best();
         const uint32_t hi = (uint32_t)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
         if (top_hi == 0) break;
+        lowest = top_hi;
         const uint32_t top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? (uint32_t)best : 0u);
         if (lane == k) { mine = (int)~top_lo; choice = unordered(top_hi); }
         held.drop(best, hi == top_hi && (uint32_t)best == top_lo);
         found = k + 1;
     }
-    if (!by_logit && !whole) {
-        float next = __shfl_down_sync(0xffffffffu, choice, 1);
-        bool behind = lane + 1 < found;                // whether `next` is a choice
-        if (a.topk == 32 && found == 32) {             // no lane is left for a candidate to spare: the best of what has not been taken stands in its place
-            const uint32_t left = __reduce_max_sync(0xffffffffu, (uint32_t)(held.best() >> 32));
-            if (lane == 31) { next = unordered(left); behind = left != 0; }
-        }
-        if (__any_sync(0xffffffffu, lane < a.topk && behind && !(choice - next > slack))) {
+    if (!BY_LOGIT && !whole) {
+        const float last = unordered(lowest), below = __shfl_down_sync(0xffffffffu, choice, 1), next = lane == 31 ? last : below;
+        if (__any_sync(0xffffffffu, lane < a.topk && lane + 1 < found && !(choice - next > slack))) {
             // candidates that were not taken are further away than fp32 can be wrong, or there are none
-            const float last = __shfl_sync(0xffffffffu, choice, found - 1), end = __shfl_sync(0xffffffffu, choice, a.topk - 1);
+            const float end = __shfl_sync(0xffffffffu, choice, a.topk - 1);
             if (found < wanted || end - last > slack) {
+                const int lanes_taken = min(found, 32);
                 double total = 1.0;
                 if (!a.sigmoid) {
                     total = 0.0;
@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
                 if (!a.sigmoid && total > 0.0) c /= total;
                 if (a.bias) c += (double)a.bias[mine];
                 int ahead = 0, placed = 0;
-                for (int k = 0; k < found; k++) {
+                for (int k = 0; k < lanes_taken; k++) {
                     const double other = __shfl_sync(0xffffffffu, c, k);
                     const int e = __shfl_sync(0xffffffffu, mine, k);
                     ahead += other > c || (other == c && e < mine);
                 }
-                for (int k = 0; k < found; k++) {
+                for (int k = 0; k < lanes_taken; k++) {
                     const int place = __shfl_sync(0xffffffffu, ahead, k), e = __shfl_sync(0xffffffffu, mine, k);
                     if (place == lane) placed = e;
                 }
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
             } else whole = true;
         }
     }
-    if (whole) {
+    if (!BY_LOGIT && whole) {
         double total = 0.0;
         if (!a.sigmoid) {
 #pragma unroll
@@ -341,16 +341,19 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     // Weights in fp32.  Renormalised ones need the chosen scores up to a common factor alone, so the exponentials are of distances to the largest chosen logit:
     // the largest of all may belong to an expert that a bias or its group keeps out, and fp32 ends 104 below it.  Sigmoids below e^-64 are e^v to
     // 2^-92 of themselves, and get the same factor where all of the chosen are that small.  Scores below e^-745, which fp64 does not hold, are 0.
+    // As a rule the largest of all is among the chosen (always, where the logits decide), as is a sigmoid that fp32 holds.
     constexpr float BARE = -64.f, LEAST = -745.f;
-    const float v = lane < a.topk ? logit(widen(row[mine])) : -INFINITY;
-    float from = a.sigmoid ? 0.f : top, w = 0.f;
-    const bool held_in_64 = v - from > LEAST;
-    if (a.renormalise) {
-        const float most = unordered(__reduce_max_sync(0xffffffffu, ordered(v)));
-        if (!a.sigmoid || most < BARE) from = most;
+    float v = -INFINITY, w = 0.f;
+    if (lane < a.topk) {
+        v = logit(widen(row[mine]));
+        w = a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top);
     }
-    if (a.sigmoid && v >= BARE) w = 1.f / (1.f + expf(-v));
-    else if (held_in_64) w = expf(v - from);
+    if constexpr (!BY_LOGIT) {
+        const float first = a.sigmoid ? 0.f : top;
+        const bool far = a.renormalise && !__any_sync(0xffffffffu, a.sigmoid ? v >= BARE : v == top);
+        const float from = far ? unordered(__reduce_max_sync(0xffffffffu, ordered(v))) : first;
+        if (far || (a.sigmoid && v < BARE)) w = v - first > LEAST ? expf(v - from) : 0.f;
+    }
     float sum = warp_sum(w);
     if (!a.renormalise) {                          // softmax over all experts, the sum in fp32 as the weights are
         sum = 0.f;
@@ -373,14 +376,20 @@ inline int launch_t(Args a, cudaStream_t st) {
     while ((epl << a.lanes_log2) < a.members) epl *= 2;
     a.wide = a.members == epl << a.lanes_log2 && aligned(a.logits, 16) && a.ld * sizeof(T) % 16 == 0 && (!a.bias || aligned(a.bias, 16));
     const dim3 grid((unsigned)((a.S + (long)WARPS - 1) / WARPS)), block(WARPS * 32);
+    const bool by_logit = !a.sigmoid && !a.bias && !a.sum2;
+    const auto launch = [&](auto experts) {
+        constexpr int N = decltype(experts)::value;
+        return by_logit ? launch_pdl(route_kernel<T, N, true>, grid, block, 0, st, a) : launch_pdl(route_kernel<T, N, false>, grid, block, 0, st, a);
+    };
+    using std::integral_constant;
     cudaError_t e;
-    if (epl <= 1) e = launch_pdl(route_kernel<T, 1>, grid, block, 0, st, a);
-    else if (epl <= 2) e = launch_pdl(route_kernel<T, 2>, grid, block, 0, st, a);
-    else if (epl <= 4) e = launch_pdl(route_kernel<T, 4>, grid, block, 0, st, a);
-    else if (epl <= 8) e = launch_pdl(route_kernel<T, 8>, grid, block, 0, st, a);
-    else if (epl <= 16) e = launch_pdl(route_kernel<T, 16>, grid, block, 0, st, a);
-    else if (epl <= 32) e = launch_pdl(route_kernel<T, 32>, grid, block, 0, st, a);
-    else e = launch_pdl(route_kernel<T, 64>, grid, block, 0, st, a);         // groups just above a power of two: 1024 / 17 experts on one lane
+    if (epl <= 1) e = launch(integral_constant<int, 1>());
+    else if (epl <= 2) e = launch(integral_constant<int, 2>());
+    else if (epl <= 4) e = launch(integral_constant<int, 4>());
+    else if (epl <= 8) e = launch(integral_constant<int, 8>());
+    else if (epl <= 16) e = launch(integral_constant<int, 16>());
+    else if (epl <= 32) e = launch(integral_constant<int, 32>());
+    else e = launch(integral_constant<int, 64>());                       // groups just above a power of two: 1024 / 17 experts on one lane
     if (e != cudaSuccess) return cuda_fail(e, "moe_route launch");
     return launch_status("moe_route");
 }
