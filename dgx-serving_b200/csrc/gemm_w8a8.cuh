@@ -20,8 +20,8 @@
 // their int32 sums to the CTA that owns the columns through distributed shared memory, and that one adds them: no workspace, no second
 // launch, and the same bits, since integers add in any order.
 //
-// Bounds and figures (us, in a graph): 2048 x 17408 x 5120 128 (2.85 POP/s; tensor pipe and L2 at three quarters each), 4096^3 52, 333 x 4091 x 3840 9.8 (what an SM takes from
-// L2, 64 bytes a cycle), 16 x 3840 x 15360 13.2 (4.5 TB/s; clusters' start and sums are 4 of it), 1 x 17408 x 5120 15.4 (5.8 TB/s).  The issuing warps stay converged and an elected
+// Bounds and figures (us, in a graph): 2048 x 17408 x 5120 128 (2.85 POP/s; tensor pipe at three quarters, L2 at 44 %), 4096^3 52, 333 x 4091 x 3840 9.8 (676 KB of
+// tiles into each of 128 CTAs, 5.4 at 64 bytes a cycle), 16 x 3840 x 15360 13.2 (4.5 TB/s; clusters' start and sums are 4 of it), 1 x 17408 x 5120 15.4 (5.8 TB/s).  The issuing warps stay converged and an elected
 // lane issues: a lane that branches off alone took 300 cycles a K-tile for waits, descriptors and commits, and the first of these shapes 217 us.
 #pragma once
 #include <cuda.h>

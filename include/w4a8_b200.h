@@ -416,7 +416,8 @@ int w4a8_moe_route(const w4a8_router *router, const void *logits, int64_t ld, in
 /* Products whose weights stay at 8 bits (the layers that lose too much at 4): wq[N][K] int8 with one fp32 scale for each output channel, xq[M][K]
  * int8 with one for each row.
  *   w4a8_quantize_rows_q8: xs = amax / 127, xq = rintf(x / xs) clamped to +-127, a row of zeros 0 (w4a8_quantize_x_q8's arithmetic over whole
- *   rows; weights are quantized offline by the same call, a channel per row).  K a multiple of 32, at most 32768.
+ *   rows; weights are quantized offline by the same call, a channel per row).  K a multiple of 32, at most 32768.  Here, in w4a8_linear_w8a8 and in w4a8_add_norm's codes an element that is not
+ *   a number has the code 0 and no part in its row's or block's amax (look for one before, if it has to be seen), and beside an infinite one all codes are 0 and the scale is infinite.
  *   w4a8_gemm_w8a8: Y[m][n] = float(sum_k xq[m][k] * wq[n][k]) * xs[m] * ws[n] + bias[n] (NULL: none), rounded once to dtype; the sum is exact, so
  *   a row's bits depend on neither M nor the way K is cut.  Y has any alignment and pitch; xq and wq are 16-byte aligned.  Any M, N up to
  *   2^31 - 1024; K a multiple of 32, at most 131040.
